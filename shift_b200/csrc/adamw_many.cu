@@ -1,0 +1,336 @@
+// One AdamW update of many tensors, moments in fp32 or in 8 bits.
+//
+// With bias corrections c1 = 1 - beta1^t and c2 = sqrt(1 - beta2^t):
+//   g  = grad * grad_scale
+//   w  = w (1 - lr wd)
+//   m += (g - m) (1 - beta1)          v = beta2 v + (1 - beta2) g^2
+//   w -= lr / c1 * m / (sqrt(v) / c2 + eps)
+// in fp32, the order of the single-buffer step in xent_adam.cu.  The 8-bit
+// form keeps m and r = sqrt(v) as e4m3 codes with a power-of-two scale per 128
+// elements (fp8.cuh).  r instead of v halves the exponent range that the codes
+// have to cover.  Magnitudes are rounded up with the probability of their
+// distance from the code below: v moves by a thousandth per step against a
+// half step of 6 %, so rounding to nearest would freeze it.  The random bits
+// are a counter hash of (seed, tensor number, element), hence the same for any
+// launch shape; elements 2^32 apart share them.
+//
+// Bound: DRAM.  The tensors' pointers travel as kernel parameters, so a step
+// is one launch per 320 tensors, needs no device table and can be captured.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "fp8.cuh"
+
+namespace sb {
+namespace adam {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;                        // elements per thread and pass
+constexpr int kChunk = kThreads * kVec;        // elements per CTA: 16 blocks of 128
+constexpr int kMaxTensors = 320;
+
+struct Entry {
+  void* p;             // parameter
+  float* w;            // fp32 master copy, or null: the parameter itself is updated
+  const void* g;
+  void *m, *v;         // fp32, or codes
+  uint8_t *ms, *vs;    // scales of the codes
+  long n;
+};
+
+struct Table {
+  Entry e[kMaxTensors];
+  uint32_t end[kMaxTensors];   // chunks of tensors 0..t, cumulated
+  uint16_t number[kMaxTensors];   // the tensor's number in the caller's list | 0x8000: vectors are aligned
+  int count;
+};
+
+struct StepArgs {
+  // 1 - beta is taken in double on the host: in fp32 it would lose the digits that beta has in common with 1
+  float lr, beta2, one_minus_beta1, one_minus_beta2, eps, wd, c1, c2, grad_scale;
+  uint32_t seed;
+  const int* sdev;       // optional: seed, lr, c1, c2 from device memory
+  const int* skip;       // optional: a non-zero word leaves everything as it is
+  int* nonfinite;        // optional: set where a scaled gradient is not finite
+};
+
+SB_DEVICE uint32_t mix32(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x7FEB352Du;
+  h = (h ^ (h >> 15)) * 0x846CA68Bu;
+  return h ^ (h >> 16);
+}
+
+// A magnitude y in [0, 448] to the e4m3 value below or above it: 16 random
+// bits are added below the three kept fraction bits, then cut off.  Below the
+// smallest normal value 2^-6 the grid is uniform, as it is in [2^-6, 2^-5), so
+// y is moved there and back.
+SB_DEVICE float round_up_sometimes(float y, uint32_t bits16) {
+  const float shift = y < 0.015625f ? 0.015625f : 0.f;
+  const uint32_t b = (__float_as_uint(y + shift) + (bits16 << 4)) & ~0xFFFFFu;
+  return __uint_as_float(b) - shift;
+}
+
+template <typename T>
+SB_DEVICE float as_float(T x);
+template <>
+SB_DEVICE float as_float<float>(float x) { return x; }
+template <>
+SB_DEVICE float as_float<__half>(__half x) { return __half2float(x); }
+template <>
+SB_DEVICE float as_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+SB_DEVICE T from_float(float x);
+template <>
+SB_DEVICE float from_float<float>(float x) { return x; }
+template <>
+SB_DEVICE __half from_float<__half>(float x) { return __float2half(x); }
+template <>
+SB_DEVICE __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
+
+template <typename T>
+SB_DEVICE void load8(const T* p, int valid, bool vec, float* f) {
+  if (vec && valid == kVec) {
+    constexpr int W = sizeof(T) * kVec / 4;
+    uint32_t raw[W];
+    if constexpr (W >= 4) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = as_float<T>(reinterpret_cast<const T*>(raw)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = i < valid ? as_float<T>(p[i]) : 0.f;
+  }
+}
+
+template <typename T>
+SB_DEVICE void store8(T* p, int valid, bool vec, const float* f) {
+  if (vec && valid == kVec) {
+    T t[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) t[i] = from_float<T>(f[i]);
+    const uint4* raw = reinterpret_cast<const uint4*>(t);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (i < valid) p[i] = from_float<T>(f[i]);
+  }
+}
+
+// Eight codes of a block times its scale.
+SB_DEVICE void load_codes(const uint8_t* p, float scale, int valid, bool vec, float* f) {
+  uint32_t raw[2] = {0, 0};
+  if (vec && valid == kVec) {
+    *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (i < valid) raw[i / 4] |= static_cast<uint32_t>(p[i]) << (8 * (i % 4));
+  }
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+        static_cast<__nv_fp8x2_storage_t>(raw[i / 2] >> (16 * (i % 2))), __NV_E4M3);
+    const float2 v = __half22float2(__half2(h));
+    f[2 * i] = v.x * scale;
+    f[2 * i + 1] = v.y * scale;
+  }
+}
+
+// Eight values of a block of 128 (16 lanes) to codes; returns the scale byte.
+SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits16, int valid, bool vec) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const float a = fabsf(f[i]);
+    top = fmaxf(top, a < INFINITY ? a : 0.f);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int byte = fp8::scale_byte(top, fp8::kE4M3);
+  const float inv = fp8::inv_scale(byte);
+  uint32_t raw[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kVec; i += 2) {
+    float y[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float x = f[i + j];
+      y[j] = fabsf(x) < INFINITY ? copysignf(round_up_sometimes(fabsf(x * inv), bits16[i + j]), x) : NAN;
+    }
+    raw[i / 4] |= fp8::pack2(y[0], y[1], fp8::kE4M3) << (16 * ((i / 2) % 2));
+  }
+  if (vec && valid == kVec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(raw[0], raw[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (i < valid) p[i] = static_cast<uint8_t>(raw[i / 4] >> (8 * (i % 4)));
+  }
+  return byte;
+}
+
+template <typename P, typename Gr, bool EIGHT>
+__global__ void __launch_bounds__(kThreads)
+adamw_many_kernel(const __grid_constant__ Table tab, StepArgs a) {
+  if (a.skip != nullptr && *a.skip != 0) return;
+  if (a.sdev != nullptr) {
+    a.seed = static_cast<uint32_t>(a.sdev[0]);
+    a.lr = __int_as_float(a.sdev[1]);
+    a.c1 = __int_as_float(a.sdev[2]);
+    a.c2 = __int_as_float(a.sdev[3]);
+  }
+  // the tensor whose chunks cover this CTA
+  int lo = 0, hi = tab.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (tab.end[mid] > blockIdx.x) hi = mid;
+    else lo = mid + 1;
+  }
+  const Entry& e = tab.e[lo];
+  const uint32_t first = lo == 0 ? 0 : tab.end[lo - 1];
+  const bool vec = (tab.number[lo] & 0x8000u) != 0;
+  const uint32_t key = mix32(mix32(a.seed) ^ ((tab.number[lo] & 0x7FFFu) * 0x9E3779B1u));
+  const long i0 = static_cast<long>(blockIdx.x - first) * kChunk + threadIdx.x * kVec;
+  const int valid = static_cast<int>(max(0l, min(static_cast<long>(kVec), e.n - i0)));
+
+  float g[kVec], w[kVec], m[kVec], v[kVec];
+  load8<Gr>(static_cast<const Gr*>(e.g) + i0, valid, vec, g);
+  if (e.w != nullptr) load8<float>(e.w + i0, valid, vec, w);
+  else load8<P>(static_cast<const P*>(e.p) + i0, valid, vec, w);
+  const long block = i0 / 128;
+  if constexpr (EIGHT) {
+    const float sm = valid > 0 ? fp8::scale_of(e.ms[block]) : 0.f, sv = valid > 0 ? fp8::scale_of(e.vs[block]) : 0.f;
+    load_codes(static_cast<const uint8_t*>(e.m) + i0, sm, valid, vec, m);
+    load_codes(static_cast<const uint8_t*>(e.v) + i0, sv, valid, vec, v);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] *= v[i];
+  } else {
+    load8<float>(static_cast<const float*>(e.m) + i0, valid, vec, m);
+    load8<float>(static_cast<const float*>(e.v) + i0, valid, vec, v);
+  }
+  bool bad = false;
+  float r[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const float gi = g[i] * a.grad_scale;
+    bad |= !(fabsf(gi) < INFINITY);
+    w[i] *= 1.f - a.lr * a.wd;
+    m[i] += (gi - m[i]) * a.one_minus_beta1;
+    v[i] = v[i] * a.beta2 + a.one_minus_beta2 * gi * gi;
+    r[i] = sqrtf(v[i]);
+    w[i] -= (a.lr / a.c1) * (m[i] / (r[i] / a.c2 + a.eps));
+  }
+  if constexpr (EIGHT) {
+    uint32_t um[kVec], uv[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const uint32_t u = mix32(static_cast<uint32_t>(i0 + i) * 0x9E3779B1u + key);
+      um[i] = u & 0xFFFFu;
+      uv[i] = u >> 16;
+    }
+    const int bm = store_codes(static_cast<uint8_t*>(e.m) + i0, m, um, valid, vec);
+    const int bv = store_codes(static_cast<uint8_t*>(e.v) + i0, r, uv, valid, vec);
+    if (threadIdx.x % 16 == 0 && valid > 0) {
+      e.ms[block] = static_cast<uint8_t>(bm);
+      e.vs[block] = static_cast<uint8_t>(bv);
+    }
+  } else {
+    store8<float>(static_cast<float*>(e.m) + i0, valid, vec, m);
+    store8<float>(static_cast<float*>(e.v) + i0, valid, vec, v);
+  }
+  if (e.w != nullptr) store8<float>(e.w + i0, valid, vec, w);
+  store8<P>(static_cast<P*>(e.p) + i0, valid, vec, w);
+  if (bad && a.nonfinite != nullptr) atomicOr(a.nonfinite, 1);
+}
+
+template <typename P, typename Gr>
+static void launch_many(const Table& t, const StepArgs& a, bool eight, cudaStream_t st) {
+  const unsigned blocks = t.end[t.count - 1];
+  if (eight) adamw_many_kernel<P, Gr, true><<<blocks, kThreads, 0, st>>>(t, a);
+  else adamw_many_kernel<P, Gr, false><<<blocks, kThreads, 0, st>>>(t, a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// Lists of equal length; w, ms and vs may be empty.  All tensors contiguous,
+// on one device; parameters of one type, gradients of one type.
+void adamw_many(const std::vector<at::Tensor>& p, const std::vector<at::Tensor>& w, const std::vector<at::Tensor>& g,
+                const std::vector<at::Tensor>& m, const std::vector<at::Tensor>& ms, const std::vector<at::Tensor>& v,
+                const std::vector<at::Tensor>& vs, const std::vector<int64_t>& numbers, double lr, double beta1,
+                double beta2, double eps, double wd, int64_t step, double grad_scale, int64_t seed,
+                const c10::optional<at::Tensor>& step_dev, const c10::optional<at::Tensor>& skip,
+                const c10::optional<at::Tensor>& nonfinite) {
+  if (p.empty()) return;
+  const at::cuda::CUDAGuard guard(p[0].device());
+  const bool eight = !ms.empty();
+  StepArgs a;
+  a.lr = static_cast<float>(lr);
+  a.beta2 = static_cast<float>(beta2);
+  a.one_minus_beta1 = static_cast<float>(1.0 - beta1);
+  a.one_minus_beta2 = static_cast<float>(1.0 - beta2);
+  a.eps = static_cast<float>(eps);
+  a.wd = static_cast<float>(wd);
+  a.c1 = static_cast<float>(1.0 - std::pow(beta1, static_cast<double>(step)));
+  a.c2 = static_cast<float>(std::sqrt(1.0 - std::pow(beta2, static_cast<double>(step))));
+  a.grad_scale = static_cast<float>(grad_scale);
+  a.seed = static_cast<uint32_t>(seed);
+  a.sdev = step_dev.has_value() ? step_dev->data_ptr<int>() : nullptr;
+  a.skip = skip.has_value() ? skip->data_ptr<int>() : nullptr;
+  a.nonfinite = nonfinite.has_value() ? nonfinite->data_ptr<int>() : nullptr;
+  const auto pt = p[0].scalar_type(), gt = g[0].scalar_type();
+  auto st = at::cuda::getCurrentCUDAStream();
+  Table tab;
+  tab.count = 0;
+  uint64_t chunks = 0;
+  auto flush = [&] {
+    if (tab.count == 0) return;
+#define SB_ADAM(PT, P)                                                                \
+  if (pt == PT) {                                                                     \
+    if (gt == at::kFloat) launch_many<P, float>(tab, a, eight, st);                   \
+    else if (gt == at::kBFloat16) launch_many<P, __nv_bfloat16>(tab, a, eight, st);   \
+    else launch_many<P, __half>(tab, a, eight, st);                                   \
+  }
+    SB_ADAM(at::kFloat, float)
+    SB_ADAM(at::kBFloat16, __nv_bfloat16)
+    SB_ADAM(at::kHalf, __half)
+#undef SB_ADAM
+    tab.count = 0;
+    chunks = 0;
+  };
+  for (size_t t = 0; t < p.size(); ++t) {
+    const long n = p[t].numel();
+    if (n == 0) continue;
+    const uint64_t add = (static_cast<uint64_t>(n) + kChunk - 1) / kChunk;
+    TORCH_CHECK(add < (1ull << 31), "adamw_many: a tensor is too long");
+    if (tab.count == kMaxTensors || chunks + add >= (1ull << 31)) flush();
+    Entry& e = tab.e[tab.count];
+    e.p = p[t].data_ptr();
+    e.w = w.empty() ? nullptr : w[t].data_ptr<float>();
+    e.g = g[t].data_ptr();
+    e.m = m[t].data_ptr();
+    e.v = v[t].data_ptr();
+    e.ms = eight ? static_cast<uint8_t*>(ms[t].data_ptr()) : nullptr;
+    e.vs = eight ? static_cast<uint8_t*>(vs[t].data_ptr()) : nullptr;
+    e.n = n;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.w) |
+                          reinterpret_cast<uintptr_t>(e.g) | reinterpret_cast<uintptr_t>(e.m) |
+                          reinterpret_cast<uintptr_t>(e.v);
+    chunks += add;
+    tab.end[tab.count] = static_cast<uint32_t>(chunks);
+    tab.number[tab.count] = static_cast<uint16_t>((numbers[t] & 0x7FFF) | ((all & 15) == 0 ? 0x8000 : 0));
+    ++tab.count;
+  }
+  flush();
+}
+
+}  // namespace adam
+}  // namespace sb

@@ -110,6 +110,115 @@ def adamw(master, m, v, grad, lr, beta1, beta2, eps, wd, step):
     return master, m, v
 
 
+# ------------------------------------------------------------- 8-bit floating point, a scale per block of 128
+def fp8_block_scale(amax: torch.Tensor, fmt: str):
+    """Scale byte (exponent + 127) and reciprocal scale of blocks with largest finite magnitude ``amax``."""
+    top = 8 if fmt == "e4m3" else 15
+    frac, ex = torch.frexp(amax.float())
+    e = ex - 1 - top + (frac > 0.875).int()
+    e = torch.where(amax > 0, e, torch.full_like(e, -127)).clamp(-127, 127)
+    return (e + 127).to(torch.uint8), ((127 - e) << 23).to(torch.int32).view(torch.float32)
+
+
+def _finite_abs(x: torch.Tensor) -> torch.Tensor:
+    a = x.abs()
+    return torch.where(torch.isfinite(a), a, torch.zeros_like(a))
+
+
+def _fp8_pack_scales(b: torch.Tensor) -> torch.Tensor:
+    b = F.pad(b, (0, -b.shape[1] % 4))
+    return b.view(b.shape[0], -1, 4).permute(1, 0, 2).contiguous()
+
+
+def _fp8_codes(x: torch.Tensor, inv: torch.Tensor, fmt: str) -> torch.Tensor:
+    dt = torch.float8_e4m3fn if fmt == "e4m3" else torch.float8_e5m2
+    out = torch.zeros(x.shape[0], -(-x.shape[1] // 16) * 16, dtype=torch.uint8)
+    out[:, :x.shape[1]] = (x * inv).to(dt).view(torch.uint8)
+    return out
+
+
+def fp8_quantize(x: torch.Tensor, fmt: str, tiles: bool, both: bool) -> list:
+    """Codes and scales (uint8) of [rows, cols] or [G, rows, cols], and of the transposes."""
+    x = (x if x.dim() == 3 else x[None]).float()
+    G, R, C = x.shape
+    if x.numel() == 0:
+        got = [torch.zeros(G * R, -(-C // 16) * 16), torch.zeros(-(-C // 512), G * R, 4)]
+        if both:
+            got += [torch.zeros(G * C, -(-R // 16) * 16), torch.zeros(-(-R // 512), G * C, 4)]
+        return [t.to(torch.uint8) for t in got]
+    rb, cb = -(-R // 128), -(-C // 128)
+    a = F.pad(_finite_abs(x), (0, cb * 128 - C, 0, rb * 128 - R)).view(G, rb, 128, cb, 128)
+    full = a.amax((2, 4), keepdim=True) if tiles else None
+    got = []
+    for t in range(2 if both else 1):
+        m = full if tiles else a.amax(2 if t else 4, keepdim=True)
+        b, inv = fp8_block_scale(m, fmt)
+        inv = inv.expand(G, rb, 128, cb, 128).reshape(G, rb * 128, cb * 128)[:, :R, :C]
+        xt, it = (x.transpose(1, 2), inv.transpose(1, 2)) if t else (x, inv)
+        n, k = (C, R) if t else (R, C)
+        if t:
+            b = b.permute(0, 3, 4, 1, 2)                     # [G, cb, 128 or 1, rb, 1]
+        b = b.expand(G, b.shape[1], 128, b.shape[3], 1).reshape(G, -1, b.shape[3])[:, :n]
+        got += [_fp8_codes(xt.reshape(G * n, k), it.reshape(G * n, k), fmt), _fp8_pack_scales(b.reshape(G * n, -1))]
+    return got
+
+
+def fp8_scales(scale: torch.Tensor) -> torch.Tensor:
+    """Scale bytes as fp32 powers of two."""
+    b = scale.view(torch.uint8).int()
+    return torch.where(b > 0, b << 23, torch.full_like(b, 1 << 22)).view(torch.float32)
+
+
+def fp8_values(data: torch.Tensor, scale: torch.Tensor, cols: int) -> torch.Tensor:
+    """fp32 values of an 8-bit matrix (``ops.fp8.BlockFp8``)."""
+    s = fp8_scales(scale).permute(1, 0, 2).reshape(data.shape[0], 4 * scale.shape[0]).repeat_interleave(128, 1)
+    return data[:, :cols].float() * s[:, :cols]
+
+
+def segments(offs: torch.Tensor, limit: int):
+    """(lo, hi) of each segment, cut to [0, limit] and never negative."""
+    o = offs.tolist()
+    out = []
+    for lo, hi in zip(o, o[1:]):
+        lo = min(max(lo, 0), limit)
+        out.append((lo, min(max(hi, lo), limit)))
+    return out
+
+
+# ------------------------------------------------------------- 8-bit moments
+_M32 = 0xFFFFFFFF
+
+
+def mix32(h):
+    """Two multiply-and-fold rounds over 32 bits (ints or int64 tensors)."""
+    h = h & _M32
+    h = ((h ^ (h >> 16)) * 0x7FEB352D) & _M32
+    h = ((h ^ (h >> 15)) * 0x846CA68B) & _M32
+    return h ^ (h >> 16)
+
+
+def moment_draws(n: int, seed: int, number: int, device=None) -> torch.Tensor:
+    """32 random bits per element of tensor ``number``: the low half rounds exp_avg, the high half exp_avg_sq."""
+    key = mix32(mix32(seed & _M32) ^ ((number * 0x9E3779B1) & _M32))
+    return mix32(torch.arange(n, dtype=torch.int64, device=device) * 0x9E3779B1 + key)
+
+
+def moment_decode(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    return code.float() * fp8_scales(scale).repeat_interleave(128)[: code.numel()]
+
+
+def moment_encode(x: torch.Tensor, bits16: torch.Tensor):
+    """x fp32 [n] -> (codes float8_e4m3fn [n], scales float8_e8m0fnu [ceil(n / 128)]); a magnitude goes to the
+    code above with the probability of its distance from the one below."""
+    n = x.numel()
+    b, inv = fp8_block_scale(F.pad(_finite_abs(x), (0, -n % 128)).view(-1, 128).amax(-1), "e4m3")
+    y = (x * inv.repeat_interleave(128)[:n]).abs()
+    shift = torch.where(y < 2.0 ** -6, 2.0 ** -6, 0.0)
+    t = (((y + shift).view(torch.int32) + (bits16 << 4).int()) & ~0xFFFFF).view(torch.float32) - shift
+    t = torch.where(torch.isfinite(x), torch.copysign(t, x), torch.full_like(t, math.nan))
+    return t.to(torch.float8_e4m3fn), b.view(torch.float8_e8m0fnu)
+
+
 def grad_of(fn, inputs, grad_out):
     """Gradients of fn(*inputs) w.r.t. the floating inputs, via autograd."""
     # cloned: an input may be a view of a buffer another rank's thread writes

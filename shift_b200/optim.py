@@ -1,0 +1,159 @@
+"""AdamW over many tensors at once, with moments in 32 or in 8 bits.
+
+``AdamWMany`` updates lists of tensors with one kernel launch per 320 of them
+(``csrc/adamw_many.cu``), in place.  It stands beside
+``ops.functional.adamw_step``, which updates one flat buffer of a fixed layout
+from one state generation into the next: use that one where the parameters
+live in ``parallel.flat.FlatParams``, and this one for parameters that are
+tensors of their own (an ordinary module, a model that is not ours).
+
+8-bit moments take 2 + 1/64 bytes per parameter instead of 8.  ``exp_avg`` and
+the square root of ``exp_avg_sq`` are e4m3 codes with one power-of-two scale
+per 128 consecutive elements, rounded stochastically from ``seed``.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from .ops import reference as ref
+from .ops._ext import ext
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class State8(NamedTuple):
+    """One moment of a tensor of n elements: ``code`` float8_e4m3fn [n], ``scale`` float8_e8m0fnu [ceil(n / 128)].
+    For ``exp_avg_sq`` the codes hold its square root."""
+    code: torch.Tensor
+    scale: torch.Tensor
+
+    @classmethod
+    def zeros(cls, param: torch.Tensor) -> "State8":
+        n = param.numel()
+        return cls(torch.zeros(n, dtype=torch.uint8, device=param.device).view(torch.float8_e4m3fn),
+                   torch.zeros(-(-n // 128), dtype=torch.uint8, device=param.device).view(torch.float8_e8m0fnu))
+
+    def values(self) -> torch.Tensor:
+        """fp32 [n]; of ``exp_avg_sq`` its square root."""
+        return ref.moment_decode(self.code, self.scale)
+
+
+def _fail(cond: bool, text: str):
+    if not cond:
+        raise ValueError("AdamWMany: " + text)
+
+
+class AdamWMany:
+    """``params``: contiguous fp32 / bf16 / fp16 tensors on one device, updated in place.
+    ``exp_avg`` / ``exp_avg_sq``: per parameter an fp32 tensor, or a ``State8``
+    (one kind for all).  ``masters``: optional fp32 tensors that hold the exact
+    weights; a parameter then is their rounded copy.  Without them a bf16 or
+    fp16 parameter is itself the weight, and each step rounds it."""
+
+    def __init__(self, params, exp_avg, exp_avg_sq, masters=None):
+        self.params, self.exp_avg, self.exp_avg_sq = list(params), list(exp_avg), list(exp_avg_sq)
+        self.masters = None if masters is None else list(masters)
+        n = len(self.params)
+        _fail(n <= 0x7FFF, f"{n} tensors, at most {0x7FFF}")
+        _fail(len(self.exp_avg) == n and len(self.exp_avg_sq) == n
+              and (self.masters is None or len(self.masters) == n), "lists of different lengths")
+        self.eight = n > 0 and isinstance(self.exp_avg[0], State8)
+        for t, p in enumerate(self.params):
+            _fail(p.dtype in _FLOATS, f"parameter {t} is {p.dtype}")
+            same = [p]
+            for s in (self.exp_avg[t], self.exp_avg_sq[t]):
+                _fail(isinstance(s, State8) == self.eight, "moments in 8 bits and in 32 bits are mixed")
+                if self.eight:
+                    _fail(s.code.dtype == torch.float8_e4m3fn and s.code.numel() == p.numel(),
+                          f"tensor {t}: {p.numel()} codes of float8_e4m3fn are expected")
+                    _fail(s.scale.dtype == torch.float8_e8m0fnu and s.scale.numel() == -(-p.numel() // 128),
+                          f"tensor {t}: {-(-p.numel() // 128)} scales of float8_e8m0fnu are expected")
+                    same += [s.code, s.scale]
+                else:
+                    _fail(s.dtype == torch.float32 and s.numel() == p.numel(),
+                          f"tensor {t}: fp32 moments of {p.numel()} elements are expected")
+                    same.append(s)
+            if self.masters is not None:
+                w = self.masters[t]
+                _fail(w.dtype == torch.float32 and w.numel() == p.numel(),
+                      f"tensor {t}: an fp32 master of {p.numel()} elements is expected")
+                same.append(w)
+            _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
+            _fail(all(x.device == self.params[0].device for x in same), f"tensor {t} or its state is on another device")
+
+    def step(self, grads, lr: float = 1.0e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1.0e-8,
+             wd: float = 0.01, step: int = 1, grad_scale: float = 1.0, seed: int | None = None, step_dev=None,
+             skip=None, nonfinite=None):
+        """One update.  ``grads``: contiguous tensors like the parameters, fp32, bf16 or fp16.
+
+        ``step`` counts from 1.  ``seed`` (8-bit moments) chooses the random
+        bits; by default it is ``step``.  ``step_dev``: int32 [>= 4] on the
+        device with seed, and lr, 1 - beta1^t, sqrt(1 - beta2^t) as float
+        bits, which replace the arguments (a replayed graph's step;
+        ``engine.StepBlock`` writes that layout).  ``skip``: int32 on the
+        device; where it is not zero nothing changes.  ``nonfinite``: int32
+        flag, set where a scaled gradient is not finite."""
+        grads = list(grads)
+        _fail(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")
+        _fail(step >= 1, f"step {step}: counted from 1")
+        dev = self.params[0].device if self.params else None
+        for t, (g, p) in enumerate(zip(grads, self.params)):
+            _fail(g.dtype in _FLOATS and g.numel() == p.numel() and g.is_contiguous() and g.device == dev,
+                  f"gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {dev}")
+        for name, x, least in (("step_dev", step_dev, 4), ("skip", skip, 1), ("nonfinite", nonfinite, 1)):
+            _fail(x is None or (x.dtype == torch.int32 and x.numel() >= least and x.is_contiguous() and x.device == dev),
+                  f"{name}: int32 [{least}] on {dev}")
+        seed = step if seed is None else seed
+        if dev is None:
+            return
+        if dev.type != "cuda":
+            self._cpu_step(grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite)
+            return
+        kinds: dict = {}
+        for t, (p, g) in enumerate(zip(self.params, grads)):
+            kinds.setdefault((p.dtype, g.dtype), []).append(t)
+        for at in kinds.values():
+            pick = lambda xs: [xs[t] for t in at]  # noqa: E731
+            m, v = pick(self.exp_avg), pick(self.exp_avg_sq)
+            ms = vs = []
+            if self.eight:
+                m, ms = [x.code for x in m], [x.scale for x in m]
+                v, vs = [x.code for x in v], [x.scale for x in v]
+            ext().adamw_many(pick(self.params), pick(self.masters) if self.masters is not None else [], pick(grads),
+                             m, ms, v, vs, at, lr, beta1, beta2, eps, wd, step, grad_scale, seed & 0xFFFFFFFF,
+                             step_dev, skip, nonfinite)
+
+    def _cpu_step(self, grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite):
+        if skip is not None and int(skip.view(-1)[0]) != 0:
+            return
+        c1, c2 = 1.0 - beta1 ** step, math.sqrt(1.0 - beta2 ** step)
+        if step_dev is not None:
+            seed = int(step_dev.view(-1)[0])
+            lr, c1, c2 = step_dev.view(-1)[1:4].view(torch.float32).tolist()
+        for t, (p, g) in enumerate(zip(self.params, grads)):
+            g = g.detach().reshape(-1).float() * grad_scale
+            if nonfinite is not None and not bool(torch.isfinite(g).all()):
+                nonfinite.view(-1)[0] = 1
+            w = (p if self.masters is None else self.masters[t]).detach().view(-1)
+            m, v = self.exp_avg[t], self.exp_avg_sq[t]
+            m32 = m.values() if self.eight else m.view(-1)
+            v32 = v.values().square() if self.eight else v.view(-1)
+            m32 = m32 + (g - m32) * (1.0 - beta1)
+            v32 = v32 * beta2 + (1.0 - beta2) * g * g
+            r = v32.sqrt()
+            new = w.float() * (1.0 - lr * wd) - (lr / c1) * (m32 / (r / c2 + eps))
+            if self.eight:
+                u = ref.moment_draws(g.numel(), seed, t)
+                for s, x, bits in ((m, m32, u & 0xFFFF), (v, r, u >> 16)):
+                    code, scale = ref.moment_encode(x, bits)
+                    s.code.view(-1).copy_(code)
+                    s.scale.copy_(scale)
+            else:
+                m.view(-1).copy_(m32)
+                v.view(-1).copy_(v32)
+            w.copy_(new)
+            if self.masters is not None:
+                p.detach().view(-1).copy_(new)
