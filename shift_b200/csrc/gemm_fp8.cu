@@ -5,10 +5,30 @@
 // Both operands have the contraction inside (K-major), see fp8.cuh for their
 // layout.  Row groups: A and D rows are cut into segments by offs[0..G], group
 // g multiplies with B rows [g N, (g + 1) N).  K groups: the contraction is cut
-// into segments that start on a block, group g writes D rows [g M, (g + 1) M).
+// into segments on block boundaries, group g writes D rows [g M, (g + 1) M).
+//
+// The block-scaled form of tcgen05.mma multiplies each product by both scales
+// itself, for runs of 32 along K: a block of 128 is four of them with the same
+// exponent.  So sums stay in one fp32 accumulator in tensor memory over the
+// whole contraction and no partial sum is ever rescaled.  The exponents of 128
+// rows and four blocks are 128 words; the scale plane is stored so that they
+// are contiguous, and tcgen05.cp spreads them over tensor memory in the order
+// the instruction wants (row r in lane r % 32, column r / 32).
+//
+// Warp roles (256 threads):
+//   warp 0      TMA loads of the operand tiles (one lane)
+//   warp 1      MMA issue (one lane)
+//   warp 2      scale words: global -> shared memory
+//   warp 3      tensor memory allocation
+//   warps 4..7  epilogue (TMEM lane quarter = warp % 4)
+// All waits are bounded (common.cuh).
+#include <cuda.h>
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+
+#include <cstring>
+#include <mutex>
 
 #include "fp8.cuh"
 
@@ -17,87 +37,452 @@ namespace fp8 {
 
 enum Mode : int { kRowGroups = 0, kKGroups = 1 };
 
+constexpr int kThreads = 256;
+constexpr int BM = 128;
+constexpr int BK = 128;            // one scale block, one 128-byte swizzled row
+constexpr int kMaxGroups = 512;
+constexpr int kScaleStages = 4;
+
+template <int BN>
+struct Cfg {
+  static constexpr int kABytes = BM * BK;
+  static constexpr int kBBytes = BN * BK;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = BN == 192 ? 4 : (BN == 128 ? 5 : 7);
+  static constexpr int kBParts = (BN + 127) / 128;               // 128-row parts of the B scales
+  static constexpr int kScaleBytes = 512 * (1 + kBParts);
+  static constexpr int kEpiBytes = 4 * 2 * 4096;                 // per warp two buffers of 32 rows x 128 bytes
+  static constexpr int kAccCols = BN <= 64 ? 64 : BN;
+  static constexpr int kScaleCols = 4 * (1 + kBParts);
+  static constexpr int kTmemCols = 512;
+  static constexpr int kScaleCol0 = 2 * kAccCols;
+  static_assert(kScaleCol0 + kScaleStages * kScaleCols <= kTmemCols, "tensor memory budget");
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 +
+                                    2 * (kMaxGroups + 1) * 4;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
 struct Args {
-  const uint8_t *a, *b;
-  const uint8_t *sa, *sb;
-  long lda, ldb;
-  long rows_a, rows_b;     // rows of the scale planes
+  const uint32_t *sa, *sb;
+  int rows_a, rows_b;      // rows of the scale planes
   int M, N, K, G, mode;
+  int split;               // row mode, one group: K ranges, partial sums into D [split][M][N] fp32
   const int* offs;
   void* D;
   long ldd;
-  bool f32, acc, a_e5m2, b_e5m2;
+  int d_rows;              // rows of the tensor that tmD describes
+  bool f32, acc, tma_store;
+  uint32_t idesc;
   int* status;
 };
 
-SB_DEVICE float decode8(uint8_t c, bool e5m2) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, e5m2 ? __NV_E5M2 : __NV_E4M3);
-  return __half2float(__half(h));
+struct Tile {
+  int m0, n0;              // first row of A / column of D within the operand
+  int a_row, b_row;        // rows of the operands
+  long d_row;              // first output row
+  int m_valid;
+  int kb0, kb;             // first block of 128, number of blocks
+};
+
+// D[tmem] (+)= A[smem] B[smem]^T with the scales in tensor memory.
+SB_DEVICE void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 bytes to 32 lanes x 4 columns, repeated in the four lane quarters.
+SB_DEVICE void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128 >> 4) << 32;      // eight rows of 16 bytes apart
+  d |= 1ull << 46;
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-// One CTA per 64 x 64 tile of one group, blocks of 32 along K in fp32.
-__global__ void __launch_bounds__(256) matmul_kernel(const Args p) {
-  __shared__ float sA[32][65], sB[32][65];
-  const int tiles_n = (p.N + 63) / 64;
-  int g = blockIdx.y;
-  int lo = 0, hi = p.mode == kRowGroups ? p.M : p.K;
-  if (p.offs != nullptr) {
-    const int lim = hi;
-    lo = min(max(p.offs[g], 0), lim);
-    hi = min(max(p.offs[g + 1], lo), lim);
-    if (p.mode == kKGroups && lo % 128 != 0 && hi > lo) {
-      if (threadIdx.x == 0) record_status(p.status, kBadShape);
-      return;
+template <int BN>
+__device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile) {
+  const int tiles_n = (p.N + BN - 1) / BN;
+  Tile t;
+  if (p.mode == kRowGroups) {
+    int lo = 0, hi = p.G - 1;                      // last group whose first tile is at most `tile`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (s_prefix[mid] <= tile) lo = mid;
+      else hi = mid - 1;
     }
-  }
-  const int tm = blockIdx.x / tiles_n, tn = blockIdx.x % tiles_n;
-  const int m_end = p.mode == kRowGroups ? hi : p.M;
-  const int m0 = (p.mode == kRowGroups ? lo : 0) + tm * 64, n0 = tn * 64;
-  if (m0 >= m_end) return;
-  const int k_lo = p.mode == kRowGroups ? 0 : lo, k_hi = p.mode == kRowGroups ? p.K : hi;
-  const long b_row0 = p.mode == kRowGroups ? static_cast<long>(g) * p.N : 0;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int k0 = k_lo; k0 < k_hi; k0 += 32) {
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      const int r = i / 32, k = k0 + i % 32;
-      float fa = 0.f, fb = 0.f;
-      if (m0 + r < m_end && k < k_hi)
-        fa = decode8(p.a[static_cast<long>(m0 + r) * p.lda + k], p.a_e5m2) *
-             scale_of(p.sa[((k / 512) * p.rows_a + m0 + r) * 4 + k / 128 % 4]);
-      if (n0 + r < p.N && k < k_hi)
-        fb = decode8(p.b[(b_row0 + n0 + r) * p.ldb + k], p.b_e5m2) *
-             scale_of(p.sb[((k / 512) * p.rows_b + b_row0 + n0 + r) * 4 + k / 128 % 4]);
-      sA[i % 32][r] = fa;
-      sB[i % 32][r] = fb;
+    int local = tile - s_prefix[lo];
+    const int blocks = (p.K + BK - 1) / BK;
+    int s = 0;
+    if (p.split > 1) {
+      const int per = (p.M + BM - 1) / BM * tiles_n;
+      s = local / per;
+      local -= s * per;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sA[k][ty + 16 * i] * sB[k][tx + 16 * j];
-    __syncthreads();
+    const int tm = local / tiles_n, tn = local % tiles_n;
+    t.m0 = s_offs[lo] + tm * BM;
+    t.n0 = tn * BN;
+    t.a_row = t.m0;
+    t.b_row = lo * p.N + t.n0;
+    t.d_row = t.m0 + static_cast<long>(s) * p.M;
+    t.m_valid = min(BM, s_offs[lo + 1] - t.m0);
+    t.kb0 = static_cast<int>(static_cast<long>(blocks) * s / p.split);
+    t.kb = static_cast<int>(static_cast<long>(blocks) * (s + 1) / p.split) - t.kb0;
+  } else {
+    const int tiles_m = (p.M + BM - 1) / BM;
+    const int per = tiles_m * tiles_n;
+    const int g = tile / per, local = tile % per;
+    const int tm = local / tiles_n, tn = local % tiles_n;
+    t.m0 = tm * BM;
+    t.n0 = tn * BN;
+    t.a_row = t.m0;
+    t.b_row = t.n0;
+    t.d_row = static_cast<long>(g) * p.M + t.m0;
+    t.m_valid = min(BM, p.M - t.m0);
+    t.kb0 = s_offs[g] / BK;
+    t.kb = (s_offs[g + 1] - s_offs[g] + BK - 1) / BK;
   }
-  const long d_row0 = p.mode == kRowGroups ? 0 : static_cast<long>(g) * p.M;
+  return t;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+              const __grid_constant__ CUtensorMap tmD, const Args p) {
+  using C = Cfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* tiles = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
+  uint8_t* epi = tiles + C::kStages * C::kStageBytes;
+  uint8_t* scales = epi + C::kEpiBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScaleStages * C::kScaleBytes);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* sf_full = empty + C::kStages;
+  uint64_t* sf_empty = sf_full + kScaleStages;
+  uint64_t* acc_full = sf_empty + kScaleStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* s_total = reinterpret_cast<int*>(tmem_slot + 1);
+  int* s_offs = s_total + 1;
+  int* s_prefix = s_offs + kMaxGroups + 1;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  for (int g = threadIdx.x; g <= p.G; g += kThreads) {
+    const int lim = p.mode == kRowGroups ? p.M : p.K;
+    s_offs[g] = p.offs != nullptr ? min(max(p.offs[g], 0), lim) : (g == 0 ? 0 : lim);
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kScaleStages; ++s) {
+      mbar_init(&sf_full[s], 1);
+      mbar_init(&sf_empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 128);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 3) {
+    tmem_alloc(tmem_slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int tiles_n = (p.N + BN - 1) / BN;
+    int total = 0;
+    if (p.mode == kRowGroups) {
+      for (int g = 0; g < p.G; ++g) {
+        s_prefix[g] = total;
+        s_offs[g + 1] = max(s_offs[g + 1], s_offs[g]);
+        total += (s_offs[g + 1] - s_offs[g] + BM - 1) / BM * tiles_n * p.split;
+      }
+      s_prefix[p.G] = total;
+    } else {
+      bool ok = true;
+      for (int g = 0; g < p.G; ++g) {
+        s_offs[g + 1] = max(s_offs[g + 1], s_offs[g]);
+        // a segment that starts or ends inside a block would take its neighbour's columns along
+        ok &= s_offs[g + 1] == s_offs[g] ||
+              (s_offs[g] % BK == 0 && (s_offs[g + 1] % BK == 0 || s_offs[g + 1] == p.K));
+      }
+      total = ok ? p.G * ((p.M + BM - 1) / BM) * tiles_n : 0;
+      if (!ok) record_status(p.status, kBadShape);
+    }
+    *s_total = total;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total = *s_total;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+        const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+        for (int i = 0; i < t.kb; ++i) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.status)) { ok = false; break; }
+          uint8_t* sA = tiles + stage * C::kStageBytes;
+          mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+          tma_load_2d(sA, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
+          tma_load_2d(sA + C::kABytes, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row);
+          if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      // an early end: wait (briefly) for the loads in flight, which must not land after the CTA has gone
+      if (!ok)
+        for (int s = 0; s < C::kStages; ++s) mbar_wait(&full[s], phase ^ (s < stage ? 0 : 1), nullptr, 200000000ull);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, acc = 0, sf = 0;
+      uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+        const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, p.status)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + acc * C::kAccCols;
+        uint32_t sfa = 0;
+        for (int i = 0; i < t.kb; ++i) {
+          const uint32_t part = (t.kb0 + i) % 4;       // the byte of the scale words
+          if (i == 0 || part == 0) {
+            if (!mbar_wait(&sf_full[sf], sf_phase, p.status)) { ok = false; break; }
+            tc_fence_after();
+            // stage sf of the words has its own columns, free since sf_empty[sf] was signalled
+            sfa = tmem + C::kScaleCol0 + sf * C::kScaleCols;
+            const uint32_t src = smem_u32(scales + sf * C::kScaleBytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 16 * i;
+            for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales(sfa + 4 * q, src + 512 * q);
+          }
+          if (!mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(tiles + stage * C::kStageBytes);
+          const uint32_t idesc = p.idesc | (part << 29) | (part << 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (m >= m_end || n >= p.N) continue;
-      const long at = (d_row0 + m) * p.ldd + n;
-      if (p.f32) {
-        float* d = static_cast<float*>(p.D) + at;
-        *d = p.acc ? *d + acc[i][j] : acc[i][j];
-      } else {
-        __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.D) + at;
-        *d = __float2bfloat16(p.acc ? __bfloat162float(*d) + acc[i][j] : acc[i][j]);
+          for (int kk = 0; kk < BK / 32; ++kk)
+            umma_scaled(d, make_sw128_desc(a_addr + kk * 32, 16, 1024),
+                        make_sw128_desc(a_addr + C::kABytes + kk * 32, 16, 1024), idesc, sfa, sfa + 4,
+                        (i | kk) != 0 ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+          if (part == 3 || i == t.kb - 1) {
+            umma_commit(&sf_empty[sf]);
+            if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
+          }
+        }
+        if (!ok) break;
+        umma_commit(&acc_full[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0, p.status);
+    }
+  } else if (warp == 2) {
+    int sf = 0;
+    uint32_t sf_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+      if (t.kb == 0) continue;
+      for (int w = t.kb0 / 4; w <= (t.kb0 + t.kb - 1) / 4; ++w) {
+        const uint32_t* wa = p.sa + static_cast<long>(w) * p.rows_a;
+        const uint32_t* wb = p.sb + static_cast<long>(w) * p.rows_b;
+        uint32_t v[4 * (1 + C::kBParts)];
+#pragma unroll
+        for (int q = 0; q < 4 * (1 + C::kBParts); ++q) {
+          const int row = q < 4 ? t.a_row + q * 32 + lane : t.b_row + (q - 4) * 32 + lane;
+          v[q] = row < (q < 4 ? p.rows_a : p.rows_b) ? __ldg((q < 4 ? wa : wb) + row) : 0u;
+        }
+        if (!mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status)) { ok = false; break; }
+        uint8_t* dst = scales + sf * C::kScaleBytes + lane * 16;
+#pragma unroll
+        for (int q = 0; q < 1 + C::kBParts; ++q)
+          *reinterpret_cast<uint4*>(dst + 512 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sf_full[sf]);
+        if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
       }
     }
+  } else if (warp >= 4) {
+    const int quarter = warp - 4;
+    const int r = quarter * 32 + lane;
+    uint8_t* buf = epi + quarter * 8192;
+    int acc = 0;
+    uint32_t acc_phase = 0, slab = 0;
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+      const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+      if (!mbar_wait(&acc_full[acc], acc_phase, p.status)) break;
+      tc_fence_after();
+      const uint32_t src = tmem + acc * C::kAccCols + ((quarter * 32) << 16);
+      const int cols = min(BN, p.N - t.n0);
+      // whole tiles, and tiles cut off by the end of D, leave through TMA
+      if (p.tma_store && t.kb > 0 && (t.m_valid == BM || t.d_row + t.m_valid >= p.d_rows)) {
+        const int step = p.f32 ? 32 : 64;             // columns of 128 bytes
+        const int n = (cols + step - 1) / step;
+#pragma unroll 1
+        for (int s = 0; s < n; ++s) {
+          uint32_t v[64];
+          tmem_ld_32x32b_x32(src + s * step, v);
+          if (!p.f32) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
+          tmem_wait_ld();
+          if (s == n - 1) {
+            tc_fence_before();
+            mbar_arrive(&acc_empty[acc]);
+          }
+          uint8_t* b = buf + (slab & 1) * 4096;
+          ++slab;
+          if (lane == 0) bulk_wait_group_read<1>();
+          __syncwarp();
+          if (p.f32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(b + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<bf16x8*>(b + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+                  float_to_bf16x8(reinterpret_cast<const float*>(v) + 8 * j);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmD, b, t.n0 + s * step, static_cast<int>(t.d_row) + quarter * 32);
+            bulk_commit_group();
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(src + c, v);
+          tmem_wait_ld();
+          const long at = (t.d_row + r) * p.ldd + t.n0 + c;
+          const int here = r < t.m_valid ? min(32, cols - c) : 0;
+          if (p.f32) {
+            float* d = static_cast<float*>(p.D) + at;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < here) {
+                const float f = t.kb > 0 ? __uint_as_float(v[i]) : 0.f;
+                d[i] = p.acc ? d[i] + f : f;
+              }
+          } else {
+            __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.D) + at;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < here) {
+                const float f = t.kb > 0 ? __uint_as_float(v[i]) : 0.f;
+                d[i] = __float2bfloat16(p.acc ? __bfloat162float(d[i]) + f : f);
+              }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&acc_empty[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
   }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 3) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+// Sum of the partial products of a split contraction, in the order of the
+// ranges, into D with the requested type and accumulation.
+__global__ void split_sum_kernel(const float* __restrict__ ws, int S, int M, int N, bool f32, bool acc, void* D,
+                                 long ldd) {
+  const long MN = static_cast<long>(M) * N;
+  for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < MN;
+       i += static_cast<long>(gridDim.x) * blockDim.x) {
+    float v = ws[i];
+    for (int s = 1; s < S; ++s) v += ws[s * MN + i];
+    const long m = i / N, at = m * ldd + (i - m * N);
+    if (f32) {
+      float* d = static_cast<float*>(D) + at;
+      *d = acc ? *d + v : v;
+    } else {
+      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(D) + at;
+      *d = __float2bfloat16(acc ? __bfloat162float(*d) + v : v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q);
+    TORCH_CHECK(e == cudaSuccess && q == cudaDriverEntryPointSuccess && ptr != nullptr,
+                "shift_b200: cannot resolve cuTensorMapEncodeTiled");
+    fn = reinterpret_cast<EncodeFn>(ptr);
+  });
+  return fn;
+}
+
+// Row-major [rows, cols] with row stride `bytes`, boxes of 128 bytes x box_rows, 128-byte swizzle.
+static CUtensorMap make_map(CUtensorMapDataType type, int elem, const void* base, long rows, long cols, long bytes,
+                            int box_rows) {
+  CUtensorMap m;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(bytes)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode_fn()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
+  return m;
+}
+
+static int num_sms(int device) {
+  static int n[64] = {};
+  int& v = n[device & 63];
+  if (v == 0) cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device);
+  return v;
+}
+
+template <int BN>
+static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Args& p, long tiles,
+                   int device, cudaStream_t st) {
+  auto kern = matmul_kernel<BN>;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::kSmemBytes));
+  const int grid = static_cast<int>(std::min<long>(num_sms(device), std::max<long>(1, tiles)));
+  kern<<<grid, kThreads, Cfg<BN>::kSmemBytes, st>>>(ta, tb, td, p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 // a, b: codes [rows, ld] with scales [words, rows, 4]; D [rows, N] (row mode)
@@ -106,32 +491,83 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
             const c10::optional<at::Tensor>& offs, int64_t M, int64_t N, int64_t K, int64_t G, int64_t mode,
             bool accumulate, const at::Tensor& status) {
   const at::cuda::CUDAGuard guard(a.device());
-  if (M == 0 || N == 0 || G == 0) return;
+  TORCH_CHECK(M < (1l << 31) - 256 && N < (1l << 31) - 256 && K < (1l << 31) - 256 && G * M < (1l << 31) - 256 &&
+                  b.size(0) < (1l << 31) - 256,
+              "fp8 matmul: a side is too long");
+  TORCH_CHECK(G >= 1 && G <= kMaxGroups, "fp8 matmul: 1 to ", kMaxGroups, " groups");
+  if (M == 0 || N == 0) return;
+  if (K == 0) {
+    if (!accumulate && !offs.has_value()) D.zero_();
+    else if (!accumulate && mode == kKGroups) D.zero_();
+    else TORCH_CHECK(accumulate, "fp8 matmul: nothing to contract");
+    return;
+  }
+  for (const auto* t : {&a, &b})
+    TORCH_CHECK(t->stride(1) == 1 && aligned16(t->data_ptr()) && (t->size(0) == 1 || t->stride(0) % 16 == 0),
+                "fp8 matmul: codes start on 16 bytes, rows a multiple of 16 bytes apart");
+  const auto st = at::cuda::getCurrentCUDAStream();
+  const int sms = num_sms(a.device().index());
   Args p;
-  p.a = static_cast<const uint8_t*>(a.data_ptr());
-  p.b = static_cast<const uint8_t*>(b.data_ptr());
-  p.sa = static_cast<const uint8_t*>(sa.data_ptr());
-  p.sb = static_cast<const uint8_t*>(sb.data_ptr());
-  p.lda = a.stride(0);
-  p.ldb = b.stride(0);
-  p.rows_a = a.size(0);
-  p.rows_b = b.size(0);
+  p.sa = static_cast<const uint32_t*>(sa.data_ptr());
+  p.sb = static_cast<const uint32_t*>(sb.data_ptr());
+  p.rows_a = static_cast<int>(a.size(0));
+  p.rows_b = static_cast<int>(b.size(0));
   p.M = static_cast<int>(M);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.G = static_cast<int>(G);
   p.mode = static_cast<int>(mode);
   p.offs = offs.has_value() ? offs->data_ptr<int>() : nullptr;
-  p.D = D.data_ptr();
-  p.ldd = D.stride(0);
-  p.f32 = D.scalar_type() == at::kFloat;
-  p.acc = accumulate;
-  p.a_e5m2 = a.scalar_type() == at::kFloat8_e5m2;
-  p.b_e5m2 = b.scalar_type() == at::kFloat8_e5m2;
   p.status = status.data_ptr<int>();
-  const dim3 grid(static_cast<unsigned>(((M + 63) / 64) * ((N + 63) / 64)), static_cast<unsigned>(G));
-  matmul_kernel<<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+
+  const long tiles_m = (M + BM - 1) / BM, blocks = (K + BK - 1) / BK;
+  const int bn = N % 192 != 0 && (N % 128 == 0 || N <= 128) ? 128 : 192;
+  const long tn = (N + bn - 1) / bn;
+  long tiles = mode == kRowGroups ? (tiles_m + (p.offs != nullptr ? G : 0)) * tn : G * tiles_m * tn;
+  p.split = 1;
+  if (p.offs == nullptr && tiles * 2 <= sms && blocks >= 8)
+    p.split = static_cast<int>(std::min<long>(sms / tiles, blocks / 4));
+
+  at::Tensor ws;
+  const bool f32 = D.scalar_type() == at::kFloat;
+  p.f32 = f32;
+  p.acc = accumulate;
+  p.D = D.data_ptr();
+  p.ldd = D.size(0) > 1 ? D.stride(0) : N;
+  long d_rows = D.size(0);
+  if (p.split > 1) {
+    ws = at::empty({p.split * M, N}, a.options().dtype(at::kFloat));
+    tiles *= p.split;
+    p.f32 = true;
+    p.acc = false;
+    p.D = ws.data_ptr();
+    p.ldd = N;
+    d_rows = p.split * M;
+  }
+  p.d_rows = static_cast<int>(d_rows);
+  const int es = p.f32 ? 4 : 2;
+  p.tma_store = !p.acc && aligned16(p.D) && (p.ldd * es) % 16 == 0;
+  // fp32 accumulator, both operands K-major, UE8M0 scales; the byte of the scale words is added per block
+  p.idesc = (static_cast<uint32_t>(a.scalar_type() == at::kFloat8_e5m2) << 7) |
+            (static_cast<uint32_t>(b.scalar_type() == at::kFloat8_e5m2) << 10) |
+            (static_cast<uint32_t>(bn >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(BM >> 4) << 24);
+
+  const long lda = a.size(0) > 1 ? a.stride(0) : (K + 15) / 16 * 16, ldb = b.size(0) > 1 ? b.stride(0) : (K + 15) / 16 * 16;
+  const CUtensorMap ta = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.data_ptr(), a.size(0), K, lda, BM);
+  const CUtensorMap tb = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.data_ptr(), b.size(0), K, ldb, bn);
+  CUtensorMap td;
+  std::memset(&td, 0, sizeof(td));
+  if (p.tma_store)
+    td = make_map(p.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, p.D, d_rows, N,
+                  p.ldd * es, 32);
+  if (bn == 192) launch<192>(ta, tb, td, p, tiles, a.device().index(), st);
+  else launch<128>(ta, tb, td, p, tiles, a.device().index(), st);
+  if (p.split > 1) {
+    const long MN = M * N;
+    split_sum_kernel<<<static_cast<unsigned>(std::min<long>((MN + 255) / 256, 148 * 8)), 256, 0, st>>>(
+        ws.data_ptr<float>(), p.split, p.M, p.N, f32, accumulate, D.data_ptr(), D.size(0) > 1 ? D.stride(0) : N);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
 }
 
 }  // namespace fp8

@@ -172,11 +172,13 @@ def grouped_wgrad(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tenso
     """out[g] (+)= a[:, seg g] @ b[:, seg g]^T with seg g = [offs[g], offs[g + 1]).
 
     For expert weight gradients: ``a`` of dy^T [N, rows], ``b`` of x^T
-    [K, rows], ``out`` [G, N, K].  Segments start on a multiple of 128, so
-    that no block of 128 is shared by two of them; the columns between a
-    segment's last row and the next start belong to the segment and have to
-    be zero (``ops.functional.gather_rows`` leaves them so).  An empty
-    segment gives zeros (or leaves ``out[g]`` with ``accumulate``)."""
+    [K, rows], ``out`` [G, N, K].  Segments start and end on a multiple of 128
+    (the last may end with the matrix), so that no block of 128 is shared by
+    two of them: rows that pad a segment belong to it and have to be zero
+    (``ops.functional.gather_rows`` leaves them so).  Other segments are
+    refused, on the GPU through the status word (``ops._ext.check_status``)
+    with ``out`` left as it was.  An empty segment gives zeros (or leaves
+    ``out[g]`` with ``accumulate``)."""
     _check_pair(a, b, "grouped_wgrad")
     _check_offs(offs, a, "grouped_wgrad")
     G, M, N, K = offs.numel() - 1, a.rows, b.rows, a.cols
@@ -186,8 +188,10 @@ def grouped_wgrad(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tenso
         _run(a, b, out.view(G * M, N), offs, M, N, K, G, 1, accumulate)
         return out
     x, y = ref.fp8_values(a.data, a.scale, K), ref.fp8_values(b.data, b.scale, K)
-    for g, (lo, hi) in enumerate(ref.segments(offs, K)):
-        _fail(lo % BLOCK == 0 or hi == lo, f"grouped_wgrad: segment {g} starts at {lo}, not on a multiple of {BLOCK}")
+    segs = ref.segments(offs, K)
+    _fail(all(hi == lo or (lo % BLOCK == 0 and (hi % BLOCK == 0 or hi == K)) for lo, hi in segs),
+          f"grouped_wgrad: segments {segs} cut a block of {BLOCK}")
+    for g, (lo, hi) in enumerate(segs):
         d = x[:, lo:hi] @ y[:, lo:hi].t()
         out[g] = (out[g].float() + d if accumulate else d).to(out.dtype)
     return out

@@ -228,14 +228,26 @@ def test_grouped_wgrad(M, N, dtype, acc):
         orc.check_product(out[g], va[:, o[g]:o[g + 1]], vb[:, o[g]:o[g + 1]], base=base[g] if acc else None)
 
 
-def test_segments_off_a_block_are_refused_by_the_status_word():
+@pytest.mark.parametrize("offs", [[0, 100, 512], [0, 128, 500]])
+def test_segments_off_a_block_are_refused_by_the_status_word(offs):
     a, b = _pair(40, 50, 512)
-    out = torch.zeros(2, 40, 50, device=DEV)
-    fp8.grouped_wgrad(a, b, torch.tensor([0, 100, 512], dtype=torch.int32, device=DEV), out)
+    out = torch.full((2, 40, 50), 3.0, device=DEV)
+    fp8.grouped_wgrad(a, b, torch.tensor(offs, dtype=torch.int32, device=DEV), out)
     torch.cuda.synchronize()
     with pytest.raises(RuntimeError, match="status"):
         check_status()
     check_status()
+    assert bool((out == 3).all())
+
+
+def test_a_last_segment_that_ends_with_the_matrix():
+    a, b = _pair(40, 50, 500)
+    out = torch.zeros(2, 40, 50, device=DEV)
+    fp8.grouped_wgrad(a, b, torch.tensor([0, 128, 500], dtype=torch.int32, device=DEV), out)
+    _done()
+    va, vb = orc.values(a), orc.values(b)
+    orc.check_product(out[0], va[:, :128], vb[:, :128])
+    orc.check_product(out[1], va[:, 128:], vb[:, 128:])
 
 
 def test_segments_outside_the_rows_are_cut():
