@@ -15,6 +15,11 @@
 // are contiguous, and tcgen05.cp spreads them over tensor memory in the order
 // the instruction wants (row r in lane r % 32, column r / 32).
 //
+// Two CTAs on neighbouring SMs work on one tile of 256 rows (cta_group::2): each
+// loads half of A's and half of B's rows, so an operand byte feeds twice as
+// many products as in a CTA of its own; the first one issues the instructions
+// for both.  Rows that fit one CTA's 128 take the single form.
+//
 // Warp roles (256 threads):
 //   warp 0      TMA loads of the operand tiles (one lane)
 //   warp 1      MMA issue (one lane)
@@ -41,25 +46,33 @@ constexpr int kThreads = 256;
 constexpr int BM = 128;
 constexpr int BK = 128;            // one scale block, one 128-byte swizzled row
 constexpr int kMaxGroups = 512;
-constexpr int kScaleStages = 4;
+constexpr int kBand = 8;           // row tiles whose column tiles are walked together
 
-template <int BN>
+// CTAS: CTAs that share a tile of 128 * CTAS rows and BN columns.  Two
+// accumulators alternate so that the epilogue of one tile runs under the next
+// one's products.  256 columns twice would leave no room for the scales, so
+// there the two share 32 columns, which the epilogue reads first.
+template <int BN, int CTAS>
 struct Cfg {
+  static constexpr int kTileM = BM * CTAS;
   static constexpr int kABytes = BM * BK;
-  static constexpr int kBBytes = BN * BK;
+  static constexpr int kBRows = BN / CTAS;                       // rows of B that one CTA loads
+  static constexpr int kBBytes = kBRows * BK;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = BN == 192 ? 4 : (BN == 128 ? 5 : 7);
+  static constexpr int kEpiBytes = 4 * 2 * 4096;                 // per warp two buffers of 32 rows x 128 bytes
   static constexpr int kBParts = (BN + 127) / 128;               // 128-row parts of the B scales
   static constexpr int kScaleBytes = 512 * (1 + kBParts);
-  static constexpr int kEpiBytes = 4 * 2 * 4096;                 // per warp two buffers of 32 rows x 128 bytes
-  static constexpr int kAccCols = BN <= 64 ? 64 : BN;
+  static constexpr bool kShared = BN == 256;
+  static constexpr int kAccCols = kShared ? 224 : BN;
+  static constexpr int kScaleStages = kShared ? 2 : 4;
   static constexpr int kScaleCols = 4 * (1 + kBParts);
   static constexpr int kTmemCols = 512;
-  static constexpr int kScaleCol0 = 2 * kAccCols;
+  static constexpr int kScaleCol0 = kAccCols + BN;
   static_assert(kScaleCol0 + kScaleStages * kScaleCols <= kTmemCols, "tensor memory budget");
-  static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 +
-                                    2 * (kMaxGroups + 1) * 4;
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static constexpr int kFixed = kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 + 2 * (kMaxGroups + 1) * 4;
+  static constexpr int kStages = (232448 - kFixed) / kStageBytes < 8 ? (232448 - kFixed) / kStageBytes : 8;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kFixed;
+  static_assert(kStages >= 3 && kStageBytes % 1024 == 0, "shared memory budget");
 };
 
 struct Args {
@@ -77,36 +90,164 @@ struct Args {
 };
 
 struct Tile {
-  int m0, n0;              // first row of A / column of D within the operand
+  int n0;                  // first column of D
   int a_row, b_row;        // rows of the operands
   long d_row;              // first output row
-  int m_valid;
+  int m_valid;             // rows of this CTA that are wanted (none: 0 or less)
   int kb0, kb;             // first block of 128, number of blocks
 };
 
 // D[tmem] (+)= A[smem] B[smem]^T with the scales in tensor memory.
+template <int CTAS>
 SB_DEVICE void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
-// 32 rows of 16 bytes to 32 lanes x 4 columns, repeated in the four lane quarters.
+// 32 rows of 16 bytes to 32 lanes x 4 columns, repeated in the four lane
+// quarters; in both CTAs of a pair, each from its own shared memory.
+template <int CTAS>
 SB_DEVICE void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
   d |= static_cast<uint64_t>(128 >> 4) << 32;      // eight rows of 16 bytes apart
   d |= 1ull << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+// Arrive on this barrier (of both CTAs of a pair) when the products issued so far are done.
+template <int CTAS>
+SB_DEVICE void commit(uint64_t* bar) {
+  if constexpr (CTAS == 1) {
+    umma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  }
+}
+// The same on this CTA's barrier alone.
+template <int CTAS>
+SB_DEVICE void commit_here(uint64_t* bar) {
+  if constexpr (CTAS == 1) umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// The first CTA's barrier at the same place, as a cluster address.
+SB_DEVICE uint32_t leader_addr(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+template <int CTAS>
+SB_DEVICE void arrive_leader(uint64_t* bar) {
+  if constexpr (CTAS == 1) {
+    mbar_arrive(bar);
+  } else {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+  }
+}
+// Wait (bounded) for a barrier that the other CTA's threads arrive on too.
+template <int CTAS>
+SB_DEVICE bool wait_both(uint64_t* bar, uint32_t phase, int* status) {
+  if constexpr (CTAS == 1) {
+    return mbar_wait(bar, phase, status);
+  } else {
+    uint64_t start = 0;
+    while (true) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000000;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(smem_u32(bar)), "r"(phase)
+          : "memory");
+      if (ok) return true;
+      const uint64_t now = globaltimer_ns();
+      if (start == 0) start = now;
+      if (now - start > kPipelineTimeoutNs) {
+        record_status(status, kTimeoutPipeline);
+        return false;
+      }
+    }
+  }
+}
+// A tile of this GPU's memory into this CTA's shared memory; completes on the first CTA's barrier.
+template <int CTAS>
+SB_DEVICE void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  if constexpr (CTAS == 1) {
+    tma_load_2d(dst, map, bar, x, y);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_addr(bar)), "r"(x), "r"(y)
+        : "memory");
+  }
+}
+template <int CTAS>
+SB_DEVICE void tmem_take(uint32_t* slot, uint32_t cols) {
+  if constexpr (CTAS == 1) {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CTAS>
+SB_DEVICE void tmem_give(uint32_t taddr, uint32_t cols) {
+  if constexpr (CTAS == 1) tmem_dealloc(taddr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+template <int CTAS>
+SB_DEVICE void sync_pair() {
+  if constexpr (CTAS == 1) {
+    __syncthreads();
+  } else {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
 }
 
-template <int BN>
-__device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile) {
+// Row and column tile of number `local` among tiles_m x tiles_n: bands of
+// kBand row tiles, rows first, so that the tiles in flight at one time share
+// few rows of both operands.
+SB_DEVICE void walk(int local, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int band = local / (kBand * tiles_n);
+  const int height = min(kBand, tiles_m - band * kBand);
+  const int in = local - band * kBand * tiles_n;
+  tn = in / height;
+  tm = band * kBand + in - tn * height;
+}
+
+// `rank`: the CTA's place in its pair.
+template <int BN, int CTAS>
+__device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile, int rank) {
+  using C = Cfg<BN, CTAS>;
   const int tiles_n = (p.N + BN - 1) / BN;
   Tile t;
+  int tm, tn;
   if (p.mode == kRowGroups) {
     int lo = 0, hi = p.G - 1;                      // last group whose first tile is at most `tile`
     while (lo < hi) {
@@ -116,43 +257,45 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
     }
     int local = tile - s_prefix[lo];
     const int blocks = (p.K + BK - 1) / BK;
+    const int rows = s_offs[lo + 1] - s_offs[lo], tiles_m = (rows + C::kTileM - 1) / C::kTileM;
     int s = 0;
     if (p.split > 1) {
-      const int per = (p.M + BM - 1) / BM * tiles_n;
+      const int per = tiles_m * tiles_n;
       s = local / per;
       local -= s * per;
     }
-    const int tm = local / tiles_n, tn = local % tiles_n;
-    t.m0 = s_offs[lo] + tm * BM;
+    walk(local, tiles_m, tiles_n, tm, tn);
+    const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
-    t.a_row = t.m0;
+    t.a_row = s_offs[lo] + m;
     t.b_row = lo * p.N + t.n0;
-    t.d_row = t.m0 + static_cast<long>(s) * p.M;
-    t.m_valid = min(BM, s_offs[lo + 1] - t.m0);
+    t.d_row = t.a_row + static_cast<long>(s) * p.M;
+    t.m_valid = min(BM, rows - m);
     t.kb0 = static_cast<int>(static_cast<long>(blocks) * s / p.split);
     t.kb = static_cast<int>(static_cast<long>(blocks) * (s + 1) / p.split) - t.kb0;
   } else {
-    const int tiles_m = (p.M + BM - 1) / BM;
+    const int tiles_m = (p.M + C::kTileM - 1) / C::kTileM;
     const int per = tiles_m * tiles_n;
-    const int g = tile / per, local = tile % per;
-    const int tm = local / tiles_n, tn = local % tiles_n;
-    t.m0 = tm * BM;
+    const int g = tile / per;
+    walk(tile % per, tiles_m, tiles_n, tm, tn);
+    const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
-    t.a_row = t.m0;
+    t.a_row = m;
     t.b_row = t.n0;
-    t.d_row = static_cast<long>(g) * p.M + t.m0;
-    t.m_valid = min(BM, p.M - t.m0);
+    t.d_row = static_cast<long>(g) * p.M + m;
+    t.m_valid = min(BM, p.M - m);
     t.kb0 = s_offs[g] / BK;
     t.kb = (s_offs[g + 1] - s_offs[g] + BK - 1) / BK;
   }
   return t;
 }
 
-template <int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int BN, int CTAS>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(CTAS, 1, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const __grid_constant__ CUtensorMap tmD, const Args p) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, CTAS>;
+  constexpr int kScaleStages = C::kScaleStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* tiles = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
@@ -171,6 +314,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   int* s_prefix = s_offs + kMaxGroups + 1;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = CTAS == 1 ? 0 : blockIdx.x % CTAS;
+  const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
 
   for (int g = threadIdx.x; g <= p.G; g += kThreads) {
     const int lim = p.mode == kRowGroups ? p.M : p.K;
@@ -182,22 +327,19 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kScaleStages; ++s) {
-      mbar_init(&sf_full[s], 1);
+      mbar_init(&sf_full[s], CTAS);
       mbar_init(&sf_empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 128);
+      mbar_init(&acc_empty[a], 4 * CTAS);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
-  if (warp == 3) {
-    tmem_alloc(tmem_slot, C::kTmemCols);
-    tmem_relinquish();
-  }
+  if (warp == 3) tmem_take<CTAS>(tmem_slot, C::kTmemCols);
   __syncthreads();
   if (threadIdx.x == 0) {
     const int tiles_n = (p.N + BN - 1) / BN;
@@ -206,7 +348,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       for (int g = 0; g < p.G; ++g) {
         s_prefix[g] = total;
         s_offs[g + 1] = max(s_offs[g + 1], s_offs[g]);
-        total += (s_offs[g + 1] - s_offs[g] + BM - 1) / BM * tiles_n * p.split;
+        total += (s_offs[g + 1] - s_offs[g] + C::kTileM - 1) / C::kTileM * tiles_n * p.split;
       }
       s_prefix[p.G] = total;
     } else {
@@ -217,13 +359,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         ok &= s_offs[g + 1] == s_offs[g] ||
               (s_offs[g] % BK == 0 && (s_offs[g + 1] % BK == 0 || s_offs[g + 1] == p.K));
       }
-      total = ok ? p.G * ((p.M + BM - 1) / BM) * tiles_n : 0;
-      if (!ok) record_status(p.status, kBadShape);
+      total = ok ? p.G * ((p.M + C::kTileM - 1) / C::kTileM) * tiles_n : 0;
+      if (!ok && blockIdx.x == 0) record_status(p.status, kBadShape);
     }
     *s_total = total;
   }
   tc_fence_before();
-  __syncthreads();
+  sync_pair<CTAS>();          // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total = *s_total;
@@ -233,42 +375,58 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
         for (int i = 0; i < t.kb; ++i) {
           if (!mbar_wait(&empty[stage], phase ^ 1, p.status)) { ok = false; break; }
           uint8_t* sA = tiles + stage * C::kStageBytes;
-          mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
-          tma_load_2d(sA, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
-          tma_load_2d(sA + C::kABytes, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], C::kStageBytes * CTAS);
+          load_tile<CTAS>(sA, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
+          load_tile<CTAS>(sA + C::kABytes, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row + rank * C::kBRows);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
         }
       }
+      // every stage's products have signalled here before this CTA may go: the other one's signals are remote
+      for (int s = 0; s < C::kStages && ok; ++s) {
+        ok = mbar_wait(&empty[stage], phase ^ 1, p.status);
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+      }
       // an early end: wait (briefly) for the loads in flight, which must not land after the CTA has gone
-      if (!ok)
+      // (the second CTA's complete on the first one's barriers; the pair leaves together)
+      if (!ok && rank == 0)
         for (int s = 0; s < C::kStages; ++s) mbar_wait(&full[s], phase ^ (s < stage ? 0 : 1), nullptr, 200000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int stage = 0, acc = 0, sf = 0;
       uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
-        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, p.status)) { ok = false; break; }
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+        // its accumulator has been read; one that shares columns with the other also waits until the tile before
+        // has read those, which it does first, and the epilogue takes tiles in order
+        if (C::kShared) {
+          if (tile != first_tile && !wait_both<CTAS>(&acc_empty[acc ^ 1], acc == 0 ? acc_phase ^ 1 : acc_phase, p.status)) {
+            ok = false;
+            break;
+          }
+        } else if (!wait_both<CTAS>(&acc_empty[acc], acc_phase ^ 1, p.status)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         const uint32_t d = tmem + acc * C::kAccCols;
         uint32_t sfa = 0;
         for (int i = 0; i < t.kb; ++i) {
           const uint32_t part = (t.kb0 + i) % 4;       // the byte of the scale words
           if (i == 0 || part == 0) {
-            if (!mbar_wait(&sf_full[sf], sf_phase, p.status)) { ok = false; break; }
+            if (!wait_both<CTAS>(&sf_full[sf], sf_phase, p.status)) { ok = false; break; }
             tc_fence_after();
             // stage sf of the words has its own columns, free since sf_empty[sf] was signalled
             sfa = tmem + C::kScaleCol0 + sf * C::kScaleCols;
             const uint32_t src = smem_u32(scales + sf * C::kScaleBytes);
 #pragma unroll
-            for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales(sfa + 4 * q, src + 512 * q);
+            for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales<CTAS>(sfa + 4 * q, src + 512 * q);
           }
           if (!mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
           tc_fence_after();
@@ -276,30 +434,31 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           const uint32_t idesc = p.idesc | (part << 29) | (part << 4);
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
-            umma_scaled(d, make_sw128_desc(a_addr + kk * 32, 16, 1024),
+            umma_scaled<CTAS>(d, make_sw128_desc(a_addr + kk * 32, 16, 1024),
                         make_sw128_desc(a_addr + C::kABytes + kk * 32, 16, 1024), idesc, sfa, sfa + 4,
                         (i | kk) != 0 ? 1u : 0u);
-          umma_commit(&empty[stage]);
+          commit<CTAS>(&empty[stage]);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
           if (part == 3 || i == t.kb - 1) {
-            umma_commit(&sf_empty[sf]);
+            commit<CTAS>(&sf_empty[sf]);
             if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
           }
         }
         if (!ok) break;
-        umma_commit(&acc_full[acc]);
+        commit<CTAS>(&acc_full[acc]);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      umma_commit(drain);
+      // whatever was issued is done before tensor memory is given back, after an early end too
+      commit_here<CTAS>(drain);
       mbar_wait(drain, 0, p.status);
     }
   } else if (warp == 2) {
     int sf = 0;
     uint32_t sf_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-      const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+    for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+      const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
       if (t.kb == 0) continue;
       for (int w = t.kb0 / 4; w <= (t.kb0 + t.kb - 1) / 4; ++w) {
         const uint32_t* wa = p.sa + static_cast<long>(w) * p.rows_a;
@@ -317,9 +476,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           *reinterpret_cast<uint4*>(dst + 512 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sf_full[sf]);
+        if (lane == 0) arrive_leader<CTAS>(&sf_full[sf]);
         if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
       }
+    }
+    for (int s = 0; s < kScaleStages && ok; ++s) {
+      ok = mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status);
+      if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
     }
   } else if (warp >= 4) {
     const int quarter = warp - 4;
@@ -327,8 +490,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     uint8_t* buf = epi + quarter * 8192;
     int acc = 0;
     uint32_t acc_phase = 0, slab = 0;
-    for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-      const Tile t = decode_tile<BN>(p, s_prefix, s_offs, tile);
+    for (int tile = first_tile; tile < total; tile += tile_step) {
+      const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
       if (!mbar_wait(&acc_full[acc], acc_phase, p.status)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * C::kAccCols + ((quarter * 32) << 16);
@@ -338,14 +501,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         const int step = p.f32 ? 32 : 64;             // columns of 128 bytes
         const int n = (cols + step - 1) / step;
 #pragma unroll 1
-        for (int s = 0; s < n; ++s) {
+        for (int i = 0; i < n; ++i) {
+          // shared columns first: the last of the first accumulator, the first of the second
+          const int s = C::kShared && acc == 0 ? n - 1 - i : i;
           uint32_t v[64];
           tmem_ld_32x32b_x32(src + s * step, v);
           if (!p.f32) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
           tmem_wait_ld();
-          if (s == n - 1) {
+          if (i == (C::kShared ? 0 : n - 1)) {
             tc_fence_before();
-            mbar_arrive(&acc_empty[acc]);
+            __syncwarp();
+            if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
           }
           uint8_t* b = buf + (slab & 1) * 4096;
           ++slab;
@@ -371,11 +537,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int q = 0; q < BN / 32; ++q) {
+          const int c = 32 * (C::kShared && acc == 0 ? BN / 32 - 1 - q : q);
           uint32_t v[32];
           __syncwarp();
           tmem_ld_32x32b_x32(src + c, v);
           tmem_wait_ld();
+          if (q == (C::kShared ? 0 : BN / 32 - 1)) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
+          }
           const long at = (t.d_row + r) * p.ldd + t.n0 + c;
           const int here = r < t.m_valid ? min(32, cols - c) : 0;
           if (p.f32) {
@@ -396,8 +568,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
               }
           }
         }
-        tc_fence_before();
-        mbar_arrive(&acc_empty[acc]);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
@@ -407,9 +577,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   }
 
   tc_fence_before();
-  __syncthreads();
+  sync_pair<CTAS>();
   tc_fence_after();
-  if (warp == 3) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == 3) tmem_give<CTAS>(tmem, C::kTmemCols);
 }
 
 // Sum of the partial products of a split contraction, in the order of the
@@ -475,14 +645,39 @@ static int num_sms(int device) {
   return v;
 }
 
-template <int BN>
+template <int BN, int CTAS>
 static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Args& p, long tiles,
                    int device, cudaStream_t st) {
-  auto kern = matmul_kernel<BN>;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::kSmemBytes));
-  const int grid = static_cast<int>(std::min<long>(num_sms(device), std::max<long>(1, tiles)));
-  kern<<<grid, kThreads, Cfg<BN>::kSmemBytes, st>>>(ta, tb, td, p);
+  using C = Cfg<BN, CTAS>;
+  auto kern = matmul_kernel<BN, CTAS>;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+  const int grid = static_cast<int>(std::min<long>(num_sms(device) / CTAS, std::max<long>(1, tiles))) * CTAS;
+  kern<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, td, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+struct Plan {
+  int ctas, bn, split;
+  long tiles;            // upper bound for the grid
+};
+
+static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, int sms) {
+  Plan p;
+  const long blocks = (K + BK - 1) / BK;
+  p.ctas = M > BM ? 2 : 1;
+  if (const char* e = getenv("SB_FP8_CTAS")) p.ctas = atoi(e);
+  p.bn = N % 192 != 0 && (N % 128 == 0 || N <= 128) ? 128 : 192;
+  if (p.ctas == 2 && N % 256 == 0) p.bn = 256;
+  if (const char* e = getenv("SB_FP8_BN")) p.bn = atoi(e);
+  const long tm = (M + BM * p.ctas - 1) / (BM * p.ctas), tn = (N + p.bn - 1) / p.bn;
+  p.tiles = mode == kRowGroups ? (tm + (offs ? G : 0)) * tn : G * tm * tn;
+  p.split = 1;
+  const long slots = sms / p.ctas;
+  if (!offs && p.tiles * 2 <= slots && blocks >= 8) {
+    p.split = static_cast<int>(std::min<long>(slots / p.tiles, blocks / 4));
+    p.tiles *= p.split;
+  }
+  return p;
 }
 
 // a, b: codes [rows, ld] with scales [words, rows, 4]; D [rows, N] (row mode)
@@ -520,13 +715,10 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   p.offs = offs.has_value() ? offs->data_ptr<int>() : nullptr;
   p.status = status.data_ptr<int>();
 
-  const long tiles_m = (M + BM - 1) / BM, blocks = (K + BK - 1) / BK;
-  const int bn = N % 192 != 0 && (N % 128 == 0 || N <= 128) ? 128 : 192;
-  const long tn = (N + bn - 1) / bn;
-  long tiles = mode == kRowGroups ? (tiles_m + (p.offs != nullptr ? G : 0)) * tn : G * tiles_m * tn;
-  p.split = 1;
-  if (p.offs == nullptr && tiles * 2 <= sms && blocks >= 8)
-    p.split = static_cast<int>(std::min<long>(sms / tiles, blocks / 4));
+  const Plan plan = make_plan(M, N, K, G, mode, p.offs != nullptr, sms);
+  const int bn = plan.bn;
+  const long tiles = plan.tiles;
+  p.split = plan.split;
 
   at::Tensor ws;
   const bool f32 = D.scalar_type() == at::kFloat;
@@ -537,7 +729,6 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   long d_rows = D.size(0);
   if (p.split > 1) {
     ws = at::empty({p.split * M, N}, a.options().dtype(at::kFloat));
-    tiles *= p.split;
     p.f32 = true;
     p.acc = false;
     p.D = ws.data_ptr();
@@ -550,18 +741,25 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   // fp32 accumulator, both operands K-major, UE8M0 scales; the byte of the scale words is added per block
   p.idesc = (static_cast<uint32_t>(a.scalar_type() == at::kFloat8_e5m2) << 7) |
             (static_cast<uint32_t>(b.scalar_type() == at::kFloat8_e5m2) << 10) |
-            (static_cast<uint32_t>(bn >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(BM >> 4) << 24);
+            (static_cast<uint32_t>(bn >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>((BM * plan.ctas) >> 4) << 24);
 
   const long lda = a.size(0) > 1 ? a.stride(0) : (K + 15) / 16 * 16, ldb = b.size(0) > 1 ? b.stride(0) : (K + 15) / 16 * 16;
   const CUtensorMap ta = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.data_ptr(), a.size(0), K, lda, BM);
-  const CUtensorMap tb = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.data_ptr(), b.size(0), K, ldb, bn);
+  const CUtensorMap tb = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.data_ptr(), b.size(0), K, ldb, bn / plan.ctas);
   CUtensorMap td;
   std::memset(&td, 0, sizeof(td));
   if (p.tma_store)
     td = make_map(p.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, p.D, d_rows, N,
                   p.ldd * es, 32);
-  if (bn == 192) launch<192>(ta, tb, td, p, tiles, a.device().index(), st);
-  else launch<128>(ta, tb, td, p, tiles, a.device().index(), st);
+  const int dev = a.device().index();
+  if (plan.ctas == 2) {
+    if (bn == 256) launch<256, 2>(ta, tb, td, p, tiles, dev, st);
+    else if (bn == 192) launch<192, 2>(ta, tb, td, p, tiles, dev, st);
+    else launch<128, 2>(ta, tb, td, p, tiles, dev, st);
+  } else {
+    if (bn == 192) launch<192, 1>(ta, tb, td, p, tiles, dev, st);
+    else launch<128, 1>(ta, tb, td, p, tiles, dev, st);
+  }
   if (p.split > 1) {
     const long MN = M * N;
     split_sum_kernel<<<static_cast<unsigned>(std::min<long>((MN + 255) / 256, 148 * 8)), 256, 0, st>>>(
