@@ -97,6 +97,16 @@ struct Tile {
   int kb0, kb;             // first block of 128, number of blocks
 };
 
+// True in one lane of a converged warp.  A role that only issues instructions
+// for the tensor cores or TMA runs under this: the compiler then knows that one
+// lane runs it and keeps descriptors and barriers in uniform registers, where
+// those instructions take them from (under `lane == 0` the four products of a
+// block took 290 clocks to issue, more than they take to run).
+SB_DEVICE bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 // D[tmem] (+)= A[smem] B[smem]^T with the scales in tensor memory.
 template <int CTAS>
 SB_DEVICE void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -371,7 +381,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   const int total = *s_total;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -397,7 +407,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         for (int s = 0; s < C::kStages; ++s) mbar_wait(&full[s], phase ^ (s < stage ? 0 : 1), nullptr, 200000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && elect_one()) {
+      const uint64_t desc0 = make_sw128_desc(smem_u32(tiles), 16, 1024);
       int stage = 0, acc = 0, sf = 0;
       uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
       bool ok = true;
@@ -430,13 +441,12 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           }
           if (!mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(tiles + stage * C::kStageBytes);
+          // the stages lie below 256 KB: adding to the address field never carries out of its 14 bits
+          const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
           const uint32_t idesc = p.idesc | (part << 29) | (part << 4);
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
-            umma_scaled<CTAS>(d, make_sw128_desc(a_addr + kk * 32, 16, 1024),
-                        make_sw128_desc(a_addr + C::kABytes + kk * 32, 16, 1024), idesc, sfa, sfa + 4,
-                        (i | kk) != 0 ? 1u : 0u);
+            umma_scaled<CTAS>(d, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfa + 4, (i | kk) != 0 ? 1u : 0u);
           commit<CTAS>(&empty[stage]);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
           if (part == 3 || i == t.kb - 1) {
@@ -454,30 +464,50 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       mbar_wait(drain, 0, p.status);
     }
   } else if (warp == 2) {
-    int sf = 0;
+    // Words of kAhead steps are in flight in registers: one step feeds four blocks of products, less than a load takes.
+    constexpr int kAhead = 4, kWords = 4 * (1 + C::kBParts);
+    int sf = 0, tile = first_tile - tile_step, w = 0, w_end = -1;
     uint32_t sf_phase = 0;
     bool ok = true;
-    for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-      const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
-      if (t.kb == 0) continue;
-      for (int w = t.kb0 / 4; w <= (t.kb0 + t.kb - 1) / 4; ++w) {
-        const uint32_t* wa = p.sa + static_cast<long>(w) * p.rows_a;
-        const uint32_t* wb = p.sb + static_cast<long>(w) * p.rows_b;
-        uint32_t v[4 * (1 + C::kBParts)];
+    Tile t = {};
+    uint32_t v[kAhead][kWords];
+    auto fetch = [&](uint32_t (&to)[kWords]) -> bool {
+      if (++w > w_end) {
+        do {
+          tile += tile_step;
+          if (tile >= total) return false;
+          t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+        } while (t.kb == 0);
+        w = t.kb0 / 4;
+        w_end = (t.kb0 + t.kb - 1) / 4;
+      }
+      const uint32_t* wa = p.sa + static_cast<long>(w) * p.rows_a;
+      const uint32_t* wb = p.sb + static_cast<long>(w) * p.rows_b;
 #pragma unroll
-        for (int q = 0; q < 4 * (1 + C::kBParts); ++q) {
-          const int row = q < 4 ? t.a_row + q * 32 + lane : t.b_row + (q - 4) * 32 + lane;
-          v[q] = row < (q < 4 ? p.rows_a : p.rows_b) ? __ldg((q < 4 ? wa : wb) + row) : 0u;
-        }
-        if (!mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status)) { ok = false; break; }
+      for (int q = 0; q < kWords; ++q) {
+        const int row = q < 4 ? t.a_row + q * 32 + lane : t.b_row + (q - 4) * 32 + lane;
+        to[q] = row < (q < 4 ? p.rows_a : p.rows_b) ? __ldg((q < 4 ? wa : wb) + row) : 0u;
+      }
+      return true;
+    };
+    bool have[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) have[j] = (j == 0 || have[j - 1]) && fetch(v[j]);
+    while (ok && have[0]) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (!ok || !have[j]) continue;
+        if (!mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status)) { ok = false; continue; }
         uint8_t* dst = scales + sf * C::kScaleBytes + lane * 16;
 #pragma unroll
         for (int q = 0; q < 1 + C::kBParts; ++q)
-          *reinterpret_cast<uint4*>(dst + 512 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          *reinterpret_cast<uint4*>(dst + 512 * q) =
+              make_uint4(v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) arrive_leader<CTAS>(&sf_full[sf]);
         if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
+        have[j] = tile < total && fetch(v[j]);
       }
     }
     for (int s = 0; s < kScaleStages && ok; ++s) {
