@@ -20,12 +20,13 @@
 // many products as in a CTA of its own; the first one issues the instructions
 // for both.  Rows that fit one CTA's 128 take the single form.
 //
-// Warp roles (256 threads):
+// Warp roles (384 threads):
 //   warp 0      TMA loads of the operand tiles (one lane)
 //   warp 1      MMA issue (one lane)
 //   warp 2      scale words: global -> shared memory
 //   warp 3      tensor memory allocation
-//   warps 4..7  epilogue (TMEM lane quarter = warp % 4)
+//   warps 4..11 epilogue: a lane quarter of tensor memory (warp % 4) is read by
+//               two warps, which take alternate columns
 // All waits are bounded (common.cuh).
 #include <cuda.h>
 #include <torch/extension.h>
@@ -42,7 +43,8 @@ namespace fp8 {
 
 enum Mode : int { kRowGroups = 0, kKGroups = 1 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
 constexpr int BM = 128;
 constexpr int BK = 128;            // one scale block, one 128-byte swizzled row
 constexpr int kMaxGroups = 512;
@@ -59,7 +61,7 @@ struct Cfg {
   static constexpr int kBRows = BN / CTAS;                       // rows of B that one CTA loads
   static constexpr int kBBytes = kBRows * BK;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = 4 * 2 * 4096;                 // per warp two buffers of 32 rows x 128 bytes
+  static constexpr int kEpiBytes = kEpiWarps * 4096;             // per warp a buffer of 32 rows x 128 bytes
   static constexpr int kBParts = (BN + 127) / 128;               // 128-row parts of the B scales
   static constexpr int kScaleBytes = 512 * (1 + kBParts);
   static constexpr bool kShared = BN == 256;
@@ -75,11 +77,28 @@ struct Cfg {
   static_assert(kStages >= 3 && kStageBytes % 1024 == 0, "shared memory budget");
 };
 
+// Division of a number below 2^31 by a fixed one: high half of a product, and
+// a shift.  With s = ceil(log2 d) and m = ceil(2^(31 + s) / d) the quotient is
+// exact, since m d - 2^(31 + s) < 2^s.
+struct Divisor {
+  unsigned m, s, d;
+  void set(unsigned by) {
+    d = by;
+    for (s = 0; (1u << s) < by; ++s) {}
+    m = static_cast<unsigned>(((1ull << (31 + s)) + by - 1) / by);
+  }
+  SB_DEVICE int operator()(int x) const {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(x)) * m) >> (31 + s));
+  }
+};
+
 struct Args {
   const uint32_t *sa, *sb;
   int rows_a, rows_b;      // rows of the scale planes
   int M, N, K, G, mode;
   int split;               // row mode, one group: K ranges, partial sums into D [split][M][N] fp32
+  int tiles_n;
+  Divisor by_band, by_tiles;   // kBand * tiles_n; row and column tiles of one group (K groups, split)
   const int* offs;
   void* D;
   long ldd;
@@ -213,6 +232,18 @@ SB_DEVICE void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int x
         : "memory");
   }
 }
+// Whether the phase is over already; does not wait.
+SB_DEVICE bool mbar_test(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
 template <int CTAS>
 SB_DEVICE void tmem_take(uint32_t* slot, uint32_t cols) {
   if constexpr (CTAS == 1) {
@@ -243,21 +274,38 @@ SB_DEVICE void sync_pair() {
 // Row and column tile of number `local` among tiles_m x tiles_n: bands of
 // kBand row tiles, rows first, so that the tiles in flight at one time share
 // few rows of both operands.
-SB_DEVICE void walk(int local, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int band = local / (kBand * tiles_n);
+SB_DEVICE void walk(const Args& p, int local, int tiles_m, int& tm, int& tn) {
+  const int band = p.by_band(local);
   const int height = min(kBand, tiles_m - band * kBand);
-  const int in = local - band * kBand * tiles_n;
-  tn = in / height;
+  const int in = local - band * kBand * p.tiles_n;
+  tn = height == kBand ? in / kBand : static_cast<int>(static_cast<unsigned>(in) / static_cast<unsigned>(height));
   tm = band * kBand + in - tn * height;
+}
+
+// The blocks that a tile contracts, all that the issuer has to know.
+SB_DEVICE void tile_blocks(const Args& p, const int* s_prefix, const int* s_offs, int tile, int& kb0, int& kb) {
+  if (p.mode == kKGroups) {
+    const int g = p.by_tiles(tile);
+    kb0 = s_offs[g] / BK;
+    kb = (s_offs[g + 1] - s_offs[g] + BK - 1) / BK;
+    return;
+  }
+  kb0 = 0;
+  kb = (p.K + BK - 1) / BK;
+  if (p.split > 1) {                               // 2^24 blocks by 148 ranges at most: 32 bits hold it
+    const unsigned s = p.by_tiles(tile), blocks = kb;
+    kb0 = blocks * s / p.split;
+    kb = blocks * (s + 1) / p.split - kb0;
+  }
 }
 
 // `rank`: the CTA's place in its pair.
 template <int BN, int CTAS>
 __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile, int rank) {
   using C = Cfg<BN, CTAS>;
-  const int tiles_n = (p.N + BN - 1) / BN;
   Tile t;
   int tm, tn;
+  tile_blocks(p, s_prefix, s_offs, tile, t.kb0, t.kb);
   if (p.mode == kRowGroups) {
     int lo = 0, hi = p.G - 1;                      // last group whose first tile is at most `tile`
     while (lo < hi) {
@@ -265,37 +313,28 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
       if (s_prefix[mid] <= tile) lo = mid;
       else hi = mid - 1;
     }
-    int local = tile - s_prefix[lo];
-    const int blocks = (p.K + BK - 1) / BK;
+    int local = tile - s_prefix[lo], s = 0;
     const int rows = s_offs[lo + 1] - s_offs[lo], tiles_m = (rows + C::kTileM - 1) / C::kTileM;
-    int s = 0;
     if (p.split > 1) {
-      const int per = tiles_m * tiles_n;
-      s = local / per;
-      local -= s * per;
+      s = p.by_tiles(local);
+      local -= s * p.by_tiles.d;
     }
-    walk(local, tiles_m, tiles_n, tm, tn);
+    walk(p, local, tiles_m, tm, tn);
     const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
     t.a_row = s_offs[lo] + m;
     t.b_row = lo * p.N + t.n0;
     t.d_row = t.a_row + static_cast<long>(s) * p.M;
     t.m_valid = min(BM, rows - m);
-    t.kb0 = static_cast<int>(static_cast<long>(blocks) * s / p.split);
-    t.kb = static_cast<int>(static_cast<long>(blocks) * (s + 1) / p.split) - t.kb0;
   } else {
-    const int tiles_m = (p.M + C::kTileM - 1) / C::kTileM;
-    const int per = tiles_m * tiles_n;
-    const int g = tile / per;
-    walk(tile % per, tiles_m, tiles_n, tm, tn);
+    const int g = p.by_tiles(tile);
+    walk(p, tile - g * p.by_tiles.d, (p.M + C::kTileM - 1) / C::kTileM, tm, tn);
     const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
     t.a_row = m;
     t.b_row = t.n0;
     t.d_row = static_cast<long>(g) * p.M + m;
     t.m_valid = min(BM, p.M - m);
-    t.kb0 = s_offs[g] / BK;
-    t.kb = (s_offs[g + 1] - s_offs[g] + BK - 1) / BK;
   }
   return t;
 }
@@ -342,7 +381,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 4 * CTAS);
+      mbar_init(&acc_empty[a], kEpiWarps * CTAS);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -352,13 +391,12 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   if (warp == 3) tmem_take<CTAS>(tmem_slot, C::kTmemCols);
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int tiles_n = (p.N + BN - 1) / BN;
     int total = 0;
     if (p.mode == kRowGroups) {
       for (int g = 0; g < p.G; ++g) {
         s_prefix[g] = total;
         s_offs[g + 1] = max(s_offs[g + 1], s_offs[g]);
-        total += (s_offs[g + 1] - s_offs[g] + C::kTileM - 1) / C::kTileM * tiles_n * p.split;
+        total += (s_offs[g + 1] - s_offs[g] + C::kTileM - 1) / C::kTileM * p.tiles_n * p.split;
       }
       s_prefix[p.G] = total;
     } else {
@@ -369,7 +407,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         ok &= s_offs[g + 1] == s_offs[g] ||
               (s_offs[g] % BK == 0 && (s_offs[g + 1] % BK == 0 || s_offs[g + 1] == p.K));
       }
-      total = ok ? p.G * ((p.M + C::kTileM - 1) / C::kTileM) * tiles_n : 0;
+      total = ok ? p.G * p.by_tiles.d : 0;
       if (!ok && blockIdx.x == 0) record_status(p.status, kBadShape);
     }
     *s_total = total;
@@ -411,9 +449,11 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       const uint64_t desc0 = make_sw128_desc(smem_u32(tiles), 16, 1024);
       int stage = 0, acc = 0, sf = 0;
       uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
-      bool ok = true;
+      uint32_t sfa = 0;
+      bool ok = true, ready = false;
       for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-        const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+        int kb0, kb;
+        tile_blocks(p, s_prefix, s_offs, tile, kb0, kb);
         // its accumulator has been read; one that shares columns with the other also waits until the tile before
         // has read those, which it does first, and the epilogue takes tiles in order
         if (C::kShared) {
@@ -427,19 +467,18 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
         tc_fence_after();
         const uint32_t d = tmem + acc * C::kAccCols;
-        uint32_t sfa = 0;
-        for (int i = 0; i < t.kb; ++i) {
-          const uint32_t part = (t.kb0 + i) % 4;       // the byte of the scale words
+        for (int i = 0; i < kb; ++i) {
+          const uint32_t part = (kb0 + i) % 4;         // the byte of the scale words
           if (i == 0 || part == 0) {
             if (!wait_both<CTAS>(&sf_full[sf], sf_phase, p.status)) { ok = false; break; }
             tc_fence_after();
-            // stage sf of the words has its own columns, free since sf_empty[sf] was signalled
+            // step sf of the words has its own columns, free since sf_empty[sf] was signalled
             sfa = tmem + C::kScaleCol0 + sf * C::kScaleCols;
             const uint32_t src = smem_u32(scales + sf * C::kScaleBytes);
 #pragma unroll
             for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales<CTAS>(sfa + 4 * q, src + 512 * q);
           }
-          if (!mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
+          if (!ready && !mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
           tc_fence_after();
           // the stages lie below 256 KB: adding to the address field never carries out of its 14 bits
           const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
@@ -449,7 +488,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             umma_scaled<CTAS>(d, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfa + 4, (i | kk) != 0 ? 1u : 0u);
           commit<CTAS>(&empty[stage]);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
-          if (part == 3 || i == t.kb - 1) {
+          ready = mbar_test(&full[stage], phase);      // asked early: the answer takes 100 clocks
+          if (part == 3 || i == kb - 1) {
             commit<CTAS>(&sf_empty[sf]);
             if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
           }
@@ -490,23 +530,32 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       }
       return true;
     };
-    bool have[kAhead];
+    auto hand_over = [&](const uint32_t (&from)[kWords]) {
+      ok = mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status);
+      if (!ok) return;
+      uint8_t* dst = scales + sf * C::kScaleBytes + lane * 16;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) have[j] = (j == 0 || have[j - 1]) && fetch(v[j]);
+      for (int q = 0; q < 1 + C::kBParts; ++q)
+        *reinterpret_cast<uint4*>(dst + 512 * q) =
+            make_uint4(from[4 * q], from[4 * q + 1], from[4 * q + 2], from[4 * q + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_leader<CTAS>(&sf_full[sf]);
+      if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
+    };
+    // the first step goes out alone, before time is spent on the next ones
+    bool have[kAhead];
+    have[0] = fetch(v[0]);
+    if (have[0]) {
+      hand_over(v[0]);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) have[j] = (j == 0 || have[j - 1]) && fetch(v[j]);
+    }
     while (ok && have[0]) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (!ok || !have[j]) continue;
-        if (!mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status)) { ok = false; continue; }
-        uint8_t* dst = scales + sf * C::kScaleBytes + lane * 16;
-#pragma unroll
-        for (int q = 0; q < 1 + C::kBParts; ++q)
-          *reinterpret_cast<uint4*>(dst + 512 * q) =
-              make_uint4(v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) arrive_leader<CTAS>(&sf_full[sf]);
-        if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
+        hand_over(v[j]);
         have[j] = tile < total && fetch(v[j]);
       }
     }
@@ -515,11 +564,11 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
     }
   } else if (warp >= 4) {
-    const int quarter = warp - 4;
+    const int quarter = warp % 4, half = (warp - 4) / 4;
     const int r = quarter * 32 + lane;
-    uint8_t* buf = epi + quarter * 8192;
+    uint8_t* buf = epi + (warp - 4) * 4096;
     int acc = 0;
-    uint32_t acc_phase = 0, slab = 0;
+    uint32_t acc_phase = 0;
     for (int tile = first_tile; tile < total; tile += tile_step) {
       const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
       if (!mbar_wait(&acc_full[acc], acc_phase, p.status)) break;
@@ -530,22 +579,24 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       if (p.tma_store && t.kb > 0 && (t.m_valid == BM || t.d_row + t.m_valid >= p.d_rows)) {
         const int step = p.f32 ? 32 : 64;             // columns of 128 bytes
         const int n = (cols + step - 1) / step;
+        if (half >= n) {                              // nothing for this warp, nor has it anything to wait for
+          if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
+        }
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
+        for (int i = half; i < n; i += 2) {
           // shared columns first: the last of the first accumulator, the first of the second
           const int s = C::kShared && acc == 0 ? n - 1 - i : i;
           uint32_t v[64];
           tmem_ld_32x32b_x32(src + s * step, v);
           if (!p.f32) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
           tmem_wait_ld();
-          if (i == (C::kShared ? 0 : n - 1)) {
+          if (C::kShared ? i < 2 : i + 2 >= n) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
           }
-          uint8_t* b = buf + (slab & 1) * 4096;
-          ++slab;
-          if (lane == 0) bulk_wait_group_read<1>();
+          uint8_t* b = buf;
+          if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
           if (p.f32) {
 #pragma unroll
@@ -567,13 +618,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
       } else {
 #pragma unroll 1
-        for (int q = 0; q < BN / 32; ++q) {
+        for (int q = half; q < BN / 32; q += 2) {
           const int c = 32 * (C::kShared && acc == 0 ? BN / 32 - 1 - q : q);
           uint32_t v[32];
           __syncwarp();
           tmem_ld_32x32b_x32(src + c, v);
           tmem_wait_ld();
-          if (q == (C::kShared ? 0 : BN / 32 - 1)) {
+          if (C::kShared ? q < 2 : q + 2 >= BN / 32) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
@@ -749,6 +800,9 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   const int bn = plan.bn;
   const long tiles = plan.tiles;
   p.split = plan.split;
+  p.tiles_n = static_cast<int>((N + bn - 1) / bn);
+  p.by_band.set(kBand * p.tiles_n);
+  p.by_tiles.set(static_cast<unsigned>((M + BM * plan.ctas - 1) / (BM * plan.ctas) * p.tiles_n));
 
   at::Tensor ws;
   const bool f32 = D.scalar_type() == at::kFloat;
