@@ -24,7 +24,7 @@
 //   warp 0      TMA loads of the operand tiles (one lane)
 //   warp 1      MMA issue (one lane)
 //   warp 2      scale words: global -> shared memory
-//   warp 3      tensor memory allocation
+//   warp 3      tensor memory allocation; in a pair, word of the scales' arrival
 //   warps 4..11 epilogue: a lane quarter of tensor memory (warp % 4) is read by
 //               two warps, which take alternate columns
 // All waits are bounded (common.cuh).
@@ -33,7 +33,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <cstring>
 #include <mutex>
 
 #include "fp8.cuh"
@@ -48,20 +47,28 @@ constexpr int kEpiWarps = 8;
 constexpr int BM = 128;
 constexpr int BK = 128;            // one scale block, one 128-byte swizzled row
 constexpr int kMaxGroups = 512;
+constexpr int kPanelBlocks = 8;    // blocks of 128 that a panel of A holds
 constexpr int kBand = 8;           // row tiles whose column tiles are walked together
 
 // CTAS: CTAs that share a tile of 128 * CTAS rows and BN columns.  Two
 // accumulators alternate so that the epilogue of one tile runs under the next
 // one's products.  256 columns twice would leave no room for the scales, so
 // there the two share 32 columns, which the epilogue reads first.
-template <int BN, int CTAS>
+// PANEL: the CTA keeps its rows of A (up to 1024 bytes each) in shared memory
+// while it walks along the columns, and only B streams.  The way from L2 into
+// an SM carries about 64 bytes a clock; without a panel a tile of 256 x 192
+// moves 28 KB for 384 clocks of products, with it 12 KB.
+template <int BN, int CTAS, bool PANEL>
 struct Cfg {
   static constexpr int kTileM = BM * CTAS;
   static constexpr int kABytes = BM * BK;
   static constexpr int kBRows = BN / CTAS;                       // rows of B that one CTA loads
   static constexpr int kBBytes = kBRows * BK;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = kEpiWarps * 4096;             // per warp a buffer of 32 rows x 128 bytes
+  static constexpr int kPanelBytes = PANEL ? kPanelBlocks * kABytes : 0;
+  static constexpr int kBOff = PANEL ? 0 : kABytes;              // of B within a stage
+  static constexpr int kStageBytes = kBOff + kBBytes;
+  static constexpr int kChunks = PANEL ? 4 : 8;                  // 16-byte pieces of a row that a warp stages
+  static constexpr int kEpiBytes = kEpiWarps * 32 * kChunks * 16;
   static constexpr int kBParts = (BN + 127) / 128;               // 128-row parts of the B scales
   static constexpr int kScaleBytes = 512 * (1 + kBParts);
   static constexpr bool kShared = BN == 256;
@@ -71,7 +78,7 @@ struct Cfg {
   static constexpr int kTmemCols = 512;
   static constexpr int kScaleCol0 = kAccCols + BN;
   static_assert(kScaleCol0 + kScaleStages * kScaleCols <= kTmemCols, "tensor memory budget");
-  static constexpr int kFixed = kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 + 2 * (kMaxGroups + 1) * 4;
+  static constexpr int kFixed = kPanelBytes + kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 + 2 * (kMaxGroups + 1) * 4;
   static constexpr int kStages = (232448 - kFixed) / kStageBytes < 8 ? (232448 - kFixed) / kStageBytes : 8;
   static constexpr int kSmemBytes = kStages * kStageBytes + kFixed;
   static_assert(kStages >= 3 && kStageBytes % 1024 == 0, "shared memory budget");
@@ -98,12 +105,11 @@ struct Args {
   int M, N, K, G, mode;
   int split;               // row mode, one group: K ranges, partial sums into D [split][M][N] fp32
   int tiles_n;
-  Divisor by_band, by_tiles;   // kBand * tiles_n; row and column tiles of one group (K groups, split)
+  Divisor by_n, by_band, by_tiles;   // tiles_n; kBand * tiles_n; tiles of one group (K groups, split)
   const int* offs;
   void* D;
   long ldd;
-  int d_rows;              // rows of the tensor that tmD describes
-  bool f32, acc, tma_store;
+  bool f32, acc, d_vec;    // d_vec: D takes 16-byte stores
   uint32_t idesc;
   int* status;
 };
@@ -244,6 +250,17 @@ SB_DEVICE bool mbar_test(uint64_t* bar, uint32_t phase) {
       : "memory");
   return ok != 0;
 }
+// The same without ordering this thread's memory accesses before it: for an
+// accumulator that has been read, which tcgen05's own fence orders.  (The
+// releasing form waits for the global stores before it, 600 clocks.)
+template <int CTAS>
+SB_DEVICE void arrive_leader_relaxed(uint64_t* bar) {
+  if constexpr (CTAS == 1) {
+    mbar_arrive(bar);
+  } else {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+  }
+}
 template <int CTAS>
 SB_DEVICE void tmem_take(uint32_t* slot, uint32_t cols) {
   if constexpr (CTAS == 1) {
@@ -268,6 +285,44 @@ SB_DEVICE void sync_pair() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
+}
+
+// 16 staged bytes to D: sums (fp32, to be added or not) or finished bf16 values.
+// `here` values of them, at `at` elements from `out`.
+SB_DEVICE void store_some(const Args& p, const uint8_t* staged, uint8_t* out, long at, int here) {
+  if (p.f32 || p.acc) {
+    const float4 w = *reinterpret_cast<const float4*>(staged);
+    float f[4] = {w.x, w.y, w.z, w.w};
+    if (p.f32) {
+      float* d = reinterpret_cast<float*>(out) + at;
+      if (p.d_vec && here == 4) {
+        float4 o = p.acc ? *reinterpret_cast<const float4*>(d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(d) = make_float4(f[0] + o.x, f[1] + o.y, f[2] + o.z, f[3] + o.w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < here) d[i] = p.acc ? d[i] + f[i] : f[i];
+      }
+    } else {
+      __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(out) + at;
+      if (p.d_vec && here == 4) {
+        const uint2 o = *reinterpret_cast<const uint2*>(d);
+        const float2 a = unpack_bf16x2(o.x), b = unpack_bf16x2(o.y);
+        *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(f[0] + a.x, f[1] + a.y), pack_bf16x2(f[2] + b.x, f[3] + b.y));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < here) d[i] = __float2bfloat16(__bfloat162float(d[i]) + f[i]);
+      }
+    }
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(staged);
+    const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+    uint16_t* d = reinterpret_cast<uint16_t*>(out) + at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < here) d[i] = static_cast<uint16_t>(e[i / 2] >> (16 * (i % 2)));
   }
 }
 
@@ -300,9 +355,9 @@ SB_DEVICE void tile_blocks(const Args& p, const int* s_prefix, const int* s_offs
 }
 
 // `rank`: the CTA's place in its pair.
-template <int BN, int CTAS>
+template <int BN, int CTAS, bool PANEL>
 __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile, int rank) {
-  using C = Cfg<BN, CTAS>;
+  using C = Cfg<BN, CTAS, PANEL>;
   Tile t;
   int tm, tn;
   tile_blocks(p, s_prefix, s_offs, tile, t.kb0, t.kb);
@@ -319,7 +374,12 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
       s = p.by_tiles(local);
       local -= s * p.by_tiles.d;
     }
-    walk(p, local, tiles_m, tm, tn);
+    if (PANEL) {                                   // along the columns, so that a panel serves many tiles
+      tm = p.by_n(local);
+      tn = local - tm * p.tiles_n;
+    } else {
+      walk(p, local, tiles_m, tm, tn);
+    }
     const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
     t.a_row = s_offs[lo] + m;
@@ -339,24 +399,28 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
   return t;
 }
 
-template <int BN, int CTAS>
+template <int BN, int CTAS, bool PANEL>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(CTAS, 1, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-              const __grid_constant__ CUtensorMap tmD, const Args p) {
-  using C = Cfg<BN, CTAS>;
+              const Args p) {
+  using C = Cfg<BN, CTAS, PANEL>;
   constexpr int kScaleStages = C::kScaleStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* tiles = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
-  uint8_t* epi = tiles + C::kStages * C::kStageBytes;
+  uint8_t* panel = tiles + C::kStages * C::kStageBytes;
+  uint8_t* epi = panel + C::kPanelBytes;
   uint8_t* scales = epi + C::kEpiBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScaleStages * C::kScaleBytes);
   uint64_t* empty = full + C::kStages;
   uint64_t* sf_full = empty + C::kStages;
   uint64_t* sf_empty = sf_full + kScaleStages;
-  uint64_t* acc_full = sf_empty + kScaleStages;
+  uint64_t* sf_here = sf_empty + kScaleStages;
+  uint64_t* acc_full = sf_here + kScaleStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* drain = acc_empty + 2;
+  uint64_t* a_full = acc_empty + 2;
+  uint64_t* a_empty = a_full + kPanelBlocks;
+  uint64_t* drain = a_empty + kPanelBlocks;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* s_total = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_offs = s_total + 1;
@@ -364,7 +428,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = CTAS == 1 ? 0 : blockIdx.x % CTAS;
-  const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
 
   for (int g = threadIdx.x; g <= p.G; g += kThreads) {
     const int lim = p.mode == kRowGroups ? p.M : p.K;
@@ -378,10 +441,15 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     for (int s = 0; s < kScaleStages; ++s) {
       mbar_init(&sf_full[s], CTAS);
       mbar_init(&sf_empty[s], 1);
+      mbar_init(&sf_here[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], kEpiWarps * CTAS);
+    }
+    for (int b = 0; b < kPanelBlocks; ++b) {
+      mbar_init(&a_full[b], 1);
+      mbar_init(&a_empty[b], 1);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -416,22 +484,39 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   sync_pair<CTAS>();          // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int total = *s_total;
+  // Tiles of this CTA (or pair): every so-and-so-many-th, or a run of neighbours, which share panels.
+  const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
+  const int first_tile = PANEL ? static_cast<int>(static_cast<long long>(*s_total) * unit / units) : unit;
+  const int total = PANEL ? static_cast<int>(static_cast<long long>(*s_total) * (unit + 1) / units) : *s_total;
+  const int tile_step = PANEL ? 1 : units;
+  const int first_n = PANEL ? first_tile - p.by_n(first_tile) * p.tiles_n : 0;   // its column tile
 
   if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
+      uint32_t panel_phase = 0;
+      int tn = first_n;
       bool ok = true;
       for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-        const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+        const Tile t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
+        const bool fresh = PANEL && (tile == first_tile || tn == 0);      // a new panel
         for (int i = 0; i < t.kb; ++i) {
+          if (PANEL && fresh) {
+            if (!mbar_wait(&a_empty[i], panel_phase ^ 1, p.status)) { ok = false; break; }
+            if (rank == 0) mbar_arrive_expect_tx(&a_full[i], C::kABytes * CTAS);
+            load_tile<CTAS>(panel + i * C::kABytes, &tmA, &a_full[i], i * BK, t.a_row);
+          }
           if (!mbar_wait(&empty[stage], phase ^ 1, p.status)) { ok = false; break; }
-          uint8_t* sA = tiles + stage * C::kStageBytes;
+          uint8_t* s = tiles + stage * C::kStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], C::kStageBytes * CTAS);
-          load_tile<CTAS>(sA, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
-          load_tile<CTAS>(sA + C::kABytes, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row + rank * C::kBRows);
+          if (!PANEL) load_tile<CTAS>(s, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
+          load_tile<CTAS>(s + C::kBOff, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row + rank * C::kBRows);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+        }
+        if (PANEL) {
+          if (fresh) panel_phase ^= 1;
+          if (++tn == p.tiles_n) tn = 0;
         }
       }
       // every stage's products have signalled here before this CTA may go: the other one's signals are remote
@@ -439,14 +524,22 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         ok = mbar_wait(&empty[stage], phase ^ 1, p.status);
         if (++stage == C::kStages) { stage = 0; phase ^= 1; }
       }
+      if (PANEL && first_tile < total)
+        for (int b = 0; b < (p.K + BK - 1) / BK && ok; ++b) ok = mbar_wait(&a_empty[b], panel_phase ^ 1, p.status);
       // an early end: wait (briefly) for the loads in flight, which must not land after the CTA has gone
       // (the second CTA's complete on the first one's barriers; the pair leaves together)
-      if (!ok && rank == 0)
+      if (!ok && rank == 0) {
         for (int s = 0; s < C::kStages; ++s) mbar_wait(&full[s], phase ^ (s < stage ? 0 : 1), nullptr, 200000000ull);
+        for (int b = 0; PANEL && b < kPanelBlocks; ++b)
+          for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait(&a_full[b], ph, nullptr, 100000000ull);
+      }
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
       const uint64_t desc0 = make_sw128_desc(smem_u32(tiles), 16, 1024);
+      const uint64_t panel0 = make_sw128_desc(smem_u32(panel), 16, 1024);
+      uint32_t panel_phase = 0;
+      int tn = first_n;
       int stage = 0, acc = 0, sf = 0;
       uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
       uint32_t sfa = 0;
@@ -467,6 +560,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
         tc_fence_after();
         const uint32_t d = tmem + acc * C::kAccCols;
+        const bool fresh = PANEL && (tile == first_tile || tn == 0);
+        const bool leave = PANEL && (tile == total - 1 || tn == p.tiles_n - 1);   // the panel's last tile
         for (int i = 0; i < kb; ++i) {
           const uint32_t part = (kb0 + i) % 4;         // the byte of the scale words
           if (i == 0 || part == 0) {
@@ -479,14 +574,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales<CTAS>(sfa + 4 * q, src + 512 * q);
           }
           if (!ready && !mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
+          if (PANEL && fresh && !mbar_wait(&a_full[i], panel_phase, p.status)) { ok = false; break; }
           tc_fence_after();
-          // the stages lie below 256 KB: adding to the address field never carries out of its 14 bits
-          const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
+          // all lies below 256 KB: adding to the address field never carries out of its 14 bits
+          const uint64_t sd = desc0 + stage * (C::kStageBytes >> 4), bd = sd + (C::kBOff >> 4);
+          const uint64_t ad = PANEL ? panel0 + i * (C::kABytes >> 4) : sd;
           const uint32_t idesc = p.idesc | (part << 29) | (part << 4);
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
             umma_scaled<CTAS>(d, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfa + 4, (i | kk) != 0 ? 1u : 0u);
           commit<CTAS>(&empty[stage]);
+          if (PANEL && leave) commit<CTAS>(&a_empty[i]);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
           ready = mbar_test(&full[stage], phase);      // asked early: the answer takes 100 clocks
           if (part == 3 || i == kb - 1) {
@@ -495,6 +593,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           }
         }
         if (!ok) break;
+        if (PANEL) {
+          if (fresh) panel_phase ^= 1;
+          if (++tn == p.tiles_n) tn = 0;
+        }
         commit<CTAS>(&acc_full[acc]);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
@@ -516,7 +618,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         do {
           tile += tile_step;
           if (tile >= total) return false;
-          t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+          t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
         } while (t.kb == 0);
         w = t.kb0 / 4;
         w_end = (t.kb0 + t.kb - 1) / 4;
@@ -540,7 +642,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             make_uint4(from[4 * q], from[4 * q + 1], from[4 * q + 2], from[4 * q + 3]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) arrive_leader<CTAS>(&sf_full[sf]);
+      if (lane == 0) mbar_arrive(CTAS == 1 ? &sf_full[sf] : &sf_here[sf]);
       if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
     };
     // the first step goes out alone, before time is spent on the next ones
@@ -563,98 +665,101 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       ok = mbar_wait(&sf_empty[sf], sf_phase ^ 1, p.status);
       if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
     }
+  } else if (warp == 3) {
+    // Tells the first CTA that words have come.  A lane of warp 2 cannot: arriving at another CTA's barrier
+    // releases, which waits for all loads of the lane, also those of the words to come.
+    if (CTAS == 2 && elect_one()) {
+      int sf = 0;
+      uint32_t sf_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        int kb0, kb;
+        tile_blocks(p, s_prefix, s_offs, tile, kb0, kb);
+        for (int w = kb0 / 4; kb > 0 && w <= (kb0 + kb - 1) / 4; ++w) {
+          if (!mbar_wait(&sf_here[sf], sf_phase, p.status)) { ok = false; break; }
+          arrive_leader<CTAS>(&sf_full[sf]);
+          if (++sf == kScaleStages) { sf = 0; sf_phase ^= 1; }
+        }
+      }
+    }
   } else if (warp >= 4) {
     const int quarter = warp % 4, half = (warp - 4) / 4;
     const int r = quarter * 32 + lane;
-    uint8_t* buf = epi + (warp - 4) * 4096;
+    uint8_t* buf = epi + (warp - 4) * 32 * C::kChunks * 16;
     int acc = 0;
     uint32_t acc_phase = 0;
+    // piece j of a staged row, turned so that neither a column of pieces nor a row meets a bank twice
+    auto staged_at = [](int row, int j) { return (row * C::kChunks + (j ^ ((C::kChunks == 8 ? row : row / 2) % C::kChunks))) * 16; };
     for (int tile = first_tile; tile < total; tile += tile_step) {
-      const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
+      const Tile t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
       if (!mbar_wait(&acc_full[acc], acc_phase, p.status)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * C::kAccCols + ((quarter * 32) << 16);
       const int cols = min(BN, p.N - t.n0);
-      // whole tiles, and tiles cut off by the end of D, leave through TMA
-      if (p.tma_store && t.kb > 0 && (t.m_valid == BM || t.d_row + t.m_valid >= p.d_rows)) {
-        const int step = p.f32 ? 32 : 64;             // columns of 128 bytes
-        const int n = (cols + step - 1) / step;
-        if (half >= n) {                              // nothing for this warp, nor has it anything to wait for
-          if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
-        }
+      // A warp's 32 rows of 128 (64) bytes go through shared memory, so that each global store covers whole runs of
+      // rows: 64 (32) columns that leave as bf16, half as many that leave as fp32 or are added to what D holds.
+      const bool wide = p.f32 || p.acc;
+      constexpr int kChunks = C::kChunks;
+      const int step = wide ? 4 * kChunks : 8 * kChunks;
+      const int n = (cols + step - 1) / step;
+      if (half >= n && lane == 0) arrive_leader_relaxed<CTAS>(&acc_empty[acc]);    // nothing for this warp to read
+      const int rows_here = min(32, t.m_valid - quarter * 32);
+      uint8_t* const out = static_cast<uint8_t*>(p.D) + ((t.d_row + quarter * 32) * p.ldd + t.n0) * (p.f32 ? 4 : 2);
 #pragma unroll 1
-        for (int i = half; i < n; i += 2) {
-          // shared columns first: the last of the first accumulator, the first of the second
-          const int s = C::kShared && acc == 0 ? n - 1 - i : i;
-          uint32_t v[64];
+      for (int i = half; i < n; i += 2) {
+        // shared columns first: the last of the first accumulator, the first of the second
+        const int s = C::kShared && acc == 0 ? n - 1 - i : i;
+        uint32_t v[8 * kChunks];
+        __syncwarp();                                  // the buffer has been read, the warp is whole
+        if constexpr (kChunks == 8) {
           tmem_ld_32x32b_x32(src + s * step, v);
-          if (!p.f32) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
-          tmem_wait_ld();
-          if (C::kShared ? i < 2 : i + 2 >= n) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
-          }
-          uint8_t* b = buf;
-          if (lane == 0) bulk_wait_group_read<0>();
-          __syncwarp();
-          if (p.f32) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(b + lane * 128 + ((j ^ (lane & 7)) * 16)) =
-                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<bf16x8*>(b + lane * 128 + ((j ^ (lane & 7)) * 16)) =
-                  float_to_bf16x8(reinterpret_cast<const float*>(v) + 8 * j);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmD, b, t.n0 + s * step, static_cast<int>(t.d_row) + quarter * 32);
-            bulk_commit_group();
-          }
+          if (!wide) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
+        } else {
+          tmem_ld_32x32b_x16(src + s * step, v);
+          if (!wide) tmem_ld_32x32b_x16(src + s * step + 16, v + 16);
         }
-      } else {
-#pragma unroll 1
-        for (int q = half; q < BN / 32; q += 2) {
-          const int c = 32 * (C::kShared && acc == 0 ? BN / 32 - 1 - q : q);
-          uint32_t v[32];
+        tmem_wait_ld();
+        if (C::kShared ? i < 2 : i + 2 >= n) {
+          tc_fence_before();
           __syncwarp();
-          tmem_ld_32x32b_x32(src + c, v);
-          tmem_wait_ld();
-          if (C::kShared ? q < 2 : q + 2 >= BN / 32) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader<CTAS>(&acc_empty[acc]);
-          }
-          const long at = (t.d_row + r) * p.ldd + t.n0 + c;
-          const int here = r < t.m_valid ? min(32, cols - c) : 0;
-          if (p.f32) {
-            float* d = static_cast<float*>(p.D) + at;
+          if (lane == 0) arrive_leader_relaxed<CTAS>(&acc_empty[acc]);
+        }
+        if (rows_here <= 0) continue;
+        if (t.kb == 0) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < here) {
-                const float f = t.kb > 0 ? __uint_as_float(v[i]) : 0.f;
-                d[i] = p.acc ? d[i] + f : f;
-              }
-          } else {
-            __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.D) + at;
+          for (int j = 0; j < 8 * kChunks; ++j) v[j] = 0u;      // nothing was contracted: zeros
+        }
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < here) {
-                const float f = t.kb > 0 ? __uint_as_float(v[i]) : 0.f;
-                d[i] = __float2bfloat16(p.acc ? __bfloat162float(d[i]) + f : f);
-              }
+        for (int j = 0; j < kChunks; ++j) {
+          uint4 w = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          if (!wide) {
+            const bf16x8 h = float_to_bf16x8(reinterpret_cast<const float*>(v) + 8 * j);
+            w = make_uint4(h.w[0], h.w[1], h.w[2], h.w[3]);
           }
+          *reinterpret_cast<uint4*>(buf + staged_at(lane, j)) = w;
+        }
+        __syncwarp();
+        const int r0 = lane / kChunks, j = lane % kChunks, per = wide ? 4 : 8, c = s * step + j * per;
+        const int here = min(per, cols - c);           // of this lane's 16 bytes
+        if (p.d_vec && here == per && !p.acc) {
+          uint8_t* d = out + (r0 * p.ldd + c) * (p.f32 ? 4 : 2);
+          const long jump = 32 / kChunks * p.ldd * (p.f32 ? 4 : 2);
+#pragma unroll
+          for (int q = 0; q < kChunks; ++q) {
+            const int row = q * (32 / kChunks) + r0;
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + staged_at(row, j));
+            if (row < rows_here) *reinterpret_cast<uint4*>(d) = w;
+            d += jump;
+          }
+        } else if (here > 0) {
+#pragma unroll 1
+          for (int row = r0; row < rows_here; row += 32 / kChunks)
+            store_some(p, buf + staged_at(row, j), out, row * p.ldd + c, here);
         }
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-    if (lane == 0) bulk_wait_group<0>();
-    __syncwarp();
   }
 
   tc_fence_before();
@@ -704,15 +809,14 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-// Row-major [rows, cols] with row stride `bytes`, boxes of 128 bytes x box_rows, 128-byte swizzle.
-static CUtensorMap make_map(CUtensorMapDataType type, int elem, const void* base, long rows, long cols, long bytes,
-                            int box_rows) {
+// Row-major bytes [rows, cols] with row stride `bytes`, boxes of 128 bytes x box_rows, 128-byte swizzle.
+static CUtensorMap make_map(const void* base, long rows, long cols, long bytes, int box_rows) {
   CUtensorMap m;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(bytes)};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode_fn()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
@@ -726,19 +830,20 @@ static int num_sms(int device) {
   return v;
 }
 
-template <int BN, int CTAS>
-static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Args& p, long tiles,
+template <int BN, int CTAS, bool PANEL>
+static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& p, long tiles,
                    int device, cudaStream_t st) {
-  using C = Cfg<BN, CTAS>;
-  auto kern = matmul_kernel<BN, CTAS>;
+  using C = Cfg<BN, CTAS, PANEL>;
+  auto kern = matmul_kernel<BN, CTAS, PANEL>;
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
   const int grid = static_cast<int>(std::min<long>(num_sms(device) / CTAS, std::max<long>(1, tiles))) * CTAS;
-  kern<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, td, p);
+  kern<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 struct Plan {
   int ctas, bn, split;
+  bool panel;
   long tiles;            // upper bound for the grid
 };
 
@@ -752,9 +857,12 @@ static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, i
   if (const char* e = getenv("SB_FP8_BN")) p.bn = atoi(e);
   const long tm = (M + BM * p.ctas - 1) / (BM * p.ctas), tn = (N + p.bn - 1) / p.bn;
   p.tiles = mode == kRowGroups ? (tm + (offs ? G : 0)) * tn : G * tm * tn;
+  p.panel = p.ctas == 2 && mode == kRowGroups && blocks <= kPanelBlocks && tn > 1;
+  if (const char* e = getenv("SB_FP8_PANEL")) p.panel = p.panel && atoi(e);
   p.split = 1;
   const long slots = sms / p.ctas;
   if (!offs && p.tiles * 2 <= slots && blocks >= 8) {
+    p.panel = false;
     p.split = static_cast<int>(std::min<long>(slots / p.tiles, blocks / 4));
     p.tiles *= p.split;
   }
@@ -801,6 +909,7 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   const long tiles = plan.tiles;
   p.split = plan.split;
   p.tiles_n = static_cast<int>((N + bn - 1) / bn);
+  p.by_n.set(p.tiles_n);
   p.by_band.set(kBand * p.tiles_n);
   p.by_tiles.set(static_cast<unsigned>((M + BM * plan.ctas - 1) / (BM * plan.ctas) * p.tiles_n));
 
@@ -810,39 +919,35 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   p.acc = accumulate;
   p.D = D.data_ptr();
   p.ldd = D.size(0) > 1 ? D.stride(0) : N;
-  long d_rows = D.size(0);
   if (p.split > 1) {
     ws = at::empty({p.split * M, N}, a.options().dtype(at::kFloat));
     p.f32 = true;
     p.acc = false;
     p.D = ws.data_ptr();
     p.ldd = N;
-    d_rows = p.split * M;
   }
-  p.d_rows = static_cast<int>(d_rows);
   const int es = p.f32 ? 4 : 2;
-  p.tma_store = !p.acc && aligned16(p.D) && (p.ldd * es) % 16 == 0;
+  p.d_vec = aligned16(p.D) && (p.ldd * es) % 16 == 0;
   // fp32 accumulator, both operands K-major, UE8M0 scales; the byte of the scale words is added per block
   p.idesc = (static_cast<uint32_t>(a.scalar_type() == at::kFloat8_e5m2) << 7) |
             (static_cast<uint32_t>(b.scalar_type() == at::kFloat8_e5m2) << 10) |
             (static_cast<uint32_t>(bn >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>((BM * plan.ctas) >> 4) << 24);
 
   const long lda = a.size(0) > 1 ? a.stride(0) : (K + 15) / 16 * 16, ldb = b.size(0) > 1 ? b.stride(0) : (K + 15) / 16 * 16;
-  const CUtensorMap ta = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.data_ptr(), a.size(0), K, lda, BM);
-  const CUtensorMap tb = make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.data_ptr(), b.size(0), K, ldb, bn / plan.ctas);
-  CUtensorMap td;
-  std::memset(&td, 0, sizeof(td));
-  if (p.tma_store)
-    td = make_map(p.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, p.D, d_rows, N,
-                  p.ldd * es, 32);
+  const CUtensorMap ta = make_map(a.data_ptr(), a.size(0), K, lda, BM);
+  const CUtensorMap tb = make_map(b.data_ptr(), b.size(0), K, ldb, bn / plan.ctas);
   const int dev = a.device().index();
-  if (plan.ctas == 2) {
-    if (bn == 256) launch<256, 2>(ta, tb, td, p, tiles, dev, st);
-    else if (bn == 192) launch<192, 2>(ta, tb, td, p, tiles, dev, st);
-    else launch<128, 2>(ta, tb, td, p, tiles, dev, st);
+  if (plan.panel) {
+    if (bn == 256) launch<256, 2, true>(ta, tb, p, tiles, dev, st);
+    else if (bn == 192) launch<192, 2, true>(ta, tb, p, tiles, dev, st);
+    else launch<128, 2, true>(ta, tb, p, tiles, dev, st);
+  } else if (plan.ctas == 2) {
+    if (bn == 256) launch<256, 2, false>(ta, tb, p, tiles, dev, st);
+    else if (bn == 192) launch<192, 2, false>(ta, tb, p, tiles, dev, st);
+    else launch<128, 2, false>(ta, tb, p, tiles, dev, st);
   } else {
-    if (bn == 192) launch<192, 1>(ta, tb, td, p, tiles, dev, st);
-    else launch<128, 1>(ta, tb, td, p, tiles, dev, st);
+    if (bn == 192) launch<192, 1, false>(ta, tb, p, tiles, dev, st);
+    else launch<128, 1, false>(ta, tb, p, tiles, dev, st);
   }
   if (p.split > 1) {
     const long MN = M * N;
