@@ -64,14 +64,21 @@ SB_DEVICE uint32_t mix32(uint32_t h) {
   return h ^ (h >> 16);
 }
 
-// A magnitude y in [0, 448] to the e4m3 value below or above it: 16 random
-// bits are added below the three kept fraction bits, then cut off.  Below the
+// y in [-448, 448] to the e4m3 value next to it towards zero or away from it:
+// random bits (16, in place) are added below the three kept fraction bits, then
+// cut off; in sign and magnitude that needs no care for the sign.  Below the
 // smallest normal value 2^-6 the grid is uniform, as it is in [2^-6, 2^-5), so
 // y is moved there and back.
-SB_DEVICE float round_up_sometimes(float y, uint32_t bits16) {
-  const float shift = y < 0.015625f ? 0.015625f : 0.f;
-  const uint32_t b = (__float_as_uint(y + shift) + (bits16 << 4)) & ~0xFFFFFu;
-  return __uint_as_float(b) - shift;
+SB_DEVICE float round_up_sometimes(float y, uint32_t bits) {
+  const float shift = fabsf(y) < 0.015625f ? __uint_as_float(0x3C800000u | (__float_as_uint(y) & 0x80000000u)) : 0.f;
+  return __uint_as_float((__float_as_uint(y + shift) + bits) & ~0xFFFFFu) - shift;
+}
+
+// One-instruction root (off by at most 2^-22 relative, zero and infinity exact).
+SB_DEVICE float root(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 template <typename T>
@@ -147,12 +154,14 @@ SB_DEVICE void load_codes(const uint8_t* p, float scale, int valid, bool vec, fl
 }
 
 // Eight values of a block of 128 (16 lanes) to codes; returns the scale byte.
-SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits16, int valid, bool vec) {
+SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits, int valid, bool vec) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const float a = fabsf(f[i]);
-    top = fmaxf(top, a < INFINITY ? a : 0.f);
+  for (int i = 0; i < kVec; ++i) top = fmaxf(top, fabsf(f[i]));
+  if (top == INFINITY) {                         // infinities do not count (fmaxf passes over NaN)
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) top = fmaxf(top, fabsf(f[i]) < INFINITY ? fabsf(f[i]) : 0.f);
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -163,10 +172,8 @@ SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits16, in
   for (int i = 0; i < kVec; i += 2) {
     float y[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float x = f[i + j];
-      y[j] = fabsf(x) < INFINITY ? copysignf(round_up_sometimes(fabsf(x * inv), bits16[i + j]), x) : NAN;
-    }
+    for (int j = 0; j < 2; ++j)                  // 0 x adds nothing to a finite value and makes NaN of any other
+      y[j] = __fmaf_rn(f[i + j], 0.f, round_up_sometimes(f[i + j] * inv, bits[i + j]));
     raw[i / 4] |= fp8::pack2(y[0], y[1], fp8::kE4M3) << (16 * ((i / 2) % 2));
   }
   if (vec && valid == kVec) {
@@ -218,25 +225,24 @@ adamw_many_kernel(const __grid_constant__ Table tab, StepArgs a) {
     load8<float>(static_cast<const float*>(e.m) + i0, valid, vec, m);
     load8<float>(static_cast<const float*>(e.v) + i0, valid, vec, v);
   }
-  bool bad = false;
-  float r[kVec];
+  float bad = 0.f, r[kVec];                      // 0 g adds nothing unless g is not finite
+  const float keep = 1.f - a.lr * a.wd, rate = a.lr / a.c1, inv_c2 = 1.f / a.c2;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const float gi = g[i] * a.grad_scale;
-    bad |= !(fabsf(gi) < INFINITY);
-    w[i] *= 1.f - a.lr * a.wd;
+    bad = __fmaf_rn(gi, 0.f, bad);
     m[i] += (gi - m[i]) * a.one_minus_beta1;
     v[i] = v[i] * a.beta2 + a.one_minus_beta2 * gi * gi;
-    r[i] = sqrtf(v[i]);
-    w[i] -= (a.lr / a.c1) * (m[i] / (r[i] / a.c2 + a.eps));
+    r[i] = root(v[i]);
+    w[i] = w[i] * keep - rate * __fdividef(m[i], r[i] * inv_c2 + a.eps);
   }
   if constexpr (EIGHT) {
     uint32_t um[kVec], uv[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const uint32_t u = mix32(static_cast<uint32_t>(i0 + i) * 0x9E3779B1u + key);
-      um[i] = u & 0xFFFFu;
-      uv[i] = u >> 16;
+      um[i] = (u << 4) & 0xFFFF0u;               // in place below the kept fraction bits
+      uv[i] = (u >> 12) & 0xFFFF0u;
     }
     const int bm = store_codes(static_cast<uint8_t*>(e.m) + i0, m, um, valid, vec);
     const int bv = store_codes(static_cast<uint8_t*>(e.v) + i0, r, uv, valid, vec);
@@ -250,7 +256,7 @@ adamw_many_kernel(const __grid_constant__ Table tab, StepArgs a) {
   }
   if (e.w != nullptr) store8<float>(e.w + i0, valid, vec, w);
   store8<P>(static_cast<P*>(e.p) + i0, valid, vec, w);
-  if (bad && a.nonfinite != nullptr) atomicOr(a.nonfinite, 1);
+  if (bad != 0.f && a.nonfinite != nullptr) atomicOr(a.nonfinite, 1);
 }
 
 template <typename P, typename Gr>

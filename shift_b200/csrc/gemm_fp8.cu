@@ -47,28 +47,20 @@ constexpr int kEpiWarps = 8;
 constexpr int BM = 128;
 constexpr int BK = 128;            // one scale block, one 128-byte swizzled row
 constexpr int kMaxGroups = 512;
-constexpr int kPanelBlocks = 8;    // blocks of 128 that a panel of A holds
 constexpr int kBand = 8;           // row tiles whose column tiles are walked together
 
 // CTAS: CTAs that share a tile of 128 * CTAS rows and BN columns.  Two
 // accumulators alternate so that the epilogue of one tile runs under the next
 // one's products.  256 columns twice would leave no room for the scales, so
 // there the two share 32 columns, which the epilogue reads first.
-// PANEL: the CTA keeps its rows of A (up to 1024 bytes each) in shared memory
-// while it walks along the columns, and only B streams.  The way from L2 into
-// an SM carries about 64 bytes a clock; without a panel a tile of 256 x 192
-// moves 28 KB for 384 clocks of products, with it 12 KB.
-template <int BN, int CTAS, bool PANEL>
+template <int BN, int CTAS>
 struct Cfg {
   static constexpr int kTileM = BM * CTAS;
   static constexpr int kABytes = BM * BK;
   static constexpr int kBRows = BN / CTAS;                       // rows of B that one CTA loads
   static constexpr int kBBytes = kBRows * BK;
-  static constexpr int kPanelBytes = PANEL ? kPanelBlocks * kABytes : 0;
-  static constexpr int kBOff = PANEL ? 0 : kABytes;              // of B within a stage
-  static constexpr int kStageBytes = kBOff + kBBytes;
-  static constexpr int kChunks = PANEL ? 4 : 8;                  // 16-byte pieces of a row that a warp stages
-  static constexpr int kEpiBytes = kEpiWarps * 32 * kChunks * 16;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kEpiBytes = kEpiWarps * 4096;             // per warp a buffer of 32 rows x 128 bytes
   static constexpr int kBParts = (BN + 127) / 128;               // 128-row parts of the B scales
   static constexpr int kScaleBytes = 512 * (1 + kBParts);
   static constexpr bool kShared = BN == 256;
@@ -78,7 +70,7 @@ struct Cfg {
   static constexpr int kTmemCols = 512;
   static constexpr int kScaleCol0 = kAccCols + BN;
   static_assert(kScaleCol0 + kScaleStages * kScaleCols <= kTmemCols, "tensor memory budget");
-  static constexpr int kFixed = kPanelBytes + kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 + 2 * (kMaxGroups + 1) * 4;
+  static constexpr int kFixed = kEpiBytes + kScaleStages * kScaleBytes + 1024 + 512 + 2 * (kMaxGroups + 1) * 4;
   static constexpr int kStages = (232448 - kFixed) / kStageBytes < 8 ? (232448 - kFixed) / kStageBytes : 8;
   static constexpr int kSmemBytes = kStages * kStageBytes + kFixed;
   static_assert(kStages >= 3 && kStageBytes % 1024 == 0, "shared memory budget");
@@ -105,7 +97,7 @@ struct Args {
   int M, N, K, G, mode;
   int split;               // row mode, one group: K ranges, partial sums into D [split][M][N] fp32
   int tiles_n;
-  Divisor by_n, by_band, by_tiles;   // tiles_n; kBand * tiles_n; tiles of one group (K groups, split)
+  Divisor by_band, by_tiles;   // kBand * tiles_n; tiles of one group (K groups, split)
   const int* offs;
   void* D;
   long ldd;
@@ -355,9 +347,9 @@ SB_DEVICE void tile_blocks(const Args& p, const int* s_prefix, const int* s_offs
 }
 
 // `rank`: the CTA's place in its pair.
-template <int BN, int CTAS, bool PANEL>
+template <int BN, int CTAS>
 __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, const int* s_offs, int tile, int rank) {
-  using C = Cfg<BN, CTAS, PANEL>;
+  using C = Cfg<BN, CTAS>;
   Tile t;
   int tm, tn;
   tile_blocks(p, s_prefix, s_offs, tile, t.kb0, t.kb);
@@ -374,12 +366,7 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
       s = p.by_tiles(local);
       local -= s * p.by_tiles.d;
     }
-    if (PANEL) {                                   // along the columns, so that a panel serves many tiles
-      tm = p.by_n(local);
-      tn = local - tm * p.tiles_n;
-    } else {
-      walk(p, local, tiles_m, tm, tn);
-    }
+    walk(p, local, tiles_m, tm, tn);
     const int m = tm * C::kTileM + rank * BM;
     t.n0 = tn * BN;
     t.a_row = s_offs[lo] + m;
@@ -399,17 +386,16 @@ __device__ __forceinline__ Tile decode_tile(const Args& p, const int* s_prefix, 
   return t;
 }
 
-template <int BN, int CTAS, bool PANEL>
+template <int BN, int CTAS>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(CTAS, 1, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const Args p) {
-  using C = Cfg<BN, CTAS, PANEL>;
+  using C = Cfg<BN, CTAS>;
   constexpr int kScaleStages = C::kScaleStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* tiles = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
-  uint8_t* panel = tiles + C::kStages * C::kStageBytes;
-  uint8_t* epi = panel + C::kPanelBytes;
+  uint8_t* epi = tiles + C::kStages * C::kStageBytes;
   uint8_t* scales = epi + C::kEpiBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScaleStages * C::kScaleBytes);
   uint64_t* empty = full + C::kStages;
@@ -418,9 +404,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   uint64_t* sf_here = sf_empty + kScaleStages;
   uint64_t* acc_full = sf_here + kScaleStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* a_full = acc_empty + 2;
-  uint64_t* a_empty = a_full + kPanelBlocks;
-  uint64_t* drain = a_empty + kPanelBlocks;
+  uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* s_total = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_offs = s_total + 1;
@@ -446,10 +430,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], kEpiWarps * CTAS);
-    }
-    for (int b = 0; b < kPanelBlocks; ++b) {
-      mbar_init(&a_full[b], 1);
-      mbar_init(&a_empty[b], 1);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -484,39 +464,22 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   sync_pair<CTAS>();          // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // Tiles of this CTA (or pair): every so-and-so-many-th, or a run of neighbours, which share panels.
-  const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
-  const int first_tile = PANEL ? static_cast<int>(static_cast<long long>(*s_total) * unit / units) : unit;
-  const int total = PANEL ? static_cast<int>(static_cast<long long>(*s_total) * (unit + 1) / units) : *s_total;
-  const int tile_step = PANEL ? 1 : units;
-  const int first_n = PANEL ? first_tile - p.by_n(first_tile) * p.tiles_n : 0;   // its column tile
+  const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS, total = *s_total;
 
   if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t panel_phase = 0;
-      int tn = first_n;
       bool ok = true;
       for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-        const Tile t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
-        const bool fresh = PANEL && (tile == first_tile || tn == 0);      // a new panel
+        const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
         for (int i = 0; i < t.kb; ++i) {
-          if (PANEL && fresh) {
-            if (!mbar_wait(&a_empty[i], panel_phase ^ 1, p.status)) { ok = false; break; }
-            if (rank == 0) mbar_arrive_expect_tx(&a_full[i], C::kABytes * CTAS);
-            load_tile<CTAS>(panel + i * C::kABytes, &tmA, &a_full[i], i * BK, t.a_row);
-          }
           if (!mbar_wait(&empty[stage], phase ^ 1, p.status)) { ok = false; break; }
           uint8_t* s = tiles + stage * C::kStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], C::kStageBytes * CTAS);
-          if (!PANEL) load_tile<CTAS>(s, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
-          load_tile<CTAS>(s + C::kBOff, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row + rank * C::kBRows);
+          load_tile<CTAS>(s, &tmA, &full[stage], (t.kb0 + i) * BK, t.a_row);
+          load_tile<CTAS>(s + C::kABytes, &tmB, &full[stage], (t.kb0 + i) * BK, t.b_row + rank * C::kBRows);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
-        }
-        if (PANEL) {
-          if (fresh) panel_phase ^= 1;
-          if (++tn == p.tiles_n) tn = 0;
         }
       }
       // every stage's products have signalled here before this CTA may go: the other one's signals are remote
@@ -524,22 +487,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         ok = mbar_wait(&empty[stage], phase ^ 1, p.status);
         if (++stage == C::kStages) { stage = 0; phase ^= 1; }
       }
-      if (PANEL && first_tile < total)
-        for (int b = 0; b < (p.K + BK - 1) / BK && ok; ++b) ok = mbar_wait(&a_empty[b], panel_phase ^ 1, p.status);
       // an early end: wait (briefly) for the loads in flight, which must not land after the CTA has gone
       // (the second CTA's complete on the first one's barriers; the pair leaves together)
-      if (!ok && rank == 0) {
+      if (!ok && rank == 0)
         for (int s = 0; s < C::kStages; ++s) mbar_wait(&full[s], phase ^ (s < stage ? 0 : 1), nullptr, 200000000ull);
-        for (int b = 0; PANEL && b < kPanelBlocks; ++b)
-          for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait(&a_full[b], ph, nullptr, 100000000ull);
-      }
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
       const uint64_t desc0 = make_sw128_desc(smem_u32(tiles), 16, 1024);
-      const uint64_t panel0 = make_sw128_desc(smem_u32(panel), 16, 1024);
-      uint32_t panel_phase = 0;
-      int tn = first_n;
       int stage = 0, acc = 0, sf = 0;
       uint32_t phase = 0, acc_phase = 0, sf_phase = 0;
       uint32_t sfa = 0;
@@ -560,8 +515,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
         tc_fence_after();
         const uint32_t d = tmem + acc * C::kAccCols;
-        const bool fresh = PANEL && (tile == first_tile || tn == 0);
-        const bool leave = PANEL && (tile == total - 1 || tn == p.tiles_n - 1);   // the panel's last tile
         for (int i = 0; i < kb; ++i) {
           const uint32_t part = (kb0 + i) % 4;         // the byte of the scale words
           if (i == 0 || part == 0) {
@@ -574,17 +527,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             for (int q = 0; q < 1 + C::kBParts; ++q) tmem_copy_scales<CTAS>(sfa + 4 * q, src + 512 * q);
           }
           if (!ready && !mbar_wait(&full[stage], phase, p.status)) { ok = false; break; }
-          if (PANEL && fresh && !mbar_wait(&a_full[i], panel_phase, p.status)) { ok = false; break; }
           tc_fence_after();
           // all lies below 256 KB: adding to the address field never carries out of its 14 bits
-          const uint64_t sd = desc0 + stage * (C::kStageBytes >> 4), bd = sd + (C::kBOff >> 4);
-          const uint64_t ad = PANEL ? panel0 + i * (C::kABytes >> 4) : sd;
+          const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
           const uint32_t idesc = p.idesc | (part << 29) | (part << 4);
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
             umma_scaled<CTAS>(d, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfa + 4, (i | kk) != 0 ? 1u : 0u);
           commit<CTAS>(&empty[stage]);
-          if (PANEL && leave) commit<CTAS>(&a_empty[i]);
           if (++stage == C::kStages) { stage = 0; phase ^= 1; }
           ready = mbar_test(&full[stage], phase);      // asked early: the answer takes 100 clocks
           if (part == 3 || i == kb - 1) {
@@ -593,10 +543,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           }
         }
         if (!ok) break;
-        if (PANEL) {
-          if (fresh) panel_phase ^= 1;
-          if (++tn == p.tiles_n) tn = 0;
-        }
         commit<CTAS>(&acc_full[acc]);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
@@ -618,7 +564,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         do {
           tile += tile_step;
           if (tile >= total) return false;
-          t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
+          t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
         } while (t.kb == 0);
         w = t.kb0 / 4;
         w_end = (t.kb0 + t.kb - 1) / 4;
@@ -685,22 +631,21 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   } else if (warp >= 4) {
     const int quarter = warp % 4, half = (warp - 4) / 4;
     const int r = quarter * 32 + lane;
-    uint8_t* buf = epi + (warp - 4) * 32 * C::kChunks * 16;
+    uint8_t* buf = epi + (warp - 4) * 4096;
     int acc = 0;
     uint32_t acc_phase = 0;
     // piece j of a staged row, turned so that neither a column of pieces nor a row meets a bank twice
-    auto staged_at = [](int row, int j) { return (row * C::kChunks + (j ^ ((C::kChunks == 8 ? row : row / 2) % C::kChunks))) * 16; };
+    auto staged_at = [](int row, int j) { return (row * 8 + (j ^ (row % 8))) * 16; };
     for (int tile = first_tile; tile < total; tile += tile_step) {
-      const Tile t = decode_tile<BN, CTAS, PANEL>(p, s_prefix, s_offs, tile, rank);
+      const Tile t = decode_tile<BN, CTAS>(p, s_prefix, s_offs, tile, rank);
       if (!mbar_wait(&acc_full[acc], acc_phase, p.status)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * C::kAccCols + ((quarter * 32) << 16);
       const int cols = min(BN, p.N - t.n0);
-      // A warp's 32 rows of 128 (64) bytes go through shared memory, so that each global store covers whole runs of
-      // rows: 64 (32) columns that leave as bf16, half as many that leave as fp32 or are added to what D holds.
+      // A warp's 32 rows of 128 bytes go through shared memory, so that each global store covers whole runs of
+      // rows: 64 columns that leave as bf16, or 32 that leave as fp32 or are added to what D holds.
       const bool wide = p.f32 || p.acc;
-      constexpr int kChunks = C::kChunks;
-      const int step = wide ? 4 * kChunks : 8 * kChunks;
+      const int step = wide ? 32 : 64;
       const int n = (cols + step - 1) / step;
       if (half >= n && lane == 0) arrive_leader_relaxed<CTAS>(&acc_empty[acc]);    // nothing for this warp to read
       const int rows_here = min(32, t.m_valid - quarter * 32);
@@ -709,15 +654,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       for (int i = half; i < n; i += 2) {
         // shared columns first: the last of the first accumulator, the first of the second
         const int s = C::kShared && acc == 0 ? n - 1 - i : i;
-        uint32_t v[8 * kChunks];
+        uint32_t v[64];
         __syncwarp();                                  // the buffer has been read, the warp is whole
-        if constexpr (kChunks == 8) {
-          tmem_ld_32x32b_x32(src + s * step, v);
-          if (!wide) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
-        } else {
-          tmem_ld_32x32b_x16(src + s * step, v);
-          if (!wide) tmem_ld_32x32b_x16(src + s * step + 16, v + 16);
-        }
+        tmem_ld_32x32b_x32(src + s * step, v);
+        if (!wide) tmem_ld_32x32b_x32(src + s * step + 32, v + 32);
         tmem_wait_ld();
         if (C::kShared ? i < 2 : i + 2 >= n) {
           tc_fence_before();
@@ -727,10 +667,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         if (rows_here <= 0) continue;
         if (t.kb == 0) {
 #pragma unroll
-          for (int j = 0; j < 8 * kChunks; ++j) v[j] = 0u;      // nothing was contracted: zeros
+          for (int j = 0; j < 64; ++j) v[j] = 0u;      // nothing was contracted: zeros
         }
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
+        for (int j = 0; j < 8; ++j) {
           uint4 w = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           if (!wide) {
             const bf16x8 h = float_to_bf16x8(reinterpret_cast<const float*>(v) + 8 * j);
@@ -739,21 +679,21 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           *reinterpret_cast<uint4*>(buf + staged_at(lane, j)) = w;
         }
         __syncwarp();
-        const int r0 = lane / kChunks, j = lane % kChunks, per = wide ? 4 : 8, c = s * step + j * per;
+        const int r0 = lane / 8, j = lane % 8, per = wide ? 4 : 8, c = s * step + j * per;
         const int here = min(per, cols - c);           // of this lane's 16 bytes
         if (p.d_vec && here == per && !p.acc) {
           uint8_t* d = out + (r0 * p.ldd + c) * (p.f32 ? 4 : 2);
-          const long jump = 32 / kChunks * p.ldd * (p.f32 ? 4 : 2);
+          const long jump = 4 * p.ldd * (p.f32 ? 4 : 2);
 #pragma unroll
-          for (int q = 0; q < kChunks; ++q) {
-            const int row = q * (32 / kChunks) + r0;
+          for (int q = 0; q < 8; ++q) {
+            const int row = q * 4 + r0;
             const uint4 w = *reinterpret_cast<const uint4*>(buf + staged_at(row, j));
             if (row < rows_here) *reinterpret_cast<uint4*>(d) = w;
             d += jump;
           }
         } else if (here > 0) {
 #pragma unroll 1
-          for (int row = r0; row < rows_here; row += 32 / kChunks)
+          for (int row = r0; row < rows_here; row += 4)
             store_some(p, buf + staged_at(row, j), out, row * p.ldd + c, here);
         }
       }
@@ -769,22 +709,35 @@ matmul_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 }
 
 // Sum of the partial products of a split contraction, in the order of the
-// ranges, into D with the requested type and accumulation.
-__global__ void split_sum_kernel(const float* __restrict__ ws, int S, int M, int N, bool f32, bool acc, void* D,
-                                 long ldd) {
-  const long MN = static_cast<long>(M) * N;
-  for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < MN;
-       i += static_cast<long>(gridDim.x) * blockDim.x) {
-    float v = ws[i];
-    for (int s = 1; s < S; ++s) v += ws[s * MN + i];
-    const long m = i / N, at = m * ldd + (i - m * N);
-    if (f32) {
-      float* d = static_cast<float*>(D) + at;
-      *d = acc ? *d + v : v;
-    } else {
-      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(D) + at;
-      *d = __float2bfloat16(acc ? __bfloat162float(*d) + v : v);
+// ranges, into D with the requested type and accumulation; four columns a
+// thread (ranges of ws are rows of N rounded up to 4).
+__global__ void split_sum_kernel(const float* __restrict__ ws, int S, int M, int N, Divisor by_quads, bool f32, bool acc,
+                                 bool vec, void* D, long ldd) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int m = by_quads(i), c = (i - m * static_cast<int>(by_quads.d)) * 4;
+  if (m >= M) return;
+  const long range = static_cast<long>(M) * by_quads.d;
+  const float4* src = reinterpret_cast<const float4*>(ws) + i;
+  float4 v = src[0];
+#pragma unroll 4
+  for (int s = 1; s < S; ++s) {
+    const float4 w = src[s * range];
+    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  const long at = m * ldd + c;
+  if (f32) {
+    float* d = static_cast<float*>(D) + at;
+    if (vec) {
+      const float4 o = acc ? *reinterpret_cast<const float4*>(d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(d) = make_float4(f[0] + o.x, f[1] + o.y, f[2] + o.z, f[3] + o.w);
+      return;
     }
+    for (int j = 0; j < 4 && c + j < N; ++j) d[j] = acc ? d[j] + f[j] : f[j];
+  } else {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(D) + at;
+    for (int j = 0; j < 4 && c + j < N; ++j)
+      d[j] = __float2bfloat16(acc ? __bfloat162float(d[j]) + f[j] : f[j]);
   }
 }
 
@@ -830,11 +783,11 @@ static int num_sms(int device) {
   return v;
 }
 
-template <int BN, int CTAS, bool PANEL>
+template <int BN, int CTAS>
 static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& p, long tiles,
                    int device, cudaStream_t st) {
-  using C = Cfg<BN, CTAS, PANEL>;
-  auto kern = matmul_kernel<BN, CTAS, PANEL>;
+  using C = Cfg<BN, CTAS>;
+  auto kern = matmul_kernel<BN, CTAS>;
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
   const int grid = static_cast<int>(std::min<long>(num_sms(device) / CTAS, std::max<long>(1, tiles))) * CTAS;
   kern<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, p);
@@ -843,26 +796,34 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& p, 
 
 struct Plan {
   int ctas, bn, split;
-  bool panel;
   long tiles;            // upper bound for the grid
 };
 
+// Up to 128 rows take one CTA per tile (a pair would compute 128 rows of
+// nothing: 1 x 32768 x 1024 in 13 us against 20), more a pair.  The width is
+// the one with the least columns walked by the busiest CTA or pair, with 64
+// added per tile for what a tile costs whatever its width.  128 columns count
+// as 176: per block they bring 24 KB into an SM for 256 clocks of products,
+// where 64 bytes a clock arrive.  Measured, 192 against 256 columns: 16384 x
+// 1536 x 1024 27.6 and 29.1 us, 16384 x 1024 x 1024 23.4 and 21.9 us.
 static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, int sms) {
   Plan p;
   const long blocks = (K + BK - 1) / BK;
   p.ctas = M > BM ? 2 : 1;
-  if (const char* e = getenv("SB_FP8_CTAS")) p.ctas = atoi(e);
-  p.bn = N % 192 != 0 && (N % 128 == 0 || N <= 128) ? 128 : 192;
-  if (p.ctas == 2 && N % 256 == 0) p.bn = 256;
-  if (const char* e = getenv("SB_FP8_BN")) p.bn = atoi(e);
-  const long tm = (M + BM * p.ctas - 1) / (BM * p.ctas), tn = (N + p.bn - 1) / p.bn;
-  p.tiles = mode == kRowGroups ? (tm + (offs ? G : 0)) * tn : G * tm * tn;
-  p.panel = p.ctas == 2 && mode == kRowGroups && blocks <= kPanelBlocks && tn > 1;
-  if (const char* e = getenv("SB_FP8_PANEL")) p.panel = p.panel && atoi(e);
+  const long slots = sms / p.ctas, tm = (M + BM * p.ctas - 1) / (BM * p.ctas);
+  long best = -1;
+  for (int bn : {256, 192, 128}) {
+    if (bn == 256 && p.ctas == 1) continue;
+    const long tn = (N + bn - 1) / bn, tiles = mode == kRowGroups ? tm * tn : G * tm * tn;
+    const long cost = (tiles + slots - 1) / slots * ((bn == 128 ? 176 : bn) + 64);
+    if (best >= 0 && cost >= best) continue;
+    best = cost;
+    p.bn = bn;
+    p.tiles = mode == kRowGroups ? (tm + (offs ? G : 0)) * tn : tiles;
+  }
+  // few tiles over a long contraction: ranges of at least four blocks to the CTAs that would have none
   p.split = 1;
-  const long slots = sms / p.ctas;
   if (!offs && p.tiles * 2 <= slots && blocks >= 8) {
-    p.panel = false;
     p.split = static_cast<int>(std::min<long>(slots / p.tiles, blocks / 4));
     p.tiles *= p.split;
   }
@@ -909,22 +870,22 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   const long tiles = plan.tiles;
   p.split = plan.split;
   p.tiles_n = static_cast<int>((N + bn - 1) / bn);
-  p.by_n.set(p.tiles_n);
   p.by_band.set(kBand * p.tiles_n);
   p.by_tiles.set(static_cast<unsigned>((M + BM * plan.ctas - 1) / (BM * plan.ctas) * p.tiles_n));
 
   at::Tensor ws;
+  const long quads = (N + 3) / 4;
   const bool f32 = D.scalar_type() == at::kFloat;
   p.f32 = f32;
   p.acc = accumulate;
   p.D = D.data_ptr();
   p.ldd = D.size(0) > 1 ? D.stride(0) : N;
   if (p.split > 1) {
-    ws = at::empty({p.split * M, N}, a.options().dtype(at::kFloat));
+    ws = at::empty({p.split * M, quads * 4}, a.options().dtype(at::kFloat));
     p.f32 = true;
     p.acc = false;
     p.D = ws.data_ptr();
-    p.ldd = N;
+    p.ldd = quads * 4;
   }
   const int es = p.f32 ? 4 : 2;
   p.d_vec = aligned16(p.D) && (p.ldd * es) % 16 == 0;
@@ -937,22 +898,22 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
   const CUtensorMap ta = make_map(a.data_ptr(), a.size(0), K, lda, BM);
   const CUtensorMap tb = make_map(b.data_ptr(), b.size(0), K, ldb, bn / plan.ctas);
   const int dev = a.device().index();
-  if (plan.panel) {
-    if (bn == 256) launch<256, 2, true>(ta, tb, p, tiles, dev, st);
-    else if (bn == 192) launch<192, 2, true>(ta, tb, p, tiles, dev, st);
-    else launch<128, 2, true>(ta, tb, p, tiles, dev, st);
-  } else if (plan.ctas == 2) {
-    if (bn == 256) launch<256, 2, false>(ta, tb, p, tiles, dev, st);
-    else if (bn == 192) launch<192, 2, false>(ta, tb, p, tiles, dev, st);
-    else launch<128, 2, false>(ta, tb, p, tiles, dev, st);
+  if (plan.ctas == 2) {
+    if (bn == 256) launch<256, 2>(ta, tb, p, tiles, dev, st);
+    else if (bn == 192) launch<192, 2>(ta, tb, p, tiles, dev, st);
+    else launch<128, 2>(ta, tb, p, tiles, dev, st);
   } else {
-    if (bn == 192) launch<192, 1, false>(ta, tb, p, tiles, dev, st);
-    else launch<128, 1, false>(ta, tb, p, tiles, dev, st);
+    if (bn == 192) launch<192, 1>(ta, tb, p, tiles, dev, st);
+    else launch<128, 1>(ta, tb, p, tiles, dev, st);
   }
   if (p.split > 1) {
-    const long MN = M * N;
-    split_sum_kernel<<<static_cast<unsigned>(std::min<long>((MN + 255) / 256, 148 * 8)), 256, 0, st>>>(
-        ws.data_ptr<float>(), p.split, p.M, p.N, f32, accumulate, D.data_ptr(), D.size(0) > 1 ? D.stride(0) : N);
+    const long n = M * quads, ldd = D.size(0) > 1 ? D.stride(0) : N;
+    TORCH_CHECK(n < (1l << 31) - 256, "fp8 matmul: too large to split");
+    Divisor by_quads;
+    by_quads.set(static_cast<unsigned>(quads));
+    const bool vec = N % 4 == 0 && aligned16(D.data_ptr()) && ldd % 4 == 0;
+    split_sum_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, st>>>(
+        ws.data_ptr<float>(), p.split, p.M, p.N, by_quads, f32, accumulate, vec, D.data_ptr(), ldd);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
 }

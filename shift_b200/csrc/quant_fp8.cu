@@ -38,6 +38,15 @@ SB_DEVICE float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;      // false for NaN too
 }
 
+// The conversion saturates: an infinity becomes NaN in e4m3, which has none, and stays one in e5m2.
+template <int FMT>
+SB_DEVICE uint32_t patch_infinities(uint32_t w, const float* y) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (isinf(y[j])) w = (w & ~(0xFFu << (8 * j))) | ((FMT == kE4M3 ? 0x7Fu : (y[j] > 0 ? 0x7Cu : 0xFCu)) << (8 * j));
+  return w;
+}
+
 struct QuantArgs {
   const void* x;
   uint8_t *q, *s, *qt, *st;
@@ -86,7 +95,8 @@ quantize_kernel(const QuantArgs a) {
     }
   }
 
-  float rmax[8], cmax[8];
+  // fmaxf passes over NaN; a maximum of infinity sends the thread through its values once more without them
+  float rmax[8], cmax[8], top = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
 #pragma unroll
@@ -94,9 +104,25 @@ quantize_kernel(const QuantArgs a) {
     rmax[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float f = finite_abs(to_f<T>(v[i].v[j]));
+      const float f = fabsf(to_f<T>(v[i].v[j]));
       rmax[i] = fmaxf(rmax[i], f);
       if (BOTH && !TILES) cmax[j] = fmaxf(cmax[j], f);
+    }
+    top = fmaxf(top, rmax[i]);
+  }
+  const bool infinite = top == INFINITY;
+  if (infinite) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      rmax[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = finite_abs(to_f<T>(v[i].v[j]));
+        rmax[i] = fmaxf(rmax[i], f);
+        if (BOTH && !TILES) cmax[j] = fmaxf(cmax[j], f);
+      }
     }
   }
   float rinv[8];
@@ -138,9 +164,7 @@ quantize_kernel(const QuantArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = to_f<T>(v[i].v[4 * h + j]) * rinv[i];
       w[h] = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (isinf(y[j])) w[h] = (w[h] & ~(0xFFu << (8 * j))) | ((FMT == kE4M3 ? 0x7Fu : (y[j] > 0 ? 0x7Cu : 0xFCu)) << (8 * j));
+      if (infinite) w[h] = patch_infinities<FMT>(w[h], y);
     }
     if (r < a.rows && c0 < a.cols)
       *reinterpret_cast<uint2*>(a.q + (g * a.rows + r) * a.ldq + c0) = make_uint2(w[0], w[1]);
@@ -198,9 +222,7 @@ quantize_kernel(const QuantArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = to_f<T>(v[4 * h + i].v[j]) * cinv[j];
         w[h] = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (isinf(y[i])) w[h] = (w[h] & ~(0xFFu << (8 * i))) | ((FMT == kE4M3 ? 0x7Fu : (y[i] > 0 ? 0x7Cu : 0xFCu)) << (8 * i));
+        if (infinite) w[h] = patch_infinities<FMT>(w[h], y);
       }
       s_t[(cg * 8 + j) * 16 + (rg ^ cg)] = static_cast<uint64_t>(w[1]) << 32 | w[0];
     }
