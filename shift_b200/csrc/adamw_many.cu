@@ -21,7 +21,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <utility>
 
 #include "fp8.cuh"
 
@@ -267,17 +270,50 @@ static void launch_many(const Table& t, const StepArgs& a, bool eight, cudaStrea
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// Lists of equal length; w, ms and vs may be empty.  All tensors contiguous,
-// on one device; parameters of one type, gradients of one type.
-void adamw_many(const std::vector<at::Tensor>& p, const std::vector<at::Tensor>& w, const std::vector<at::Tensor>& g,
-                const std::vector<at::Tensor>& m, const std::vector<at::Tensor>& ms, const std::vector<at::Tensor>& v,
-                const std::vector<at::Tensor>& vs, const std::vector<int64_t>& numbers, double lr, double beta1,
-                double beta2, double eps, double wd, int64_t step, double grad_scale, int64_t seed,
-                const c10::optional<at::Tensor>& step_dev, const c10::optional<at::Tensor>& skip,
-                const c10::optional<at::Tensor>& nonfinite) {
-  if (p.empty()) return;
-  const at::cuda::CUDAGuard guard(p[0].device());
-  const bool eight = !ms.empty();
+template <typename P>
+static void launch_types(at::ScalarType g, const Table& t, const StepArgs& a, bool eight, cudaStream_t st) {
+  if (g == at::kFloat) launch_many<P, float>(t, a, eight, st);
+  else if (g == at::kBFloat16) launch_many<P, __nv_bfloat16>(t, a, eight, st);
+  else launch_many<P, __half>(t, a, eight, st);
+}
+
+// The tensors of an optimizer, checked once; kept by its Python object.  w, ms
+// and vs may be empty.  Addresses are read from the tensors at every step.
+struct Many {
+  std::vector<at::Tensor> p, w, m, ms, v, vs;
+};
+
+std::shared_ptr<Many> adamw_many_plan(std::vector<at::Tensor> p, std::vector<at::Tensor> w, std::vector<at::Tensor> m,
+                                      std::vector<at::Tensor> ms, std::vector<at::Tensor> v,
+                                      std::vector<at::Tensor> vs) {
+  return std::make_shared<Many>(Many{std::move(p), std::move(w), std::move(m), std::move(ms), std::move(v), std::move(vs)});
+}
+
+void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, double beta1, double beta2, double eps,
+                double wd, int64_t step, double grad_scale, int64_t seed, const c10::optional<at::Tensor>& step_dev,
+                const c10::optional<at::Tensor>& skip, const c10::optional<at::Tensor>& nonfinite) {
+  TORCH_CHECK_VALUE(g.size() == t.p.size(), "AdamWMany: ", g.size(), " gradients for ", t.p.size(), " parameters");
+  if (g.empty()) return;
+  const auto dev = t.p[0].device();
+  const bool eight = !t.ms.empty();
+  auto is_float = [](at::ScalarType x) { return x == at::kFloat || x == at::kBFloat16 || x == at::kHalf; };
+  for (size_t i = 0; i < g.size(); ++i) {
+    const long n = t.p[i].numel();
+    TORCH_CHECK_VALUE(is_float(g[i].scalar_type()) && g[i].numel() == n && g[i].is_contiguous() && g[i].device() == dev,
+                      "AdamWMany: gradient ", i, ": contiguous, ", n, " elements, fp32 / bf16 / fp16, on ", dev);
+    // a tensor can be given other memory (.data, resize_) after the check at construction
+    TORCH_CHECK_VALUE(t.p[i].is_contiguous() && t.m[i].numel() == n && t.v[i].numel() == n && t.p[i].device() == dev &&
+                          (t.w.empty() || t.w[i].numel() == n) &&
+                          (!eight || (t.ms[i].numel() == (n + 127) / 128 && t.vs[i].numel() == (n + 127) / 128)),
+                      "AdamWMany: tensor ", i, " has changed its size or place");
+  }
+  const std::pair<const char*, const c10::optional<at::Tensor>*> words[] = {
+      {"step_dev", &step_dev}, {"skip", &skip}, {"nonfinite", &nonfinite}};
+  for (const auto& [name, x] : words)
+    TORCH_CHECK_VALUE(!x->has_value() || ((*x)->scalar_type() == at::kInt && (*x)->is_contiguous() && (*x)->device() == dev &&
+                                          (*x)->numel() >= (x == &step_dev ? 4 : 1)),
+                      "AdamWMany: ", name, ": int32 on ", dev);
+  const at::cuda::CUDAGuard guard(dev);
   StepArgs a;
   a.lr = static_cast<float>(lr);
   a.beta2 = static_cast<float>(beta2);
@@ -292,51 +328,60 @@ void adamw_many(const std::vector<at::Tensor>& p, const std::vector<at::Tensor>&
   a.sdev = step_dev.has_value() ? step_dev->data_ptr<int>() : nullptr;
   a.skip = skip.has_value() ? skip->data_ptr<int>() : nullptr;
   a.nonfinite = nonfinite.has_value() ? nonfinite->data_ptr<int>() : nullptr;
-  const auto pt = p[0].scalar_type(), gt = g[0].scalar_type();
   auto st = at::cuda::getCurrentCUDAStream();
+  // one table after another for each pair of parameter and gradient types that occurs
+  std::vector<std::pair<at::ScalarType, at::ScalarType>> kinds;
+  for (size_t i = 0; i < g.size(); ++i) {
+    const auto k = std::make_pair(t.p[i].scalar_type(), g[i].scalar_type());
+    if (std::find(kinds.begin(), kinds.end(), k) == kinds.end()) kinds.push_back(k);
+  }
   Table tab;
-  tab.count = 0;
-  uint64_t chunks = 0;
-  auto flush = [&] {
-    if (tab.count == 0) return;
-#define SB_ADAM(PT, P)                                                                \
-  if (pt == PT) {                                                                     \
-    if (gt == at::kFloat) launch_many<P, float>(tab, a, eight, st);                   \
-    else if (gt == at::kBFloat16) launch_many<P, __nv_bfloat16>(tab, a, eight, st);   \
-    else launch_many<P, __half>(tab, a, eight, st);                                   \
-  }
-    SB_ADAM(at::kFloat, float)
-    SB_ADAM(at::kBFloat16, __nv_bfloat16)
-    SB_ADAM(at::kHalf, __half)
-#undef SB_ADAM
+  for (const auto& [pt, gt] : kinds) {
     tab.count = 0;
-    chunks = 0;
-  };
-  for (size_t t = 0; t < p.size(); ++t) {
-    const long n = p[t].numel();
-    if (n == 0) continue;
-    const uint64_t add = (static_cast<uint64_t>(n) + kChunk - 1) / kChunk;
-    TORCH_CHECK(add < (1ull << 31), "adamw_many: a tensor is too long");
-    if (tab.count == kMaxTensors || chunks + add >= (1ull << 31)) flush();
-    Entry& e = tab.e[tab.count];
-    e.p = p[t].data_ptr();
-    e.w = w.empty() ? nullptr : w[t].data_ptr<float>();
-    e.g = g[t].data_ptr();
-    e.m = m[t].data_ptr();
-    e.v = v[t].data_ptr();
-    e.ms = eight ? static_cast<uint8_t*>(ms[t].data_ptr()) : nullptr;
-    e.vs = eight ? static_cast<uint8_t*>(vs[t].data_ptr()) : nullptr;
-    e.n = n;
-    const uintptr_t all = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.w) |
-                          reinterpret_cast<uintptr_t>(e.g) | reinterpret_cast<uintptr_t>(e.m) |
-                          reinterpret_cast<uintptr_t>(e.v);
-    chunks += add;
-    tab.end[tab.count] = static_cast<uint32_t>(chunks);
-    tab.number[tab.count] = static_cast<uint16_t>((numbers[t] & 0x7FFF) | ((all & 15) == 0 ? 0x8000 : 0));
-    ++tab.count;
+    uint64_t chunks = 0;
+    auto flush = [&] {
+      if (tab.count == 0) return;
+      if (pt == at::kFloat) launch_types<float>(gt, tab, a, eight, st);
+      else if (pt == at::kBFloat16) launch_types<__nv_bfloat16>(gt, tab, a, eight, st);
+      else launch_types<__half>(gt, tab, a, eight, st);
+      tab.count = 0;
+      chunks = 0;
+    };
+    for (size_t i = 0; i < g.size(); ++i) {
+      const long n = t.p[i].numel();
+      if (n == 0 || t.p[i].scalar_type() != pt || g[i].scalar_type() != gt) continue;
+      const uint64_t add = (static_cast<uint64_t>(n) + kChunk - 1) / kChunk;
+      TORCH_CHECK(add < (1ull << 31), "AdamWMany: a tensor is too long");
+      if (tab.count == kMaxTensors || chunks + add >= (1ull << 31)) flush();
+      Entry& e = tab.e[tab.count];
+      e.p = t.p[i].data_ptr();
+      e.w = t.w.empty() ? nullptr : t.w[i].data_ptr<float>();
+      e.g = g[i].data_ptr();
+      e.m = t.m[i].data_ptr();
+      e.v = t.v[i].data_ptr();
+      e.ms = eight ? static_cast<uint8_t*>(t.ms[i].data_ptr()) : nullptr;
+      e.vs = eight ? static_cast<uint8_t*>(t.vs[i].data_ptr()) : nullptr;
+      e.n = n;
+      const uintptr_t all = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.w) |
+                            reinterpret_cast<uintptr_t>(e.g) | reinterpret_cast<uintptr_t>(e.m) |
+                            reinterpret_cast<uintptr_t>(e.v);
+      chunks += add;
+      tab.end[tab.count] = static_cast<uint32_t>(chunks);
+      tab.number[tab.count] = static_cast<uint16_t>((i & 0x7FFF) | ((all & 15) == 0 ? 0x8000 : 0));
+      ++tab.count;
+    }
+    flush();
   }
-  flush();
+  for (const auto& x : t.p) x.unsafeGetTensorImpl()->bump_version();   // as any write in place: autograd notices
 }
 
 }  // namespace adam
 }  // namespace sb
+
+// called by bindings.cpp, which has no other reason to know the plan's type
+void bind_adamw_many(pybind11::module& m) {
+  namespace py = pybind11;
+  py::class_<sb::adam::Many, std::shared_ptr<sb::adam::Many>>(m, "AdamWManyPlan");
+  m.def("adamw_many_plan", &sb::adam::adamw_many_plan);
+  m.def("adamw_many", &sb::adam::adamw_many, "AdamW over many tensors, moments in fp32 or 8 bits");
+}

@@ -50,19 +50,11 @@ void adamw_step(const at::Tensor& master, const at::Tensor& m, const at::Tensor&
                 const c10::optional<at::Tensor>& nonfinite, const c10::optional<at::Tensor>& step_dev);
 void nonfinite_check(const at::Tensor& x, at::Tensor& flag);
 }  // namespace adam
-namespace adam {
-void adamw_many(const std::vector<at::Tensor>& p, const std::vector<at::Tensor>& w, const std::vector<at::Tensor>& g,
-                const std::vector<at::Tensor>& m, const std::vector<at::Tensor>& ms, const std::vector<at::Tensor>& v,
-                const std::vector<at::Tensor>& vs, const std::vector<int64_t>& numbers, double lr, double beta1,
-                double beta2, double eps, double wd, int64_t step, double grad_scale, int64_t seed,
-                const c10::optional<at::Tensor>& step_dev, const c10::optional<at::Tensor>& skip,
-                const c10::optional<at::Tensor>& nonfinite);
-}  // namespace adam
 namespace fp8 {
 std::vector<at::Tensor> quantize(const at::Tensor& x, int64_t fmt, bool tiles, bool both);
-void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, at::Tensor& D,
-            const c10::optional<at::Tensor>& offs, int64_t M, int64_t N, int64_t K, int64_t G, int64_t mode,
-            bool accumulate, const at::Tensor& status);
+at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at::Tensor& b, const at::Tensor& sb,
+                  int64_t Kb, const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& offs, int64_t mode,
+                  bool accumulate, bool make_f32, const at::Tensor& status);
 }  // namespace fp8
 namespace fa {
 std::vector<at::Tensor> fwd(const at::Tensor& qkv, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, double scale,
@@ -94,6 +86,8 @@ namespace digest {
 at::Tensor sha256_leaves(const at::Tensor& t, int64_t leaf, const at::Tensor& consts);
 }  // namespace digest
 }  // namespace sb
+
+void bind_adamw_many(pybind11::module& m);   // adamw_many.cu
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "shift_b200 sm_100a kernels";
@@ -133,7 +127,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("beta2"), py::arg("eps"), py::arg("wd"), py::arg("step"), py::arg("grad_scale"),
         py::arg("nonfinite") = py::none(), py::arg("step_dev") = py::none());
   m.def("nonfinite_check", &sb::adam::nonfinite_check);
-  m.def("adamw_many", &sb::adam::adamw_many, "AdamW over many tensors, moments in fp32 or 8 bits");
+  bind_adamw_many(m);
   m.def("fp8_quantize", &sb::fp8::quantize, "block quantiser to 8-bit floating point");
   m.def("fp8_matmul", &sb::fp8::matmul, "product of 8-bit matrices with block scales (dense / grouped)");
   m.def("attn_fwd", &sb::fa::fwd, "tcgen05 causal flash attention forward");

@@ -33,6 +33,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "fp8.cuh"
@@ -788,7 +789,12 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& p, 
                    int device, cudaStream_t st) {
   using C = Cfg<BN, CTAS>;
   auto kern = matmul_kernel<BN, CTAS>;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+  static std::atomic<uint64_t> ready{0};          // devices that know the kernel's shared memory size
+  const uint64_t bit = 1ull << (device & 63);
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int grid = static_cast<int>(std::min<long>(num_sms(device) / CTAS, std::max<long>(1, tiles))) * CTAS;
   kern<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -830,22 +836,62 @@ static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, i
   return p;
 }
 
-// a, b: codes [rows, ld] with scales [words, rows, 4]; D [rows, N] (row mode)
-// or [G * M, N] (K mode), bf16 or fp32, inner stride 1.
-void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, at::Tensor& D,
-            const c10::optional<at::Tensor>& offs, int64_t M, int64_t N, int64_t K, int64_t G, int64_t mode,
-            bool accumulate, const at::Tensor& status) {
+static void check_operand(const at::Tensor& q, const at::Tensor& scale, int64_t cols) {
+  const auto t = q.scalar_type();
+  TORCH_CHECK_VALUE(q.dim() == 2 && (t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2),
+                    "fp8 product: codes are a matrix of float8_e4m3fn or float8_e5m2, got ", t);
+  TORCH_CHECK_VALUE(cols >= 0 && q.size(1) >= cols, "fp8 product: ", q.size(1), " columns of codes, ", cols, " are said");
+  TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat8_e8m0fnu && scale.is_contiguous() && scale.dim() == 3 &&
+                        scale.size(0) == (cols + 511) / 512 && scale.size(1) == q.size(0) && scale.size(2) == 4,
+                    "fp8 product: scales [", (cols + 511) / 512, ", ", q.size(0),
+                    ", 4] of float8_e8m0fnu, contiguous, got ", scale.sizes(), " of ", scale.scalar_type());
+  TORCH_CHECK_VALUE(scale.device() == q.device() && q.is_cuda(), "fp8 product: codes and scales on one CUDA device");
+}
+
+// a, b: codes [rows, ld] with scales [words, rows, 4] and `K` columns each.
+// Without offs: out [a.rows, b.rows].  With offs [G + 1]: mode 0 (row groups)
+// out [a.rows, b.rows / G], mode 1 (K groups) out [G, a.rows, b.rows].  An out
+// that is not given is made, in fp32 or bf16.
+at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at::Tensor& b, const at::Tensor& sb,
+                  int64_t Kb, const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& offs, int64_t mode,
+                  bool accumulate, bool make_f32, const at::Tensor& status) {
+  check_operand(a, sa, K);
+  check_operand(b, sb, Kb);
+  TORCH_CHECK_VALUE(K == Kb, "fp8 product: the operands contract ", K, " and ", Kb, " values");
+  TORCH_CHECK_VALUE(a.device() == b.device(), "fp8 product: operands on ", a.device(), " and ", b.device());
+  int64_t G = 1;
+  if (offs.has_value()) {
+    TORCH_CHECK_VALUE(offs->dim() == 1 && offs->numel() >= 2 && offs->scalar_type() == at::kInt && offs->is_contiguous() &&
+                          offs->device() == a.device(),
+                      "fp8 product: offs are int32 [groups + 1] on the operands' device");
+    G = offs->numel() - 1;
+    TORCH_CHECK_VALUE(mode == kKGroups || b.size(0) % G == 0, "fp8 product: ", b.size(0), " rows of b for ", G, " groups");
+  }
+  const int64_t M = a.size(0), N = mode == kRowGroups ? b.size(0) / G : b.size(0);
+  TORCH_CHECK_VALUE(out.has_value() || !accumulate, "fp8 product: accumulate needs out");
   const at::cuda::CUDAGuard guard(a.device());
+  at::Tensor result = out.has_value() ? *out : at::empty({M, N}, a.options().dtype(make_f32 ? at::kFloat : at::kBFloat16));
+  if (mode == kKGroups) {
+    TORCH_CHECK_VALUE(result.dim() == 3 && result.size(0) == G && result.size(1) == M && result.size(2) == N &&
+                          result.is_contiguous(),
+                      "fp8 product: out ", result.sizes(), ", expected [", G, ", ", M, ", ", N, "], contiguous");
+  } else {
+    TORCH_CHECK_VALUE(result.dim() == 2 && result.size(0) == M && result.size(1) == N && (N <= 1 || result.stride(1) == 1),
+                      "fp8 product: out ", result.sizes(), ", expected [", M, ", ", N, "] with inner stride 1");
+  }
+  TORCH_CHECK_VALUE(result.scalar_type() == at::kFloat || result.scalar_type() == at::kBFloat16,
+                    "fp8 product: out in bf16 or fp32, got ", result.scalar_type());
+  TORCH_CHECK_VALUE(result.device() == a.device(), "fp8 product: out on ", result.device(), ", operands on ", a.device());
+  const at::Tensor D = mode == kKGroups ? result.view({G * M, N}) : result;
   TORCH_CHECK(M < (1l << 31) - 256 && N < (1l << 31) - 256 && K < (1l << 31) - 256 && G * M < (1l << 31) - 256 &&
                   b.size(0) < (1l << 31) - 256,
               "fp8 matmul: a side is too long");
   TORCH_CHECK(G >= 1 && G <= kMaxGroups, "fp8 matmul: 1 to ", kMaxGroups, " groups");
-  if (M == 0 || N == 0) return;
+  if (M == 0 || N == 0) return result;
   if (K == 0) {
-    if (!accumulate && !offs.has_value()) D.zero_();
-    else if (!accumulate && mode == kKGroups) D.zero_();
-    else TORCH_CHECK(accumulate, "fp8 matmul: nothing to contract");
-    return;
+    TORCH_CHECK_VALUE(!offs.has_value() || mode == kKGroups, "fp8 product: nothing to contract");
+    if (!accumulate) D.zero_();
+    return result;
   }
   for (const auto* t : {&a, &b})
     TORCH_CHECK(t->stride(1) == 1 && aligned16(t->data_ptr()) && (t->size(0) == 1 || t->stride(0) % 16 == 0),
@@ -916,6 +962,7 @@ void matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, cons
         ws.data_ptr<float>(), p.split, p.M, p.N, by_quads, f32, accumulate, vec, D.data_ptr(), ldd);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
+  return result;
 }
 
 }  // namespace fp8

@@ -252,30 +252,29 @@ static void launch_quant(const QuantArgs& a, bool tiles, bool both, long blocks,
 
 // x [rows, cols] or [groups, rows, cols], inner stride 1.  Returns
 // (codes, scales) or (codes, scales, codes of the transpose, its scales);
-// codes uint8 [groups * rows, round_up(cols, 16)], scales uint8 [words, rows, 4].
+// codes [groups * rows, round_up(cols, 16)], scales [words, rows, 4].
 std::vector<at::Tensor> quantize(const at::Tensor& x, int64_t fmt, bool tiles, bool both) {
   TORCH_CHECK(x.is_cuda(), "quantize: CUDA tensor required");
-  TORCH_CHECK(x.dim() == 2 || x.dim() == 3, "quantize: a matrix, or a batch of matrices, is required");
-  TORCH_CHECK(fmt == kE4M3 || fmt == kE5M2, "quantize: unknown 8-bit type");
   const at::cuda::CUDAGuard guard(x.device());
   const long groups = x.dim() == 3 ? x.size(0) : 1;
   const long rows = x.size(-2), cols = x.size(-1);
   TORCH_CHECK(rows < (1l << 31) - 128 && cols < (1l << 31) - 512, "quantize: a side is too long");
   TORCH_CHECK(x.stride(-1) == 1 || cols <= 1, "quantize: the inner dimension must be contiguous");
-  const auto u8 = x.options().dtype(at::kByte);
+  const auto codes = x.options().dtype(fmt == kE4M3 ? at::kFloat8_e4m3fn : at::kFloat8_e5m2);
+  const auto scales = x.options().dtype(at::kFloat8_e8m0fnu);
   const long ldq = (cols + 15) / 16 * 16, ldqt = (rows + 15) / 16 * 16;
-  std::vector<at::Tensor> out = {at::empty({groups * rows, ldq}, u8), at::empty({(cols + 511) / 512, groups * rows, 4}, u8)};
+  std::vector<at::Tensor> out = {at::empty({groups * rows, ldq}, codes), at::empty({(cols + 511) / 512, groups * rows, 4}, scales)};
   if (both) {
-    out.push_back(at::empty({groups * cols, ldqt}, u8));
-    out.push_back(at::empty({(rows + 511) / 512, groups * cols, 4}, u8));
+    out.push_back(at::empty({groups * cols, ldqt}, codes));
+    out.push_back(at::empty({(rows + 511) / 512, groups * cols, 4}, scales));
   }
   if (x.numel() == 0) return out;
   QuantArgs a;
   a.x = x.data_ptr();
-  a.q = out[0].data_ptr<uint8_t>();
-  a.s = out[1].data_ptr<uint8_t>();
-  a.qt = both ? out[2].data_ptr<uint8_t>() : nullptr;
-  a.st = both ? out[3].data_ptr<uint8_t>() : nullptr;
+  a.q = static_cast<uint8_t*>(out[0].data_ptr());
+  a.s = static_cast<uint8_t*>(out[1].data_ptr());
+  a.qt = both ? static_cast<uint8_t*>(out[2].data_ptr()) : nullptr;
+  a.st = both ? static_cast<uint8_t*>(out[3].data_ptr()) : nullptr;
   a.ld = x.stride(-2);
   a.gstride = x.dim() == 3 ? x.stride(0) : 0;
   a.rows = static_cast<int>(rows);

@@ -60,71 +60,70 @@ class BlockFp8(NamedTuple):
         return self.data.device
 
 
-def _fail(cond: bool, text: str):
-    if not cond:
-        raise ValueError(text)
-
-
 def quantize(x: torch.Tensor, fmt: str = "e4m3", tiles: bool = False, both: bool = False):
     """x [rows, cols] or [G, rows, cols], bf16 / fp16 / fp32, inner stride 1.
 
     Returns the ``BlockFp8`` of x (rows G * rows), or with ``both`` the pair
     of it and that of each matrix's transpose (rows G * cols)."""
-    _fail(fmt in FORMATS, f"quantize: 8-bit type {fmt!r}, expected one of {sorted(FORMATS)}")
-    _fail(x.dim() in (2, 3), f"quantize: a matrix or a batch of matrices, got {x.dim()} dimensions")
-    _fail(x.dtype in (torch.bfloat16, torch.float16, torch.float32), f"quantize: bf16, fp16 or fp32, got {x.dtype}")
+    if fmt not in FORMATS:
+        raise ValueError(f"quantize: 8-bit type {fmt!r}, expected one of {sorted(FORMATS)}")
+    if x.dim() not in (2, 3):
+        raise ValueError(f"quantize: a matrix or a batch of matrices, got {x.dim()} dimensions")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"quantize: bf16, fp16 or fp32, got {x.dtype}")
     rows, cols = x.shape[-2:]
     if x.is_cuda:
-        got = ext().fp8_quantize(x, 0 if fmt == "e4m3" else 1, tiles, both)
+        got = ext().fp8_quantize(x, fmt == "e5m2", tiles, both)
     else:
         got = ref.fp8_quantize(x, fmt, tiles, both)
-    q = BlockFp8(got[0].view(FORMATS[fmt]), got[1].view(torch.float8_e8m0fnu), cols)
-    if not both:
-        return q
-    return q, BlockFp8(got[2].view(FORMATS[fmt]), got[3].view(torch.float8_e8m0fnu), rows)
+        got = [t.view(torch.float8_e8m0fnu if i % 2 else FORMATS[fmt]) for i, t in enumerate(got)]
+    q = BlockFp8(got[0], got[1], cols)
+    return (q, BlockFp8(got[2], got[3], rows)) if both else q
 
 
 def dequantize(q: BlockFp8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values [rows, cols]; exact in fp32 and bf16 down to their smallest values."""
+    """The values [rows, cols], each rounded once to ``dtype`` (fp32 and bf16 hold them exactly, but for those that
+    were rounded up past the type's largest value, which become infinite, or lie below its smallest)."""
     _check(q, "dequantize")
     return ref.fp8_values(q.data, q.scale, q.cols).to(dtype)
 
 
+# The CUDA entry point checks its arguments itself (csrc/gemm_fp8.cu); these are for CPU tensors.
 def _check(q: BlockFp8, who: str):
-    _fail(q.data.dim() == 2 and q.data.dtype in FORMATS.values(),
-          f"{who}: codes are a matrix of float8_e4m3fn or float8_e5m2, got {q.data.dtype}")
-    _fail(q.cols >= 0 and q.data.shape[1] >= q.cols, f"{who}: {q.data.shape[1]} columns of codes, {q.cols} are said")
-    _fail(q.scale.dtype == torch.float8_e8m0fnu and q.scale.is_contiguous()
-          and tuple(q.scale.shape) == (-(-q.cols // 512), q.data.shape[0], 4),
-          f"{who}: scales [{-(-q.cols // 512)}, {q.data.shape[0]}, 4] of float8_e8m0fnu, contiguous, got "
-          f"{tuple(q.scale.shape)} of {q.scale.dtype}")
-    _fail(q.scale.device == q.data.device, f"{who}: codes and scales on one device")
+    if q.data.dim() != 2 or q.data.dtype not in FORMATS.values():
+        raise ValueError(f"{who}: codes are a matrix of float8_e4m3fn or float8_e5m2, got {q.data.dtype}")
+    if q.cols < 0 or q.data.shape[1] < q.cols:
+        raise ValueError(f"{who}: {q.data.shape[1]} columns of codes, {q.cols} are said")
+    if (q.scale.dtype != torch.float8_e8m0fnu or not q.scale.is_contiguous() or q.scale.device != q.data.device
+            or tuple(q.scale.shape) != (-(-q.cols // 512), q.data.shape[0], 4)):
+        raise ValueError(f"{who}: scales [{-(-q.cols // 512)}, {q.data.shape[0]}, 4] of float8_e8m0fnu, contiguous, "
+                         f"beside the codes, got {tuple(q.scale.shape)} of {q.scale.dtype}")
 
 
 def _check_pair(a: BlockFp8, b: BlockFp8, who: str):
     _check(a, who)
     _check(b, who)
-    _fail(a.cols == b.cols, f"{who}: the operands contract {a.cols} and {b.cols} values")
-    _fail(a.device == b.device, f"{who}: operands on {a.device} and {b.device}")
+    if a.cols != b.cols:
+        raise ValueError(f"{who}: the operands contract {a.cols} and {b.cols} values")
+    if a.device != b.device:
+        raise ValueError(f"{who}: operands on {a.device} and {b.device}")
 
 
 def _check_out(out: torch.Tensor, shape: tuple, a: BlockFp8, who: str):
-    _fail(tuple(out.shape) == shape, f"{who}: out {tuple(out.shape)}, expected {shape}")
-    _fail(out.dtype in (torch.bfloat16, torch.float32), f"{who}: out in bf16 or fp32, got {out.dtype}")
-    _fail(out.device == a.device, f"{who}: out on {out.device}, operands on {a.device}")
-    _fail(out.shape[-1] <= 1 or out.stride(-1) == 1, f"{who}: out's inner stride must be 1")
+    if tuple(out.shape) != shape or (out.shape[-1] > 1 and out.stride(-1) != 1):
+        raise ValueError(f"{who}: out {tuple(out.shape)}, expected {shape} with inner stride 1")
+    if out.dtype not in (torch.bfloat16, torch.float32) or out.device != a.device:
+        raise ValueError(f"{who}: out in bf16 or fp32 beside the operands, got {out.dtype} on {out.device}")
 
 
 def _check_offs(offs: torch.Tensor, a: BlockFp8, who: str):
-    _fail(offs.dim() == 1 and offs.numel() >= 2 and offs.dtype == torch.int32 and offs.is_contiguous(),
-          f"{who}: offs are int32 [groups + 1]")
-    _fail(offs.device == a.device, f"{who}: offs on {offs.device}, operands on {a.device}")
+    if offs.dim() != 1 or offs.numel() < 2 or offs.dtype != torch.int32 or offs.device != a.device:
+        raise ValueError(f"{who}: offs are int32 [groups + 1] beside the operands")
 
 
-def _run(a, b, out, offs, M, N, K, G, mode, accumulate):
-    ext().fp8_matmul(a.data, a.scale, b.data, b.scale, out, offs, M, N, K, G, mode, accumulate,
-                     status_word(a.device))
-    return out
+def _run(a, b, out, offs, mode, accumulate, make_f32=False):
+    return ext().fp8_matmul(a.data, a.scale, a.cols, b.data, b.scale, b.cols, out, offs, mode, accumulate, make_f32,
+                            status_word(a.data.device))
 
 
 def matmul(a: BlockFp8, b: BlockFp8, out: torch.Tensor | None = None, accumulate: bool = False,
@@ -132,15 +131,17 @@ def matmul(a: BlockFp8, b: BlockFp8, out: torch.Tensor | None = None, accumulate
     """D [a.rows, b.rows] = a @ b^T, summed in fp32 and rounded once to
     ``out``'s type (bf16 or fp32; ``out_dtype`` where no ``out`` is given).
     ``accumulate`` adds to what ``out`` holds."""
-    _check_pair(a, b, "matmul")
-    M, N, K = a.rows, b.rows, a.cols
-    if out is None:
-        _fail(not accumulate, "matmul: accumulate needs out")
-        out = torch.empty(M, N, dtype=out_dtype, device=a.device)
-    _check_out(out, (M, N), a, "matmul")
+    if out is None and out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"matmul: out in bf16 or fp32, got {out_dtype}")
     if a.data.is_cuda:
-        return _run(a, b, out, None, M, N, K, 1, 0, accumulate)
-    y = ref.fp8_values(a.data, a.scale, K) @ ref.fp8_values(b.data, b.scale, K).t()
+        return _run(a, b, out, None, 0, accumulate, out_dtype == torch.float32)
+    _check_pair(a, b, "matmul")
+    if out is None:
+        if accumulate:
+            raise ValueError("matmul: accumulate needs out")
+        out = torch.empty(a.rows, b.rows, dtype=out_dtype)
+    _check_out(out, (a.rows, b.rows), a, "matmul")
+    y = ref.fp8_values(a.data, a.scale, a.cols) @ ref.fp8_values(b.data, b.scale, b.cols).t()
     return out.copy_(out.float() + y if accumulate else y)
 
 
@@ -151,16 +152,17 @@ def grouped_matmul(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tens
     [G, N, K]); ``offs`` is int32 [G + 1] on the device, rising.  Rows of
     ``out`` that no segment covers are left as they were (unwritten memory
     where no ``out`` is given)."""
+    if a.data.is_cuda:
+        return _run(a, b, out, offs, 0, False)
     _check_pair(a, b, "grouped_matmul")
     _check_offs(offs, a, "grouped_matmul")
     G = offs.numel() - 1
-    _fail(b.rows % G == 0, f"grouped_matmul: {b.rows} rows of b for {G} groups")
+    if b.rows % G:
+        raise ValueError(f"grouped_matmul: {b.rows} rows of b for {G} groups")
     R, N, K = a.rows, b.rows // G, a.cols
     if out is None:
-        out = torch.empty(R, N, dtype=torch.bfloat16, device=a.device)
+        out = torch.empty(R, N, dtype=torch.bfloat16)
     _check_out(out, (R, N), a, "grouped_matmul")
-    if a.data.is_cuda:
-        return _run(a, b, out, offs, R, N, K, G, 0, False)
     x, w = ref.fp8_values(a.data, a.scale, K), ref.fp8_values(b.data, b.scale, K).view(G, N, K)
     for g, (lo, hi) in enumerate(ref.segments(offs, R)):
         out[lo:hi] = (x[lo:hi] @ w[g].t()).to(out.dtype)
@@ -179,18 +181,18 @@ def grouped_wgrad(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tenso
     refused, on the GPU through the status word (``ops._ext.check_status``)
     with ``out`` left as it was.  An empty segment gives zeros (or leaves
     ``out[g]`` with ``accumulate``)."""
+    if a.data.is_cuda:
+        return _run(a, b, out, offs, 1, accumulate)
     _check_pair(a, b, "grouped_wgrad")
     _check_offs(offs, a, "grouped_wgrad")
-    G, M, N, K = offs.numel() - 1, a.rows, b.rows, a.cols
-    _check_out(out, (G, M, N), a, "grouped_wgrad")
-    _fail(out.is_contiguous(), "grouped_wgrad: out must be contiguous")
-    if a.data.is_cuda:
-        _run(a, b, out.view(G * M, N), offs, M, N, K, G, 1, accumulate)
-        return out
+    G, K = offs.numel() - 1, a.cols
+    _check_out(out, (G, a.rows, b.rows), a, "grouped_wgrad")
+    if not out.is_contiguous():
+        raise ValueError("grouped_wgrad: out must be contiguous")
     x, y = ref.fp8_values(a.data, a.scale, K), ref.fp8_values(b.data, b.scale, K)
     segs = ref.segments(offs, K)
-    _fail(all(hi == lo or (lo % BLOCK == 0 and (hi % BLOCK == 0 or hi == K)) for lo, hi in segs),
-          f"grouped_wgrad: segments {segs} cut a block of {BLOCK}")
+    if not all(hi == lo or (lo % BLOCK == 0 and (hi % BLOCK == 0 or hi == K)) for lo, hi in segs):
+        raise ValueError(f"grouped_wgrad: segments {segs} cut a block of {BLOCK}")
     for g, (lo, hi) in enumerate(segs):
         d = x[:, lo:hi] @ y[:, lo:hi].t()
         out[g] = (out[g].float() + d if accumulate else d).to(out.dtype)

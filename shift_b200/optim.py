@@ -83,6 +83,13 @@ class AdamWMany:
                 same.append(w)
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
             _fail(all(x.device == self.params[0].device for x in same), f"tensor {t} or its state is on another device")
+        self._plan = None
+        if n > 0 and self.params[0].is_cuda:
+            m, v, ms, vs = self.exp_avg, self.exp_avg_sq, [], []
+            if self.eight:
+                m, ms = [x.code for x in m], [x.scale for x in m]
+                v, vs = [x.code for x in v], [x.scale for x in v]
+            self._plan = ext().adamw_many_plan(self.params, self.masters or [], m, ms, v, vs)
 
     def step(self, grads, lr: float = 1.0e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1.0e-8,
              wd: float = 0.01, step: int = 1, grad_scale: float = 1.0, seed: int | None = None, step_dev=None,
@@ -96,35 +103,24 @@ class AdamWMany:
         ``engine.StepBlock`` writes that layout).  ``skip``: int32 on the
         device; where it is not zero nothing changes.  ``nonfinite``: int32
         flag, set where a scaled gradient is not finite."""
+        if step < 1:
+            raise ValueError(f"AdamWMany: step {step}: counted from 1")
+        seed = (step if seed is None else seed) & 0xFFFFFFFF
+        if self._plan is not None:
+            ext().adamw_many(self._plan, grads if isinstance(grads, list) else list(grads), lr, beta1, beta2, eps, wd,
+                             step, grad_scale, seed, step_dev, skip, nonfinite)
+            return
         grads = list(grads)
-        _fail(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")
-        _fail(step >= 1, f"step {step}: counted from 1")
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamWMany: {len(grads)} gradients for {len(self.params)} parameters")
         dev = self.params[0].device if self.params else None
         for t, (g, p) in enumerate(zip(grads, self.params)):
-            _fail(g.dtype in _FLOATS and g.numel() == p.numel() and g.is_contiguous() and g.device == dev,
-                  f"gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {dev}")
+            if g.dtype not in _FLOATS or g.numel() != p.numel() or not g.is_contiguous() or g.device != dev:
+                raise ValueError(f"AdamWMany: gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {dev}")
         for name, x, least in (("step_dev", step_dev, 4), ("skip", skip, 1), ("nonfinite", nonfinite, 1)):
-            _fail(x is None or (x.dtype == torch.int32 and x.numel() >= least and x.is_contiguous() and x.device == dev),
-                  f"{name}: int32 [{least}] on {dev}")
-        seed = step if seed is None else seed
-        if dev is None:
-            return
-        if dev.type != "cuda":
-            self._cpu_step(grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite)
-            return
-        kinds: dict = {}
-        for t, (p, g) in enumerate(zip(self.params, grads)):
-            kinds.setdefault((p.dtype, g.dtype), []).append(t)
-        for at in kinds.values():
-            pick = lambda xs: [xs[t] for t in at]  # noqa: E731
-            m, v = pick(self.exp_avg), pick(self.exp_avg_sq)
-            ms = vs = []
-            if self.eight:
-                m, ms = [x.code for x in m], [x.scale for x in m]
-                v, vs = [x.code for x in v], [x.scale for x in v]
-            ext().adamw_many(pick(self.params), pick(self.masters) if self.masters is not None else [], pick(grads),
-                             m, ms, v, vs, at, lr, beta1, beta2, eps, wd, step, grad_scale, seed & 0xFFFFFFFF,
-                             step_dev, skip, nonfinite)
+            if x is not None and (x.dtype != torch.int32 or x.numel() < least or x.device != dev):
+                raise ValueError(f"AdamWMany: {name}: int32 [{least}] on {dev}")
+        self._cpu_step(grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite)
 
     def _cpu_step(self, grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite):
         if skip is not None and int(skip.view(-1)[0]) != 0:
