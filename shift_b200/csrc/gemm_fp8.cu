@@ -818,7 +818,7 @@ static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, i
   p.ctas = M > BM ? 2 : 1;
   const long slots = sms / p.ctas, tm = (M + BM * p.ctas - 1) / (BM * p.ctas);
   long best = -1;
-  for (int bn : {256, 192, 128}) {
+  for (int bn : {256, 224, 192, 128}) {
     if (bn == 256 && p.ctas == 1) continue;
     const long tn = (N + bn - 1) / bn, tiles = mode == kRowGroups ? tm * tn : G * tm * tn;
     const long cost = (tiles + slots - 1) / slots * ((bn == 128 ? 176 : bn) + 64);
@@ -946,10 +946,12 @@ at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at
   const int dev = a.device().index();
   if (plan.ctas == 2) {
     if (bn == 256) launch<256, 2>(ta, tb, p, tiles, dev, st);
+    else if (bn == 224) launch<224, 2>(ta, tb, p, tiles, dev, st);
     else if (bn == 192) launch<192, 2>(ta, tb, p, tiles, dev, st);
     else launch<128, 2>(ta, tb, p, tiles, dev, st);
   } else {
-    if (bn == 192) launch<192, 1>(ta, tb, p, tiles, dev, st);
+    if (bn == 224) launch<224, 1>(ta, tb, p, tiles, dev, st);
+    else if (bn == 192) launch<192, 1>(ta, tb, p, tiles, dev, st);
     else launch<128, 1>(ta, tb, p, tiles, dev, st);
   }
   if (p.split > 1) {

@@ -18,20 +18,49 @@ namespace fp8 {
 
 constexpr int kQThreads = 256;
 
-// Eight consecutive values of a row as loaded (16 bytes, or 32 for fp32).
+// Sixteen consecutive values of a row in 32-bit words as loaded: pairs of
+// 2-byte values, or single fp32 values.
 template <typename T>
-struct alignas(16) Vec8 {
-  T v[8];
+struct alignas(16) Row16 {
+  static constexpr int kWords = 4 * sizeof(T);
+  uint32_t w[kWords];
 };
 
+SB_DEVICE float value(const Row16<float>& r, int j) { return __uint_as_float(r.w[j]); }
+SB_DEVICE float value(const Row16<__nv_bfloat16>& r, int j) {
+  return __uint_as_float(j % 2 ? r.w[j / 2] & 0xFFFF0000u : r.w[j / 2] << 16);
+}
+SB_DEVICE float value(const Row16<__half>& r, int j) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&r.w[j / 2]);
+  return j % 2 ? __high2float(h) : __low2float(h);
+}
+// Magnitudes of a word's values, and the larger ones of two words: both values
+// of a pair at once.  NaN loses against a number.
 template <typename T>
-SB_DEVICE float to_f(T x);
+SB_DEVICE uint32_t magnitude(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu); }
+template <typename T>
+SB_DEVICE uint32_t larger(uint32_t a, uint32_t b);
 template <>
-SB_DEVICE float to_f<float>(float x) { return x; }
+SB_DEVICE uint32_t larger<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
 template <>
-SB_DEVICE float to_f<__half>(__half x) { return __half2float(x); }
+SB_DEVICE uint32_t larger<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
 template <>
-SB_DEVICE float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+SB_DEVICE uint32_t larger<__half>(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// Value `hi` of a word of magnitudes.
+template <typename T>
+SB_DEVICE float part(uint32_t w, int hi) {
+  Row16<T> r;
+  r.w[0] = w;
+  return value(r, sizeof(T) == 4 ? 0 : hi);
+}
 
 SB_DEVICE float finite_abs(float x) {
   const float a = fabsf(x);
@@ -52,179 +81,182 @@ struct QuantArgs {
   uint8_t *q, *s, *qt, *st;
   long ld, gstride;        // input strides, elements
   int rows, cols;          // of one group
+  int groups;
   int rb, cb;              // tiles per group
   long ldq, ldqt;          // output row strides
   long all_rows, all_cols; // groups * rows, groups * cols: rows of the scale planes
   bool vec;                // 16-byte loads are aligned
 };
 
-// thread (rg, cg): rows rg * 8 .. +8, columns cg * 8 .. +8 of the tile, so 16
-// lanes read 256 contiguous bytes of a row (2-byte types) and a column's codes
-// of 8 rows are one 8-byte word of the transposed tile.
+// Thread (rg, cg): rows 4 rg .. +4, columns 16 cg .. +16 of the tile, so 8 lanes
+// hold a row, a thread stores 16 codes of a row at once, and four rows of a
+// column are one word of the transposed tile.  Maxima are taken on pairs as
+// they were loaded.  (8 columns by 8 rows a thread, in fp32, issued 17 and 24
+// instructions a value for one and two orientations, 22.5 and 27.6 us for
+// 16384 x 1024.)
 template <typename T, int FMT, bool TILES, bool BOTH>
 __global__ void __launch_bounds__(kQThreads)
 quantize_kernel(const QuantArgs a) {
-  __shared__ float s_max[8][128];
+  using R = Row16<T>;
+  constexpr int kWords = R::kWords, kPer = 16 / kWords;   // values of a word
+  constexpr bool kCols = BOTH && !TILES;
+  __shared__ uint32_t s_max[8][8 * kWords];               // [warp][column group, word]: largest of a warp's 16 rows
   __shared__ float s_inv[128];
-  __shared__ uint64_t s_t[BOTH ? 128 * 16 : 1];
-  const int cg = threadIdx.x % 16, rg = threadIdx.x / 16;
+  __shared__ alignas(16) uint32_t s_t[BOTH ? 128 * 32 : 4];
+  const int cg = threadIdx.x % 8, rg = threadIdx.x / 8;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long per = static_cast<long>(a.rb) * a.cb;
-  const long g = blockIdx.x / per;
-  const int tile = static_cast<int>(blockIdx.x - g * per);
-  const int tr = tile / a.cb, tc = tile % a.cb;
-  const int r0 = tr * 128 + rg * 8, c0 = tc * 128 + cg * 8;
-  const T* x = reinterpret_cast<const T*>(a.x) + g * a.gstride;
+  const unsigned per = static_cast<unsigned>(a.rb) * a.cb;
+  const int g = a.groups == 1 ? 0 : static_cast<int>(blockIdx.x / per);
+  const unsigned tile = blockIdx.x - g * per;
+  const int tr = tile / static_cast<unsigned>(a.cb), tc = tile - tr * a.cb;
+  const int r0 = tr * 128 + rg * 4, c0 = tc * 128 + cg * 16;
+  const T* x = reinterpret_cast<const T*>(a.x) + g * a.gstride + static_cast<long>(r0) * a.ld + c0;
 
-  Vec8<T> v[8];
+  R v[4];
+  if (a.vec && c0 + 16 <= a.cols && r0 + 4 <= a.rows) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i;
-    const T* p = x + static_cast<long>(r) * a.ld + c0;
-    uint4* dst = reinterpret_cast<uint4*>(&v[i]);
-    if (r < a.rows && a.vec && c0 + 8 <= a.cols) {
-      const uint4* src = reinterpret_cast<const uint4*>(p);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 0; w < static_cast<int>(sizeof(T)) / 2; ++w) dst[w] = __ldg(src + w);
-    } else {
+      for (int q = 0; q < kWords / 4; ++q)
+        reinterpret_cast<uint4*>(v[i].w)[q] = __ldg(reinterpret_cast<const uint4*>(x + i * a.ld) + q);
+  } else {
 #pragma unroll
-      for (int w = 0; w < static_cast<int>(sizeof(T)) / 2; ++w) dst[w] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r < a.rows && c0 + j < a.cols) v[i].v[j] = p[j];
+      for (int q = 0; q < kWords; ++q) v[i].w[q] = 0u;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (r0 + i < a.rows && c0 + j < a.cols) reinterpret_cast<T*>(v[i].w)[j] = x[i * a.ld + j];
     }
   }
 
-  // fmaxf passes over NaN; a maximum of infinity sends the thread through its values once more without them
-  float rmax[8], cmax[8], top = 0.f;
+  // the largest magnitudes, of the rows and (pairwise) of the columns
+  float rmax[4], top = 0.f;
+  uint32_t cmax[kWords];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    rmax[i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = fabsf(to_f<T>(v[i].v[j]));
-      rmax[i] = fmaxf(rmax[i], f);
-      if (BOTH && !TILES) cmax[j] = fmaxf(cmax[j], f);
+    for (int q = 0; q < kWords; ++q) {
+      const uint32_t w = magnitude<T>(v[i].w[q]);
+      m = larger<T>(m, w);
+      if (kCols) cmax[q] = i == 0 ? larger<T>(0u, w) : larger<T>(cmax[q], w);
     }
+    rmax[i] = fmaxf(part<T>(m, 0), part<T>(m, 1));
     top = fmaxf(top, rmax[i]);
   }
+  // infinities do not count: a thread that met one looks again without them
   const bool infinite = top == INFINITY;
   if (infinite) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       rmax[i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float f = finite_abs(to_f<T>(v[i].v[j]));
-        rmax[i] = fmaxf(rmax[i], f);
-        if (BOTH && !TILES) cmax[j] = fmaxf(cmax[j], f);
+      for (int j = 0; j < 16; ++j) rmax[i] = fmaxf(rmax[i], finite_abs(value(v[i], j)));
+    }
+    if (kCols) {
+#pragma unroll
+      for (int q = 0; q < kWords; ++q) {
+        cmax[q] = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w = magnitude<T>(v[i].w[q]);
+#pragma unroll
+          for (int h = 0; h < kPer; ++h)
+            if (!(part<T>(w, h) < INFINITY)) w &= kPer == 1 ? 0u : (h ? 0x0000FFFFu : 0xFFFF0000u);
+          cmax[q] = larger<T>(cmax[q], w);
+        }
       }
     }
   }
-  float rinv[8];
-  int rbyte[8];
+
+  int rbyte[4];
+  float rinv[4];
   if constexpr (TILES) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, rmax[i]);
-    m = warp_max(m);
-    if (lane == 0) s_max[0][warp] = m;
+    float m = warp_max(fmaxf(fmaxf(rmax[0], rmax[1]), fmaxf(rmax[2], rmax[3])));
+    float* s = reinterpret_cast<float*>(&s_max[0][0]);
+    if (lane == 0) s[warp] = m;
     __syncthreads();
-    m = s_max[0][0];
+    m = s[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) m = fmaxf(m, s_max[0][w]);
-    const int byte = scale_byte(m, FMT);
+    for (int w = 1; w < 8; ++w) m = fmaxf(m, s[w]);
+    rbyte[0] = scale_byte(m, FMT);
+    rinv[0] = inv_scale(rbyte[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      rbyte[i] = byte;
-      rinv[i] = inv_scale(byte);
-    }
+    for (int i = 1; i < 4; ++i) rbyte[i] = rbyte[0], rinv[i] = rinv[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
+      for (int o = 4; o > 0; o >>= 1) rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
       rbyte[i] = scale_byte(rmax[i], FMT);
       rinv[i] = inv_scale(rbyte[i]);
     }
   }
 
   // codes along the rows
+  uint8_t* q = a.q + (static_cast<long>(g) * a.rows + r0) * a.ldq + c0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i;
-    uint32_t w[2];
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 4; ++h) {
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = to_f<T>(v[i].v[4 * h + j]) * rinv[i];
+      for (int j = 0; j < 4; ++j) y[j] = value(v[i], 4 * h + j) * rinv[i];
       w[h] = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
       if (infinite) w[h] = patch_infinities<FMT>(w[h], y);
     }
-    if (r < a.rows && c0 < a.cols)
-      *reinterpret_cast<uint2*>(a.q + (g * a.rows + r) * a.ldq + c0) = make_uint2(w[0], w[1]);
-    // scale bytes of this tile, and zeros for the columns that the last word lacks
-    if (cg == 0 && r < a.rows) {
-      uint8_t* s = a.s + ((tc / 4) * a.all_rows + g * a.rows + r) * 4;
-      s[tc % 4] = static_cast<uint8_t>(rbyte[i]);
-      if (tc == a.cb - 1)
-        for (int j = tc % 4 + 1; j < 4; ++j) s[j] = 0;
-    }
+    if (r0 + i < a.rows && c0 < a.cols) *reinterpret_cast<uint4*>(q + i * a.ldq) = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  // scale bytes of this tile, and zeros for the columns that the last word lacks: four lanes of a row group, a row each
+  if (cg < 4 && r0 + cg < a.rows) {
+    const int byte = cg == 0 ? rbyte[0] : cg == 1 ? rbyte[1] : cg == 2 ? rbyte[2] : rbyte[3];
+    uint8_t* s = a.s + ((tc / 4) * a.all_rows + static_cast<long>(g) * a.rows + r0 + cg) * 4;
+    s[tc % 4] = static_cast<uint8_t>(byte);
+    if (tc == a.cb - 1)
+      for (int j = tc % 4 + 1; j < 4; ++j) s[j] = 0;
+  }
+
   if constexpr (BOTH) {
-    float cinv[8];
-    if constexpr (TILES) {
+    if constexpr (kCols) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cinv[j] = rinv[0];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cmax[j] = fmaxf(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
-        if (lane < 16) s_max[warp][cg * 8 + j] = cmax[j];
+      for (int w = 0; w < kWords; ++w) {
+        cmax[w] = larger<T>(cmax[w], __shfl_xor_sync(0xffffffffu, cmax[w], 8));
+        cmax[w] = larger<T>(cmax[w], __shfl_xor_sync(0xffffffffu, cmax[w], 16));
+        if (lane < 8) s_max[warp][cg * kWords + w] = cmax[w];
       }
       __syncthreads();
     }
     if (threadIdx.x < 128) {
       const int c = tc * 128 + threadIdx.x;
       int byte = rbyte[0];
-      if constexpr (!TILES) {
-        float m = s_max[0][threadIdx.x];
+      if constexpr (kCols) {
+        uint32_t m = s_max[0][threadIdx.x / kPer];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) m = fmaxf(m, s_max[w][threadIdx.x]);
-        byte = scale_byte(m, FMT);
+        for (int w = 1; w < 8; ++w) m = larger<T>(m, s_max[w][threadIdx.x / kPer]);
+        byte = scale_byte(part<T>(m, threadIdx.x % kPer), FMT);
         s_inv[threadIdx.x] = inv_scale(byte);
       }
       if (c < a.cols) {
-        uint8_t* s = a.st + ((tr / 4) * a.all_cols + g * a.cols + c) * 4;
+        uint8_t* s = a.st + ((tr / 4) * a.all_cols + static_cast<long>(g) * a.cols + c) * 4;
         s[tr % 4] = static_cast<uint8_t>(byte);
         if (tr == a.rb - 1)
           for (int j = tr % 4 + 1; j < 4; ++j) s[j] = 0;
       }
     }
-    if constexpr (!TILES) {
-      __syncthreads();
+    if constexpr (kCols) __syncthreads();
+    // Word rg of column c lies at rg ^ 4 (c / 16): the eight column groups and four row groups of a warp store to 32
+    // different banks, and four words that make 16 bytes of a column stay together.
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cinv[j] = s_inv[cg * 8 + j];
-    }
-    // 8 rows of a column are one 8-byte word; words are swizzled by the column
-    // group so that the 16 lanes of a row group write 16 different banks pairs
+    for (int j = 0; j < 16; ++j) {
+      const float inv = kCols ? s_inv[cg * 16 + j] : rinv[0];
+      float y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t w[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = to_f<T>(v[4 * h + i].v[j]) * cinv[j];
-        w[h] = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
-        if (infinite) w[h] = patch_infinities<FMT>(w[h], y);
-      }
-      s_t[(cg * 8 + j) * 16 + (rg ^ cg)] = static_cast<uint64_t>(w[1]) << 32 | w[0];
+      for (int i = 0; i < 4; ++i) y[i] = value(v[i], j) * inv;
+      uint32_t w = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
+      if (infinite) w = patch_infinities<FMT>(w, y);
+      s_t[(cg * 16 + j) * 32 + (rg ^ (4 * cg))] = w;
     }
     __syncthreads();
 #pragma unroll
@@ -232,10 +264,9 @@ quantize_kernel(const QuantArgs a) {
       const int idx = k * kQThreads + threadIdx.x;
       const int c = idx / 8, ch = idx % 8;        // column of the tile, 16-row chunk
       const int col = tc * 128 + c, row = tr * 128 + ch * 16;
-      if (col < a.cols && row < a.rows) {
-        const uint64_t lo = s_t[c * 16 + ((2 * ch) ^ (c / 8))], hi = s_t[c * 16 + ((2 * ch + 1) ^ (c / 8))];
-        *reinterpret_cast<ulonglong2*>(a.qt + (g * a.cols + col) * a.ldqt + row) = make_ulonglong2(lo, hi);
-      }
+      if (col < a.cols && row < a.rows)
+        *reinterpret_cast<uint4*>(a.qt + (static_cast<long>(g) * a.cols + col) * a.ldqt + row) =
+            *reinterpret_cast<const uint4*>(&s_t[c * 32 + ((4 * ch) ^ (4 * (c / 16)))]);
     }
   }
 }
@@ -277,6 +308,7 @@ std::vector<at::Tensor> quantize(const at::Tensor& x, int64_t fmt, bool tiles, b
   a.st = both ? static_cast<uint8_t*>(out[3].data_ptr()) : nullptr;
   a.ld = x.stride(-2);
   a.gstride = x.dim() == 3 ? x.stride(0) : 0;
+  a.groups = static_cast<int>(groups);
   a.rows = static_cast<int>(rows);
   a.cols = static_cast<int>(cols);
   a.rb = static_cast<int>((rows + 127) / 128);
