@@ -302,7 +302,7 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
     TORCH_CHECK_VALUE(is_float(g[i].scalar_type()) && g[i].numel() == n && g[i].is_contiguous() && g[i].device() == dev,
                       "AdamWMany: gradient ", i, ": contiguous, ", n, " elements, fp32 / bf16 / fp16, on ", dev);
     // a tensor can be given other memory (.data, resize_) after the check at construction
-    TORCH_CHECK_VALUE(t.p[i].is_contiguous() && t.m[i].numel() == n && t.v[i].numel() == n && t.p[i].device() == dev &&
+    TORCH_CHECK_VALUE(is_float(t.p[i].scalar_type()) && t.p[i].is_contiguous() && t.m[i].numel() == n && t.v[i].numel() == n && t.p[i].device() == dev &&
                           (t.w.empty() || t.w[i].numel() == n) &&
                           (!eight || (t.ms[i].numel() == (n + 127) / 128 && t.vs[i].numel() == (n + 127) / 128)),
                       "AdamWMany: tensor ", i, " has changed its size or place");

@@ -1,6 +1,6 @@
 """Kernel micro-benchmarks at the shapes of the 0.494B MoE training step.
 
-    python -m shift_b200.ops.microbench [--ops gemm,attn,mem,fused] [--iters N]
+    python -m shift_b200.ops.microbench [--ops gemm,attn,mem,fused,fp8] [--iters N]
 
 Each case is timed with CUDA events on the launching stream after warm-up,
 with a synchronize on both sides; inputs of the timed cases are larger than
@@ -298,6 +298,41 @@ def run_fused(iters):
     return rows
 
 
+def run_fp8(iters, T=16384, H=1024):
+    """8-bit operators: quantiser and optimizer against the copy bandwidth, products against twice the bf16 rate."""
+    from ..optim import AdamWMany, State8
+    from . import fp8
+    pk = peaks()
+    rows = []
+
+    def mem(name, fn, nbytes):
+        t = timeit(fn, iters)
+        rows.append({"case": name, "ms": round(t, 4), "gbs": round(nbytes / t / 1e6, 1),
+                     "frac_of_peak": round(nbytes / t / 1e6 / pk["hbm_gbs"], 3)})
+
+    x = bf(T, H)
+    mem(f"fp8.quantize rows {T}x{H}", lambda: fp8.quantize(x), T * H * 3)
+    mem(f"fp8.quantize both {T}x{H}", lambda: fp8.quantize(x, both=True), T * H * 4)
+    for name, M, N, K in (("qkv.fwd", T, 1536, H), ("o.fwd", T, H, H), ("lm_head.fwd", T, 32768, H),
+                          ("qkv.wgrad", 1536, H, T), ("square", 8192, 8192, 8192), ("one token head", 1, 32768, H)):
+        a, b = fp8.quantize(bf(M, K)), fp8.quantize(bf(N, K))
+        out = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+        t = timeit(lambda: fp8.matmul(a, b, out=out), iters)
+        tf = 2 * M * N * K / t / 1e9
+        rows.append({"case": f"fp8.matmul {name} {M}x{N}x{K}", "ms": round(t, 4), "tflops": round(tf, 1),
+                     "frac_of_peak": round(tf / (2 * pk["bf16_tflops"]), 3)})
+    n = 124_000_000
+    for eight in (True, False):
+        p, g = [bf(n // 8) for _ in range(8)], [bf(n // 8) for _ in range(8)]
+        state = lambda: [State8.zeros(q) if eight else torch.zeros(q.numel(), device="cuda") for q in p]  # noqa: E731
+        opt = AdamWMany(p, state(), state(), [q.float() for q in p])
+        mem(f"adamw many {n} {8 if eight else 32}-bit", lambda: opt.step(g), n * (12 + (4 if eight else 16)))
+    from ._ext import check_status
+    torch.cuda.synchronize()
+    check_status()
+    return rows
+
+
 def main():
     p = argparse.ArgumentParser()
     p.add_argument("--ops", default="gemm,attn,mem")
@@ -318,6 +353,8 @@ def main():
         out["mem"] = run_mem(args.iters)
     if "fused" in ops:
         out["fused"] = run_fused(args.iters)
+    if "fp8" in ops:
+        out["fp8"] = run_fp8(args.iters)
     for k, v in out.items():
         if isinstance(v, list):
             for r in v:

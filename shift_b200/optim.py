@@ -83,13 +83,20 @@ class AdamWMany:
                 same.append(w)
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
             _fail(all(x.device == self.params[0].device for x in same), f"tensor {t} or its state is on another device")
+        own = [x.data_ptr() for p, *state in zip(self.params, *self._states()) for x in (p, *state) if x.numel()]
+        _fail(len(set(own)) == len(own), "a tensor is there twice, or two share memory")
         self._plan = None
         if n > 0 and self.params[0].is_cuda:
-            m, v, ms, vs = self.exp_avg, self.exp_avg_sq, [], []
-            if self.eight:
-                m, ms = [x.code for x in m], [x.scale for x in m]
-                v, vs = [x.code for x in v], [x.scale for x in v]
+            lists = self._states()
+            m, ms, v, vs = lists[:4] if self.eight else (lists[0], [], lists[1], [])
             self._plan = ext().adamw_many_plan(self.params, self.masters or [], m, ms, v, vs)
+
+    def _states(self):
+        """The lists of tensors that a step writes beside the parameters."""
+        lists = [self.exp_avg, self.exp_avg_sq]
+        if self.eight:
+            lists = [[s[i] for s in x] for x in lists for i in (0, 1)]
+        return lists + ([] if self.masters is None else [self.masters])
 
     def step(self, grads, lr: float = 1.0e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1.0e-8,
              wd: float = 0.01, step: int = 1, grad_scale: float = 1.0, seed: int | None = None, step_dev=None,
@@ -153,3 +160,76 @@ class AdamWMany:
             w.copy_(new)
             if self.masters is not None:
                 p.detach().view(-1).copy_(new)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``AdamWMany`` as a ``torch.optim`` optimizer: a script's ``torch.optim.AdamW`` with its state in 8 bits
+    (``state_bits=8``: 2 + 1/64 bytes per parameter, where 32 bits take 8) or 32, updated by one kernel per group.
+
+    ``master_weights`` keeps fp32 weights beside bf16 or fp16 parameters.  Under ``ft.transparent`` it is adopted like
+    any other optimizer: its state is part of ``state_dict`` and heals with it.  State tensors are made at a
+    parameter's first gradient; a parameter without a gradient is left alone in that step."""
+
+    def __init__(self, params, lr: float = 1.0e-3, betas=(0.9, 0.999), eps: float = 1.0e-8, weight_decay: float = 1.0e-2,
+                 state_bits: int = 8, master_weights: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state in 8 or 32 bits, got {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights))
+        self._many: dict = {}
+
+    def _init_state(self, p, group):
+        st = self.state[p]
+        st["step"] = 0
+        for name in ("exp_avg", "exp_avg_sq"):
+            if group["state_bits"] == 8:
+                code, scale = State8.zeros(p)
+                # as bytes: what copies or ships a state dict need not know the 8-bit types
+                st[name], st[name + "_scale"] = code.view(torch.uint8), scale.view(torch.uint8)
+            else:
+                st[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        if group["master_weights"]:
+            st["master"] = p.detach().float().clone()
+
+    def _moment(self, p, name, group):
+        st = self.state[p]
+        if group["state_bits"] == 8:
+            return State8(st[name].view(torch.float8_e4m3fn), st[name + "_scale"].view(torch.float8_e8m0fnu))
+        return st[name]
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts floating-point and byte states to the parameter's type: put back what was saved
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            for name, x in saved.get(i, {}).items():
+                self.state[p][name] = x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
+        self._many.clear()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for k, group in enumerate(self.param_groups):
+            live = [p for p in group["params"] if p.grad is not None]
+            by_step: dict = {}
+            for p in live:
+                if "step" not in self.state[p]:
+                    self._init_state(p, group)
+                self.state[p]["step"] += 1
+                by_step.setdefault((self.state[p]["step"], p.device), []).append(p)
+            for (t, _), ps in by_step.items():
+                # the lists of a group are checked and handed over once, as long as the same parameters take part
+                held = self._many.get((k, ps[0]))
+                if held is None or len(held[0]) != len(ps) or any(a is not b for a, b in zip(held[0], ps)):
+                    many = AdamWMany(ps, [self._moment(p, "exp_avg", group) for p in ps],
+                                     [self._moment(p, "exp_avg_sq", group) for p in ps],
+                                     [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
+                    held = self._many[(k, ps[0])] = (ps, many)
+                beta1, beta2 = group["betas"]
+                held[1].step([p.grad for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
+                             wd=group["weight_decay"], step=int(t))
+        return loss

@@ -90,7 +90,9 @@ def _done():
 
 
 SIZES = [(1, 16, 16), (1, 1, 1), (1, 1000, 1024), (5, 33, 700), (64, 640, 96), (128, 128, 128), (129, 225, 129),
-         (256, 448, 1024), (300, 1000, 2061), (1000, 8, 4096), (2050, 1536, 640), (40, 3000, 513)]
+         (256, 448, 1024), (300, 1000, 2061), (1000, 8, 4096), (2050, 1536, 640), (40, 3000, 513),
+         # every tile width, by one CTA and by a pair, several tiles to each
+         (1, 32768, 200), (100, 28000, 130), (4096, 4096, 2500), (16384, 672, 200), (5000, 1344, 1024)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -110,7 +112,8 @@ def test_matmul_types(fa, fb):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("M,N,K", [(384, 256, 8192), (200, 100, 3000), (1536, 1024, 4096), (17, 9, 5000)])
+@pytest.mark.parametrize("M,N,K", [(384, 256, 8192), (200, 100, 3000), (1536, 1024, 4096), (17, 9, 5000),
+                                   (4096, 4096, 300)])
 def test_matmul_accumulate(M, N, K, dtype):
     a, b = _pair(M, N, K, "e5m2", "e4m3", spread=1.0)
     base = torch.randn(M, N, device=DEV).to(dtype)

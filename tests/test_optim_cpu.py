@@ -127,6 +127,7 @@ def test_refusals():
                 lambda: AdamWMany(params, [x.half() for x in m], v),
                 lambda: AdamWMany([p.t() if p.dim() == 2 else p for p in params],
                                   [x.t() if x.dim() == 2 else x for x in m], v),
+                lambda: AdamWMany(params + params[:1], m + m[:1], v + v[:1]), lambda: AdamWMany(params, m, m),
                 lambda: AdamWMany(params, m8, [s._replace(scale=s.scale[:0]) for s in m8]),
                 lambda: AdamWMany(params, m, v).step(grads[:-1]), lambda: AdamWMany(params, m, v).step(grads, step=0),
                 lambda: AdamWMany(params, m, v).step([g.double() for g in grads]),
@@ -135,3 +136,55 @@ def test_refusals():
         with pytest.raises(ValueError):
             bad()
     AdamWMany([], [], []).step([])
+
+
+@pytest.mark.parametrize("bits,master", [(8, False), (8, True), (32, True)])
+def test_torch_optimizer_and_its_saved_state(bits, master):
+    from shift_b200.optim import AdamW
+
+    def model():
+        torch.manual_seed(3)
+        net = torch.nn.Sequential(torch.nn.Linear(40, 30), torch.nn.Linear(30, 7, bias=False)).to(torch.bfloat16)
+        return net, AdamW(net.parameters(), lr=1e-2, state_bits=bits, master_weights=master)
+
+    def grads(net, i):
+        g = torch.Generator().manual_seed(i)
+        for j, p in enumerate(net.parameters()):
+            # the second tensor has no gradient in the first step: its count then lags behind
+            p.grad = None if i == 0 and j == 1 else torch.randn(p.shape, generator=g).to(p.dtype)
+
+    net, opt = model()
+    for i in range(3):
+        grads(net, i)
+        opt.step()
+    steps = [opt.state[p]["step"] for p in net.parameters()]
+    assert steps == [3, 2, 3]
+    twin, other = model()
+    twin.load_state_dict(net.state_dict())
+    other.load_state_dict(opt.state_dict())
+    for a, b in zip(net.parameters(), twin.parameters()):
+        for k, x in opt.state[a].items():
+            assert (torch.equal(x, other.state[b][k]) and x.dtype == other.state[b][k].dtype) if k != "step" \
+                else x == other.state[b][k]
+    for i in range(3, 5):
+        for n, o in ((net, opt), (twin, other)):
+            grads(n, i)
+            o.step()
+    assert all(torch.equal(a, b) for a, b in zip(net.parameters(), twin.parameters()))
+
+
+def test_torch_optimizer_follows_the_stock_one_with_32_bit_state():
+    from shift_b200.optim import AdamW
+    torch.manual_seed(4)
+    a = [torch.nn.Parameter(torch.randn(50, 3)), torch.nn.Parameter(torch.randn(129))]
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    ours, stock = AdamW(a, lr=1e-2, state_bits=32), torch.optim.AdamW(b, lr=1e-2)
+    for i in range(5):
+        for p, q in zip(a, b):
+            p.grad = torch.randn(p.shape)
+            q.grad = p.grad.clone()
+        ours.step()
+        stock.step()
+    # both round each of five updates of at most 1e-2 and the weight a dozen times in fp32
+    for p, q in zip(a, b):
+        assert bool(((p - q).abs() <= 5 * 12 * 2.0 ** -24 * (q.abs() + 0.05)).all())
