@@ -6,8 +6,8 @@
 // Bound: DRAM.  It reads each value once and writes one byte per orientation;
 // a CTA owns one 128 x 128 tile, holds it in registers, and finds the row and
 // column maxima there, so the second orientation costs no second read.
-// 16384 x 1024 bf16: 13.3 us for one orientation (3.8 TB/s), 22.7 us for both
-// (3.0 TB/s); what is left is waiting, 16 warps fit an SM.
+// 16384 x 1024 bf16: 14 us for one orientation (3.5 TB/s), 18.4 us for both
+// (3.7 TB/s); what is left is waiting, 24 warps fit an SM.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -64,19 +64,9 @@ SB_DEVICE float part(uint32_t w, int hi) {
   return value(r, sizeof(T) == 4 ? 0 : hi);
 }
 
-SB_DEVICE float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a < INFINITY ? a : 0.f;      // false for NaN too
-}
-
-// The conversion saturates: an infinity becomes NaN in e4m3, which has none, and stays one in e5m2.
-template <int FMT>
-SB_DEVICE uint32_t patch_infinities(uint32_t w, const float* y) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (isinf(y[j])) w = (w & ~(0xFFu << (8 * j))) | ((FMT == kE4M3 ? 0x7Fu : (y[j] > 0 ? 0x7Cu : 0xFCu)) << (8 * j));
-  return w;
-}
+SB_DEVICE float as_float(float x) { return x; }
+SB_DEVICE float as_float(__half x) { return __half2float(x); }
+SB_DEVICE float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 struct QuantArgs {
   const void* x;
@@ -94,10 +84,10 @@ struct QuantArgs {
 // hold a row, a thread stores 16 codes of a row at once, and four rows of a
 // column are one word of the transposed tile.  Maxima are taken on pairs as
 // they were loaded.  (8 columns by 8 rows a thread, in fp32, issued 17 and 24
-// instructions a value for one and two orientations, 22.5 and 27.6 us for
+// instructions a value for one and two orientations: 22.5 and 27.6 us for
 // 16384 x 1024.)
 template <typename T, int FMT, bool TILES, bool BOTH>
-__global__ void __launch_bounds__(kQThreads)
+__global__ void __launch_bounds__(kQThreads, BOTH && sizeof(T) == 2 ? 3 : 1)
 quantize_kernel(const QuantArgs a) {
   using R = Row16<T>;
   constexpr int kWords = R::kWords, kPer = 16 / kWords;   // values of a word
@@ -132,45 +122,38 @@ quantize_kernel(const QuantArgs a) {
     }
   }
 
-  // the largest magnitudes, of the rows and (pairwise) of the columns
-  float rmax[4], top = 0.f;
+  // The largest magnitudes, of the rows and (pairwise) of the columns.  Infinities do not count: a thread that meets
+  // one puts zeros in their place and looks again; their codes are set apart, from the input, at the end.
+  float rmax[4];
   uint32_t cmax[kWords];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int q = 0; q < kWords; ++q) {
-      const uint32_t w = magnitude<T>(v[i].w[q]);
-      m = larger<T>(m, w);
-      if (kCols) cmax[q] = i == 0 ? larger<T>(0u, w) : larger<T>(cmax[q], w);
-    }
-    rmax[i] = fmaxf(part<T>(m, 0), part<T>(m, 1));
-    top = fmaxf(top, rmax[i]);
-  }
-  // infinities do not count: a thread that met one looks again without them
-  const bool infinite = top == INFINITY;
-  if (infinite) {
+  bool infinite = false;
+#pragma unroll 1
+  while (true) {
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      rmax[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) rmax[i] = fmaxf(rmax[i], finite_abs(value(v[i], j)));
-    }
-    if (kCols) {
+      uint32_t m = 0u;
 #pragma unroll
       for (int q = 0; q < kWords; ++q) {
-        cmax[q] = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w = magnitude<T>(v[i].w[q]);
-#pragma unroll
-          for (int h = 0; h < kPer; ++h)
-            if (!(part<T>(w, h) < INFINITY)) w &= kPer == 1 ? 0u : (h ? 0x0000FFFFu : 0xFFFF0000u);
-          cmax[q] = larger<T>(cmax[q], w);
-        }
+        const uint32_t w = magnitude<T>(v[i].w[q]);
+        m = larger<T>(m, w);
+        if (kCols) cmax[q] = i == 0 ? larger<T>(0u, w) : larger<T>(cmax[q], w);
       }
+      rmax[i] = fmaxf(part<T>(m, 0), part<T>(m, 1));
+      top = fmaxf(top, rmax[i]);
     }
+    if (top != INFINITY) break;
+    infinite = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < kWords; ++q)
+#pragma unroll
+        for (int h = 0; h < kPer; ++h)
+          if (fabsf(part<T>(v[i].w[q], h)) == INFINITY) v[i].w[q] &= kPer == 1 ? 0u : (h ? 0x0000FFFFu : 0xFFFF0000u);
   }
+  // code of an infinity: NaN in e4m3, which has none
+  auto infinity_code = [](float f) -> uint8_t { return FMT == kE4M3 ? 0x7F : (f > 0.f ? 0x7C : 0xFC); };
 
   int rbyte[4];
   float rinv[4];
@@ -207,9 +190,17 @@ quantize_kernel(const QuantArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = value(v[i], 4 * h + j) * rinv[i];
       w[h] = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
-      if (infinite) w[h] = patch_infinities<FMT>(w[h], y);
     }
     if (r0 + i < a.rows && c0 < a.cols) *reinterpret_cast<uint4*>(q + i * a.ldq) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (infinite) {
+#pragma unroll 1
+    for (int e = 0; e < 64; ++e) {
+      const int i = e / 16, j = e % 16;
+      if (r0 + i >= a.rows || c0 + j >= a.cols) continue;
+      const float f = as_float(x[i * a.ld + j]);
+      if (fabsf(f) == INFINITY) q[i * a.ldq + j] = infinity_code(f);
+    }
   }
   // scale bytes of this tile, and zeros for the columns that the last word lacks: four lanes of a row group, a row each
   if (cg < 4 && r0 + cg < a.rows) {
@@ -221,6 +212,11 @@ quantize_kernel(const QuantArgs a) {
   }
 
   if constexpr (BOTH) {
+    // The values are unpacked anew: kept from above they would fill 64 registers and halve the CTAs of an SM.
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) asm volatile("" : "+r"(v[i].w[w]));
     if constexpr (kCols) {
 #pragma unroll
       for (int w = 0; w < kWords; ++w) {
@@ -257,8 +253,17 @@ quantize_kernel(const QuantArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = value(v[i], j) * inv;
       uint32_t w = pack2(y[0], y[1], FMT) | (pack2(y[2], y[3], FMT) << 16);
-      if (infinite) w = patch_infinities<FMT>(w, y);
       s_t[(cg * 16 + j) * 32 + (rg ^ (4 * cg))] = w;
+    }
+    if (infinite) {
+#pragma unroll 1
+      for (int e = 0; e < 64; ++e) {
+        const int i = e / 16, j = e % 16;
+        if (r0 + i >= a.rows || c0 + j >= a.cols) continue;
+        const float f = as_float(x[i * a.ld + j]);
+        if (fabsf(f) == INFINITY)
+          reinterpret_cast<uint8_t*>(&s_t[(cg * 16 + j) * 32 + (rg ^ (4 * cg))])[i] = infinity_code(f);
+      }
     }
     __syncthreads();
 #pragma unroll
