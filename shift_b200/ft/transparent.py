@@ -148,7 +148,9 @@ class TransparentRuntime:
         for o, sd in zip(self.optimizers, payload["optimizers"]):
             o.load_state_dict(sd)
         self.progress.update(payload["progress"])
-        torch.set_rng_state(payload["torch_rng"])
+        # a copy of its own: in the received buffer it starts wherever other byte tensors (8-bit optimizer state) end,
+        # and the generator reads it as aligned words
+        torch.set_rng_state(payload["torch_rng"].clone())
         random.setstate(payload["python_rng"])
         ok = self.hashes() == payload["hashes"]
         self.event("restored", step=payload["step"], load_seconds=time.monotonic() - t0, hashes_match=ok,
