@@ -296,3 +296,31 @@ def test_another_stream_and_a_captured_graph():
     eager = layer()
     _done()
     assert all(torch.equal(a, b) for a, b in zip(replayed, eager))
+
+
+def test_two_streams_at_once():
+    """Products, split ones among them, on two streams that nothing orders, next to bf16 products."""
+    from shift_b200.ops import gemm as G
+    cases = [_pair(384, 256, 8192), _pair(1000, 1344, 1024), _pair(1, 4096, 512), _pair(300, 200, 5000)]
+    want = [fp8.matmul(a, b, out_dtype=torch.float32) for a, b in cases]
+    x, w = _matrix(512, 256, 1, spread=0.1), _matrix(384, 256, 2, spread=0.1)
+    plain = G.linear_fwd(x, w)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for turn in range(10):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                order = cases if k == 0 else cases[::-1]
+                got[k] = [fp8.matmul(a, b, out_dtype=torch.float32) for a, b in order] + [G.linear_fwd(x, w)]
+    _done()
+    for k in range(2):
+        mine = got[k][:-1] if k == 0 else got[k][:-1][::-1]
+        assert all(torch.equal(a, b) for a, b in zip(mine, want)) and torch.equal(got[k][-1], plain)
+
+
+def test_the_same_operand_twice_and_its_own_sum():
+    a, _ = _pair(300, 16, 700)
+    y = fp8.matmul(a, a, out_dtype=torch.float32)
+    _done()
+    orc.check_product(y, orc.values(a), orc.values(a))
