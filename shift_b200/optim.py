@@ -230,6 +230,6 @@ class AdamW(torch.optim.Optimizer):
                                      [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
                     held = self._many[(k, ps[0])] = (ps, many)
                 beta1, beta2 = group["betas"]
-                held[1].step([p.grad for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
+                held[1].step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
                              wd=group["weight_decay"], step=int(t))
         return loss
