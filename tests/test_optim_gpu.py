@@ -114,3 +114,28 @@ def test_skip_flag_nonfinite_and_a_captured_step():
     grads[4][5] = float("nan")
     opt.step(grads, nonfinite=flag, step=3, **H)
     assert int(flag) == 1
+
+
+@pytest.mark.parametrize("bits,master", [(8, True), (32, False)])
+def test_torch_optimizer_on_the_gpu_follows_the_cpu(bits, master):
+    """Ten steps from the same start: weights of both agree to the moments' rounding borders (8 bits: a few values in
+    10^4 may take the next code, 2^-3 of a moment, in one step; an update of lr 1e-3 then moves by at most 2.5e-4)."""
+    from shift_b200.optim import AdamW
+
+    def run(device):
+        torch.manual_seed(5)
+        ps = [torch.nn.Parameter(torch.randn(s).to(device)) for s in ((300, 40), (1000,), (3, 5, 7))]
+        opt = AdamW(ps, lr=1e-3, state_bits=bits, master_weights=master)
+        g = torch.Generator().manual_seed(6)
+        for _ in range(10):
+            for p in ps:
+                p.grad = torch.randn(p.shape, generator=g).to(device)
+                if p.dim() == 2:
+                    p.grad = p.grad.t().contiguous().t()         # another layout
+            opt.step()
+        return [p.detach().cpu() for p in ps]
+
+    for a, b in zip(run(DEV), run("cpu")):
+        off = (a - b).abs()
+        assert float((off > 1e-6 + 16 * 2.0 ** -24 * b.abs()).float().mean()) <= (1e-2 if bits == 8 else 0.0)
+        assert float(off.max()) <= (10 * 2.5e-4 if bits == 8 else 1e-5)
