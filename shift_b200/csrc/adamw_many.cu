@@ -10,9 +10,12 @@
 // elements (fp8.cuh).  r instead of v halves the exponent range that the codes
 // have to cover.  Magnitudes are rounded up with the probability of their
 // distance from the code below: v moves by a thousandth per step against a
-// half step of 6 %, so rounding to nearest would freeze it.  The random bits
-// are a counter hash of (seed, tensor number, element), hence the same for any
-// launch shape; elements 2^32 apart share them.
+// half step of 6 %, so rounding to nearest would freeze it.  A root above zero
+// never goes to code 0, though: m of the same element may keep a code, and an
+// update divided by nothing is hundreds of learning rates (an element 1e-6 of
+// its block's largest).  At code 1 its update is too small instead.  The random
+// bits are a counter hash of (seed, tensor number, element), hence the same for
+// any launch shape; elements 2^32 apart share them.
 //
 // Bound: DRAM with 32-bit moments (0.494 B elements: 2.05 ms, 6.7 TB/s);
 // instructions with 8-bit ones (1.88 ms, 4.2 TB/s, 94 instructions an element).
@@ -161,7 +164,9 @@ SB_DEVICE void load_codes(const uint8_t* p, float scale, int valid, bool vec, fl
 }
 
 // Eight values of a block of 128 (16 lanes) to codes; returns the scale byte.
-SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits, int valid, bool vec) {
+// ROOT: values of zero or more, of which those above zero get code 1 at least.
+template <bool ROOT>
+SB_DEVICE int store_codes(uint8_t* p, float* f, const uint32_t* bits, int valid, bool vec) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) top = fmaxf(top, fabsf(f[i]));
@@ -174,6 +179,16 @@ SB_DEVICE int store_codes(uint8_t* p, const float* f, const uint32_t* bits, int 
   for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const int byte = fp8::scale_byte(top, fp8::kE4M3);
   const float inv = fp8::inv_scale(byte);
+  if constexpr (ROOT) {
+    const float one = fp8::scale_of(byte) * 0.001953125f;      // what code 1 stands for, exactly
+    float low = f[0];
+#pragma unroll
+    for (int i = 1; i < kVec; ++i) low = fminf(low, f[i]);
+    if (low < one) {                             // rare: a look at each of the eight only then
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) f[i] = f[i] > 0.f ? fmaxf(f[i], one) : f[i];
+    }
+  }
   uint32_t raw[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < kVec; i += 2) {
@@ -251,8 +266,8 @@ adamw_many_kernel(const __grid_constant__ Table tab, StepArgs a) {
       um[i] = (u << 4) & 0xFFFF0u;               // in place below the kept fraction bits
       uv[i] = (u >> 12) & 0xFFFF0u;
     }
-    const int bm = store_codes(static_cast<uint8_t*>(e.m) + i0, m, um, valid, vec);
-    const int bv = store_codes(static_cast<uint8_t*>(e.v) + i0, r, uv, valid, vec);
+    const int bm = store_codes<false>(static_cast<uint8_t*>(e.m) + i0, m, um, valid, vec);
+    const int bv = store_codes<true>(static_cast<uint8_t*>(e.v) + i0, r, uv, valid, vec);
     if (threadIdx.x % 16 == 0 && valid > 0) {
       e.ms[block] = static_cast<uint8_t>(bm);
       e.vs[block] = static_cast<uint8_t>(bv);

@@ -207,12 +207,15 @@ def moment_decode(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return code.float() * fp8_scales(scale).repeat_interleave(128)[: code.numel()]
 
 
-def moment_encode(x: torch.Tensor, bits16: torch.Tensor):
+def moment_encode(x: torch.Tensor, bits16: torch.Tensor, root: bool = False):
     """x fp32 [n] -> (codes float8_e4m3fn [n], scales float8_e8m0fnu [ceil(n / 128)]); a magnitude goes to the
-    code above with the probability of its distance from the one below."""
+    code above with the probability of its distance from the one below.  ``root``: x are roots of second moments, of
+    which those above zero get code 1 at least (an update is divided by them)."""
     n = x.numel()
     b, inv = fp8_block_scale(F.pad(_finite_abs(x), (0, -n % 128)).view(-1, 128).amax(-1), "e4m3")
     y = (x * inv.repeat_interleave(128)[:n]).abs()
+    if root:
+        y = torch.where(x > 0, y.clamp(min=2.0 ** -9), y)
     shift = torch.where(y < 2.0 ** -6, 2.0 ** -6, 0.0)
     t = (((y + shift).view(torch.int32) + (bits16 << 4).int()) & ~0xFFFFF).view(torch.float32) - shift
     t = torch.where(torch.isfinite(x), torch.copysign(t, x), torch.full_like(t, math.nan))

@@ -9,7 +9,10 @@ tensors of their own (an ordinary module, a model that is not ours).
 
 8-bit moments take 2 + 1/64 bytes per parameter instead of 8.  ``exp_avg`` and
 the square root of ``exp_avg_sq`` are e4m3 codes with one power-of-two scale
-per 128 consecutive elements, rounded stochastically from ``seed``.
+per 128 consecutive elements, rounded stochastically from ``seed``.  The codes
+span 18 binades: an element whose gradients are smaller than 4e-6 of its
+block's largest is updated as if its root were that large, so by less than with
+32-bit moments.
 """
 from __future__ import annotations
 
@@ -150,8 +153,8 @@ class AdamWMany:
             new = w.float() * (1.0 - lr * wd) - (lr / c1) * (m32 / (r / c2 + eps))
             if self.eight:
                 u = ref.moment_draws(g.numel(), seed, t)
-                for s, x, bits in ((m, m32, u & 0xFFFF), (v, r, u >> 16)):
-                    code, scale = ref.moment_encode(x, bits)
+                for s, x, bits, root in ((m, m32, u & 0xFFFF, False), (v, r, u >> 16, True)):
+                    code, scale = ref.moment_encode(x, bits, root)
                     s.code.view(-1).copy_(code)
                     s.scale.copy_(scale)
             else:
