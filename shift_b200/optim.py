@@ -225,14 +225,18 @@ class AdamW(torch.optim.Optimizer):
                 self.state[p]["step"] += 1
                 by_step.setdefault((self.state[p]["step"], p.device), []).append(p)
             for (t, _), ps in by_step.items():
-                # the lists of a group are checked and handed over once, as long as the same parameters take part
+                # the lists of a group are checked and handed over once, as long as the same tensors take part: state can
+                # be cleared, or given other tensors or other memory
+                use = [group["state_bits"], group["master_weights"], *ps]
+                use += [x for p in ps for x in self.state[p].values() if isinstance(x, torch.Tensor)]
+                at = [x.data_ptr() for x in use[2 + len(ps):]]
                 held = self._many.get((k, ps[0]))
-                if held is None or len(held[0]) != len(ps) or any(a is not b for a, b in zip(held[0], ps)):
+                if held is None or len(held[0]) != len(use) or held[1] != at or any(a is not b for a, b in zip(held[0], use)):
                     many = AdamWMany(ps, [self._moment(p, "exp_avg", group) for p in ps],
                                      [self._moment(p, "exp_avg_sq", group) for p in ps],
                                      [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
-                    held = self._many[(k, ps[0])] = (ps, many)
+                    held = self._many[(k, ps[0])] = (use, at, many)
                 beta1, beta2 = group["betas"]
-                held[1].step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
+                held[2].step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
                              wd=group["weight_decay"], step=int(t))
         return loss

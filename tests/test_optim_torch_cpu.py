@@ -1,0 +1,70 @@
+"""``optim.AdamW`` as scripts handle a torch optimizer: state that is cleared, replaced, copied or saved by others."""
+import pytest
+import torch
+
+from shift_b200.optim import AdamW
+
+KINDS = [(8, False), (8, True), (32, False), (32, True)]
+
+
+def params(seed=0, dtype=torch.float32, shapes=((40, 7), (130,))):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=g).to(dtype)) for s in shapes]
+
+
+def grads(ps, i):
+    g = torch.Generator().manual_seed(100 + i)
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g).to(p.dtype)
+
+
+def run(ps, opt, turns):
+    for i in turns:
+        grads(ps, i)
+        opt.step()
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def same_state(a, pa, b, pb):
+    for p, q in zip(pa, pb):
+        assert a.state[p].keys() == b.state[q].keys()
+        for k, x in a.state[p].items():
+            assert torch.equal(x, b.state[q][k]) if isinstance(x, torch.Tensor) else x == b.state[q][k]
+
+
+# ----------------------------------------------------------------------------- state from outside
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_cleared_state_starts_anew(bits, master):
+    ps = params()
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, master_weights=master)
+    run(ps, opt, range(3))
+    opt.state.clear()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = AdamW(qs, lr=1e-2, state_bits=bits, master_weights=master)
+    run(ps, opt, [5, 6])
+    run(qs, other, [5, 6])
+    assert same(ps, qs)
+    same_state(opt, ps, other, qs)
+
+
+@pytest.mark.parametrize("how", ["tensor", "memory"])
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_replaced_state_is_used_and_updated(bits, master, how):
+    ps, qs = params(), params()
+    opt, other = (AdamW(x, lr=1e-2, state_bits=bits, master_weights=master) for x in (ps, qs))
+    run(ps, opt, range(3))
+    run(qs, other, [7])
+    for p, q in zip(ps, qs):                           # the other optimizer's state, as it is after one step
+        p.data.copy_(q.data)
+        for k, x in other.state[q].items():
+            if isinstance(x, torch.Tensor) and how == "memory":
+                opt.state[p][k].data = x.clone()
+            else:
+                opt.state[p][k] = x.clone() if isinstance(x, torch.Tensor) else x
+    run(ps, opt, [8, 9])
+    run(qs, other, [8, 9])
+    assert same(ps, qs)
+    same_state(opt, ps, other, qs)
