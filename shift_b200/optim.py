@@ -181,6 +181,10 @@ class AdamW(torch.optim.Optimizer):
                                       master_weights=master_weights))
         self._many: dict = {}
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._many = {}                                # a copy or an unpickled optimizer has tensors of its own
+
     def _init_state(self, p, group):
         st = self.state[p]
         st["step"] = 0

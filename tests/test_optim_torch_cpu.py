@@ -1,4 +1,7 @@
 """``optim.AdamW`` as scripts handle a torch optimizer: state that is cleared, replaced, copied or saved by others."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -66,5 +69,23 @@ def test_replaced_state_is_used_and_updated(bits, master, how):
                 opt.state[p][k] = x.clone() if isinstance(x, torch.Tensor) else x
     run(ps, opt, [8, 9])
     run(qs, other, [8, 9])
+    assert same(ps, qs)
+    same_state(opt, ps, other, qs)
+
+
+# ----------------------------------------------------------------------------- copies
+@pytest.mark.parametrize("started", [False, True])
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_copies_go_on_by_themselves(bits, master, how, started):
+    ps = params()
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, master_weights=master)
+    run(ps, opt, range(2 if started else 0))
+    other = how(opt)
+    qs = other.param_groups[0]["params"]
+    before = [p.detach().clone() for p in ps]
+    run(qs, other, [5, 6])
+    assert same(ps, before)                            # the copy has its own tensors
+    run(ps, opt, [5, 6])
     assert same(ps, qs)
     same_state(opt, ps, other, qs)
