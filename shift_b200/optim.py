@@ -220,27 +220,46 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for k, group in enumerate(self.param_groups):
-            live = [p for p in group["params"] if p.grad is not None]
-            by_step: dict = {}
-            for p in live:
-                if "step" not in self.state[p]:
-                    self._init_state(p, group)
-                self.state[p]["step"] += 1
-                by_step.setdefault((self.state[p]["step"], p.device), []).append(p)
-            for (t, _), ps in by_step.items():
-                # the lists of a group are checked and handed over once, as long as the same tensors take part: state can
-                # be cleared, or given other tensors or other memory
-                use = [group["state_bits"], group["master_weights"], *ps]
-                use += [x for p in ps for x in self.state[p].values() if isinstance(x, torch.Tensor)]
-                at = [x.data_ptr() for x in use[2 + len(ps):]]
-                held = self._many.get((k, ps[0]))
-                if held is None or len(held[0]) != len(use) or held[1] != at or any(a is not b for a, b in zip(held[0], use)):
-                    many = AdamWMany(ps, [self._moment(p, "exp_avg", group) for p in ps],
-                                     [self._moment(p, "exp_avg_sq", group) for p in ps],
-                                     [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
-                    held = self._many[(k, ps[0])] = (use, at, many)
-                beta1, beta2 = group["betas"]
-                held[2].step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
-                             wd=group["weight_decay"], step=int(t))
+        jobs, made = [], []
+        try:                                           # all that may be refused comes before the first update
+            for k, group in enumerate(self.param_groups):
+                self._gather(k, group, jobs, made)
+        except Exception:
+            for p in made:
+                del self.state[p]
+            raise
+        for group, t, ps, many in jobs:
+            beta1, beta2 = group["betas"]
+            many.step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2,
+                      eps=group["eps"], wd=group["weight_decay"], step=t)
+            for p in ps:
+                self.state[p]["step"] = t
         return loss
+
+    def _gather(self, k, group, jobs, made):
+        """Adds group ``k``'s (group, step, parameters, AdamWMany) to ``jobs``, parameters with new state to ``made``."""
+        by_step: dict = {}
+        for p in group["params"]:
+            if p.grad is None:
+                continue
+            g = p.grad
+            if g.layout != torch.strided or g.dtype not in _FLOATS or g.shape != p.shape or g.device != p.device:
+                raise ValueError(f"AdamW: gradient {tuple(g.shape)} of {g.dtype}, {g.layout}, on {g.device} for a "
+                                 f"parameter {tuple(p.shape)} on {p.device}: dense, fp32 / bf16 / fp16, beside it")
+            if "step" not in self.state[p]:
+                made.append(p)
+                self._init_state(p, group)
+            by_step.setdefault((int(self.state[p]["step"]) + 1, p.device), []).append(p)
+        for (t, _), ps in by_step.items():
+            # the lists of a group are checked and handed over once, as long as the same tensors take part: state can
+            # be cleared, or given other tensors or other memory
+            use = [group["state_bits"], group["master_weights"], *ps]
+            use += [x for p in ps for x in self.state[p].values() if isinstance(x, torch.Tensor)]
+            at = [x.data_ptr() for x in use[2 + len(ps):]]
+            held = self._many.get((k, ps[0]))
+            if held is None or len(held[0]) != len(use) or held[1] != at or any(a is not b for a, b in zip(held[0], use)):
+                many = AdamWMany(ps, [self._moment(p, "exp_avg", group) for p in ps],
+                                 [self._moment(p, "exp_avg_sq", group) for p in ps],
+                                 [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
+                held = self._many[(k, ps[0])] = (use, at, many)
+            jobs.append((group, t, ps, held[2]))

@@ -89,3 +89,36 @@ def test_copies_go_on_by_themselves(bits, master, how, started):
     run(ps, opt, [5, 6])
     assert same(ps, qs)
     same_state(opt, ps, other, qs)
+
+
+# ----------------------------------------------------------------------------- refusals
+def _double(p):
+    p.data = p.data.double()
+    p.grad = torch.ones_like(p)
+
+
+def _sparse(p):
+    p.grad = torch.ones_like(p).to_sparse()
+
+
+@pytest.mark.parametrize("started", [False, True])
+@pytest.mark.parametrize("spoil", [_double, _sparse])
+def test_a_refused_step_changes_nothing(spoil, started):
+    ps, bad = params(), torch.nn.Parameter(torch.randn(30, 4))
+    opt = AdamW([{"params": ps, "lr": 1e-2}, {"params": [bad]}], state_bits=8)
+    if started:
+        run(ps + [bad], opt, range(2))
+    kept = bad.data
+    grads(ps, 7)
+    spoil(bad)
+    before, state = [p.detach().clone() for p in ps], copy.deepcopy(opt.state_dict()["state"])
+    with pytest.raises(ValueError):
+        opt.step()
+    assert same(ps, before)
+    now = opt.state_dict()["state"]
+    assert now.keys() == state.keys()
+    for i, x in state.items():
+        assert all(torch.equal(y, now[i][k]) if isinstance(y, torch.Tensor) else y == now[i][k] for k, y in x.items())
+    bad.grad, bad.data = None, kept
+    opt.step()
+    assert [opt.state[p]["step"] for p in ps] == [3 if started else 1] * 2
