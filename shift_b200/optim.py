@@ -220,6 +220,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        place = {p: i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
         jobs, made = [], []
         try:                                           # all that may be refused comes before the first update
             for k, group in enumerate(self.param_groups):
@@ -228,10 +229,11 @@ class AdamW(torch.optim.Optimizer):
             for p in made:
                 del self.state[p]
             raise
+        # the random bits hang on the seed and on a tensor's number in its list: each list has a seed of its own
         for group, t, ps, many in jobs:
             beta1, beta2 = group["betas"]
             many.step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2,
-                      eps=group["eps"], wd=group["weight_decay"], step=t)
+                      eps=group["eps"], wd=group["weight_decay"], step=t, seed=t + 0x9E3779B1 * place[ps[0]])
             for p in ps:
                 self.state[p]["step"] = t
         return loss

@@ -122,3 +122,28 @@ def test_a_refused_step_changes_nothing(spoil, started):
     bad.grad, bad.data = None, kept
     opt.step()
     assert [opt.state[p]["step"] for p in ps] == [3 if started else 1] * 2
+
+
+# ----------------------------------------------------------------------------- random bits
+@pytest.mark.parametrize("late", [False, True])
+def test_groups_do_not_share_random_bits(late):
+    """Two equal tensors, in two groups or at two step counts of one: codes that are rounded by independent bits differ
+    in about a quarter of the places and more (a value within its step is uniform: 2 u (1 - u), 1/3 in the mean)."""
+    w, g = torch.randn(2, 4096, generator=torch.Generator().manual_seed(2)).unbind()
+    ps = [torch.nn.Parameter(w.clone()) for _ in range(2)]
+    opt = AdamW(ps if late else [{"params": [p]} for p in ps], state_bits=8)
+    if late:                                           # the second one has steps of its own from here on
+        ps[0].grad = torch.zeros(4096)
+        opt.step()
+    ps[0].grad, ps[1].grad = g.clone(), g.clone()
+    opt.step()
+    if late:
+        assert [opt.state[p]["step"] for p in ps] == [2, 1]
+    off = (opt.state[ps[0]]["exp_avg"] != opt.state[ps[1]]["exp_avg"]).double().mean()
+    assert float(off) > 0.2
+    # and a parameter alone still takes the bits of its step
+    alone = AdamW([torch.nn.Parameter(w.clone())], state_bits=8)
+    alone.param_groups[0]["params"][0].grad = g.clone()
+    alone.step()
+    if not late:
+        assert torch.equal(alone.state[alone.param_groups[0]["params"][0]]["exp_avg"], opt.state[ps[0]]["exp_avg"])
