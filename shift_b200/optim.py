@@ -171,7 +171,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``master_weights`` keeps fp32 weights beside bf16 or fp16 parameters.  Under ``ft.transparent`` it is adopted like
     any other optimizer: its state is part of ``state_dict`` and heals with it.  State tensors are made at a
-    parameter's first gradient; a parameter without a gradient is left alone in that step."""
+    parameter's first gradient; a parameter without a gradient is left alone in that step.  State is row-major whatever
+    a parameter's layout; a parameter that is not (channels_last, transposed) is copied to that order and back."""
 
     def __init__(self, params, lr: float = 1.0e-3, betas=(0.9, 0.999), eps: float = 1.0e-8, weight_decay: float = 1.0e-2,
                  state_bits: int = 8, master_weights: bool = False):
@@ -180,10 +181,11 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights))
         self._many: dict = {}
+        self._packed: dict = {}                        # row-major copies of parameters of another layout
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._many = {}                                # a copy or an unpickled optimizer has tensors of its own
+        self._many, self._packed = {}, {}              # a copy or an unpickled optimizer has tensors of its own
 
     def _init_state(self, p, group):
         st = self.state[p]
@@ -196,7 +198,10 @@ class AdamW(torch.optim.Optimizer):
             else:
                 st[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         if group["master_weights"]:
-            st["master"] = p.detach().float().clone()
+            st["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+
+    def _flat(self, p):
+        return p if p.is_contiguous() else self._packed[p]
 
     def _moment(self, p, name, group):
         st = self.state[p]
@@ -231,9 +236,14 @@ class AdamW(torch.optim.Optimizer):
             raise
         # the random bits hang on the seed and on a tensor's number in its list: each list has a seed of its own
         for group, t, ps, many in jobs:
+            moved = [p for p in ps if not p.is_contiguous()]
+            for p in moved:
+                self._packed[p].copy_(p)
             beta1, beta2 = group["betas"]
             many.step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2,
                       eps=group["eps"], wd=group["weight_decay"], step=t, seed=t + 0x9E3779B1 * place[ps[0]])
+            for p in moved:
+                p.copy_(self._packed[p])
             for p in ps:
                 self.state[p]["step"] = t
         return loss
@@ -251,16 +261,21 @@ class AdamW(torch.optim.Optimizer):
             if "step" not in self.state[p]:
                 made.append(p)
                 self._init_state(p, group)
+            held = self._packed.get(p)
+            if p.is_contiguous():
+                self._packed.pop(p, None)
+            elif held is None or (held.shape, held.dtype, held.device) != (p.shape, p.dtype, p.device):
+                self._packed[p] = torch.empty(p.shape, dtype=p.dtype, device=p.device)
             by_step.setdefault((int(self.state[p]["step"]) + 1, p.device), []).append(p)
         for (t, _), ps in by_step.items():
             # the lists of a group are checked and handed over once, as long as the same tensors take part: state can
             # be cleared, or given other tensors or other memory
-            use = [group["state_bits"], group["master_weights"], *ps]
+            use = [group["state_bits"], group["master_weights"], *(self._flat(p) for p in ps)]
             use += [x for p in ps for x in self.state[p].values() if isinstance(x, torch.Tensor)]
             at = [x.data_ptr() for x in use[2 + len(ps):]]
             held = self._many.get((k, ps[0]))
             if held is None or len(held[0]) != len(use) or held[1] != at or any(a is not b for a, b in zip(held[0], use)):
-                many = AdamWMany(ps, [self._moment(p, "exp_avg", group) for p in ps],
+                many = AdamWMany([self._flat(p) for p in ps], [self._moment(p, "exp_avg", group) for p in ps],
                                  [self._moment(p, "exp_avg_sq", group) for p in ps],
                                  [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
                 held = self._many[(k, ps[0])] = (use, at, many)

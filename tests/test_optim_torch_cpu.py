@@ -147,3 +147,46 @@ def test_groups_do_not_share_random_bits(late):
     alone.step()
     if not late:
         assert torch.equal(alone.state[alone.param_groups[0]["params"][0]]["exp_avg"], opt.state[ps[0]]["exp_avg"])
+
+
+# ----------------------------------------------------------------------------- layouts
+def check_layouts(bits, master, device="cpu"):
+    """Parameters in other layouts are updated like their row-major copies, keep their layout, and state moves between."""
+    def make(other):
+        g = torch.Generator().manual_seed(4)
+        x = [torch.randn(6, 5, 4, 3, generator=g).to(device), torch.randn(40, 30, generator=g).to(device),
+             torch.randn(9, generator=g).to(device)]
+        if other:
+            x[0] = x[0].to(memory_format=torch.channels_last)
+            x[1] = x[1].t().contiguous().t()
+        ps = [torch.nn.Parameter(y) for y in x]
+        return ps, AdamW(ps, lr=1e-2, state_bits=bits, master_weights=master)
+
+    (ps, opt), (qs, other) = make(True), make(False)
+    for i in range(2):
+        for x, o in ((ps, opt), (qs, other)):
+            g = torch.Generator().manual_seed(100 + i)
+            for p in x:                                # a gradient in the parameter's layout
+                p.grad = torch.empty_like(p).copy_(torch.randn(p.shape, generator=g))
+            o.step()
+    assert ps[0].is_contiguous(memory_format=torch.channels_last) and not ps[1].is_contiguous()
+    assert same(ps, qs)
+    same_state(opt, ps, other, qs)
+    rs, third = make(True)
+    third.load_state_dict(other.state_dict())
+    for r, q in zip(rs, qs):
+        r.data.copy_(q.data)
+    for x, o in ((rs, third), (qs, other)):
+        for p in x:
+            p.grad = torch.empty_like(p).fill_(0.5)
+        o.step()
+    assert same(rs, qs)
+    rs[1].data = rs[1].data.contiguous()               # and back to row-major in the middle
+    for x, o in ((rs, third), (qs, other)):
+        o.step()
+    assert same(rs, qs)
+
+
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_parameters_of_any_layout(bits, master):
+    check_layouts(bits, master)
