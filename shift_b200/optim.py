@@ -210,14 +210,51 @@ class AdamW(torch.optim.Optimizer):
         return st[name]
 
     def load_state_dict(self, state_dict):
+        """Takes what this class saved, and what ``torch.optim.AdamW`` did: the group then keeps this optimizer's
+        ``state_bits`` and ``master_weights``, moments are rounded to nearest and master weights start from the
+        parameters.  Saved state of another rule (``amsgrad``, ``maximize``, coupled weight decay) is refused."""
+        kinds = [{name: g[name] for name in ("state_bits", "master_weights")} for g in self.param_groups]
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        for g in groups:
+            other = [name for name in ("amsgrad", "maximize") if g.get(name)]
+            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                other.append("coupled weight decay")
+            other += ["no " + name for name in ("lr", "betas", "eps", "weight_decay") if name not in g]
+            if other:
+                raise ValueError(f"AdamW: a saved state with {', '.join(other)}")
+            for i in () if "state_bits" in g else g["params"]:
+                if i in saved and not {"step", "exp_avg", "exp_avg_sq"} <= saved[i].keys():
+                    raise ValueError(f"AdamW: saved state with {sorted(saved[i])}, not step, exp_avg and exp_avg_sq")
         super().load_state_dict(state_dict)
-        # the base class casts floating-point and byte states to the parameter's type: put back what was saved
-        saved = state_dict["state"]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            for name, x in saved.get(i, {}).items():
-                self.state[p][name] = x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
+        for mine, theirs, kind in zip(self.param_groups, groups, kinds):
+            mine.update({name: x for name, x in kind.items() if name not in theirs})
+            for i, p in zip(theirs["params"], mine["params"]):
+                if i not in saved:
+                    continue
+                if "state_bits" not in theirs:
+                    self._take(p, mine, saved[i])
+                    continue
+                # the base class casts floating-point and byte states to the parameter's type: put back what was saved
+                for name, x in saved[i].items():
+                    self.state[p][name] = x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
         self._many.clear()
+
+    def _take(self, p, group, saved):
+        """State of ``p`` from that of torch.optim.AdamW: moments of the parameter's shape in any floating type."""
+        self.state.pop(p, None)
+        self._init_state(p, group)
+        st = self.state[p]
+        st["step"] = int(saved["step"])
+        m, v = (saved[name].to(p.device, torch.float32).contiguous() for name in ("exp_avg", "exp_avg_sq"))
+        if group["state_bits"] == 32:
+            st["exp_avg"].copy_(m)
+            st["exp_avg_sq"].copy_(v)
+            return
+        half = torch.full((p.numel(),), 0x8000, device=p.device)
+        for name, x, root in (("exp_avg", m, False), ("exp_avg_sq", v.sqrt(), True)):
+            code, scale = ref.moment_encode(x.view(-1), half, root)
+            st[name].copy_(code.view(torch.uint8))
+            st[name + "_scale"].copy_(scale.view(torch.uint8))
 
     @torch.no_grad()
     def step(self, closure=None):

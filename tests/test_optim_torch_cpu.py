@@ -190,3 +190,83 @@ def check_layouts(bits, master, device="cpu"):
 @pytest.mark.parametrize("bits,master", KINDS)
 def test_parameters_of_any_layout(bits, master):
     check_layouts(bits, master)
+
+
+# ----------------------------------------------------------------------------- another optimizer's state
+def stock_state(dtype=torch.float32, device="cpu", **kw):
+    ps = [torch.nn.Parameter(p.detach().to(device)) for p in params(1, dtype)]
+    ps[0].data = ps[0].data.t().contiguous().t()       # its moments have this layout too
+    opt = torch.optim.AdamW(ps, lr=3e-3, weight_decay=0.1, **kw)
+    run_on(ps, opt, range(4))
+    return ps, opt
+
+
+def run_on(ps, opt, turns):
+    for i in turns:
+        g = torch.Generator().manual_seed(100 + i)
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g).to(p)
+        opt.step()
+
+
+def check_stock_state(bits, master, dtype, device="cpu"):
+    qs, stock = stock_state(dtype, device)
+    ps = [torch.nn.Parameter(q.detach().clone(memory_format=torch.contiguous_format)) for q in qs]
+    opt = AdamW(ps, state_bits=bits, master_weights=master)
+    opt.load_state_dict(stock.state_dict())
+    assert opt.param_groups[0]["lr"] == 3e-3 and opt.param_groups[0]["state_bits"] == bits
+    for p, q in zip(ps, qs):
+        assert opt.state[p]["step"] == 4
+        for name in ("exp_avg", "exp_avg_sq"):
+            want = stock.state[q][name].double().reshape(-1)
+            if bits == 32:
+                assert torch.equal(opt.state[p][name].double().reshape(-1), want)
+                continue
+            want = want if name == "exp_avg" else want.sqrt()
+            got = opt._moment(p, name, opt.param_groups[0])
+            # half a step: 2^-4 of the value, 2^-10 of the scale below the smallest normal code, and a root's code 1
+            low = got.scale.double().repeat_interleave(128)[: p.numel()] * 2.0 ** (-10 if name == "exp_avg" else -9)
+            assert bool(((got.values().double() - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, low) * (1 + 1e-6)).all())
+    before = [(p.detach().double(), *(stock.state[q][name].double() for name in ("exp_avg", "exp_avg_sq")))
+              for p, q in zip(ps, qs)]
+    run_on(ps, opt, [9])
+    run_on(qs, stock, [9])
+    lr, c1, c2 = 3e-3, 1 - 0.9 ** 5, (1 - 0.999 ** 5) ** 0.5
+    for p, q, (w, m, v) in zip(ps, qs, before):
+        # One step from equal weights.  8 bits: exp_avg off by 1/16 of itself (or 2^-10 of a scale, at most its block's
+        # largest / 224), the root by 1/16 of itself.  Then the roundings: the weight to its type on either side, the
+        # stock one's bf16 state (half a step of 2^-8 on m and v each), and 32 for fp32.
+        g = p.grad.double()
+        m1, r1 = 0.9 * m + 0.1 * g, (0.999 * v + 0.001 * g * g).sqrt()
+        update = lr / c1 * m1.abs() / (r1 / c2)
+        dm = 0.9 * torch.maximum(m.abs() / 16, m.abs().max() / 224 * 2.0 ** -10) if bits == 8 else torch.zeros_like(m)
+        tol = lr / c1 * dm / (r1 * 15 / 16 / c2) + (update / 15 if bits == 8 else 0)
+        half = torch.finfo(dtype).eps / 2
+        tol += 4 * half * (w.abs() + lr) + 3 * half * lr / c1 * (m1.abs() + 0.9 * m.abs()) / (r1 / c2) + 32 * 2.0 ** -24 * (w.abs() + update)
+        assert not torch.equal(p.double(), w)
+        assert bool(((p.double() - q.double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_the_stock_optimizers_saved_state(bits, master, dtype):
+    check_stock_state(bits, master, dtype)
+
+
+def test_saved_state_of_other_rules_is_refused():
+    ps = params(1)
+    opt = AdamW(ps, lr=1e-2)
+    run(ps, opt, [0])
+    before = copy.deepcopy(opt.state_dict())
+    for sd in (stock_state(amsgrad=True)[1].state_dict(), stock_state(maximize=True)[1].state_dict()):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(sd)
+    adam = torch.optim.Adam(params(1), weight_decay=0.1)
+    sgd = torch.optim.SGD(params(1), lr=0.1, momentum=0.9)
+    for other in (adam, sgd):
+        run(other.param_groups[0]["params"], other, [0])
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other.state_dict())
+    now = opt.state_dict()
+    assert now["param_groups"] == before["param_groups"]
+    assert all(torch.equal(x, now["state"][i][k]) for i, st in before["state"].items() for k, x in st.items() if k != "step")

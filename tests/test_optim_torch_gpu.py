@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from shift_b200.optim import AdamW
-from test_optim_torch_cpu import KINDS, check_layouts, same, same_state
+from test_optim_torch_cpu import KINDS, check_layouts, check_stock_state, same, same_state
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -55,3 +55,9 @@ def test_cleared_replaced_and_copied_state(bits, master):
         turn(x, o, 3)
     assert same(ps, qs)
     same_state(opt, ps, other, qs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits,master", KINDS)
+def test_the_stock_optimizers_saved_state(bits, master, dtype):
+    check_stock_state(bits, master, dtype, DEV)
