@@ -332,6 +332,12 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
     TORCH_CHECK_VALUE(!x->has_value() || ((*x)->scalar_type() == at::kInt && (*x)->is_contiguous() && (*x)->device() == dev &&
                                           (*x)->numel() >= (x == &step_dev ? 4 : 1)),
                       "AdamWMany: ", name, ": int32 on ", dev);
+  // one CTA writes the flag while others have yet to read these words
+  if (nonfinite.has_value())
+    for (const auto* x : {&skip, &step_dev})
+      TORCH_CHECK_VALUE(!x->has_value() || nonfinite->data_ptr<int>() < (*x)->data_ptr<int>() ||
+                            nonfinite->data_ptr<int>() >= (*x)->data_ptr<int>() + (x == &step_dev ? 4 : 1),
+                        "AdamWMany: nonfinite is a word that the step reads");
   const at::cuda::CUDAGuard guard(dev);
   StepArgs a;
   a.lr = static_cast<float>(lr);

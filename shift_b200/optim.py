@@ -112,7 +112,8 @@ class AdamWMany:
         bits, which replace the arguments (a replayed graph's step;
         ``engine.StepBlock`` writes that layout).  ``skip``: int32 on the
         device; where it is not zero nothing changes.  ``nonfinite``: int32
-        flag, set where a scaled gradient is not finite."""
+        flag, set where a scaled gradient is not finite.  ``skip`` is read
+        while ``nonfinite`` is written: not the same word."""
         if step < 1:
             raise ValueError(f"AdamWMany: step {step}: counted from 1")
         seed = (step if seed is None else seed) & 0xFFFFFFFF
@@ -130,6 +131,9 @@ class AdamWMany:
         for name, x, least in (("step_dev", step_dev, 4), ("skip", skip, 1), ("nonfinite", nonfinite, 1)):
             if x is not None and (x.dtype != torch.int32 or x.numel() < least or x.device != dev):
                 raise ValueError(f"AdamWMany: {name}: int32 [{least}] on {dev}")
+        if nonfinite is not None and any(x is not None and x.data_ptr() <= nonfinite.data_ptr() < x.data_ptr() + 4 * n
+                                         for x, n in ((skip, 1), (step_dev, 4))):
+            raise ValueError("AdamWMany: nonfinite is a word that the step reads")
         self._cpu_step(grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite)
 
     def _cpu_step(self, grads, lr, beta1, beta2, eps, wd, step, grad_scale, seed, step_dev, skip, nonfinite):

@@ -1,0 +1,21 @@
+"""What ``AdamWMany`` refuses on the GPU: the checks are the extension's."""
+import pytest
+import torch
+
+from test_optim_refusals_cpu import make, words
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("k", range(4))
+def test_the_flag_is_not_a_word_that_is_read(k):
+    opt, p, g = make(DEV)
+    skip, step_dev, flag = words(DEV)[k]
+    with pytest.raises(ValueError, match="nonfinite"):
+        opt.step(g, skip=skip, step_dev=step_dev, nonfinite=flag)
+    assert bool((p == 1).all())
+    block = torch.zeros(8, dtype=torch.int32, device=DEV)
+    block[1:4] = torch.tensor([1e-3, 0.1, 0.03]).view(torch.int32)
+    opt.step(g, step_dev=block, skip=block[4:], nonfinite=block[5:])          # neighbours are no matter
+    assert bool((p != 1).all())
