@@ -262,6 +262,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            # a replay would repeat this step's bias corrections and random bits and leave the counts behind
+            raise RuntimeError("AdamW: step() cannot be captured into a graph; AdamWMany.step takes step_dev for that")
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -270,3 +270,18 @@ def test_saved_state_of_other_rules_is_refused():
     now = opt.state_dict()
     assert now["param_groups"] == before["param_groups"]
     assert all(torch.equal(x, now["state"][i][k]) for i, st in before["state"].items() for k, x in st.items() if k != "step")
+
+
+def test_a_captured_step_is_refused(monkeypatch):
+    ps = params()
+    opt = AdamW(ps)
+    grads(ps, 0)
+    before = [p.detach().clone() for p in ps]
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    monkeypatch.undo()
+    assert same(ps, before) and not opt.state
+    opt.step()
+    assert opt.state[ps[0]]["step"] == 1

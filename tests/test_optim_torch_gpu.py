@@ -61,3 +61,21 @@ def test_cleared_replaced_and_copied_state(bits, master):
 @pytest.mark.parametrize("bits,master", KINDS)
 def test_the_stock_optimizers_saved_state(bits, master, dtype):
     check_stock_state(bits, master, dtype, DEV)
+
+
+def test_a_captured_step_is_refused():
+    """The refusal comes before any launch, so the capture ends as an empty one and the optimizer goes on."""
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = AdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+    assert opt.state[p]["step"] == 1
+    opt.step()
+    torch.cuda.synchronize()
+    assert opt.state[p]["step"] == 2 and bool((x == 0).all())
