@@ -86,8 +86,9 @@ class AdamWMany:
                 same.append(w)
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
             _fail(all(x.device == self.params[0].device for x in same), f"tensor {t} or its state is on another device")
-        own = [x.data_ptr() for p, *state in zip(self.params, *self._states()) for x in (p, *state) if x.numel()]
-        _fail(len(set(own)) == len(own), "a tensor is there twice, or two share memory")
+        own = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                     for p, *state in zip(self.params, *self._states()) for x in (p, *state) if x.numel())
+        _fail(all(end <= start for (_, end), (start, _) in zip(own, own[1:])), "a tensor is there twice, or two share memory")
         self._plan = None
         if n > 0 and self.params[0].is_cuda:
             lists = self._states()

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from shift_b200.optim import AdamWMany
+from shift_b200.optim import AdamWMany, State8
 
 
 def words(device="cpu"):
@@ -27,3 +27,24 @@ def test_the_flag_is_not_a_word_that_is_read(k):
     block[1:4] = torch.tensor([1e-3, 0.1, 0.03]).view(torch.int32)
     opt.step(g, step_dev=block, skip=block[4:], nonfinite=block[5:])          # neighbours are no matter
     assert bool((p != 1).all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_tensors_that_share_a_part_of_their_memory(eight):
+    def new(n):
+        return State8.zeros(torch.empty(n)) if eight else torch.zeros(n)
+
+    flat = torch.zeros(400)
+    a, b = flat[:200], flat[199:]
+    with pytest.raises(ValueError, match="share memory"):
+        AdamWMany([a, b], [new(200), new(201)], [new(200), new(201)])
+    with pytest.raises(ValueError, match="share memory"):
+        AdamWMany([torch.zeros(200), torch.zeros(201)], [new(200), new(201)], [new(200), new(201)], masters=[a, b])
+    if eight:
+        code = torch.zeros(300, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        s = new(200)
+        with pytest.raises(ValueError, match="share memory"):
+            AdamWMany([torch.zeros(200)], [s._replace(code=code[:200])], [s._replace(code=code[100:], scale=s.scale.clone())])
+    opt = AdamWMany([flat[:200], flat[200:]], [new(200), new(200)], [new(200), new(200)])         # neighbours may
+    opt.step([torch.ones(200), torch.ones(200)])
+    assert bool((flat < 0).all())
