@@ -35,6 +35,9 @@ setup(
             sources=sources,
             include_dirs=[os.path.join(ROOT, CSRC)],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": cuda_flags},
+            # A compiler that links its C++ library in statically would give the extension a second copy beside
+            # torch's, and a refusal that prints a number would end the process in the copy's locale tables.
+            extra_link_args=["-l:libstdc++.so.6"],
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
