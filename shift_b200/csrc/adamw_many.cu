@@ -300,12 +300,15 @@ static void launch_types(at::ScalarType g, const Table& t, const StepArgs& a, bo
 // and vs may be empty.  Addresses are read from the tensors at every step.
 struct Many {
   std::vector<at::Tensor> p, w, m, ms, v, vs;
+  c10::Device dev;
 };
 
 std::shared_ptr<Many> adamw_many_plan(std::vector<at::Tensor> p, std::vector<at::Tensor> w, std::vector<at::Tensor> m,
                                       std::vector<at::Tensor> ms, std::vector<at::Tensor> v,
                                       std::vector<at::Tensor> vs) {
-  return std::make_shared<Many>(Many{std::move(p), std::move(w), std::move(m), std::move(ms), std::move(v), std::move(vs)});
+  const c10::Device dev = p.at(0).device();
+  return std::make_shared<Many>(
+      Many{std::move(p), std::move(w), std::move(m), std::move(ms), std::move(v), std::move(vs), dev});
 }
 
 void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, double beta1, double beta2, double eps,
@@ -313,18 +316,23 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
                 const c10::optional<at::Tensor>& skip, const c10::optional<at::Tensor>& nonfinite) {
   TORCH_CHECK_VALUE(g.size() == t.p.size(), "AdamWMany: ", g.size(), " gradients for ", t.p.size(), " parameters");
   if (g.empty()) return;
-  const auto dev = t.p[0].device();
+  const auto dev = t.dev;
   const bool eight = !t.ms.empty();
   auto is_float = [](at::ScalarType x) { return x == at::kFloat || x == at::kBFloat16 || x == at::kHalf; };
   for (size_t i = 0; i < g.size(); ++i) {
     const long n = t.p[i].numel();
     TORCH_CHECK_VALUE(is_float(g[i].scalar_type()) && g[i].numel() == n && g[i].is_contiguous() && g[i].device() == dev,
                       "AdamWMany: gradient ", i, ": contiguous, ", n, " elements, fp32 / bf16 / fp16, on ", dev);
-    // a tensor can be given other memory (.data, resize_) after the check at construction
-    TORCH_CHECK_VALUE(is_float(t.p[i].scalar_type()) && t.p[i].is_contiguous() && t.m[i].numel() == n && t.v[i].numel() == n && t.p[i].device() == dev &&
-                          (t.w.empty() || t.w[i].numel() == n) &&
-                          (!eight || (t.ms[i].numel() == (n + 127) / 128 && t.vs[i].numel() == (n + 127) / 128)),
-                      "AdamWMany: tensor ", i, " has changed its size or place");
+    // a tensor can be given other memory (.data, resize_) of any type after the check at construction
+    auto still = [&](const at::Tensor& x, at::ScalarType type, long size) {
+      return x.scalar_type() == type && x.numel() == size && x.is_contiguous() && x.device() == dev;
+    };
+    const auto moment = eight ? at::kFloat8_e4m3fn : at::kFloat;
+    TORCH_CHECK_VALUE(is_float(t.p[i].scalar_type()) && still(t.p[i], t.p[i].scalar_type(), n) && still(t.m[i], moment, n) &&
+                          still(t.v[i], moment, n) && (t.w.empty() || still(t.w[i], at::kFloat, n)) &&
+                          (!eight || (still(t.ms[i], at::kFloat8_e8m0fnu, (n + 127) / 128) &&
+                                      still(t.vs[i], at::kFloat8_e8m0fnu, (n + 127) / 128))),
+                      "AdamWMany: tensor ", i, " has changed its type, size or place");
   }
   const std::pair<const char*, const c10::optional<at::Tensor>*> words[] = {
       {"step_dev", &step_dev}, {"skip", &skip}, {"nonfinite", &nonfinite}};

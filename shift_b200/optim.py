@@ -64,6 +64,20 @@ class AdamWMany:
         _fail(len(self.exp_avg) == n and len(self.exp_avg_sq) == n
               and (self.masters is None or len(self.masters) == n), "lists of different lengths")
         self.eight = n > 0 and isinstance(self.exp_avg[0], State8)
+        self.device = self.params[0].device if n > 0 else None
+        self._check()
+        own = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                     for p, *state in zip(self.params, *self._states()) for x in (p, *state) if x.numel())
+        _fail(all(end <= start for (_, end), (start, _) in zip(own, own[1:])), "a tensor is there twice, or two share memory")
+        self._plan = None
+        if n > 0 and self.params[0].is_cuda:
+            lists = self._states()
+            m, ms, v, vs = lists[:4] if self.eight else (lists[0], [], lists[1], [])
+            self._plan = ext().adamw_many_plan(self.params, self.masters or [], m, ms, v, vs)
+
+    def _check(self):
+        """Types, sizes and places of all tensors; a step looks again (the extension's itself on the GPU), since a tensor
+        can be given other memory."""
         for t, p in enumerate(self.params):
             _fail(p.dtype in _FLOATS, f"parameter {t} is {p.dtype}")
             same = [p]
@@ -85,15 +99,7 @@ class AdamWMany:
                       f"tensor {t}: an fp32 master of {p.numel()} elements is expected")
                 same.append(w)
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
-            _fail(all(x.device == self.params[0].device for x in same), f"tensor {t} or its state is on another device")
-        own = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
-                     for p, *state in zip(self.params, *self._states()) for x in (p, *state) if x.numel())
-        _fail(all(end <= start for (_, end), (start, _) in zip(own, own[1:])), "a tensor is there twice, or two share memory")
-        self._plan = None
-        if n > 0 and self.params[0].is_cuda:
-            lists = self._states()
-            m, ms, v, vs = lists[:4] if self.eight else (lists[0], [], lists[1], [])
-            self._plan = ext().adamw_many_plan(self.params, self.masters or [], m, ms, v, vs)
+            _fail(all(x.device == self.device for x in same), f"tensor {t} or its state is on another device")
 
     def _states(self):
         """The lists of tensors that a step writes beside the parameters."""
@@ -125,7 +131,8 @@ class AdamWMany:
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"AdamWMany: {len(grads)} gradients for {len(self.params)} parameters")
-        dev = self.params[0].device if self.params else None
+        self._check()
+        dev = self.device
         for t, (g, p) in enumerate(zip(grads, self.params)):
             if g.dtype not in _FLOATS or g.numel() != p.numel() or not g.is_contiguous() or g.device != dev:
                 raise ValueError(f"AdamWMany: gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {dev}")

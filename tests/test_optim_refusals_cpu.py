@@ -48,3 +48,36 @@ def test_tensors_that_share_a_part_of_their_memory(eight):
     opt = AdamWMany([flat[:200], flat[200:]], [new(200), new(200)], [new(200), new(200)])         # neighbours may
     opt.step([torch.ones(200), torch.ones(200)])
     assert bool((flat < 0).all())
+
+
+def spoilt(eight, device="cpu"):
+    """Optimizers, made of sound tensors of which one was given other memory since."""
+    other = [lambda x: x.float().half(), lambda x: x[:100].clone(),
+             lambda x: torch.zeros(300, 2, device=device).to(x.dtype)[:, 0]]
+    for which in ("exp_avg", "exp_avg_sq", "masters", "params"):
+        for k, f in enumerate(other):
+            if which == "params" and k == 0:
+                continue                               # another floating type is a parameter's right
+            p, w = torch.ones(300, device=device).bfloat16(), torch.ones(300, device=device)
+            m, v = ((State8.zeros(p), State8.zeros(p)) if eight else (torch.zeros_like(w), torch.zeros_like(w)))
+            opt = AdamWMany([p], [m], [v], [w])
+            x = getattr(opt, which)[0]
+            x = x.code if isinstance(x, State8) else x
+            x.data = f(x)
+            yield opt, p, [torch.ones(x.numel() if which == "params" else 300, device=device)], which, k
+    if eight:
+        p = torch.ones(300, device=device)
+        for field in range(4):
+            m, v = State8.zeros(p), State8.zeros(p)
+            opt = AdamWMany([p], [m], [v])
+            (m, v)[field // 2].scale.data = (m.scale[:1].clone() if field % 2 else m.scale.float())
+            yield opt, p, [torch.ones(300, device=device)], "scale", field
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_tensors_that_were_given_other_memory(eight):
+    for opt, p, g, which, k in spoilt(eight):
+        before = p.clone()
+        with pytest.raises(ValueError):
+            opt.step(g)
+        assert torch.equal(p, before), (which, k)
