@@ -862,6 +862,8 @@ static void check_operand(const at::Tensor& q, const at::Tensor& scale, int64_t 
 at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at::Tensor& b, const at::Tensor& sb,
                   int64_t Kb, const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& offs, int64_t mode,
                   bool accumulate, bool make_f32, const at::Tensor& status) {
+  // a contraction by segments is never cut into ranges: without segments it has no form
+  TORCH_CHECK_VALUE(mode == kRowGroups || (mode == kKGroups && offs.has_value()), "fp8 product: groups of the contraction need offs");
   check_operand(a, sa, K);
   check_operand(b, sb, Kb);
   TORCH_CHECK_VALUE(K == Kb, "fp8 product: the operands contract ", K, " and ", Kb, " values");

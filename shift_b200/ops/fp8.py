@@ -116,6 +116,11 @@ def _check_out(out: torch.Tensor, shape: tuple, a: BlockFp8, who: str):
         raise ValueError(f"{who}: out in bf16 or fp32 beside the operands, got {out.dtype} on {out.device}")
 
 
+def _need_offs(offs, who: str):
+    if offs is None:                       # the extension takes none for a dense product
+        raise ValueError(f"{who}: offs are int32 [groups + 1] beside the operands")
+
+
 def _check_offs(offs: torch.Tensor, a: BlockFp8, who: str):
     if offs.dim() != 1 or offs.numel() < 2 or offs.dtype != torch.int32 or offs.device != a.device:
         raise ValueError(f"{who}: offs are int32 [groups + 1] beside the operands")
@@ -152,6 +157,7 @@ def grouped_matmul(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tens
     [G, N, K]); ``offs`` is int32 [G + 1] on the device, rising.  Rows of
     ``out`` that no segment covers are left as they were (unwritten memory
     where no ``out`` is given)."""
+    _need_offs(offs, "grouped_matmul")
     if a.data.is_cuda:
         return _run(a, b, out, offs, 0, False)
     _check_pair(a, b, "grouped_matmul")
@@ -181,6 +187,7 @@ def grouped_wgrad(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tenso
     refused, on the GPU through the status word (``ops._ext.check_status``)
     with ``out`` left as it was.  An empty segment gives zeros (or leaves
     ``out[g]`` with ``accumulate``)."""
+    _need_offs(offs, "grouped_wgrad")
     if a.data.is_cuda:
         return _run(a, b, out, offs, 1, accumulate)
     _check_pair(a, b, "grouped_wgrad")

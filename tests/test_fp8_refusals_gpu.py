@@ -4,6 +4,7 @@ import torch
 
 from shift_b200.ops import fp8
 from shift_b200.optim import AdamWMany, State8
+from test_fp8_refusals_cpu import check_segments_are_needed
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -46,3 +47,14 @@ def test_optimizer(eight):
     assert bool((p == 1).all())
     opt.step(g)
     assert bool((p != 1).all())
+
+
+def test_segments_are_needed():
+    """The extension itself refuses too: it would cut the contraction and sum ranges that nothing wrote."""
+    from shift_b200.ops._ext import ext, status_word
+    check_segments_are_needed(DEV)
+    a, b = fp8.quantize(torch.ones(4, 4096, device=DEV)), fp8.quantize(torch.ones(6, 4096, device=DEV))
+    for mode in (1, 2, -1):
+        with pytest.raises(ValueError, match="offs"):
+            ext().fp8_matmul(a.data, a.scale, a.cols, b.data, b.scale, b.cols, torch.zeros(1, 4, 6, device=DEV), None, mode,
+                             False, False, status_word(a.device))
