@@ -852,6 +852,8 @@ static void check_operand(const at::Tensor& q, const at::Tensor& scale, int64_t 
                         scale.size(0) == (cols + 511) / 512 && scale.size(1) == q.size(0) && scale.size(2) == 4,
                     "fp8 product: scales [", (cols + 511) / 512, ", ", q.size(0),
                     ", 4] of float8_e8m0fnu, contiguous, got ", scale.sizes(), " of ", scale.scalar_type());
+  // four scales are read as one word; a view of bytes can start anywhere
+  TORCH_CHECK_VALUE((reinterpret_cast<uintptr_t>(scale.data_ptr()) & 3) == 0, "fp8 product: scales start on 4 bytes");
   TORCH_CHECK_VALUE(scale.device() == q.device() && q.is_cuda(), "fp8 product: codes and scales on one CUDA device");
 }
 

@@ -3,6 +3,9 @@ import pytest
 import torch
 
 from shift_b200.ops import fp8
+from shift_b200.ops._ext import available, ext
+
+needs_ext = pytest.mark.skipif(not available(), reason="the extension is not built")
 
 
 def check_segments_are_needed(device):
@@ -18,3 +21,22 @@ def check_segments_are_needed(device):
 
 def test_segments_are_needed():
     check_segments_are_needed("cpu")
+
+
+def moved(x, by):
+    """The same bytes, starting ``by`` bytes behind a boundary."""
+    flat = torch.zeros(x.numel() + 16, dtype=torch.uint8, device=x.device)
+    flat[by:by + x.numel()] = x.reshape(-1).view(torch.uint8)
+    return flat[by:by + x.numel()].view(x.dtype).view(x.shape)
+
+
+@needs_ext
+@pytest.mark.parametrize("by", [1, 2, 3])
+def test_scales_off_their_words_are_refused(by):
+    """The extension's check of an operand, which comes before that of its device: no GPU is needed to see it."""
+    a, b = (fp8.quantize(torch.ones(n, 600)) for n in (4, 6))
+    a = a._replace(scale=moved(a.scale, by))
+    assert bool((fp8.matmul(a, b) == 600).all())       # on the CPU any place will do
+    with pytest.raises(ValueError, match="4 bytes"):
+        ext().fp8_matmul(a.data, a.scale, 600, b.data, b.scale, 600, None, None, 0, False, False,
+                         torch.zeros(1, dtype=torch.int32))

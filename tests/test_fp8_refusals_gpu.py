@@ -4,7 +4,7 @@ import torch
 
 from shift_b200.ops import fp8
 from shift_b200.optim import AdamWMany, State8
-from test_fp8_refusals_cpu import check_segments_are_needed
+from test_fp8_refusals_cpu import check_segments_are_needed, moved
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -58,3 +58,15 @@ def test_segments_are_needed():
         with pytest.raises(ValueError, match="offs"):
             ext().fp8_matmul(a.data, a.scale, a.cols, b.data, b.scale, b.cols, torch.zeros(1, 4, 6, device=DEV), None, mode,
                              False, False, status_word(a.device))
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_scales_off_their_words_are_refused(side):
+    q = [fp8.quantize(torch.ones(n, 600, device=DEV)) for n in (4, 6)]
+    scale = q[side].scale
+    for by in (1, 2, 3):
+        q[side] = q[side]._replace(scale=moved(scale, by))
+        with pytest.raises(ValueError, match="4 bytes"):
+            fp8.matmul(*q)
+    q[side] = q[side]._replace(scale=moved(scale, 4))
+    assert bool((fp8.matmul(*q) == 600).all())
