@@ -156,7 +156,8 @@ def grouped_matmul(a: BlockFp8, b: BlockFp8, offs: torch.Tensor, out: torch.Tens
     """D[r] = a[r] @ b[g]^T for the rows r in [offs[g], offs[g + 1]).
 
     ``b`` holds the groups' matrices one after the other (``quantize`` of
-    [G, N, K]); ``offs`` is int32 [G + 1] on the device, rising.  Rows of
+    [G, N, K]); ``offs`` is int32 [G + 1] on the device, rising (cut to
+    the rows; one below the one before counts as that one).  Rows of
     ``out`` that no segment covers are left as they were (unwritten memory
     where no ``out`` is given)."""
     _need_offs(offs, "grouped_matmul")

@@ -176,13 +176,11 @@ def fp8_values(data: torch.Tensor, scale: torch.Tensor, cols: int) -> torch.Tens
 
 
 def segments(offs: torch.Tensor, limit: int):
-    """(lo, hi) of each segment, cut to [0, limit] and never negative."""
-    o = offs.tolist()
-    out = []
-    for lo, hi in zip(o, o[1:]):
-        lo = min(max(lo, 0), limit)
-        out.append((lo, min(max(hi, lo), limit)))
-    return out
+    """(lo, hi) of each segment, cut to [0, limit]; an offset below the one before counts as that one."""
+    o = [min(max(x, 0), limit) for x in offs.tolist()]
+    for g in range(1, len(o)):
+        o[g] = max(o[g], o[g - 1])
+    return list(zip(o, o[1:]))
 
 
 # ------------------------------------------------------------- 8-bit moments
