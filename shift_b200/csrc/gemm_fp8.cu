@@ -889,6 +889,7 @@ at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at
   } else {
     TORCH_CHECK_VALUE(result.dim() == 2 && result.size(0) == M && result.size(1) == N && (N <= 1 || result.stride(1) == 1),
                       "fp8 product: out ", result.sizes(), ", expected [", M, ", ", N, "] with inner stride 1");
+    TORCH_CHECK_VALUE(M <= 1 || N == 0 || result.stride(0) >= N, "fp8 product: rows of out overlap");
   }
   TORCH_CHECK_VALUE(result.scalar_type() == at::kFloat || result.scalar_type() == at::kBFloat16,
                     "fp8 product: out in bf16 or fp32, got ", result.scalar_type());

@@ -114,6 +114,8 @@ def _check_pair(a: BlockFp8, b: BlockFp8, who: str):
 def _check_out(out: torch.Tensor, shape: tuple, a: BlockFp8, who: str):
     if tuple(out.shape) != shape or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"{who}: out {tuple(out.shape)}, expected {shape} with inner stride 1")
+    if out.shape[-2] > 1 and out.stride(-2) < out.shape[-1]:
+        raise ValueError(f"{who}: rows of out overlap")
     if out.dtype not in (torch.bfloat16, torch.float32) or out.device != a.device:
         raise ValueError(f"{who}: out in bf16 or fp32 beside the operands, got {out.dtype} on {out.device}")
 

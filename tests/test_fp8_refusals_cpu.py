@@ -40,3 +40,26 @@ def test_scales_off_their_words_are_refused(by):
     with pytest.raises(ValueError, match="4 bytes"):
         ext().fp8_matmul(a.data, a.scale, 600, b.data, b.scale, 600, None, None, 0, False, False,
                          torch.zeros(1, dtype=torch.int32))
+
+
+def check_out_rows_apart(device):
+    a, b = fp8.quantize(torch.ones(4, 40, device=device)), fp8.quantize(torch.ones(8, 40, device=device))
+    offs = torch.tensor([0, 2, 4], dtype=torch.int32, device=device)
+    flat = torch.zeros(100, device=device)
+    for out in (flat[:8].expand(4, 8), flat.as_strided((4, 8), (7, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            fp8.matmul(a, b, out=out)
+        if out.stride(0):
+            with pytest.raises(ValueError, match="overlap"):
+                fp8.matmul(a, b, out=out, accumulate=True)
+    for out in (flat[:4].expand(4, 4), flat.as_strided((4, 4), (3, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            fp8.grouped_matmul(a, b, offs, out=out)
+    assert bool((flat == 0).all())
+    assert bool((fp8.matmul(a, b, out=flat.as_strided((4, 8), (8, 1))) == 40).all())
+    one = fp8.quantize(torch.ones(1, 40, device=device))
+    assert bool((fp8.matmul(one, b, out=flat[:8].expand(1, 8)) == 40).all())       # a single row has no neighbour
+
+
+def test_out_rows_apart():
+    check_out_rows_apart("cpu")

@@ -4,7 +4,7 @@ import torch
 
 from shift_b200.ops import fp8
 from shift_b200.optim import AdamWMany, State8
-from test_fp8_refusals_cpu import check_segments_are_needed, moved
+from test_fp8_refusals_cpu import check_out_rows_apart, check_segments_are_needed, moved
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -70,3 +70,7 @@ def test_scales_off_their_words_are_refused(side):
             fp8.matmul(*q)
     q[side] = q[side]._replace(scale=moved(scale, 4))
     assert bool((fp8.matmul(*q) == 600).all())
+
+
+def test_out_rows_apart():
+    check_out_rows_apart(DEV)
