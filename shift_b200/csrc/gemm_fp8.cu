@@ -905,6 +905,8 @@ at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at
     if (!accumulate) D.zero_();
     return result;
   }
+  for (const auto* t : {&a, &b})                   // a tensor map's strides are whole: no row repeats another
+    TORCH_CHECK_VALUE(t->size(0) <= 1 || t->stride(0) >= K, "fp8 product: rows of codes overlap");
   for (const auto* t : {&a, &b})
     TORCH_CHECK(t->stride(1) == 1 && aligned16(t->data_ptr()) && (t->size(0) == 1 || t->stride(0) % 16 == 0),
                 "fp8 matmul: codes start on 16 bytes, rows a multiple of 16 bytes apart");

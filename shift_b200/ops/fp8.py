@@ -47,7 +47,7 @@ class BlockFp8(NamedTuple):
     [ceil(cols / 512), rows, 4] powers of two (float8_e8m0fnu): entry (w, r, j) scales
     columns [512 w + 128 j, + 128) of row r.  A batch of G matrices has their rows one
     after the other.  Products on the GPU want codes that start on 16 bytes in rows a multiple
-    of 16 bytes apart, and scales that start on 4 bytes, as ``quantize`` makes them: views of a
+    of 16 bytes apart (none over another), and scales that start on 4 bytes, as ``quantize`` makes them: views of a
     byte buffer that lie otherwise are refused and have to be cloned."""
     data: torch.Tensor
     scale: torch.Tensor

@@ -74,3 +74,15 @@ def test_scales_off_their_words_are_refused(side):
 
 def test_out_rows_apart():
     check_out_rows_apart(DEV)
+
+
+def test_rows_of_codes_that_overlap():
+    """Broadcast or overlapping rows have no tensor map; a single row may have any stride."""
+    a, b = fp8.quantize(torch.ones(4, 40, device=DEV)), fp8.quantize(torch.ones(8, 40, device=DEV))
+    raw = a.data.view(torch.uint8)
+    for bad in (raw[:1].expand(4, 48), raw.as_strided((4, 48), (32, 1))):
+        for pair in ((a._replace(data=bad.view(a.data.dtype)), b), (b, a._replace(data=bad.view(a.data.dtype)))):
+            with pytest.raises(ValueError, match="overlap"):
+                fp8.matmul(*pair)
+    one = fp8.BlockFp8(raw.as_strided((1, 48), (0, 1)).view(a.data.dtype), a.scale[:, :1].clone(), 40)
+    assert bool((fp8.matmul(one, b) == 40).all())
