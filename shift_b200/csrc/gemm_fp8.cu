@@ -900,9 +900,14 @@ at::Tensor matmul(const at::Tensor& a, const at::Tensor& sa, int64_t K, const at
               "fp8 matmul: a side is too long");
   TORCH_CHECK(G >= 1 && G <= kMaxGroups, "fp8 matmul: 1 to ", kMaxGroups, " groups");
   if (M == 0 || N == 0) return result;
-  if (K == 0) {
-    TORCH_CHECK_VALUE(!offs.has_value() || mode == kKGroups, "fp8 product: nothing to contract");
-    if (!accumulate) D.zero_();
+  if (K == 0) {                                    // nothing to contract: zeros, by group in the rows of the segments
+    if (accumulate) return result;
+    if (mode == kKGroups || !offs.has_value()) {
+      D.zero_();
+    } else {
+      const at::Tensor row = at::arange(M, offs->options());
+      D.masked_fill_(row.ge(offs->narrow(0, 0, 1)).__and__(row.lt(offs->max())).unsqueeze(1), 0);
+    }
     return result;
   }
   for (const auto* t : {&a, &b})                   // a tensor map's strides are whole: no row repeats another

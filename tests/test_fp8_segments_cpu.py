@@ -45,3 +45,17 @@ def test_rows(o):
 @pytest.mark.parametrize("o", FALLING)
 def test_contraction(o):
     check_contraction(o, "cpu")
+
+
+def check_nothing_to_contract(o, device):
+    a = fp8.quantize(torch.ones(200, 0, device=device))
+    b = fp8.quantize(torch.ones(3, 32, 0, device=device), tiles=True)
+    out = torch.full((200, 32), -64.0, device=device)
+    fp8.grouped_matmul(a, b, torch.tensor(o, dtype=torch.int32, device=device), out=out)
+    want = torch.tensor([0.0 if g >= 0 else -64.0 for g in taken(o, 200)])
+    assert torch.equal(out.cpu(), want[:, None].expand(200, 32))
+
+
+@pytest.mark.parametrize("o", FALLING + [[20, 30, 30, 90]])
+def test_nothing_to_contract(o):
+    check_nothing_to_contract(o, "cpu")

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from shift_b200.ops._ext import check_status
-from test_fp8_segments_cpu import FALLING, check_contraction, check_rows
+from test_fp8_segments_cpu import FALLING, check_contraction, check_nothing_to_contract, check_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,8 @@ def test_contraction(o):
     check_contraction(o, "cuda")
     torch.cuda.synchronize()
     check_status()
+
+
+@pytest.mark.parametrize("o", FALLING + [[20, 30, 30, 90]])
+def test_nothing_to_contract(o):
+    check_nothing_to_contract(o, "cuda")
