@@ -346,6 +346,8 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
       TORCH_CHECK_VALUE(!x->has_value() || nonfinite->data_ptr<int>() < (*x)->data_ptr<int>() ||
                             nonfinite->data_ptr<int>() >= (*x)->data_ptr<int>() + (x == &step_dev ? 4 : 1),
                         "AdamWMany: nonfinite is a word that the step reads");
+  // As any write in place: autograd notices.  Before the first launch: a tensor made in inference mode refuses it.
+  for (const auto& x : t.p) x.unsafeGetTensorImpl()->bump_version();
   const at::cuda::CUDAGuard guard(dev);
   StepArgs a;
   a.lr = static_cast<float>(lr);
@@ -405,7 +407,6 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
     }
     flush();
   }
-  for (const auto& x : t.p) x.unsafeGetTensorImpl()->bump_version();   // as any write in place: autograd notices
 }
 
 }  // namespace adam

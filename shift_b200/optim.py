@@ -98,6 +98,8 @@ class AdamWMany:
                 _fail(w.dtype == torch.float32 and w.numel() == p.numel(),
                       f"tensor {t}: an fp32 master of {p.numel()} elements is expected")
                 same.append(w)
+            _fail(torch.is_inference_mode_enabled() or not any(x.is_inference() for x in same),
+                  f"tensor {t} or its state was made in inference mode")
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
             _fail(all(x.device == self.device for x in same), f"tensor {t} or its state is on another device")
 

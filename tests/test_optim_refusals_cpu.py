@@ -81,3 +81,21 @@ def test_tensors_that_were_given_other_memory(eight):
         with pytest.raises(ValueError):
             opt.step(g)
         assert torch.equal(p, before), (which, k)
+
+
+def check_inference_tensors(device):
+    with torch.inference_mode():
+        opt, p, g = make(device)
+        m = opt.exp_avg[0]
+        opt.step(g)                                    # inside the mode they are as good as any
+        before, moment = p.clone(), m.clone()
+        assert bool((p != 1).all())
+    with pytest.raises((ValueError, RuntimeError), match="nference"):
+        opt.step(g)
+    assert torch.equal(p, before) and torch.equal(m, moment)
+    with pytest.raises(ValueError, match="inference"):
+        AdamWMany([p], [m], [opt.exp_avg_sq[0]])
+
+
+def test_inference_tensors_are_refused_before_they_change():
+    check_inference_tensors("cpu")

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_optim_refusals_cpu import make, spoilt, words
+from test_optim_refusals_cpu import check_inference_tensors, make, spoilt, words
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -44,3 +44,7 @@ def test_tensors_that_were_moved_to_the_host(eight):
     p.data = p.data.to(DEV)
     opt.step([torch.ones(300, device=DEV)])
     assert bool((p != 1).all())
+
+
+def test_inference_tensors_are_refused_before_they_change():
+    check_inference_tensors(DEV)
