@@ -311,14 +311,13 @@ std::shared_ptr<Many> adamw_many_plan(std::vector<at::Tensor> p, std::vector<at:
       Many{std::move(p), std::move(w), std::move(m), std::move(ms), std::move(v), std::move(vs), dev});
 }
 
-void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, double beta1, double beta2, double eps,
-                double wd, int64_t step, double grad_scale, int64_t seed, const c10::optional<at::Tensor>& step_dev,
-                const c10::optional<at::Tensor>& skip, const c10::optional<at::Tensor>& nonfinite) {
+static bool is_float(at::ScalarType x) { return x == at::kFloat || x == at::kBFloat16 || x == at::kHalf; }
+
+// What a step refuses of its gradients, and of the tensors as they are by now.
+void adamw_many_check(const Many& t, const std::vector<at::Tensor>& g) {
   TORCH_CHECK_VALUE(g.size() == t.p.size(), "AdamWMany: ", g.size(), " gradients for ", t.p.size(), " parameters");
-  if (g.empty()) return;
   const auto dev = t.dev;
   const bool eight = !t.ms.empty();
-  auto is_float = [](at::ScalarType x) { return x == at::kFloat || x == at::kBFloat16 || x == at::kHalf; };
   for (size_t i = 0; i < g.size(); ++i) {
     const long n = t.p[i].numel();
     TORCH_CHECK_VALUE(is_float(g[i].scalar_type()) && g[i].numel() == n && g[i].is_contiguous() && g[i].device() == dev,
@@ -334,6 +333,15 @@ void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, doub
                                       still(t.vs[i], at::kFloat8_e8m0fnu, (n + 127) / 128))),
                       "AdamWMany: tensor ", i, " has changed its type, size or place");
   }
+}
+
+void adamw_many(const Many& t, const std::vector<at::Tensor>& g, double lr, double beta1, double beta2, double eps,
+                double wd, int64_t step, double grad_scale, int64_t seed, const c10::optional<at::Tensor>& step_dev,
+                const c10::optional<at::Tensor>& skip, const c10::optional<at::Tensor>& nonfinite) {
+  adamw_many_check(t, g);
+  if (g.empty()) return;
+  const auto dev = t.dev;
+  const bool eight = !t.ms.empty();
   const std::pair<const char*, const c10::optional<at::Tensor>*> words[] = {
       {"step_dev", &step_dev}, {"skip", &skip}, {"nonfinite", &nonfinite}};
   for (const auto& [name, x] : words)
@@ -417,5 +425,6 @@ void bind_adamw_many(pybind11::module& m) {
   namespace py = pybind11;
   py::class_<sb::adam::Many, std::shared_ptr<sb::adam::Many>>(m, "AdamWManyPlan");
   m.def("adamw_many_plan", &sb::adam::adamw_many_plan);
+  m.def("adamw_many_check", &sb::adam::adamw_many_check);
   m.def("adamw_many", &sb::adam::adamw_many, "AdamW over many tensors, moments in fp32 or 8 bits");
 }

@@ -17,6 +17,7 @@ block's largest is updated as if its root were that large, so by less than with
 from __future__ import annotations
 
 import math
+import operator
 from typing import NamedTuple
 
 import torch
@@ -103,6 +104,18 @@ class AdamWMany:
             _fail(all(x.is_contiguous() for x in same), f"tensor {t} or its state is not contiguous")
             _fail(all(x.device == self.device for x in same), f"tensor {t} or its state is on another device")
 
+    def check(self, grads):
+        """Raises what ``step`` would of these gradients, and of the tensors as they are by now."""
+        if self._plan is not None:
+            ext().adamw_many_check(self._plan, grads)
+            return
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamWMany: {len(grads)} gradients for {len(self.params)} parameters")
+        self._check()
+        for t, (g, p) in enumerate(zip(grads, self.params)):
+            if g.dtype not in _FLOATS or g.numel() != p.numel() or not g.is_contiguous() or g.device != self.device:
+                raise ValueError(f"AdamWMany: gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {self.device}")
+
     def _states(self):
         """The lists of tensors that a step writes beside the parameters."""
         lists = [self.exp_avg, self.exp_avg_sq]
@@ -131,13 +144,8 @@ class AdamWMany:
                              step, grad_scale, seed, step_dev, skip, nonfinite)
             return
         grads = list(grads)
-        if len(grads) != len(self.params):
-            raise ValueError(f"AdamWMany: {len(grads)} gradients for {len(self.params)} parameters")
-        self._check()
+        self.check(grads)
         dev = self.device
-        for t, (g, p) in enumerate(zip(grads, self.params)):
-            if g.dtype not in _FLOATS or g.numel() != p.numel() or not g.is_contiguous() or g.device != dev:
-                raise ValueError(f"AdamWMany: gradient {t}: contiguous, {p.numel()} elements, fp32 / bf16 / fp16, on {dev}")
         for name, x, least in (("step_dev", step_dev, 4), ("skip", skip, 1), ("nonfinite", nonfinite, 1)):
             if x is not None and (x.dtype != torch.int32 or x.numel() < least or x.device != dev):
                 raise ValueError(f"AdamWMany: {name}: int32 [{least}] on {dev}")
@@ -194,12 +202,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state in 8 or 32 bits, got {state_bits}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights))
-        self._many: dict = {}
+        self._lists = None                             # what was handed over, and what that hangs on
         self._packed: dict = {}                        # row-major copies of parameters of another layout
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._many, self._packed = {}, {}              # a copy or an unpickled optimizer has tensors of its own
+        self._lists, self._packed = None, {}           # a copy or an unpickled optimizer has tensors of its own
 
     def _init_state(self, p, group):
         st = self.state[p]
@@ -251,7 +259,7 @@ class AdamW(torch.optim.Optimizer):
                 # the base class casts floating-point and byte states to the parameter's type: put back what was saved
                 for name, x in saved[i].items():
                     self.state[p][name] = x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
-        self._many.clear()
+        self._lists = None
 
     def _take(self, p, group, saved):
         """State of ``p`` from that of torch.optim.AdamW: moments of the parameter's shape in any floating type."""
@@ -279,58 +287,93 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        place = {p: i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
-        jobs, made = [], []
+        live = [[(p, g) for p in group["params"] if (g := p.grad) is not None] for group in self.param_groups]
+        made = []
         try:                                           # all that may be refused comes before the first update
-            for k, group in enumerate(self.param_groups):
-                self._gather(k, group, jobs, made)
+            jobs = self._jobs(live, made)
         except Exception:
             for p in made:
                 del self.state[p]
+            self._lists = None
             raise
-        # the random bits hang on the seed and on a tensor's number in its list: each list has a seed of its own
-        for group, t, ps, many in jobs:
-            moved = [p for p in ps if not p.is_contiguous()]
+        for (k, ps, states, many, _, place), t, grads in jobs:
+            group = self.param_groups[k]
+            moved = [p for p in ps if p in self._packed] if self._packed else ()
             for p in moved:
                 self._packed[p].copy_(p)
             beta1, beta2 = group["betas"]
-            many.step([p.grad.contiguous() for p in ps], lr=float(group["lr"]), beta1=beta1, beta2=beta2,
-                      eps=group["eps"], wd=group["weight_decay"], step=t, seed=t + 0x9E3779B1 * place[ps[0]])
+            # the random bits hang on the seed and on a tensor's number in its list: each list has a seed of its own
+            many.step(grads, lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
+                      wd=group["weight_decay"], step=t, seed=t + 0x9E3779B1 * place)
             for p in moved:
                 p.copy_(self._packed[p])
-            for p in ps:
-                self.state[p]["step"] = t
+            for st in states:
+                st["step"] = t
         return loss
 
-    def _gather(self, k, group, jobs, made):
-        """Adds group ``k``'s (group, step, parameters, AdamWMany) to ``jobs``, parameters with new state to ``made``."""
-        by_step: dict = {}
-        for p in group["params"]:
-            if p.grad is None:
-                continue
-            g = p.grad
-            if g.layout != torch.strided or g.dtype not in _FLOATS or g.shape != p.shape or g.device != p.device:
-                raise ValueError(f"AdamW: gradient {tuple(g.shape)} of {g.dtype}, {g.layout}, on {g.device} for a "
-                                 f"parameter {tuple(p.shape)} on {p.device}: dense, fp32 / bf16 / fp16, beside it")
-            if "step" not in self.state[p]:
-                made.append(p)
-                self._init_state(p, group)
-            held = self._packed.get(p)
-            if p.is_contiguous():
-                self._packed.pop(p, None)
-            elif held is None or (held.shape, held.dtype, held.device) != (p.shape, p.dtype, p.device):
-                self._packed[p] = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-            by_step.setdefault((int(self.state[p]["step"]) + 1, p.device), []).append(p)
-        for (t, _), ps in by_step.items():
-            # the lists of a group are checked and handed over once, as long as the same tensors take part: state can
-            # be cleared, or given other tensors or other memory
-            use = [group["state_bits"], group["master_weights"], *(self._flat(p) for p in ps)]
-            use += [x for p in ps for x in self.state[p].values() if isinstance(x, torch.Tensor)]
-            at = [x.data_ptr() for x in use[2 + len(ps):]]
-            held = self._many.get((k, ps[0]))
-            if held is None or len(held[0]) != len(use) or held[1] != at or any(a is not b for a, b in zip(held[0], use)):
+    def _used(self, live):
+        """What the lists handed over hang on: objects, and the addresses of state tensors (``None`` where a state is
+        not as this class makes it).  State can be cleared, or given other tensors or other memory."""
+        objects, places = [*self.state, *self.state.values()], []
+        for group, pairs in zip(self.param_groups, live):
+            objects += (group["state_bits"], group["master_weights"], None)
+            for p, _ in pairs:
+                objects += (p, p.is_contiguous())
+        for st in self.state.values():
+            if next(iter(st), None) != "step":
+                return objects, None
+            tensors = [x for x in st.values() if x.__class__ is not int]
+            objects += tensors
+            try:
+                places += [x.data_ptr() for x in tensors]
+            except AttributeError:
+                return objects, None
+        return objects, places
+
+    def _jobs(self, live, made):
+        """(list handed over, step, gradients) of every update; parameters with new state are added to ``made``."""
+        for p, g in (pair for pairs in live for pair in pairs):
+            if g.layout is not torch.strided:
+                raise ValueError(f"AdamW: gradient of layout {g.layout} of a parameter {tuple(p.shape)}: dense ones only")
+        objects, places = self._used(live)
+        held = self._lists
+        if (held is None or places is None or places != held[1] or len(objects) != len(held[0])
+                or not all(map(operator.is_, objects, held[0]))
+                or any(st["step"] != states[0]["step"] for _, _, states, *_ in held[2] for st in states)):
+            lists = self._hand_over(live, made)
+            held = self._lists = (*self._used(live), lists)
+        jobs = []
+        for one in held[2]:
+            k, ps, states, many, index, _ = one
+            grads = [live[k][i][1].contiguous() for i in index]
+            for p in ps if self._packed else ():
+                if p in self._packed and self._packed[p].shape != p.shape:
+                    raise ValueError(f"AdamW: a parameter has changed its shape to {tuple(p.shape)}")
+            many.check(grads)
+            jobs.append((one, int(states[0]["step"]) + 1, grads))
+        return jobs
+
+    def _hand_over(self, live, made):
+        """The lists that are updated by one call each: (group, parameters, their state, AdamWMany, their places among
+        the group's live ones, the first one's number in the optimizer)."""
+        place = {p: i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
+        lists = []
+        for k, (group, pairs) in enumerate(zip(self.param_groups, live)):
+            by_step: dict = {}
+            for i, (p, _) in enumerate(pairs):
+                if "step" not in self.state[p]:
+                    made.append(p)
+                    self._init_state(p, group)
+                held = self._packed.get(p)
+                if p.is_contiguous():
+                    self._packed.pop(p, None)
+                elif held is None or (held.shape, held.dtype, held.device) != (p.shape, p.dtype, p.device):
+                    self._packed[p] = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+                by_step.setdefault((int(self.state[p]["step"]), p.device), []).append((i, p))
+            for some in by_step.values():
+                index, ps = zip(*some)
                 many = AdamWMany([self._flat(p) for p in ps], [self._moment(p, "exp_avg", group) for p in ps],
                                  [self._moment(p, "exp_avg_sq", group) for p in ps],
                                  [self.state[p]["master"] for p in ps] if group["master_weights"] else None)
-                held = self._many[(k, ps[0])] = (use, at, many)
-            jobs.append((group, t, ps, held[2]))
+                lists.append((k, ps, [self.state[p] for p in ps], many, index, place[ps[0]]))
+        return lists
