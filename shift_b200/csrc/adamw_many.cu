@@ -68,6 +68,8 @@ struct StepArgs {
   int* nonfinite;        // optional: set where a scaled gradient is not finite
 };
 
+// Integer mix of two multiplications, constants and shifts as Chris Wellons published them ("Prospecting for hash
+// functions", 2018); stated again in ops/reference.py.
 SB_DEVICE uint32_t mix32(uint32_t h) {
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;

@@ -251,8 +251,10 @@ SB_DEVICE bool mbar_test(uint64_t* bar, uint32_t phase) {
   return ok != 0;
 }
 // The same without ordering this thread's memory accesses before it: for an
-// accumulator that has been read, which tcgen05's own fence orders.  (The
-// releasing form waits for the global stores before it, 600 clocks.)
+// accumulator that has been read.  What orders it is tcgen05.wait::ld: after it
+// the columns are in registers, so nothing of the reads is left that the next
+// products could overtake, and nothing else is handed over.  (The releasing
+// form waits for the global stores before it, 600 clocks.)
 template <int CTAS>
 SB_DEVICE void arrive_leader_relaxed(uint64_t* bar) {
   if constexpr (CTAS == 1) {

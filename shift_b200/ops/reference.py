@@ -188,7 +188,8 @@ _M32 = 0xFFFFFFFF
 
 
 def mix32(h):
-    """Two multiply-and-fold rounds over 32 bits (ints or int64 tensors)."""
+    """Two multiply-and-fold rounds over 32 bits (ints or int64 tensors); the constants are those that Chris Wellons
+    published ("Prospecting for hash functions", 2018)."""
     h = h & _M32
     h = ((h ^ (h >> 16)) * 0x7FEB352D) & _M32
     h = ((h ^ (h >> 15)) * 0x846CA68B) & _M32
