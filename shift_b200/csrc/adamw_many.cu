@@ -15,10 +15,11 @@
 // update divided by nothing is hundreds of learning rates (an element 1e-6 of
 // its block's largest).  At code 1 its update is too small instead.  The random
 // bits are a counter hash of (seed, tensor number, element), hence the same for
-// any launch shape; elements 2^32 apart share them.
+// any launch shape; elements 2^32 apart share them.  Codes and scales are those
+// of the CPU's statement, bit for bit but for the sign of a zero.
 //
-// Bound: DRAM with 32-bit moments (0.494 B elements: 2.05 ms, 6.7 TB/s);
-// instructions with 8-bit ones (1.88 ms, 4.2 TB/s, 94 instructions an element).
+// Bound: DRAM with 32-bit moments (0.494 B elements: 2.07 ms, 6.7 TB/s);
+// instructions with 8-bit ones (2.03 ms, 3.9 TB/s, 105 instructions an element).
 // The tensors' pointers travel as kernel parameters, so a step is one launch
 // per 320 tensors, needs no device table and can be captured.  One pass of 8
 // elements a thread: four passes of a CTA, for one search of its tensor, were
@@ -253,11 +254,21 @@ adamw_many_kernel(const __grid_constant__ Table tab, StepArgs a) {
   const float keep = 1.f - a.lr * a.wd, rate = a.lr / a.c1, inv_c2 = 1.f / a.c2;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const float gi = g[i] * a.grad_scale;
+    const float gi = __fmul_rn(g[i], a.grad_scale);
     bad = __fmaf_rn(gi, 0.f, bad);
-    m[i] += (gi - m[i]) * a.one_minus_beta1;
-    v[i] = v[i] * a.beta2 + a.one_minus_beta2 * gi * gi;
-    r[i] = root(v[i]);
+    if constexpr (EIGHT) {
+      // Each operation rounded by itself, as on the CPU: a last bit decides between two codes, 2^-3 apart, so only the
+      // same last bits make the same codes (0.494 B elements: 2.03 ms; 1.90 with fused additions and the short root).
+      m[i] = __fadd_rn(m[i], __fmul_rn(__fsub_rn(gi, m[i]), a.one_minus_beta1));
+      v[i] = __fadd_rn(__fmul_rn(v[i], a.beta2), __fmul_rn(__fmul_rn(a.one_minus_beta2, gi), gi));
+      r[i] = __fsqrt_rn(v[i]);
+    } else {
+      // The root only divides the update, whose error of 2^-21 is below the weight's last bit (2.07 ms; 2.11 with the
+      // exact root and separate additions, 2.16 with an exact division too).
+      m[i] += (gi - m[i]) * a.one_minus_beta1;
+      v[i] = v[i] * a.beta2 + a.one_minus_beta2 * gi * gi;
+      r[i] = root(v[i]);
+    }
     w[i] = w[i] * keep - rate * __fdividef(m[i], r[i] * inv_c2 + a.eps);
   }
   if constexpr (EIGHT) {

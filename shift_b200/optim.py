@@ -171,7 +171,7 @@ class AdamWMany:
             v32 = v.values().square() if self.eight else v.view(-1)
             m32 = m32 + (g - m32) * (1.0 - beta1)
             v32 = v32 * beta2 + (1.0 - beta2) * g * g
-            r = v32.sqrt()
+            r = v32.double().sqrt().float()            # rounded correctly: fp32's own root here is a bit off at times
             new = w.float() * (1.0 - lr * wd) - (lr / c1) * (m32 / (r / c2 + eps))
             if self.eight:
                 u = ref.moment_draws(g.numel(), seed, t)
