@@ -320,7 +320,7 @@ class AdamW(torch.optim.Optimizer):
             for p, _ in pairs:
                 objects += (p, p.is_contiguous())
         for st in self.state.values():
-            if next(iter(st), None) != "step":
+            if not isinstance(st, dict) or next(iter(st), None) != "step":
                 return objects, None
             tensors = [x for x in st.values() if x.__class__ is not int]
             objects += tensors

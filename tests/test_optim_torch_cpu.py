@@ -73,6 +73,19 @@ def test_replaced_state_is_used_and_updated(bits, master, how):
     same_state(opt, ps, other, qs)
 
 
+def test_state_that_others_add_is_left_alone():
+    """Entries of another's making, beside the parameters' and among their state, and state in another order."""
+    ps, qs = params(), params()
+    opt, other = AdamW(ps, lr=1e-2), AdamW(qs, lr=1e-2)
+    for i in range(3):
+        run(ps, opt, [i])
+        run(qs, other, [i])
+        opt.state["note"] = 1.5
+        opt.state[ps[0]]["tag"] = 0.5
+        opt.state[ps[1]] = dict(reversed(opt.state[ps[1]].items()))
+    assert same(ps, qs) and opt.state["note"] == 1.5 and opt.state[ps[0]]["tag"] == 0.5
+
+
 # ----------------------------------------------------------------------------- copies
 @pytest.mark.parametrize("started", [False, True])
 @pytest.mark.parametrize("how", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
