@@ -29,8 +29,8 @@
 //               two warps, which take alternate columns
 // All waits are bounded (common.cuh).
 //
-// Bound: operations where the contraction is long (8192^3: 0.369 ms, 2982
-// TFLOP/s, 512 of every 590 clocks a block are products; 0.455 ms under the
+// Bound: operations where the contraction is long (8192^3: 0.374 ms, 2943
+// TFLOP/s, 512 of every 590 clocks a block are products; 0.466 ms under the
 // power cap), the way from L2 where it is short (16384 x 1536 x 1024: 27 us
 // from a warm L2, 34 us from DRAM): a pair's tile of 256 x 256 brings 32 KB
 // into each SM per block, which takes 64 bytes a clock for the 512 clocks that
@@ -820,7 +820,9 @@ struct Plan {
 // added per tile for what a tile costs whatever its width.  128 columns count
 // as 176: per block they bring 24 KB into an SM for 256 clocks of products,
 // where 64 bytes a clock arrive.  Measured, 192 against 256 columns: 16384 x
-// 1536 x 1024 27.6 and 29.1 us, 16384 x 1024 x 1024 23.4 and 21.9 us.
+// 1536 x 1024 27.6 and 29.1 us, 16384 x 1024 x 1024 23.4 and 21.9 us.  The split
+// is looked at after the width: 1536 x 1024 x 16384 takes 48 tiles of 128
+// columns on 74 pairs and is not split (50 us).
 static Plan make_plan(long M, long N, long K, long G, int64_t mode, bool offs, int sms) {
   Plan p;
   const long blocks = (K + BK - 1) / BK;
