@@ -25,7 +25,7 @@ cuda_flags = [
 if os.environ.get("SHIFT_DEBUG_BOUNDS"):
     cuda_flags.append("-DSHIFT_DEBUG_BOUNDS=1")
 
-sources = sorted(glob.glob(os.path.join(CSRC, "*.cu"))) + [os.path.join(CSRC, "bindings.cpp")]
+sources = sorted(glob.glob(os.path.join(CSRC, "*.cu"))) + sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
 
 setup(
     name="shift_b200",

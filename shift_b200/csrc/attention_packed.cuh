@@ -1,0 +1,253 @@
+// Causal attention over packed sequences on the 5th-generation tensor cores (sm_100a).
+//
+//   s = scale q k^T for the keys start(q) <= k <= q,  p = exp(s - lse),  o = p v,  lse = log sum exp s
+//   dp = do v^T,  delta = do . o,  ds = p (dp - delta),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do
+//
+// Rows are tiled by 128 without regard to where sequences begin: what a query sees is the interval [start(q), q], and
+// what sees a key is [key, stop(key)), so a tile that holds several sequences masks by two numbers a row, the number of
+// tiles is known to the host, and short sequences share tiles (tiles of one sequence each would take 128 rows for every
+// sequence of one token).  Only blocks at an interval's border pay for the mask.
+//
+// All kernels run persistently: a CTA takes its next tile from the hardware's list of CTAs that have not started
+// (cluster launch control), the costliest tiles first.  Twelve warps: two groups of four softmax warps (a thread has one
+// row of 128), one warp that loads tiles by TMA, one that issues tcgen05.mma.  Scores live in tensor memory; the
+// probabilities go back there as 16-bit operands of the second product and never to shared memory.
+//
+// What others hold.  Products run over whole blocks, so a masked value is a product with zero, which is zero unless the
+// other factor is infinite or NaN.  Rows that no sequence covers are cleared in shared memory after they were loaded.  Rows
+// of other sequences (or later ones of the same) that are not finite would leave NaN in a result: such results are
+// recognised when they are stored and computed again row by row from what they see.
+//
+// Every wait is bounded; on expiry the kernel records a status code and winds down.
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "attention_packed.h"
+#include "common.cuh"
+#include "lowp.cuh"
+
+namespace sb {
+namespace pa {
+
+constexpr int kThreads = 384;      // 8 softmax warps, loader, MMA issuer, two idle (a whole group of four for setmaxnreg)
+constexpr int kLoader = 8, kIssuer = 9;
+constexpr int kReaders = 10;       // warps that read a scheduling slot
+constexpr int kChunk = 128 * 128;  // bytes of 128 rows of 64 16-bit columns
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// O is rescaled only when a row's maximum rises by more than 2^8 over the one in use: the probabilities then stay below
+// 2^8 (fp16 holds them), and after a row's first blocks it hardly ever happens.
+constexpr float kRescale = 8.f;
+
+SB_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two fp32 operations in one instruction
+SB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+SB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+SB_DEVICE float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1;
+  static SB_DEVICE uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <>
+struct Half<__half> {
+  static constexpr uint32_t kFormat = 0;
+  static SB_DEVICE uint32_t pack(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+
+// instruction descriptor: fp32 accumulator, operands of type T, B along N where b_mn
+template <typename T>
+constexpr uint32_t idesc(int M, int N, int b_mn) {
+  return (1u << 4) | (Half<T>::kFormat << 7) | (Half<T>::kFormat << 10) | (static_cast<uint32_t>(b_mn) << 16) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+SB_DEVICE uint64_t kdesc(uint32_t addr) { return make_sw128_desc(addr, 16, 1024); }
+// B along N: the second 64 columns lie `next` bytes behind the first
+SB_DEVICE uint64_t mndesc(uint32_t addr, uint32_t next) { return make_sw128_desc(addr, next, 1024); }
+
+SB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int N>
+SB_DEVICE void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+SB_DEVICE void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// 384 threads are launched with 168 registers each: 256 x 216 + 128 x 72 = 384 x 168
+constexpr int kLaunchRegs = 168, kSoftRegs = 216, kOtherRegs = 72;
+static_assert(256 * kSoftRegs + 128 * kOtherRegs == kThreads * kLaunchRegs, "register shares");
+
+// ---------------------------------------------------------------------------
+// Scheduling: request n (made while item n is worked on) has the answer's slot n & 1.
+// ---------------------------------------------------------------------------
+struct Sched {
+  uint4* answer;              // [2]
+  uint64_t* full;             // [2]
+  uint64_t* empty;            // [2], kReaders arrivals
+};
+SB_DEVICE bool sched_request(const Sched& s, int n, int* status) {
+  const int b = n & 1;
+  if (!mbar_wait(&s.empty[b], ((n >> 1) & 1) ^ 1, status)) return false;
+  mbar_arrive_expect_tx(&s.full[b], 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(&s.answer[b])),
+               "r"(smem_u32(&s.full[b]))
+               : "memory");
+  return true;
+}
+// The next item, or -1 (none left, or a wait ran out).  By a whole warp.
+SB_DEVICE int sched_next(const Sched& s, int n, int* status) {
+  const int b = n & 1;
+  if (!__all_sync(0xffffffffu, mbar_wait(&s.full[b], (n >> 1) & 1, status))) return -1;
+  uint32_t ok, x = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "+r"(x)
+      : "r"(smem_u32(&s.answer[b]))
+      : "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) mbar_arrive(&s.empty[b]);
+  return ok != 0 ? static_cast<int>(x) : -1;
+}
+
+// Rows [row0, row0 + n) of a loaded tile (64-column chunks `next` bytes apart) that no sequence covers become zeros.
+SB_DEVICE void clear_rows(uint8_t* tile, int n, int chunks, int next, int row0, int first, int last) {
+  const int lane = threadIdx.x % 32;
+  for (int r = lane / 8; r < n; r += 4)
+    if (row0 + r < first || row0 + r >= last)
+      for (int c = 0; c < chunks; ++c)
+        *reinterpret_cast<uint4*>(tile + c * next + r * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+template <int D, typename T>
+SB_DEVICE void load_part(const T* p, float* f) {       // this lane's D / 32 columns
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) f[i] = to_float(p[(threadIdx.x % 32) * (D / 32) + i]);
+}
+template <int N>
+SB_DEVICE float dot(const float* a, const float* b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += a[i] * b[i];
+  return warp_sum(s);
+}
+
+// One row of O by a whole warp, from what the row sees alone.
+template <int D, typename T>
+__device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float lse2) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x % 32;
+  const T* x = static_cast<const T*>(a.qkv);
+  const long kc = static_cast<long>(a.Hq + h / a.group) * D, vc = kc + static_cast<long>(a.Hkv) * D;
+  float q[N], k[N], v[N], acc[N] = {};
+  load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
+  for (int j = st; j <= row; ++j) {
+    load_part<D>(x + j * a.ld + kc, k);
+    load_part<D>(x + j * a.ld + vc, v);
+    const float p = ex2(dot<N>(q, k) * a.scale_log2 - lse2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += p * v[i];
+  }
+  T* out = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D + lane * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = from_float<T>(acc[i]);
+}
+
+SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // -lse, -delta of query q (64 apart)
+  return a.rows + (static_cast<long>(h) * (a.tiles * 2) + q / 64) * 128 + q % 64;
+}
+
+// One row of dQ, columns [c0, c1).
+template <int D, typename T>
+__device__ __noinline__ void slow_dq(const Args& a, int row, int h, int st, int c0, int c1) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x % 32;
+  const T* x = static_cast<const T*>(a.qkv);
+  const long kc = static_cast<long>(a.Hq + h / a.group) * D, vc = kc + static_cast<long>(a.Hkv) * D;
+  float q[N], g[N], k[N], v[N], acc[N] = {};
+  load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
+  load_part<D>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D, g);
+  const float* rb = row_block(a, h, row);
+  for (int j = st; j <= row; ++j) {
+    load_part<D>(x + j * a.ld + kc, k);
+    load_part<D>(x + j * a.ld + vc, v);
+    const float ds = ex2(dot<N>(q, k) * a.scale_log2 + rb[0]) * (dot<N>(g, v) + rb[64]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += ds * k[i];
+  }
+  T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(h) * D;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (lane * N + i >= c0 && lane * N + i < c1) out[lane * N + i] = from_float<T>(acc[i] * a.scale);
+}
+
+// One row of dK (want_k) or dV of key head kvh, over query heads [h0, h1), to 16 bits or, where a split's sum follows, fp32.
+template <int D, typename T>
+__device__ __noinline__ void slow_dkv(const Args& a, int row, int kvh, int h0, int h1, int end, bool want_k, float* partial) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x % 32;
+  const T* x = static_cast<const T*>(a.qkv);
+  const long kc = static_cast<long>(a.Hq + kvh) * D, vc = kc + static_cast<long>(a.Hkv) * D;
+  float q[N], g[N], k[N], v[N], acc[N] = {};
+  load_part<D>(x + row * a.ld + kc, k);
+  load_part<D>(x + row * a.ld + vc, v);
+  for (int h = h0; h < h1; ++h)
+    for (int j = row; j < end; ++j) {
+      load_part<D>(x + j * a.ld + static_cast<long>(h) * D, q);
+      load_part<D>(static_cast<const T*>(a.dout) + j * a.do_ld + static_cast<long>(h) * D, g);
+      const float* rb = row_block(a, h, j);
+      const float p = ex2(dot<N>(q, k) * a.scale_log2 + rb[0]);
+      const float ds = p * (dot<N>(g, v) + rb[64]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += want_k ? ds * q[i] : p * g[i];
+    }
+  T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + (want_k ? kc : vc);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = want_k ? acc[i] * a.scale : acc[i];
+    if (partial != nullptr) partial[lane * N + i] = y;
+    else out[lane * N + i] = from_float<T>(y);
+  }
+}
+
+}  // namespace pa
+}  // namespace sb

@@ -1,0 +1,696 @@
+// Backward kernels of causal attention over packed sequences (attention_packed.cuh has the design).
+//
+// Two passes, each with the products it needs, so that every sum stays in one tensor memory accumulator and no order hangs
+// on timing: dK / dV by tiles of 128 keys (S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q), dQ by tiles of 128
+// queries (S = Q K^T, dP = dO V^T, dQ += dS K).  Seven products instead of five; one pass would add dQ across CTAs in the
+// order in which they get there.
+//
+// In both, the other side comes in blocks of 64 and the two groups of softmax warps take them in turn: S and dP of block n
+// are in buffer n & 1 (64 columns each), P and dS go over them as 16-bit operands.  While a group works on block n, the
+// products of block n + 1 fill the other buffer.
+#include "attention_packed.cuh"
+
+namespace sb {
+namespace pa {
+
+constexpr int kSub = 64 * 128;     // bytes of 64 rows of 64 16-bit columns
+
+// -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
+// a row of a head.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args a, float* __restrict__ out) {
+  constexpr int L = D / 8;
+  const long i = static_cast<long>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  const int sub = threadIdx.x % L, h = static_cast<int>(i % a.Hq);
+  const long row = i / a.Hq;
+  if (row >= static_cast<long>(a.tiles) * 128) return;         // whole groups of L lanes; a warp's last group shuffles alone
+  const unsigned lanes = (L == 8 ? 0xffu : 0xffffu) << (threadIdx.x % 32 / L * L);
+  float s = 0.f, nl = 0.f;
+  if (row < a.T && a.start[row] <= row) {
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D + sub * 8);
+    const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D + sub * 8);
+    const T *x = reinterpret_cast<const T*>(&u), *y = reinterpret_cast<const T*>(&g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += to_float(x[k]) * to_float(y[k]);
+    nl = -a.lse[static_cast<long>(h) * a.T + row] * kLog2e;
+  }
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(lanes, s, o);
+  if (sub == 0) {
+    float* p = out + (static_cast<long>(h) * (a.tiles * 2) + row / 64) * 128 + row % 64;
+    p[0] = nl;
+    p[64] = -s;
+  }
+}
+
+// ============================ dK, dV ============================
+template <int D>
+struct Dkv {
+  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
+  static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock + 512;      // Q, dO, -lse and -delta of 64 queries
+  static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
+};
+
+struct DkvItem {
+  int kvh, part, k0, first_h, heads, blocks, subs;      // `blocks` of 64 queries a head
+  SB_DEVICE DkvItem(const Args& a, int idx) {
+    const int per = a.Hkv * a.split, r = idx % per;
+    kvh = r / a.split;
+    part = r % a.split;
+    heads = a.group / a.split;
+    first_h = kvh * a.group + part * heads;
+    k0 = a.order[idx / per] * 128;
+    const int end = a.stop[min(k0 + 127, a.T - 1)];
+    blocks = k0 < a.ends[1] && k0 + 128 > a.ends[0] ? (end - k0 + 63) / 64 : 0;
+    subs = blocks * heads;
+  }
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUtensorMap tm64,
+           const __grid_constant__ CUtensorMap tmo, const __grid_constant__ Args a) {
+  using F = Dkv<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* sK = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint8_t* sV = sK + F::kTile;
+  uint8_t* sQ = sV + F::kTile;                                  // [stages][Q | dO]
+  float* sR = reinterpret_cast<float*>(sQ + F::kStages * 2 * F::kBlock);          // [stages][2][64]
+  uint4* answer = reinterpret_cast<uint4*>(sR + F::kStages * 128);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
+  uint64_t *kv_full = bar, *kv_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
+  uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
+  const Sched sched{answer, p_full + 2, p_full + 4};
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_full + 6);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(kv_empty, 1);
+    mbar_init(land, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 8);
+    mbar_init(drain, 1);
+    for (int i = 0; i < F::kStages; ++i) {
+      mbar_init(&in_full[i], 1);
+      mbar_init(&in_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&sched.full[i], 1);
+      mbar_init(&sched.empty[i], kReaders);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kIssuer) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot, tdV = tbase + 256, tdK = tbase + 256 + D;
+
+  if (warp >= 8) {
+    regs_down<kOtherRegs>();
+    if (warp == kLoader) {
+      const int first = a.ends[0], last = min(a.ends[1], a.T);
+      int g = 0, nkv = 0, nl = 0;
+      bool ok = true;
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        if (lane == 0) ok = sched_request(sched, n, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        const DkvItem it(a, idx);
+        if (ok && it.subs > 0) {
+          if (lane == 0) {
+            ok = mbar_wait(kv_empty, (nkv & 1) ^ 1, a.status);
+            if (ok) {
+              mbar_arrive_expect_tx(kv_full, 2 * F::kTile);
+              for (int c = 0; c < F::kHalves; ++c) {
+                tma_load_2d(sK + c * kChunk, &tm128, kv_full, (a.Hq + it.kvh) * D + c * 64, it.k0);
+                tma_load_2d(sV + c * kChunk, &tm128, kv_full, (a.Hq + a.Hkv + it.kvh) * D + c * 64, it.k0);
+              }
+            }
+          }
+          ++nkv;
+          ok = __all_sync(0xffffffffu, ok);
+          for (int s = 0; s < it.subs && ok; ++s, ++g) {
+            const int st = g % F::kStages, h = it.first_h + s / it.blocks, row = it.k0 + s % it.blocks * 64;
+            const bool clear = row < first || min(row + 64, a.T) > last;
+            uint8_t* in = sQ + st * 2 * F::kBlock;
+            if (lane == 0) {
+              ok = mbar_wait(&in_empty[st], ((g / F::kStages) & 1) ^ 1, a.status);
+              if (ok) {
+                uint64_t* to = clear ? land : &in_full[st];
+                mbar_arrive_expect_tx(to, F::kStage);
+                for (int c = 0; c < F::kHalves; ++c) {
+                  tma_load_2d(in + c * kSub, &tm64, to, h * D + c * 64, row);
+                  tma_load_2d(in + F::kBlock + c * kSub, &tmo, to, h * D + c * 64, row);
+                }
+                bulk_load(sR + st * 128, row_block(a, h, row), 512, to);
+              }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (clear && ok) {
+              ok = __all_sync(0xffffffffu, mbar_wait(land, nl & 1, a.status));
+              ++nl;
+              if (ok) {
+                clear_rows(in, 64, F::kHalves, kSub, row, first, last);
+                clear_rows(in + F::kBlock, 64, F::kHalves, kSub, row, first, last);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&in_full[st]);
+              }
+            }
+          }
+        }
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+    } else if (warp == kIssuer) {
+      constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
+      const uint32_t ka = smem_u32(sK), va = smem_u32(sV);
+      int g = 0, nkv = 0;
+      bool ok = true;
+      auto scores = [&](int g) -> bool {               // S^T and dP^T of block g to its buffer
+        const int st = g % F::kStages;
+        if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
+        tc_fence_after();
+        const uint32_t qa = smem_u32(sQ + st * 2 * F::kBlock), oa = qa + F::kBlock, ts = tbase + (g & 1) * 128;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
+          umma_f16(ts, kdesc(ka + off), kdesc(qa + sub), idS, kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
+          umma_f16(ts + 64, kdesc(va + off), kdesc(oa + sub), idS, kk > 0);
+        }
+        umma_commit(&s_full[g & 1]);
+        return true;
+      };
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        const DkvItem it(a, idx);
+        if (lane == 0 && it.subs > 0) {
+          ok = mbar_wait(kv_full, nkv & 1, a.status);
+          if (ok) ok = scores(g);
+          for (int s = 0; s < it.subs && ok; ++s, ++g) {
+            if (s + 1 < it.subs) ok = scores(g + 1);
+            if (ok && s == max(0, it.subs - 2)) umma_commit(kv_empty);                    // the last scores were issued
+            if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
+            if (ok && s == 0 && nkv > 0) ok = mbar_wait(acc_free, (nkv - 1) & 1, a.status);
+            if (!ok) break;
+            tc_fence_after();
+            const int st = g % F::kStages;
+            const uint32_t qa = smem_u32(sQ + st * 2 * F::kBlock), oa = qa + F::kBlock, ts = tbase + (g & 1) * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tdV, ts + kk * 8, mndesc(oa + kk * 2048, kSub), idG, s > 0 || kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tdK, ts + 64 + kk * 8, mndesc(qa + kk * 2048, kSub), idG, s > 0 || kk > 0);
+            umma_commit(&in_empty[st]);
+          }
+          if (ok) umma_commit(acc_full);
+          ++nkv;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {
+        umma_commit(drain);
+        mbar_wait(drain, 0, a.status);
+      }
+      __syncwarp();
+    }
+  } else {
+    regs_up<kSoftRegs>();
+    const int w = warp / 4;                            // this group's buffer; at the end, 0 stores dV and 1 dK
+    const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t ts = tbase + w * 128 + lane_off;
+    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    int g = 0, nkv = 0;
+    bool ok = true;
+    for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+      const DkvItem it(a, idx);
+      const int row = it.k0 + (warp % 4) * 32 + lane;
+      const int end = row < a.T ? a.stop[row] : row;
+      const int least = a.stop[it.k0];                 // the tile's earliest end
+      for (int s = 0; s < it.subs; ++s, ++g) {
+        if ((g & 1) != w) continue;
+        const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * 64;
+        // -lse and -delta came with Q and dO; S cannot be there before them
+        if (!__all_sync(0xffffffffu, mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status) &&
+                                         mbar_wait(&s_full[w], (g >> 1) & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const float4* nl4 = reinterpret_cast<const float4*>(sR + st * 128);
+        const bool masked = q0 < it.k0 + 127 || q0 + 64 > least;
+        const int from = row - q0, to_c = end - q0;    // visible: from <= column < to_c
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t vs[32], vd[32];
+          tmem_ld_32x32b_x32(ts + c, vs);
+          tmem_ld_32x32b_x32(ts + 64 + c, vd);
+          tmem_wait_ld();
+          uint32_t pp[16], pd[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 nl = nl4[(c + k) / 4], nd = nl4[16 + (c + k) / 4];
+            float2 z[2], e[2];
+            z[0] = fma2(make_float2(__uint_as_float(vs[k]), __uint_as_float(vs[k + 1])), sc2, make_float2(nl.x, nl.y));
+            z[1] = fma2(make_float2(__uint_as_float(vs[k + 2]), __uint_as_float(vs[k + 3])), sc2, make_float2(nl.z, nl.w));
+            e[0] = add2(make_float2(__uint_as_float(vd[k]), __uint_as_float(vd[k + 1])), make_float2(nd.x, nd.y));
+            e[1] = add2(make_float2(__uint_as_float(vd[k + 2]), __uint_as_float(vd[k + 3])), make_float2(nd.z, nd.w));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              z[u].x = ex2(z[u].x);
+              z[u].y = ex2(z[u].y);
+              e[u] = mul2(e[u], z[u]);
+            }
+            if (masked) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int col = c + k + 2 * u;
+                if (col < from || col >= to_c) z[u].x = e[u].x = 0.f;
+                if (col + 1 < from || col + 1 >= to_c) z[u].y = e[u].y = 0.f;
+              }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              pp[k / 2 + u] = Half<T>::pack(z[u].x, z[u].y);
+              pd[k / 2 + u] = Half<T>::pack(e[u].x, e[u].y);
+            }
+          }
+          tmem_st_32x32b_x16(ts + c / 2, pp);
+          tmem_st_32x32b_x16(ts + 64 + c / 2, pd);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+      }
+      if (!ok) break;
+      const bool covered = row < a.T && end > row;
+      const bool dk = w == 1;
+      const long col = static_cast<long>(a.Hq + (dk ? 0 : a.Hkv) + it.kvh) * D;
+      T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + col;
+      float* partial = nullptr;
+      if (a.split > 1)
+        partial = a.partial + ((static_cast<long>(it.part) * a.Hkv + it.kvh) * a.T + row) * (2 * D) + (dk ? 0 : D);
+      bool bad = false;
+      if (it.subs > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_full, nkv & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        ++nkv;
+        tc_fence_after();
+        const float f = dk ? a.scale : 1.f;
+        float chk = 0.f;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32((dk ? tdK : tdV) + lane_off + c, o);
+          tmem_wait_ld();
+          if (c + 32 == D) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float y = __uint_as_float(o[k]) * f;
+            chk = fmaf(y, 0.f, chk);
+            o[k] = __float_as_uint(y);
+          }
+          if (covered && partial != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(partial + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          } else if (covered) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                y[e] = Half<T>::pack(__uint_as_float(o[k + 2 * e]), __uint_as_float(o[k + 2 * e + 1]));
+              *reinterpret_cast<uint4*>(out + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+        }
+        bad = covered && chk != 0.f;
+      }
+      if (row < a.T && !covered && a.fill && it.part == 0)
+#pragma unroll
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
+        const int who = __ffs(some) - 1, r = __shfl_sync(0xffffffffu, row, who);
+        slow_dkv<D, T>(a, r, it.kvh, it.first_h, it.first_h + it.heads, __shfl_sync(0xffffffffu, end, who), dk,
+                       partial == nullptr ? nullptr : partial + static_cast<long>(r - row) * (2 * D));
+      }
+      idx = sched_next(sched, n, a.status);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer) tmem_dealloc(tbase, 512);
+}
+
+// Sums of a split, in order: one thread has 8 values of a row's [dK | dV].
+template <int D, typename T>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
+  const long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  const int c = static_cast<int>(i % (2 * D / 8)) * 8;
+  const long r = i / (2 * D / 8);
+  const int row = static_cast<int>(r % a.T), kvh = static_cast<int>(r / a.T);
+  if (kvh >= a.Hkv || a.stop[row] <= row) return;
+  float s[8] = {};
+  for (int p = 0; p < a.split; ++p) {
+    const float4* x = reinterpret_cast<const float4*>(a.partial + ((static_cast<long>(p) * a.Hkv + kvh) * a.T + row) * (2 * D) + c);
+    const float4 u = x[0], v = x[1];
+    s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+    s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+  }
+  const long col = static_cast<long>(a.Hq + kvh + (c < D ? 0 : a.Hkv)) * D + c % D;
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.dqkv) + row * a.dqkv_ld + col) =
+      make_uint4(Half<T>::pack(s[0], s[1]), Half<T>::pack(s[2], s[3]), Half<T>::pack(s[4], s[5]), Half<T>::pack(s[6], s[7]));
+}
+
+// ============================ dQ ============================
+template <int D>
+struct Dq {
+  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
+  static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock;             // K, V of 64 keys
+  static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
+};
+
+struct DqItem {
+  int h, kvh, q0, lo, hi;                              // blocks of 64 keys
+  SB_DEVICE DqItem(const Args& a, int idx) {
+    h = idx % a.Hq;
+    kvh = h / a.group;
+    q0 = a.order[idx / a.Hq] * 128;
+    lo = hi = 0;
+    if (q0 < a.ends[1] && q0 + 128 > a.ends[0]) {
+      lo = a.start[q0] / 64;
+      hi = min(q0 / 64 + 2, (a.T + 63) / 64);
+    }
+  }
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUtensorMap tm64,
+          const __grid_constant__ CUtensorMap tmo, const __grid_constant__ Args a) {
+  using F = Dq<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* sQ = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint8_t* sO = sQ + F::kTile;
+  uint8_t* sK = sO + F::kTile;                                  // [stages][K | V]
+  uint4* answer = reinterpret_cast<uint4*>(sK + F::kStages * F::kStage);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
+  uint64_t *q_full = bar, *q_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
+  uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
+  const Sched sched{answer, p_full + 2, p_full + 4};
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_full + 6);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(land, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 8);
+    mbar_init(drain, 1);
+    for (int i = 0; i < F::kStages; ++i) {
+      mbar_init(&in_full[i], 1);
+      mbar_init(&in_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&sched.full[i], 1);
+      mbar_init(&sched.empty[i], kReaders);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kIssuer) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot, tdQ = tbase + 256;
+
+  if (warp >= 8) {
+    regs_down<kOtherRegs>();
+    if (warp == kLoader) {
+      const int first = a.ends[0], last = min(a.ends[1], a.T);
+      int g = 0, nq = 0, nl = 0;
+      bool ok = true;
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        if (lane == 0) ok = sched_request(sched, n, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        const DqItem it(a, idx);
+        if (ok && it.hi > it.lo) {
+          if (lane == 0) {
+            ok = mbar_wait(q_empty, (nq & 1) ^ 1, a.status);
+            if (ok) {
+              mbar_arrive_expect_tx(q_full, 2 * F::kTile);
+              for (int c = 0; c < F::kHalves; ++c) {
+                tma_load_2d(sQ + c * kChunk, &tm128, q_full, it.h * D + c * 64, it.q0);
+                tma_load_2d(sO + c * kChunk, &tmo, q_full, it.h * D + c * 64, it.q0);
+              }
+            }
+          }
+          ++nq;
+          ok = __all_sync(0xffffffffu, ok);
+          for (int j = it.lo; j < it.hi && ok; ++j, ++g) {
+            const int st = g % F::kStages, row = j * 64;
+            const bool clear = row < first || min(row + 64, a.T) > last;
+            uint8_t* in = sK + st * F::kStage;
+            if (lane == 0) {
+              ok = mbar_wait(&in_empty[st], ((g / F::kStages) & 1) ^ 1, a.status);
+              if (ok) {
+                uint64_t* to = clear ? land : &in_full[st];
+                mbar_arrive_expect_tx(to, F::kStage);
+                for (int c = 0; c < F::kHalves; ++c) {
+                  tma_load_2d(in + c * kSub, &tm64, to, (a.Hq + it.kvh) * D + c * 64, row);
+                  tma_load_2d(in + F::kBlock + c * kSub, &tm64, to, (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
+                }
+              }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (clear && ok) {                         // K alone is multiplied by masked values
+              ok = __all_sync(0xffffffffu, mbar_wait(land, nl & 1, a.status));
+              ++nl;
+              if (ok) {
+                clear_rows(in, 64, F::kHalves, kSub, row, first, last);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&in_full[st]);
+              }
+            }
+          }
+        }
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+    } else if (warp == kIssuer) {
+      constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
+      const uint32_t qa = smem_u32(sQ), oa = smem_u32(sO);
+      int g = 0, nq = 0;
+      bool ok = true;
+      auto scores = [&](int g) -> bool {
+        const int st = g % F::kStages;
+        if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(sK + st * F::kStage), va = ka + F::kBlock, ts = tbase + (g & 1) * 128;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
+          umma_f16(ts, kdesc(qa + off), kdesc(ka + sub), idS, kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
+          umma_f16(ts + 64, kdesc(oa + off), kdesc(va + sub), idS, kk > 0);
+        }
+        umma_commit(&s_full[g & 1]);
+        return true;
+      };
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        const DqItem it(a, idx);
+        const int subs = it.hi - it.lo;
+        if (lane == 0 && subs > 0) {
+          ok = mbar_wait(q_full, nq & 1, a.status);
+          if (ok) ok = scores(g);
+          for (int s = 0; s < subs && ok; ++s, ++g) {
+            if (s + 1 < subs) ok = scores(g + 1);
+            if (ok && s == max(0, subs - 2)) umma_commit(q_empty);             // the last scores were issued
+            if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
+            if (ok && s == 0 && nq > 0) ok = mbar_wait(acc_free, (nq - 1) & 1, a.status);
+            if (!ok) break;
+            tc_fence_after();
+            const int st = g % F::kStages;
+            const uint32_t ka = smem_u32(sK + st * F::kStage), ts = tbase + (g & 1) * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tdQ, ts + kk * 8, mndesc(ka + kk * 2048, kSub), idG, s > 0 || kk > 0);
+            umma_commit(&in_empty[st]);
+          }
+          if (ok) umma_commit(acc_full);
+          ++nq;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {
+        umma_commit(drain);
+        mbar_wait(drain, 0, a.status);
+      }
+      __syncwarp();
+    }
+  } else {
+    regs_up<kSoftRegs>();
+    const int w = warp / 4;                            // this group's buffer; at the end, its half of the columns
+    const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t ts = tbase + w * 128 + lane_off;
+    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    int g = 0, nq = 0;
+    bool ok = true;
+    for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+      const DqItem it(a, idx);
+      const int row = it.q0 + (warp % 4) * 32 + lane;
+      const int st = row < a.T ? a.start[row] : row + 1;
+      const int most = a.start[min(it.q0 + 127, a.T - 1)];
+      const float* rb = row_block(a, it.h, row);       // there are rows up to a multiple of 128
+      const float2 nl = make_float2(rb[0], rb[0]), nd = make_float2(rb[64], rb[64]);
+      for (int j = it.lo; j < it.hi; ++j, ++g) {
+        if ((g & 1) != w) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (g >> 1) & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const bool masked = j * 64 < most || j * 64 + 63 > it.q0;
+        const int from = st - j * 64, to_c = row - j * 64;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t vs[32], vd[32], pd[16];
+          tmem_ld_32x32b_x32(ts + c, vs);
+          tmem_ld_32x32b_x32(ts + 64 + c, vd);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float2 z = fma2(make_float2(__uint_as_float(vs[k]), __uint_as_float(vs[k + 1])), sc2, nl);
+            float2 e = add2(make_float2(__uint_as_float(vd[k]), __uint_as_float(vd[k + 1])), nd);
+            z.x = ex2(z.x);
+            z.y = ex2(z.y);
+            e = mul2(e, z);
+            if (masked) {
+              if (c + k < from || c + k > to_c) e.x = 0.f;
+              if (c + k + 1 < from || c + k + 1 > to_c) e.y = 0.f;
+            }
+            pd[k / 2] = Half<T>::pack(e.x, e.y);
+          }
+          tmem_st_32x32b_x16(ts + c / 2, pd);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+      }
+      if (!ok) break;
+      const bool covered = row < a.T && st <= row;
+      T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(it.h) * D;
+      bool bad = false;
+      if (it.hi > it.lo) {
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_full, nq & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        tc_fence_after();
+        float chk = 0.f;
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) {
+          const int c = w * (D / 2) + u * 32;
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tdQ + lane_off + c, o);
+          tmem_wait_ld();
+          if (u + 1 == D / 64) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = __uint_as_float(o[k + 2 * e]) * a.scale, y1 = __uint_as_float(o[k + 2 * e + 1]) * a.scale;
+              chk = fmaf(y0, 0.f, fmaf(y1, 0.f, chk));
+              y[e] = Half<T>::pack(y0, y1);
+            }
+            if (covered) *reinterpret_cast<uint4*>(out + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        bad = covered && chk != 0.f;
+      }
+      if (row < a.T && !covered && a.fill)
+#pragma unroll
+        for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + w * (D / 2) + c) = make_uint4(0, 0, 0, 0);
+      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
+        const int who = __ffs(some) - 1;
+        slow_dq<D, T>(a, __shfl_sync(0xffffffffu, row, who), it.h, __shfl_sync(0xffffffffu, st, who), w * (D / 2),
+                      (w + 1) * (D / 2));
+      }
+      idx = sched_next(sched, n, a.status);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer) tmem_dealloc(tbase, 512);
+}
+
+template <int D, typename T>
+static void launch(const CUtensorMap& tm128, const CUtensorMap& tm64, const CUtensorMap& do128, const CUtensorMap& do64,
+                   Args a, const int* q_order, const int* k_order, float* rows, cudaStream_t stream) {
+  const long work = static_cast<long>(a.tiles) * 128 * a.Hq;
+  rows_kernel<D, T><<<static_cast<unsigned>((work + 256 / (D / 8) - 1) / (256 / (D / 8))), 256, 0, stream>>>(a, rows);
+  a.rows = rows;
+  cudaFuncSetAttribute(dkv_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dkv<D>::kSmem);
+  cudaFuncSetAttribute(dq_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dq<D>::kSmem);
+  a.order = k_order;
+  dkv_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hkv * a.split), kThreads, Dkv<D>::kSmem, stream>>>(tm128, tm64, do64, a);
+  if (a.split > 1) {
+    const long n = static_cast<long>(a.Hkv) * a.T * (2 * D / 8);
+    join_kernel<D, T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(a);
+  }
+  a.order = q_order;
+  dq_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hq), kThreads, Dq<D>::kSmem, stream>>>(tm128, tm64, do128, a);
+}
+
+void launch_bwd(int D, bool half, const CUtensorMap& tm128, const CUtensorMap& tm64, const CUtensorMap& do128,
+                const CUtensorMap& do64, const Args& a, const int* q_order, const int* k_order, float* rows,
+                cudaStream_t stream) {
+  if (D == 64) {
+    if (half) launch<64, __half>(tm128, tm64, do128, do64, a, q_order, k_order, rows, stream);
+    else launch<64, __nv_bfloat16>(tm128, tm64, do128, do64, a, q_order, k_order, rows, stream);
+  } else {
+    if (half) launch<128, __half>(tm128, tm64, do128, do64, a, q_order, k_order, rows, stream);
+    else launch<128, __nv_bfloat16>(tm128, tm64, do128, do64, a, q_order, k_order, rows, stream);
+  }
+}
+
+}  // namespace pa
+}  // namespace sb

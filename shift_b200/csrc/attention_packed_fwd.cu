@@ -1,0 +1,396 @@
+// Forward kernel of causal attention over packed sequences (attention_packed.cuh has the design).
+#include "attention_packed.cuh"
+
+namespace sb {
+namespace pa {
+
+// ============================ forward ============================
+// An item is two tiles of 128 queries that share a loop over key blocks.  Group w of softmax warps has tile w.
+//   issuer   S_w = Q_w K_j^T (128 x 128),  O_w += P_w V_j (128 x D), P_w read from tensor memory
+//   softmax  a thread's whole row of S to registers, running maximum and sum, P back to tensor memory
+// Heads of 64: S, P and O of both tiles have columns of their own (2 x (128 + 64 + 64)), so the next S is computed while a
+// group is still at its exponentials.  Heads of 128: P lies over S (2 x (128 + 128)).
+template <int D>
+struct Fwd {
+  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk;
+  static constexpr int kK = D == 64 ? 4 : 3, kV = D == 64 ? 4 : 2;     // stages
+  static constexpr bool kOver = D == 128;                              // P over S
+  static constexpr int kSmem = 1024 + 2 * kTile + (kK + kV) * kTile + 512;
+  static constexpr int kP = kOver ? 0 : 256, kPStep = kOver ? 128 : 64, kO = kOver ? 256 : 384;
+};
+
+struct FwdItem {
+  int h[2], q0[2], lo[2], hi[2], all_lo, all_hi, kvh;
+  SB_DEVICE FwdItem(const Args& a, int idx) {
+    const int per = a.pair_heads ? a.Hq / 2 : a.Hq;
+    const int t = a.order[idx / per], r = idx % per;
+    const int first = a.ends[0], last = a.ends[1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[i] = a.pair_heads ? 2 * r + i : r;
+      q0[i] = a.pair_heads ? t * 128 : t * 256 + i * 128;
+      lo[i] = hi[i] = 0;
+      if (q0[i] < a.T && q0[i] < last && q0[i] + 128 > first) {
+        lo[i] = a.start[q0[i]] / 128;
+        hi[i] = q0[i] / 128 + 1;
+      }
+    }
+    const bool one = hi[0] > lo[0], two = hi[1] > lo[1];
+    all_lo = one && two ? min(lo[0], lo[1]) : one ? lo[0] : lo[1];
+    all_hi = max(hi[0], hi[1]);
+    kvh = h[0] / a.group;
+  }
+  SB_DEVICE bool has(int i, int j) const { return j >= lo[i] && j < hi[i]; }
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Args a) {
+  using F = Fwd<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* sQ = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint8_t* sK = sQ + 2 * F::kTile;
+  uint8_t* sV = sK + F::kK * F::kTile;
+  uint4* answer = reinterpret_cast<uint4*>(sV + F::kV * F::kTile);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
+  uint64_t *q_full = bar, *q_empty = bar + 1, *land = bar + 2, *k_full = bar + 3, *k_empty = k_full + F::kK;
+  uint64_t *v_full = k_empty + F::kK, *v_empty = v_full + F::kV, *s_full = v_empty + F::kV, *s_empty = s_full + 2;
+  uint64_t *p_full = s_empty + 2, *o_full = p_full + 2, *o_free = o_full + 2, *drain = o_free + 2;
+  const Sched sched{answer, drain + 1, drain + 3};
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 5);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(land, 1);
+    mbar_init(drain, 1);
+    for (int i = 0; i < F::kK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < F::kV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 4);
+      mbar_init(&sched.full[i], 1);
+      mbar_init(&sched.empty[i], kReaders);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kIssuer) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot;
+
+  if (warp >= 8) {
+    regs_down<kOtherRegs>();
+    if (warp == kLoader) {
+      const int first = a.ends[0], last = min(a.ends[1], a.T);
+      int nk = 0, nv = 0, nq = 0, nl = 0;
+      bool ok = true;
+      if (lane == 0) tma_prefetch_desc(&tm);
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        if (lane == 0) ok = sched_request(sched, n, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        const FwdItem it(a, idx);
+        if (ok && it.all_hi > it.all_lo) {
+          if (lane == 0) {
+            ok = mbar_wait(q_empty, (nq & 1) ^ 1, a.status);
+            if (ok) {
+              mbar_arrive_expect_tx(q_full, 2 * F::kTile);
+              for (int i = 0; i < 2; ++i)
+                for (int c = 0; c < F::kHalves; ++c)
+                  tma_load_2d(sQ + i * F::kTile + c * kChunk, &tm, q_full, it.h[i] * D + c * 64, it.q0[i]);
+            }
+          }
+          ++nq;
+          ok = __all_sync(0xffffffffu, ok);
+          for (int j = it.all_lo; j < it.all_hi && ok; ++j, ++nk, ++nv) {
+            const int sk = nk % F::kK, sv = nv % F::kV, row = j * 128;
+            const bool clear = row < first || min(row + 128, a.T) > last;
+            if (lane == 0) {
+              ok = mbar_wait(&k_empty[sk], ((nk / F::kK) & 1) ^ 1, a.status);
+              if (ok) {
+                mbar_arrive_expect_tx(&k_full[sk], F::kTile);
+                for (int c = 0; c < F::kHalves; ++c)
+                  tma_load_2d(sK + sk * F::kTile + c * kChunk, &tm, &k_full[sk], (a.Hq + it.kvh) * D + c * 64, row);
+                ok = mbar_wait(&v_empty[sv], ((nv / F::kV) & 1) ^ 1, a.status);
+              }
+              if (ok) {
+                uint64_t* to = clear ? land : &v_full[sv];
+                mbar_arrive_expect_tx(to, F::kTile);
+                for (int c = 0; c < F::kHalves; ++c)
+                  tma_load_2d(sV + sv * F::kTile + c * kChunk, &tm, to, (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
+              }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (clear && ok) {
+              ok = __all_sync(0xffffffffu, mbar_wait(land, nl & 1, a.status));
+              ++nl;
+              if (ok) {
+                clear_rows(sV + sv * F::kTile, 128, F::kHalves, kChunk, row, first, last);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[sv]);
+              }
+            }
+          }
+        }
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+    } else if (warp == kIssuer) {
+      constexpr uint32_t idS = idesc<T>(128, 128, 0), idO = idesc<T>(128, D, 1);
+      int nk = 0, nv = 0, nq = 0, nb[2] = {0, 0}, no[2] = {0, 0};   // blocks and items of each tile so far
+      bool ok = true;
+      const uint32_t qa = smem_u32(sQ);
+      auto issue_s = [&](int i, int sk) {              // S_i of the key block in stage sk
+        const uint32_t ka = smem_u32(sK + sk * F::kTile), q = qa + i * F::kTile;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32;
+          umma_f16(tbase + i * 128, kdesc(q + off), kdesc(ka + off), idS, kk > 0);
+        }
+        umma_commit(&s_full[i]);
+      };
+      auto issue_o = [&](int i, int sv, bool fresh) {
+        const uint32_t va = smem_u32(sV + sv * F::kTile);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16_ts(tbase + F::kO + i * D, tbase + F::kP + i * F::kPStep + kk * 8, mndesc(va + kk * 2048, kChunk), idO,
+                      !(fresh && kk == 0));
+        umma_commit(&o_full[i]);
+      };
+      for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+        const FwdItem it(a, idx);
+        if (lane == 0 && it.all_hi > it.all_lo) {
+          ok = mbar_wait(q_full, nq & 1, a.status);
+          ++nq;
+          // S of block j: its stage is nk % kK
+          auto scores = [&](int j, int i) -> bool {
+            if (!F::kOver && nb[i] > 0 && !mbar_wait(&s_empty[i], (nb[i] - 1) & 1, a.status)) return false;
+            tc_fence_after();
+            issue_s(i, nk % F::kK);
+            ++nb[i];
+            return true;
+          };
+          auto keys = [&]() -> bool { return mbar_wait(&k_full[nk % F::kK], (nk / F::kK) & 1, a.status); };
+          auto keys_done = [&](int j) {
+            umma_commit(&k_empty[nk % F::kK]);
+            ++nk;
+            if (j == it.all_hi - 1) umma_commit(q_empty);
+          };
+          int np[2] = {nb[0], nb[1]};                  // blocks whose P was used
+          if (ok) ok = keys();
+          for (int i = 0; i < 2 && ok; ++i)
+            if (it.has(i, it.all_lo)) ok = scores(it.all_lo, i);
+          if (ok) keys_done(it.all_lo);
+          for (int j = it.all_lo; j < it.all_hi && ok; ++j) {
+            const bool more = j + 1 < it.all_hi;
+            if (more) ok = keys();
+            if (!F::kOver && more) {
+              for (int i = 0; i < 2 && ok; ++i)
+                if (it.has(i, j + 1)) ok = scores(j + 1, i);
+              if (ok) keys_done(j + 1);
+            }
+            const int sv = nv % F::kV;
+            if (ok) ok = mbar_wait(&v_full[sv], (nv / F::kV) & 1, a.status);
+            for (int i = 0; i < 2 && ok; ++i) {
+              if (it.has(i, j)) {
+                ok = mbar_wait(&p_full[i], np[i] & 1, a.status);
+                ++np[i];
+                if (ok && j == it.lo[i] && no[i] > 0) ok = mbar_wait(&o_free[i], (no[i] - 1) & 1, a.status);
+                if (!ok) break;
+                tc_fence_after();
+                issue_o(i, sv, j == it.lo[i]);
+              }
+              if (F::kOver && more && it.has(i, j + 1)) ok = scores(j + 1, i);
+            }
+            if (!ok) break;
+            umma_commit(&v_empty[sv]);
+            ++nv;
+            if (F::kOver && more) keys_done(j + 1);
+          }
+          for (int i = 0; i < 2; ++i) no[i] += it.hi[i] > it.lo[i];
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {                                 // nothing of this CTA is in flight when tensor memory is given back
+        umma_commit(drain);
+        mbar_wait(drain, 0, a.status);
+      }
+      __syncwarp();
+    }
+  } else {
+    regs_up<kSoftRegs>();
+    const int w = warp / 4;                            // tile
+    const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * F::kPStep + lane_off;
+    const uint32_t to = tbase + F::kO + w * D + lane_off;
+    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    int nb = 0;
+    bool ok = true;
+    for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
+      const FwdItem it(a, idx);
+      const int q0 = w ? it.q0[1] : it.q0[0], lo = w ? it.lo[1] : it.lo[0], hi = w ? it.hi[1] : it.hi[0];
+      const int h = w ? it.h[1] : it.h[0];
+      const int row = q0 + (warp % 4) * 32 + lane;
+      const int st = row < a.T ? a.start[row] : row + 1;
+      const int most = q0 < a.T ? a.start[min(q0 + 127, a.T - 1)] : 0;     // the tile's latest start
+      float m = -INFINITY, l = 0.f;
+      for (int j = lo; j < hi; ++j, ++nb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], nb & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t v[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld_32x32b_x32(ts + c, v + c);
+        tmem_wait_ld();
+        if (!F::kOver) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[w]);
+        }
+        if (j * 128 < most || j * 128 + 127 > q0) {
+          const int from = st - j * 128, to_c = row - j * 128;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c < from || c > to_c) v[c] = 0xff800000u;
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            m4[k] = fmaxf(fmaxf(m4[k], __uint_as_float(v[c + 2 * k])), __uint_as_float(v[c + 2 * k + 1]));
+        const float mx = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2);
+        if (j > lo) {                                  // P of the block before was read, and O holds it
+          if (!__all_sync(0xffffffffu, mbar_wait(&o_full[w], (nb - 1) & 1, a.status))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        if (__any_sync(0xffffffffu, mx > m + kRescale)) {
+          if (j > lo) {
+            const float f = mx == -INFINITY ? 1.f : ex2(m - mx);
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {          // few at a time: S is still in registers
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(to + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st_32x32b_x16(to + c, o);
+            }
+            tmem_wait_st();
+            l *= f;
+          }
+          m = mx;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const float2 nm2 = make_float2(nm, nm);
+        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float2 z = fma2(make_float2(__uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1])), sc2, nm2);
+            z.x = ex2(z.x);
+            z.y = ex2(z.y);
+            l2[k & 1] = add2(l2[k & 1], z);
+            pk[k] = Half<T>::pack(z.x, z.y);
+          }
+          tmem_st_32x32b_x16(tp + c / 2, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+        l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+      }
+      if (!ok) break;
+      const bool covered = row < a.T && st <= row;
+      float lse2 = -INFINITY;
+      bool bad = false;
+      T* orow = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D;
+      if (hi > lo) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&o_full[w], (nb - 1) & 1, a.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const float inv = 1.f / l;
+        float chk = 0.f;
+        lse2 = m + log2f(l);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(to + c, o);
+          tmem_wait_ld();
+          if (c + 32 == D) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[w]);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = __uint_as_float(o[k + 2 * e]) * inv, y1 = __uint_as_float(o[k + 2 * e + 1]) * inv;
+              chk = fmaf(y0, 0.f, fmaf(y1, 0.f, chk));
+              y[e] = Half<T>::pack(y0, y1);
+            }
+            if (covered) *reinterpret_cast<uint4*>(orow + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        bad = covered && chk != 0.f && fabsf(lse2) < INFINITY;
+      }
+      if (row < a.T) {
+        a.lse[static_cast<long>(h) * a.T + row] = covered ? lse2 * kLn2 : -INFINITY;
+        if (!covered && a.fill)
+#pragma unroll
+          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
+      }
+      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
+        const int who = __ffs(some) - 1;
+        slow_o<D, T>(a, __shfl_sync(0xffffffffu, row, who), h, __shfl_sync(0xffffffffu, st, who),
+                     __shfl_sync(0xffffffffu, lse2, who));
+      }
+      idx = sched_next(sched, n, a.status);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer) tmem_dealloc(tbase, 512);
+}
+
+template <int D, typename T>
+static void launch(const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
+  cudaFuncSetAttribute(fwd_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fwd<D>::kSmem);
+  fwd_kernel<D, T><<<items, kThreads, Fwd<D>::kSmem, stream>>>(tm, a);
+}
+
+void launch_fwd(int D, bool half, const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
+  if (D == 64) half ? launch<64, __half>(tm, a, items, stream) : launch<64, __nv_bfloat16>(tm, a, items, stream);
+  else half ? launch<128, __half>(tm, a, items, stream) : launch<128, __nv_bfloat16>(tm, a, items, stream);
+}
+
+}  // namespace pa
+}  // namespace sb

@@ -87,7 +87,10 @@ at::Tensor sha256_leaves(const at::Tensor& t, int64_t leaf, const at::Tensor& co
 }  // namespace digest
 }  // namespace sb
 
-void bind_adamw_many(pybind11::module& m);   // adamw_many.cu
+void bind_adamw_many(pybind11::module& m);        // adamw_many.cu
+void bind_packed(pybind11::module& m);            // packed.cu
+void bind_packed_attention(pybind11::module& m);  // attention_packed_host.cpp
+void bind_objectives(pybind11::module& m);        // objectives_host.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "shift_b200 sm_100a kernels";
@@ -128,6 +131,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("nonfinite") = py::none(), py::arg("step_dev") = py::none());
   m.def("nonfinite_check", &sb::adam::nonfinite_check);
   bind_adamw_many(m);
+  bind_packed(m);
+  bind_packed_attention(m);
+  bind_objectives(m);
   m.def("fp8_quantize", &sb::fp8::quantize, "block quantiser to 8-bit floating point");
   m.def("fp8_matmul", &sb::fp8::matmul, "product of 8-bit matrices with block scales (dense / grouped)");
   m.def("attn_fwd", &sb::fa::fwd, "tcgen05 causal flash attention forward");

@@ -1,0 +1,373 @@
+// Losses of label log-probabilities, straight from the logits: the log-probability of every row's label with its gradient,
+// the clipped policy loss with a KL term, the preference loss of pairs of sequences.
+//
+//   lse = log sum_v exp z_v,   logp = z_label - lse,   dL/dz_v = d ([v = label] - exp(z_v - lse)),   d = dL/dlogp
+//
+// All of them move logits: a row has V values of 2 or 4 bytes and a few of its own.  Rows are cut over a cluster of 1, 2,
+// 4 or 8 CTAs (joined over distributed shared memory in rank order) where a slice would not stay in shared memory, or
+// where there are too few rows for the SMs.  Maxima and sums are fp32, one running pair a thread; what follows from a
+// row's sum (its logarithm, ratios, the clip's comparison) is computed once a row in 64 bits, because a ratio next to the
+// clip's border decides a whole row's gradient.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "lowp.cuh"
+#include "objectives.h"
+
+namespace cg = cooperative_groups;
+
+namespace sb {
+namespace obj {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+SB_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// exp(z - m); m is finite.  The difference is rounded before it is scaled, so the error goes with |z - m|, not with |z|.
+SB_DEVICE float exp_diff(float z, float m) { return ex2((z - m) * kLog2e); }
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static SB_DEVICE void unpack(const uint4& u, float* f) { bf16x8_to_float(reinterpret_cast<const bf16x8&>(u), f); }
+  static SB_DEVICE uint4 pack(const float* f) {
+    bf16x8 v = float_to_bf16x8(f);
+    return reinterpret_cast<uint4&>(v);
+  }
+};
+template <>
+struct Elem<__half> {
+  static SB_DEVICE void unpack(const uint4& u, float* f) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(h[i]);
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  }
+  static SB_DEVICE uint4 pack(const float* f) {
+    uint4 u;
+    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    return u;
+  }
+};
+template <>
+struct Elem<float> {
+  static SB_DEVICE void unpack(const uint4& u, float* f) {
+    f[0] = __uint_as_float(u.x);
+    f[1] = __uint_as_float(u.y);
+    f[2] = __uint_as_float(u.z);
+    f[3] = __uint_as_float(u.w);
+  }
+  static SB_DEVICE uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+// The part of a row that one CTA of a cluster has: whole 16-byte vectors [v0, v1) of the row's aligned middle; rank 0 also
+// the single values before and behind it (a row may start on any value's alignment).
+template <typename T>
+struct Slice {
+  static constexpr int E = 16 / sizeof(T);
+  T* row;
+  int head, tail, V, v0, v1;
+  bool edges;
+  SB_DEVICE Slice(T* r, int V_, int rank, int ranks) : row(r), V(V_) {
+    head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / static_cast<int>(sizeof(T)));
+    const int nv = (V - head) / E;
+    tail = V - head - nv * E;
+    v0 = static_cast<int>(static_cast<long>(nv) * rank / ranks);
+    v1 = static_cast<int>(static_cast<long>(nv) * (rank + 1) / ranks);
+    edges = rank == 0;
+  }
+  SB_DEVICE uint4* vec(int v) const { return reinterpret_cast<uint4*>(row + head) + v; }
+  // the edge value of this thread, or -1 (there are at most 2 E - 2 of them)
+  SB_DEVICE int edge() const {
+    const int t = threadIdx.x;
+    return !edges || t >= head + tail ? -1 : t < head ? t : V - tail + (t - head);
+  }
+};
+
+// Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.
+struct Run {
+  float m = -INFINITY, s = 0.f;
+  template <int N>
+  SB_DEVICE void add(const float* z) {
+    float b = z[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) b = fmaxf(b, z[i]);
+    if (b > m) {
+      s *= m == -INFINITY ? 0.f : exp_diff(m, b);
+      m = b;
+    }
+    // NaN has no place in a maximum, so a row of NaN and -inf alone gets there with m = -inf
+    const float at = m == -INFINITY ? 0.f : m;
+    if (m == INFINITY) {                           // the sum counts the infinite ones, so that its logarithm adds nothing
+#pragma unroll
+      for (int i = 0; i < N; ++i) s += z[i] == INFINITY ? 1.f : exp_diff(z[i], at);
+      return;
+    }
+    float part[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i & 1] += exp_diff(z[i], at);
+    s += part[0] + part[1];
+  }
+  static SB_DEVICE float share(float m, float s, float top) {
+    return m == top ? 1.f : m == -INFINITY ? (s == s ? 0.f : 1.f) : exp_diff(m, top);
+  }
+  SB_DEVICE void join(float m2, float s2) {
+    const float top = fmaxf(m, m2);
+    s = s * share(m, s, top) + s2 * share(m2, s2, top);
+    m = top;
+  }
+};
+
+// All threads' runs joined over the CTA and the cluster, in an order that does not change; every thread gets the result.
+SB_DEVICE Run join_all(Run r, int ranks) {
+  __shared__ float2 warps[kThreads / 32];
+  __shared__ float2 mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r.join(__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o));
+  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = make_float2(r.m, r.s);
+  __syncthreads();
+  Run all;
+  all.m = warps[0].x;
+  all.s = warps[0].y;
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) all.join(warps[w].x, warps[w].y);
+  if (ranks == 1) return all;
+  if (threadIdx.x == 0) mine = make_float2(all.m, all.s);
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  Run row;
+  for (int k = 0; k < ranks; ++k) {
+    const float2 p = *cl.map_shared_rank(&mine, k);
+    if (k == 0) {
+      row.m = p.x;
+      row.s = p.y;
+    } else {
+      row.join(p.x, p.y);
+    }
+  }
+  cl.sync();                                       // nobody leaves, or writes `mine` again, while it is read
+  return row;
+}
+
+// d (onehot - softmax) over the slice.  `get` yields a vector's values, p(z) the softmax.
+template <typename T, typename Get, typename P>
+SB_DEVICE void write_grad(const Slice<T>& s, int label, float d, const Get& get, const P& p) {
+  constexpr int E = Slice<T>::E;
+  int owner = -1;                                  // the slice's vector that holds the label
+  if (label >= s.head && label < s.V - s.tail) owner = (label - s.head) / E;
+  if (d == 0.f) {                                  // rows without a label, or clipped: no value of theirs is looked at
+    for (int v = s.v0 + threadIdx.x; v < s.v1; v += kThreads) *s.vec(v) = make_uint4(0, 0, 0, 0);
+    const int e = s.edge();
+    if (e >= 0) s.row[e] = from_float<T>(0.f);
+    return;
+  }
+#pragma unroll 4
+  for (int v = s.v0 + threadIdx.x; v < s.v1; v += kThreads) {
+    float z[E];
+    Elem<T>::unpack(get(v), z);
+#pragma unroll
+    for (int i = 0; i < E; ++i) z[i] = -d * p(z[i]);
+    if (v == owner) {
+      const int at = (label - s.head) % E;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i == at) z[i] += d;
+    }
+    *s.vec(v) = Elem<T>::pack(z);
+  }
+  const int e = s.edge();
+  if (e >= 0) s.row[e] = from_float<T>((e == label ? d : 0.f) - d * p(to_float(s.row[e])));
+}
+
+template <typename T, typename Keep>
+SB_DEVICE Run read_row(const Slice<T>& s, const Keep& keep) {
+  constexpr int E = Slice<T>::E, U = 4;            // vectors in flight
+  Run r;
+  for (int v = s.v0 + threadIdx.x; v < s.v1; v += U * kThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < s.v1) u[k] = *s.vec(v + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < s.v1) {
+        float z[E];
+        keep(v + k * kThreads, u[k]);
+        Elem<T>::unpack(u[k], z);
+        r.add<E>(z);
+      }
+  }
+  const int e = s.edge();
+  if (e >= 0) {
+    const float z = to_float(s.row[e]);
+    r.add<1>(&z);
+  }
+  return r;
+}
+
+// logp and lse of every row: one pass over the logits.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logp_kernel(const Args a) {
+  const long r = blockIdx.x / a.ranks;
+  const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
+  const Run run = join_all(read_row(s, [](int, const uint4&) {}), a.ranks);
+  if (threadIdx.x == 0 && s.edges) {
+    const int label = a.labels[r];
+    const bool live = label >= 0 && label < a.V;
+    const double l = log(static_cast<double>(run.s));
+    a.lse[r] = static_cast<float>(static_cast<double>(run.m) + l);
+    a.logp[r] = live ? static_cast<float>(static_cast<double>(to_float(s.row[label])) - static_cast<double>(run.m) - l) : 0.f;
+  }
+}
+
+// The gradient at the logits, over them, from lse and dL/dlogp: read and write once.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) grad_kernel(const Args a) {
+  const long r = blockIdx.x / a.ranks;
+  const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
+  const int label = a.labels[r];
+  const float d = label >= 0 && label < a.V ? a.dlogp[r] : 0.f;
+  const float lse = a.lse[r];
+  write_grad(s, label, d, [&](int v) { return *s.vec(v); }, [&](float z) { return exp_diff(z, lse); });
+}
+
+// Loss, log-probability and gradient of every row in one pass: the row's slice waits in shared memory (KEEP) for its sum.
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
+  extern __shared__ uint4 held[];
+  const long r = blockIdx.x / a.ranks;
+  const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
+  const int label = a.labels[r];
+  const bool live = label >= 0 && label < a.V;
+  __shared__ float s_d;
+  float zl = 0.f;
+  if (threadIdx.x == 0 && live) zl = to_float(s.row[label]);          // before it is written over (by any CTA of the row)
+  const Run run = join_all(read_row(s, [&](int v, const uint4& u) { if (KEEP) held[v - s.v0] = u; }), a.ranks);
+  if (threadIdx.x == 0) {
+    double loss = 0, logp = 0, d = 0;
+    if (live) {
+      logp = static_cast<double>(zl) - static_cast<double>(run.m) - log(static_cast<double>(run.s));
+      const double ratio = exp(logp - static_cast<double>(a.t.old[r])), adv = a.t.adv[r];
+      const double clipped = fmin(fmax(ratio, 1.0 - a.t.low), 1.0 + a.t.high);
+      const double gain = adv == 0.0 ? 0.0 : ratio * adv, cut = clipped * adv;
+      const bool open = gain <= cut;
+      loss = -(open ? gain : cut);
+      d = open ? -gain : 0.0;
+      if (gain != gain) loss = d = gain;
+      if (a.t.ref != nullptr && a.t.kl != 0.0) {
+        const double gap = static_cast<double>(a.t.ref[r]) - logp, e = expm1(gap);
+        loss += a.t.kl * (e - gap);
+        d -= a.t.kl * e;
+      }
+      d *= a.t.weight != nullptr ? a.t.scale * a.t.weight[r] : a.t.scale;
+    }
+    s_d = static_cast<float>(d);
+    if (s.edges) {
+      a.t.loss[r] = static_cast<float>(loss);
+      a.logp[r] = static_cast<float>(logp);
+    }
+  }
+  __syncthreads();
+  const float inv = 1.f / run.s, m = run.m;
+  write_grad(s, label, s_d, [&](int v) { return KEEP ? held[v - s.v0] : *s.vec(v); },
+             [&](float z) { return exp_diff(z, m) * inv; });
+}
+
+// Pairs of sequences (2 p chosen, 2 p + 1 rejected): one CTA a pair sums logp - ref over each sequence's labelled rows,
+// and writes the loss, the margin and every row's dL/dlogp.  Rows of no pair get 0.
+__global__ void __launch_bounds__(kThreads)
+pair_kernel(const float* __restrict__ logp, const float* __restrict__ ref, const int* __restrict__ labels, int V,
+            const int* __restrict__ offs, int T, float beta, float scale, float* __restrict__ loss,
+            float* __restrict__ margin, float* __restrict__ dlogp) {
+  __shared__ int bound[3];
+  __shared__ double part[kThreads / 32];
+  const int p = blockIdx.x, warp = threadIdx.x / 32;
+  if (threadIdx.x < 3) bound[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i <= 2 * p + 2; i += kThreads) {       // an offset below one before counts as that one
+    const int b = min(offs[i], T);
+    for (int k = max(0, i - 2 * p); k < 3; ++k) atomicMax(&bound[k], b);
+  }
+  __syncthreads();
+  double sums[2];
+  for (int k = 0; k < 2; ++k) {
+    double sum = 0;
+    for (int r = bound[k] + threadIdx.x; r < bound[k + 1]; r += kThreads)
+      if (labels[r] >= 0 && labels[r] < V) sum += static_cast<double>(logp[r]) - static_cast<double>(ref[r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x % 32 == 0) part[warp] = sum;
+    __syncthreads();
+    sums[k] = part[0];
+    for (int w = 1; w < kThreads / 32; ++w) sums[k] += part[w];
+    __syncthreads();
+  }
+  const double h = static_cast<double>(beta) * (sums[0] - sums[1]);
+  if (threadIdx.x == 0) {
+    margin[p] = static_cast<float>(h);
+    loss[p] = static_cast<float>(fmax(-h, 0.0) + log1p(exp(-fabs(h))));
+    if (h != h) loss[p] = static_cast<float>(h);
+  }
+  const float d = static_cast<float>(static_cast<double>(beta) * scale / (1.0 + exp(h)));
+  for (int r = bound[0] + threadIdx.x; r < bound[2]; r += kThreads) dlogp[r] = r < bound[1] ? -d : d;
+  if (p == 0)
+    for (int r = threadIdx.x; r < bound[0]; r += kThreads) dlogp[r] = 0.f;
+  if (p == static_cast<int>(gridDim.x) - 1)
+    for (int r = bound[2] + threadIdx.x; r < T; r += kThreads) dlogp[r] = 0.f;
+}
+
+template <typename F>
+static cudaError_t launch(F* kernel, const Args& a, size_t smem, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows * a.ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(a.ranks);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMost);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <typename T>
+static cudaError_t run_typed(Kernel k, const Args& a, cudaStream_t stream) {
+  switch (k) {
+    case kLogp: return launch(logp_kernel<T>, a, 0, stream);
+    case kGrad: return launch(grad_kernel<T>, a, 0, stream);
+    default: break;
+  }
+  const size_t held = (static_cast<size_t>(a.V) * sizeof(T) / 16 / a.ranks + 1) * 16;
+  return held <= kHeldMost ? launch(policy_kernel<T, true>, a, held, stream) : launch(policy_kernel<T, false>, a, 0, stream);
+}
+
+cudaError_t run(Kernel k, Type type, const Args& a, cudaStream_t stream) {
+  return type == kBf16 ? run_typed<__nv_bfloat16>(k, a, stream)
+         : type == kF16 ? run_typed<__half>(k, a, stream) : run_typed<float>(k, a, stream);
+}
+
+cudaError_t run_pairs(int pairs, const float* logp, const float* ref, const int* labels, int V, const int* offs, int T,
+                      float beta, float scale, float* loss, float* margin, float* dlogp, cudaStream_t stream) {
+  pair_kernel<<<pairs, kThreads, 0, stream>>>(logp, ref, labels, V, offs, T, beta, scale, loss, margin, dlogp);
+  return cudaGetLastError();
+}
+
+}  // namespace obj
+}  // namespace sb

@@ -1,0 +1,309 @@
+// Packed sequences: what a buffer's offsets say of every row, and rotary positions.
+//
+// A packed buffer holds sequences of different lengths one after the other:
+// sequence g is rows [offs[g], offs[g + 1]).  Offsets rise; they are cut to the
+// buffer, and one below the one before counts as that one.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <limits>
+
+#include "common.cuh"
+#include "lowp.cuh"
+
+namespace sb {
+namespace packed {
+
+constexpr int kRows = 256;     // rows (and threads) of a CTA of the plan kernel
+constexpr int kBins = 4096;    // costs of the tile orders; larger ones share the last bin
+
+// start, pos, stop of every row.  A row's sequence begins at the last offset at or before it and ends at the first one
+// behind it, so the offsets that fall into a CTA's 256 rows are marked in a bit set and the nearest ones outside are kept
+// beside it: no search per row.  Every CTA walks all offsets (a prefix maximum, 256 at a time).
+__global__ void __launch_bounds__(kRows)
+rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start, int* __restrict__ pos,
+            int* __restrict__ stop, int* __restrict__ ends) {
+  __shared__ unsigned mark[kRows / 32];
+  __shared__ int part[kRows / 32], s_before, s_after;
+  const int r0 = blockIdx.x * kRows, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x < kRows / 32) mark[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    s_before = -1;
+    s_after = INT_MAX;
+  }
+  int carry = 0;                 // the largest offset so far, at least 0
+  __syncthreads();
+  for (int base = 0; base < n; base += kRows) {
+    const int i = base + threadIdx.x;
+    int b = i < n ? min(offs[i], T) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, b, o);
+      if (lane >= o) b = max(b, up);
+    }
+    if (lane == 31) part[warp] = b;
+    __syncthreads();
+    int top = carry;
+    for (int w = 0; w < kRows / 32; ++w) {
+      if (w < warp) b = max(b, part[w]);
+      top = max(top, part[w]);
+    }
+    b = max(b, carry);
+    carry = top;
+    if (i < n) {
+      if (b < r0) atomicMax(&s_before, b);
+      else if (b < r0 + kRows) atomicOr(&mark[(b - r0) / 32], 1u << ((b - r0) % 32));
+      else atomicMin(&s_after, b);
+      if (blockIdx.x == 0 && i == 0) ends[0] = b;
+    }
+    __syncthreads();             // part is written again
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) ends[1] = carry;
+  const int r = r0 + threadIdx.x;
+  if (r >= T) return;
+  int first = s_before, behind = s_after;
+  unsigned m = mark[warp] & (0xffffffffu >> (31 - lane));            // offsets at rows up to this one
+  int w = warp;
+  while (m == 0 && w > 0) m = mark[--w];
+  if (m != 0) first = r0 + w * 32 + 31 - __clz(m);
+  m = lane == 31 ? 0 : mark[warp] & (0xffffffffu << (lane + 1));
+  w = warp;
+  while (m == 0 && w < kRows / 32 - 1) m = mark[++w];
+  if (m != 0) behind = r0 + w * 32 + __ffs(m) - 1;
+  const bool covered = first >= 0 && behind != INT_MAX;
+  start[r] = covered ? first : r + 1;
+  pos[r] = covered ? r - first : -1;
+  stop[r] = covered ? behind : r;
+}
+
+// Orders of the attention kernels' tiles, the costliest first: a counting sort by the number of 128-row blocks that a
+// tile meets.  Block 0: tiles of 128 queries; 1: of 256 queries; 2: of 128 keys.  The order decides when a tile runs,
+// nothing else.
+__global__ void __launch_bounds__(1024)
+order_kernel(const int* __restrict__ start, const int* __restrict__ stop, int T, int* __restrict__ fwd,
+             int* __restrict__ fwd2, int* __restrict__ bwd) {
+  __shared__ int bins[kBins];
+  const int rows = blockIdx.x == 1 ? 256 : 128;
+  const int nt = (T + rows - 1) / rows;
+  int* out = blockIdx.x == 0 ? fwd : blockIdx.x == 1 ? fwd2 : bwd;
+  auto cost = [&](int t) {
+    const int lo = t * rows, hi = min(lo + rows, T);
+    const int blocks = blockIdx.x == 2 ? (stop[hi - 1] - lo + 127) / 128 : (hi + 127) / 128 - start[lo] / 128;
+    return kBins - 1 - max(0, min(blocks, kBins - 1));
+  };
+  for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
+  __syncthreads();
+  for (int t = threadIdx.x; t < nt; t += 1024) atomicAdd(&bins[cost(t)], 1);
+  __syncthreads();
+  // exclusive sum over the bins, four to a thread
+  __shared__ int warps[32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int4 b = reinterpret_cast<int4*>(bins)[threadIdx.x];
+  const int mine = b.x + b.y + b.z + b.w;
+  int run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) warps[warp] = run;
+  __syncthreads();
+  run -= mine;
+  for (int w = 0; w < warp; ++w) run += warps[w];
+  reinterpret_cast<int4*>(bins)[threadIdx.x] = make_int4(run, run + b.x, run + b.x + b.y, run + b.x + b.y + b.z);
+  __syncthreads();
+  for (int t = threadIdx.x; t < nt; t += 1024) out[atomicAdd(&bins[cost(t)], 1)] = t;
+}
+
+// [start, pos, stop: T each | first covered row, row behind the last one | orders: nt, nt2, nt]
+std::vector<at::Tensor> sequences(const at::Tensor& offs, int64_t rows) {
+  TORCH_CHECK(offs.is_cuda() && offs.scalar_type() == at::kInt && offs.dim() == 1 && offs.numel() >= 2 &&
+                  offs.is_contiguous(),
+              "sequences: offs are int32 [sequences + 1], contiguous, on the device");
+  TORCH_CHECK(rows >= 0 && rows <= (1 << 30), "sequences: 0 to 2^30 rows, got ", rows);
+  const at::cuda::CUDAGuard guard(offs.device());
+  const int64_t nt = (rows + 127) / 128, nt2 = (rows + 255) / 256;
+  auto flat = at::empty({3 * rows + 2 + 2 * nt + nt2}, offs.options());
+  auto part = [&](int64_t at, int64_t n) { return flat.narrow(0, at, n); };
+  std::vector<at::Tensor> got = {part(0, rows), part(rows, rows), part(2 * rows, rows), part(3 * rows, 2),
+                                 part(3 * rows + 2, nt), part(3 * rows + 2 + nt, nt2),
+                                 part(3 * rows + 2 + nt + nt2, nt)};
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const int T = static_cast<int>(rows);
+  int* p = flat.data_ptr<int>();
+  rows_kernel<<<std::max(1, (T + kRows - 1) / kRows), kRows, 0, stream>>>(
+      offs.data_ptr<int>(), static_cast<int>(offs.numel()), T, p, p + T, p + 2L * T, p + 3L * T);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (T > 0) {
+    int* o = p + 3L * T + 2;
+    order_kernel<<<3, 1024, 0, stream>>>(p, p + 2L * T, T, o, o + nt, o + nt + nt2);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return got;
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions:  y1 = m (x1 cos a - x2 sin a),  y2 = m (x2 cos a + x1 sin a),  a = pos * f
+//
+// The frequency of a pair is given as a 64-bit fraction of a turn, F = f / (2 pi) * 2^64.  pos * F modulo 2^64 is then
+// the angle's fraction of a turn, exact for every position (in fp32, pos * f is off by 0.06 rad at a million), and no
+// table of cosines is read.  A thread has `V` elements of one row's pairs (16 bytes where alignment allows), computes
+// their sines once and rotates them in up to kHeads heads.  Bound by memory: each rotated value read and written once.
+// ---------------------------------------------------------------------------
+constexpr int kHeads = 4;
+
+struct RotaryArgs {
+  const void* x;
+  void* out;
+  const int* pos;
+  const long long* turns;     // [rot / 2]
+  long xs, os;                // row strides, elements
+  int T, heads, dim, rot, chunks, live;   // chunks of a head a thread each; the first `live` rotate, the others copy
+  float size;
+  int inverse;
+};
+
+template <typename T, int V, int ALIGN>
+struct alignas(ALIGN) Vec {
+  T e[V];
+};
+
+// ALIGN: alignment of a chunk in bytes; below sizeof(T) * V its elements are read one by one
+template <typename T, int V, bool INTER, int ALIGN>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+  using VT = Vec<T, V, ALIGN>;
+  const long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  const int groups = (a.heads + kHeads - 1) / kHeads;
+  const int c = static_cast<int>(i % a.chunks);
+  const long rest = i / a.chunks;
+  const int g = static_cast<int>(rest % groups);
+  const long row = rest / groups;
+  if (row >= a.T) return;
+  const int h0 = g * kHeads, nh = min(kHeads, a.heads - h0);
+  const T* xr = static_cast<const T*>(a.x) + row * a.xs + static_cast<long>(h0) * a.dim;
+  T* yr = static_cast<T*>(a.out) + row * a.os + static_cast<long>(h0) * a.dim;
+  if (c >= a.live) {                                       // columns behind the rotated ones
+    const int at = a.rot + (c - a.live) * V;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+      if (h < nh) *reinterpret_cast<VT*>(yr + h * a.dim + at) = *reinterpret_cast<const VT*>(xr + h * a.dim + at);
+    return;
+  }
+  constexpr int P = INTER ? V / 2 : V;                     // pairs
+  const int p0 = c * P, at = c * V, half = a.rot / 2;
+  float cs[P], sn[P];
+  const long long pos = a.pos[row];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const long long frac = static_cast<long long>(static_cast<unsigned long long>(pos) *
+                                                  static_cast<unsigned long long>(a.turns[p0 + j]));
+    // half turns in [-1, 1): the 64-bit fraction keeps its leading bits however small the angle is
+    sincospif(__ll2float_rn(frac) * 1.0842021724855044e-19f /* 2^-63 */, &sn[j], &cs[j]);
+    cs[j] *= a.size;
+    sn[j] *= a.inverse ? -a.size : a.size;
+  }
+  VT u[kHeads], v[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+    if (h < nh) {
+      u[h] = *reinterpret_cast<const VT*>(xr + h * a.dim + at);
+      if (!INTER) v[h] = *reinterpret_cast<const VT*>(xr + h * a.dim + half + at);
+    }
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (h >= nh) break;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      T& e1 = INTER ? u[h].e[2 * j] : u[h].e[j];
+      T& e2 = INTER ? u[h].e[2 * j + 1] : v[h].e[j];
+      const float x1 = to_float(e1), x2 = to_float(e2);
+      // spelled out, so that every width of access rounds alike
+      e1 = from_float<T>(__fmaf_rn(x1, cs[j], -__fmul_rn(x2, sn[j])));
+      e2 = from_float<T>(__fmaf_rn(x2, cs[j], __fmul_rn(x1, sn[j])));
+    }
+    *reinterpret_cast<VT*>(yr + h * a.dim + at) = u[h];
+    if (!INTER) *reinterpret_cast<VT*>(yr + h * a.dim + half + at) = v[h];
+  }
+}
+
+template <typename T, int V, int ALIGN = V * static_cast<int>(sizeof(T))>
+static void rotary_launch(RotaryArgs a, bool inter, bool copy, cudaStream_t stream) {
+  a.live = (inter ? a.rot : a.rot / 2) / V;
+  a.chunks = a.live + (copy ? (a.dim - a.rot) / V : 0);
+  const long work = static_cast<long>(a.T) * ((a.heads + kHeads - 1) / kHeads) * a.chunks;
+  const long blocks = (work + 255) / 256;
+  TORCH_CHECK(blocks < (1L << 31), "rotary: too many rows and heads for one launch");
+  if (inter) {
+    if constexpr (V >= 2) rotary_kernel<T, V, true, ALIGN><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+  } else {
+    rotary_kernel<T, V, false, ALIGN><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+  }
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// Elements per access: the most, up to 16 bytes, that divide every column that a chunk begins at, the row strides and the
+// bases.  (16384 rows of 24 heads of 64, bf16: 16-byte accesses 17 us, 2-byte ones 70 us.)
+template <typename T>
+static void rotary_typed(const RotaryArgs& a, bool inter, bool copy, cudaStream_t stream) {
+  const uint64_t all = static_cast<uint64_t>(a.dim) | static_cast<uint64_t>(inter ? a.rot : a.rot / 2) |
+                       static_cast<uint64_t>(a.rot) | static_cast<uint64_t>(a.xs) | static_cast<uint64_t>(a.os) |
+                       reinterpret_cast<uint64_t>(a.x) / sizeof(T) | reinterpret_cast<uint64_t>(a.out) / sizeof(T);
+  if constexpr (sizeof(T) == 2) {
+    if (all % 8 == 0) return rotary_launch<T, 8>(a, inter, copy, stream);
+  }
+  if (all % 4 == 0) return rotary_launch<T, 4>(a, inter, copy, stream);
+  if (all % 2 == 0) return rotary_launch<T, 2>(a, inter, copy, stream);
+  if (inter) return rotary_launch<T, 2, sizeof(T)>(a, inter, copy, stream);
+  rotary_launch<T, 1>(a, inter, copy, stream);
+}
+
+void rotary(const at::Tensor& x, at::Tensor& out, const at::Tensor& pos, const at::Tensor& turns, int64_t heads,
+            int64_t dim, int64_t rot, bool inter, double size, bool inverse) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && out.dim() == 2, "rotary: matrices [rows, columns] on the device");
+  TORCH_CHECK(x.device() == out.device() && x.device() == pos.device() && x.device() == turns.device(),
+              "rotary: x, out, positions and the plan on one device");
+  TORCH_CHECK(x.scalar_type() == out.scalar_type(), "rotary: out is ", out.scalar_type(), ", x ", x.scalar_type());
+  TORCH_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.numel() == x.size(0) && pos.is_contiguous(),
+              "rotary: positions are int32, one for each of the ", x.size(0), " rows, contiguous");
+  TORCH_CHECK(heads >= 0 && x.size(1) >= heads * dim && out.size(1) >= heads * dim && out.size(0) == x.size(0),
+              "rotary: ", heads, " heads of ", dim, " columns do not fit x [", x.size(0), ", ", x.size(1), "] or out [",
+              out.size(0), ", ", out.size(1), "]");
+  TORCH_CHECK(turns.scalar_type() == at::kLong && turns.is_contiguous() && turns.numel() == rot / 2 && rot >= 2 &&
+                  rot % 2 == 0 && rot <= dim, "rotary: a plan of another size");
+  for (const at::Tensor& t : {x, out})
+    TORCH_CHECK((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
+                "rotary: rows of stride 1 inside that do not overlap");
+  const bool same = x.data_ptr() == out.data_ptr() && (x.size(0) <= 1 || x.stride(0) == out.stride(0));
+  if (!same && x.numel() > 0) {
+    auto range = [](const at::Tensor& t) {
+      const char* p = static_cast<const char*>(t.data_ptr());
+      return std::make_pair(p, p + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size());
+    };
+    const auto a = range(x), b = range(out);
+    TORCH_CHECK(a.second <= b.first || b.second <= a.first, "rotary: out overlaps x and is not x itself");
+  }
+  if (x.size(0) == 0 || heads == 0) return;
+  const at::cuda::CUDAGuard guard(x.device());
+  RotaryArgs a{x.data_ptr(), out.data_ptr(), pos.data_ptr<int>(),
+               reinterpret_cast<const long long*>(turns.data_ptr<int64_t>()),
+               x.size(0) > 1 ? x.stride(0) : 0, x.size(0) > 1 ? out.stride(0) : 0, static_cast<int>(x.size(0)),
+               static_cast<int>(heads), static_cast<int>(dim), static_cast<int>(rot), 0, 0, static_cast<float>(size),
+               inverse ? 1 : 0};
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const bool copy = !same && dim > rot;
+  switch (x.scalar_type()) {
+    case at::kBFloat16: rotary_typed<__nv_bfloat16>(a, inter, copy, stream); break;
+    case at::kHalf: rotary_typed<__half>(a, inter, copy, stream); break;
+    case at::kFloat: rotary_typed<float>(a, inter, copy, stream); break;
+    default: TORCH_CHECK(false, "rotary: bf16, fp16 or fp32, got ", x.scalar_type());
+  }
+}
+
+}  // namespace packed
+}  // namespace sb
+
+void bind_packed(pybind11::module& m) {
+  m.def("packed_sequences", &sb::packed::sequences, "start, position and end of every row of a packed buffer, tile orders");
+  m.def("rotary", &sb::packed::rotary, "rotary positions of the first heads of every row");
+}

@@ -183,6 +183,84 @@ def segments(offs: torch.Tensor, limit: int):
     return list(zip(o, o[1:]))
 
 
+# ------------------------------------------------------------- packed sequences
+def packed_rows(offs: torch.Tensor, rows: int):
+    """start, pos, stop of every row and the covered range (``ops.packed.Sequences``)."""
+    row = torch.arange(rows, dtype=torch.int32)
+    start, pos, stop = row + 1, torch.full_like(row, -1), row.clone()
+    segs = segments(offs, rows)
+    for lo, hi in segs:
+        start[lo:hi], stop[lo:hi], pos[lo:hi] = lo, hi, row[lo:hi] - lo
+    return start, pos, stop, torch.tensor([segs[0][0], segs[-1][1]], dtype=torch.int32)
+
+
+def rotary(x: torch.Tensor, pos: torch.Tensor, freq: torch.Tensor, rot: int, layout: str, size: float,
+           inverse: bool) -> torch.Tensor:
+    """x [T, H, D] rotated by pos * freq (64-bit angles) in its first ``rot`` columns."""
+    angle = pos.double()[:, None] * freq
+    c, s = (size * angle.cos()).float()[:, None], (size * angle.sin()).float()[:, None]
+    s = -s if inverse else s
+    y = x.float().clone()
+    one, two = (slice(0, rot // 2), slice(rot // 2, rot)) if layout == "half" else (slice(0, rot, 2), slice(1, rot, 2))
+    a, b = y[..., one].clone(), y[..., two].clone()
+    y[..., one], y[..., two] = a * c - b * s, b * c + a * s
+    return y.to(x.dtype)
+
+
+def packed_attention(qkv: torch.Tensor, segs, Hq: int, Hkv: int, D: int, scale: float):
+    """Causal attention inside every segment: (o [T, Hq * D] fp32, lse [Hq, T] fp32), zeros and -inf elsewhere."""
+    T, g = qkv.shape[0], Hq // Hkv
+    q, k, v = qkv.float().view(T, Hq + 2 * Hkv, D).split([Hq, Hkv, Hkv], 1)
+    outs, lses, at = [], [], 0
+    for lo, hi in [*segs, (T, T)]:
+        outs.append(qkv.new_zeros(lo - at, Hq * D, dtype=torch.float32))
+        lses.append(torch.full((Hq, lo - at), -math.inf))
+        if hi > lo:
+            qs, ks, vs = (t[lo:hi].transpose(0, 1) for t in (q, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)))
+            s = (qs @ ks.transpose(1, 2) * scale).masked_fill(torch.ones(hi - lo, hi - lo, dtype=torch.bool).triu(1), -math.inf)
+            outs.append((torch.softmax(s, -1) @ vs).transpose(0, 1).reshape(hi - lo, Hq * D))
+            lses.append(torch.logsumexp(s.detach(), -1))
+        at = hi
+    return torch.cat(outs), torch.cat(lses, 1)
+
+
+# ------------------------------------------------------------- label log-probabilities
+def has_label(labels: torch.Tensor, vocab: int) -> torch.Tensor:
+    return (labels >= 0) & (labels < vocab)
+
+
+def label_logp(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor) -> torch.Tensor:
+    """logits[label] - lse in 64 bits, 0 without a label."""
+    live = has_label(labels, logits.shape[1])
+    at = torch.where(live, labels, torch.zeros_like(labels)).long()
+    logp = logits.gather(1, at[:, None])[:, 0].double() - lse
+    return torch.where(live, logp, torch.zeros_like(logp))
+
+
+def label_logp_grad_(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, d: torch.Tensor) -> torch.Tensor:
+    """logits <- d (onehot - softmax); rows without a label, or of d = 0, become zeros."""
+    live = has_label(labels, logits.shape[1]) & (d != 0)
+    g = -d.double()[:, None] * torch.exp(logits.double() - lse.double()[:, None])
+    rows = live.nonzero()[:, 0]
+    g[rows, labels[rows].long()] += d[rows].double()
+    logits.copy_(torch.where(live[:, None], g, torch.zeros_like(g)))
+    return logits
+
+
+def policy_terms(logp, old_logp, adv, ref_logp, low: float, high: float, kl: float):
+    """Loss and its derivative at logp (64 bits) of the clipped policy loss with a KL term."""
+    adv = adv.double()
+    ratio = torch.exp(logp - old_logp.double())
+    gain = torch.where(adv == 0, torch.zeros_like(adv), ratio * adv)
+    cut = ratio.clamp(1 - low, 1 + high) * adv
+    loss = -torch.minimum(gain, cut)
+    d = torch.where(gain <= cut, -gain, torch.where(gain.isnan(), gain, torch.zeros_like(gain)))
+    if ref_logp is not None and kl != 0:
+        gap = ref_logp.double() - logp
+        loss, d = loss + kl * (torch.expm1(gap) - gap), d - kl * torch.expm1(gap)
+    return loss, d
+
+
 # ------------------------------------------------------------- 8-bit moments
 _M32 = 0xFFFFFFFF
 
