@@ -47,6 +47,15 @@ SB_DEVICE float ex2(float x) {
   return y;
 }
 
+// True in one lane of a converged warp.  What issues to the tensor cores runs under it as a whole: the compiler then keeps
+// descriptors and barriers in uniform registers, where those instructions take them from (under `lane == 0` the sixteen
+// products of a 128 x 128 block of heads of 128 took 2900 clocks to issue; they run in 1024).
+SB_DEVICE bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // two fp32 operations in one instruction
 SB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -68,6 +77,48 @@ SB_DEVICE float2 mul2(float2 a, float2 b) {
       : "=l"(reinterpret_cast<uint64_t&>(d))
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
+}
+
+SB_DEVICE float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values on the FMA and integer pipes, for x <= 126: x = j + r with j the nearest whole number (left in the low
+// bits of x + 1.5 * 2^23) and r in [-1/2, 1/2]; 2^r by a polynomial of degree 4 fitted to the relative error over that
+// interval (least squares, reweighted; at most 2.7e-6), j added to the exponent.  Values below -126 count as -126.
+__device__ constexpr float kEx2[5] = {0.99999928f, 0.69312179f, 0.24024744f, 0.055917863f, 0.0095701013f};
+SB_DEVICE float2 ex2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
+  const float2 j = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 r = fma2(j, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(make_float2(kEx2[4], kEx2[4]), r, make_float2(kEx2[3], kEx2[3]));
+  p = fma2(p, r, make_float2(kEx2[2], kEx2[2]));
+  p = fma2(p, r, make_float2(kEx2[1], kEx2[1]));
+  p = fma2(p, r, make_float2(kEx2[0], kEx2[0]));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// Whether a barrier's phase is over; asked early, since the answer takes a hundred clocks.
+SB_DEVICE bool mbar_test(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
+// The wait of a whole warp; `ready`: the answer to an earlier question.
+SB_DEVICE bool warp_wait(uint64_t* bar, uint32_t phase, int* status, bool ready = false) {
+  if (__all_sync(0xffffffffu, ready)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase, status));
 }
 
 template <typename T>
@@ -129,10 +180,13 @@ SB_DEVICE bool sched_request(const Sched& s, int n, int* status) {
                : "memory");
   return true;
 }
-// The next item, or -1 (none left, or a wait ran out).  By a whole warp.
+// The next item, or -1 (none left, or a wait ran out).  By a whole warp, or (WARP false) by the one lane that runs.
+template <bool WARP = true>
 SB_DEVICE int sched_next(const Sched& s, int n, int* status) {
   const int b = n & 1;
-  if (!__all_sync(0xffffffffu, mbar_wait(&s.full[b], (n >> 1) & 1, status))) return -1;
+  bool there = mbar_wait(&s.full[b], (n >> 1) & 1, status);
+  if (WARP) there = __all_sync(0xffffffffu, there);
+  if (!there) return -1;
   uint32_t ok, x = 0;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
@@ -144,8 +198,8 @@ SB_DEVICE int sched_next(const Sched& s, int n, int* status) {
       : "r"(smem_u32(&s.answer[b]))
       : "memory");
   fence_proxy_async_smem();
-  __syncwarp();
-  if (threadIdx.x % 32 == 0) mbar_arrive(&s.empty[b]);
+  if (WARP) __syncwarp();
+  if (!WARP || threadIdx.x % 32 == 0) mbar_arrive(&s.empty[b]);
   return ok != 0 ? static_cast<int>(x) : -1;
 }
 

@@ -170,30 +170,34 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
-      const uint32_t ka = smem_u32(sK), va = smem_u32(sV);
-      int g = 0, nkv = 0;
-      bool ok = true;
+      // all of shared memory lies below 256 KB: adding to a descriptor's address field (16-byte units) never carries out
+      const uint64_t dk = kdesc(smem_u32(sK)), dv = kdesc(smem_u32(sV)), din = kdesc(smem_u32(sQ));
+      const uint64_t din_mn = mndesc(smem_u32(sQ), kSub);
       auto scores = [&](int g) -> bool {               // S^T and dP^T of block g to its buffer
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
         tc_fence_after();
-        const uint32_t qa = smem_u32(sQ + st * 2 * F::kBlock), oa = qa + F::kBlock, ts = tbase + (g & 1) * 128;
+        const uint64_t q = din + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
+        const uint32_t ts = tbase + (g & 1) * 128;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
-          umma_f16(ts, kdesc(ka + off), kdesc(qa + sub), idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
+          umma_f16(ts, dk + off, q + sub, idS, kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
-          umma_f16(ts + 64, kdesc(va + off), kdesc(oa + sub), idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
+          umma_f16(ts + 64, dv + off, o + sub, idS, kk > 0);
         }
         umma_commit(&s_full[g & 1]);
         return true;
       };
+      if (elect_one()) {
+      int g = 0, nkv = 0;
+      bool ok = true;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         const DkvItem it(a, idx);
-        if (lane == 0 && it.subs > 0) {
+        if (it.subs > 0) {
           ok = mbar_wait(kv_full, nkv & 1, a.status);
           if (ok) ok = scores(g);
           for (int s = 0; s < it.subs && ok; ++s, ++g) {
@@ -204,24 +208,21 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
-            const uint32_t qa = smem_u32(sQ + st * 2 * F::kBlock), oa = qa + F::kBlock, ts = tbase + (g & 1) * 128;
+            const uint64_t q = din_mn + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
+            const uint32_t ts = tbase + (g & 1) * 128;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16_ts(tdV, ts + kk * 8, mndesc(oa + kk * 2048, kSub), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdV, ts + kk * 8, o + kk * (2048 >> 4), idG, s > 0 || kk > 0);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16_ts(tdK, ts + 64 + kk * 8, mndesc(qa + kk * 2048, kSub), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdK, ts + 64 + kk * 8, q + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
           }
           if (ok) umma_commit(acc_full);
           ++nkv;
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) idx = sched_next(sched, n, a.status);
+        if (ok) idx = sched_next<false>(sched, n, a.status);
       }
-      if (lane == 0) {
-        umma_commit(drain);
-        mbar_wait(drain, 0, a.status);
+      umma_commit(drain);
+      mbar_wait(drain, 0, a.status);
       }
       __syncwarp();
     }
@@ -505,31 +506,34 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
-      const uint32_t qa = smem_u32(sQ), oa = smem_u32(sO);
-      int g = 0, nq = 0;
-      bool ok = true;
+      const uint64_t dq = kdesc(smem_u32(sQ)), dob = kdesc(smem_u32(sO)), din = kdesc(smem_u32(sK));
+      const uint64_t din_mn = mndesc(smem_u32(sK), kSub);
       auto scores = [&](int g) -> bool {
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
         tc_fence_after();
-        const uint32_t ka = smem_u32(sK + st * F::kStage), va = ka + F::kBlock, ts = tbase + (g & 1) * 128;
+        const uint64_t k = din + st * (F::kStage >> 4), v = k + (F::kBlock >> 4);
+        const uint32_t ts = tbase + (g & 1) * 128;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
-          umma_f16(ts, kdesc(qa + off), kdesc(ka + sub), idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
+          umma_f16(ts, dq + off, k + sub, idS, kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32, sub = (kk >> 2) * kSub + (kk & 3) * 32;
-          umma_f16(ts + 64, kdesc(oa + off), kdesc(va + sub), idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
+          umma_f16(ts + 64, dob + off, v + sub, idS, kk > 0);
         }
         umma_commit(&s_full[g & 1]);
         return true;
       };
+      if (elect_one()) {
+      int g = 0, nq = 0;
+      bool ok = true;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         const DqItem it(a, idx);
         const int subs = it.hi - it.lo;
-        if (lane == 0 && subs > 0) {
+        if (subs > 0) {
           ok = mbar_wait(q_full, nq & 1, a.status);
           if (ok) ok = scores(g);
           for (int s = 0; s < subs && ok; ++s, ++g) {
@@ -540,21 +544,19 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
-            const uint32_t ka = smem_u32(sK + st * F::kStage), ts = tbase + (g & 1) * 128;
+            const uint64_t k = din_mn + st * (F::kStage >> 4);
+            const uint32_t ts = tbase + (g & 1) * 128;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16_ts(tdQ, ts + kk * 8, mndesc(ka + kk * 2048, kSub), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdQ, ts + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
           }
           if (ok) umma_commit(acc_full);
           ++nq;
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) idx = sched_next(sched, n, a.status);
+        if (ok) idx = sched_next<false>(sched, n, a.status);
       }
-      if (lane == 0) {
-        umma_commit(drain);
-        mbar_wait(drain, 0, a.status);
+      umma_commit(drain);
+      mbar_wait(drain, 0, a.status);
       }
       __syncwarp();
     }

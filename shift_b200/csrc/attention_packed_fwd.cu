@@ -43,6 +43,8 @@ struct FwdItem {
   SB_DEVICE bool has(int i, int j) const { return j >= lo[i] && j < hi[i]; }
 };
 
+constexpr int kOnFma = 3;      // of 8 exponentials, those computed on the FMA pipe
+
 template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Args a) {
   using F = Fwd<D>;
@@ -151,29 +153,31 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 128, 0), idO = idesc<T>(128, D, 1);
-      int nk = 0, nv = 0, nq = 0, nb[2] = {0, 0}, no[2] = {0, 0};   // blocks and items of each tile so far
-      bool ok = true;
-      const uint32_t qa = smem_u32(sQ);
+      // all of shared memory lies below 256 KB: adding to a descriptor's address field (16-byte units) never carries out
+      const uint64_t dq = kdesc(smem_u32(sQ)), dk = kdesc(smem_u32(sK)), dv = mndesc(smem_u32(sV), kChunk);
       auto issue_s = [&](int i, int sk) {              // S_i of the key block in stage sk
-        const uint32_t ka = smem_u32(sK + sk * F::kTile), q = qa + i * F::kTile;
+        const uint64_t q = dq + i * (F::kTile >> 4), k = dk + sk * (F::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32;
-          umma_f16(tbase + i * 128, kdesc(q + off), kdesc(ka + off), idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+          umma_f16(tbase + i * 128, q + off, k + off, idS, kk > 0);
         }
         umma_commit(&s_full[i]);
       };
-      auto issue_o = [&](int i, int sv, bool fresh) {
-        const uint32_t va = smem_u32(sV + sv * F::kTile);
+      auto issue_o = [&](int i, int sv, bool fresh, bool last) {
+        const uint64_t v = dv + sv * (F::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_f16_ts(tbase + F::kO + i * D, tbase + F::kP + i * F::kPStep + kk * 8, mndesc(va + kk * 2048, kChunk), idO,
+          umma_f16_ts(tbase + F::kO + i * D, tbase + F::kP + i * F::kPStep + kk * 8, v + kk * (2048 >> 4), idO,
                       !(fresh && kk == 0));
-        umma_commit(&o_full[i]);
+        if (!F::kOver || last) umma_commit(&o_full[i]);
       };
+      if (elect_one()) {
+      int nk = 0, nv = 0, nq = 0, nb[2] = {0, 0}, no[2] = {0, 0};   // blocks and items of each tile so far
+      bool ok = true;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         const FwdItem it(a, idx);
-        if (lane == 0 && it.all_hi > it.all_lo) {
+        if (it.all_hi > it.all_lo) {
           ok = mbar_wait(q_full, nq & 1, a.status);
           ++nq;
           // S of block j: its stage is nk % kK
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
                 if (ok && j == it.lo[i] && no[i] > 0) ok = mbar_wait(&o_free[i], (no[i] - 1) & 1, a.status);
                 if (!ok) break;
                 tc_fence_after();
-                issue_o(i, sv, j == it.lo[i]);
+                issue_o(i, sv, j == it.lo[i], j == it.hi[i] - 1);
               }
               if (F::kOver && more && it.has(i, j + 1)) ok = scores(j + 1, i);
             }
@@ -223,12 +227,10 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           }
           for (int i = 0; i < 2; ++i) no[i] += it.hi[i] > it.lo[i];
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) idx = sched_next(sched, n, a.status);
+        if (ok) idx = sched_next<false>(sched, n, a.status);
       }
-      if (lane == 0) {                                 // nothing of this CTA is in flight when tensor memory is given back
-        umma_commit(drain);
-        mbar_wait(drain, 0, a.status);
+      umma_commit(drain);                              // nothing of this CTA is in flight when tensor memory is given back
+      mbar_wait(drain, 0, a.status);
       }
       __syncwarp();
     }
@@ -239,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * F::kPStep + lane_off;
     const uint32_t to = tbase + F::kO + w * D + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-    int nb = 0;
-    bool ok = true;
+    int nb = 0, items = 0;
+    bool ok = true, s_ready = false;
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const FwdItem it(a, idx);
       const int q0 = w ? it.q0[1] : it.q0[0], lo = w ? it.lo[1] : it.lo[0], hi = w ? it.hi[1] : it.hi[0];
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       const int most = q0 < a.T ? a.start[min(q0 + 127, a.T - 1)] : 0;     // the tile's latest start
       float m = -INFINITY, l = 0.f;
       for (int j = lo; j < hi; ++j, ++nb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], nb & 1, a.status))) {
+        if (!warp_wait(&s_full[w], nb & 1, a.status, s_ready)) {
           ok = false;
           break;
         }
@@ -270,15 +272,18 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           for (int c = 0; c < 128; ++c)
             if (c < from || c > to_c) v[c] = 0xff800000u;
         }
+        // P V of the block before must be done before P is written again or O rescaled: where P lies over S, this block's
+        // S was issued behind it
+        const bool o_ready = !F::kOver && j > lo && mbar_test(&o_full[w], (nb - 1) & 1);
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 128; c += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            m4[k] = fmaxf(fmaxf(m4[k], __uint_as_float(v[c + 2 * k])), __uint_as_float(v[c + 2 * k + 1]));
+            m4[k] = max3(m4[k], __uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1]));
         const float mx = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2);
-        if (j > lo) {                                  // P of the block before was read, and O holds it
-          if (!__all_sync(0xffffffffu, mbar_wait(&o_full[w], (nb - 1) & 1, a.status))) {
+        if (!F::kOver && j > lo) {
+          if (!warp_wait(&o_full[w], (nb - 1) & 1, a.status, o_ready)) {
             ok = false;
             break;
           }
@@ -303,25 +308,30 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
         }
         const float nm = m == -INFINITY ? 0.f : -m;
         const float2 nm2 = make_float2(nm, nm);
-        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float2 l2[4] = {};
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
+          float2 z[16];
           uint32_t pk[16];
 #pragma unroll
+          for (int k = 0; k < 16; ++k)
+            z[k] = fma2(make_float2(__uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1])), sc2, nm2);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) z[k] = k % 8 < kOnFma ? ex2_fma(z[k]) : make_float2(ex2(z[k].x), ex2(z[k].y));
+#pragma unroll
           for (int k = 0; k < 16; ++k) {
-            float2 z = fma2(make_float2(__uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1])), sc2, nm2);
-            z.x = ex2(z.x);
-            z.y = ex2(z.y);
-            l2[k & 1] = add2(l2[k & 1], z);
-            pk[k] = Half<T>::pack(z.x, z.y);
+            l2[k & 3] = add2(l2[k & 3], z[k]);
+            pk[k] = Half<T>::pack(z[k].x, z[k].y);
           }
           tmem_st_32x32b_x16(tp + c / 2, pk);
         }
+        s_ready = j + 1 < hi && mbar_test(&s_full[w], (nb + 1) & 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[w]);
-        l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        l2[0] = add2(add2(l2[0], l2[1]), add2(l2[2], l2[3]));
+        l += l2[0].x + l2[0].y;
       }
       if (!ok) break;
       const bool covered = row < a.T && st <= row;
@@ -329,10 +339,11 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       bool bad = false;
       T* orow = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D;
       if (hi > lo) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&o_full[w], (nb - 1) & 1, a.status))) {
+        if (!warp_wait(&o_full[w], (F::kOver ? items : nb - 1) & 1, a.status)) {
           ok = false;
           break;
         }
+        ++items;
         tc_fence_after();
         const float inv = 1.f / l;
         float chk = 0.f;
