@@ -121,6 +121,12 @@ SB_DEVICE bool warp_wait(uint64_t* bar, uint32_t phase, int* status, bool ready 
   return __all_sync(0xffffffffu, mbar_wait(bar, phase, status));
 }
 
+// Bits [from, to] of a word, clipped to it: which of 32 columns are seen.
+SB_DEVICE uint32_t seen(int from, int to) {
+  const uint32_t low = to >= 31 ? 0xffffffffu : to < 0 ? 0u : (2u << to) - 1u;
+  return from <= 0 ? low : from > 31 ? 0u : low & (0xffffffffu << from);
+}
+
 template <typename T>
 struct Half;
 template <>

@@ -267,10 +267,14 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           if (lane == 0) mbar_arrive(&s_empty[w]);
         }
         if (j * 128 < most || j * 128 + 127 > q0) {
-          const int from = st - j * 128, to_c = row - j * 128;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c < from || c > to_c) v[c] = 0xff800000u;
+          for (int c = 0; c < 128; c += 32) {
+            const uint32_t bits = seen(st - j * 128 - c, row - j * 128 - c);
+            if (!__all_sync(0xffffffffu, bits == 0xffffffffu))
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!(bits >> k & 1)) v[c + k] = 0xff800000u;
+          }
         }
         // P V of the block before must be done before P is written again or O rescaled: where P lies over S, this block's
         // S was issued behind it
