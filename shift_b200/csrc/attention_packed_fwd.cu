@@ -175,9 +175,16 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       if (elect_one()) {
       int nk = 0, nv = 0, nq = 0, nb[2] = {0, 0}, no[2] = {0, 0};   // blocks and items of each tile so far
       bool ok = true;
+      FwdItem it(a, blockIdx.x);
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-        const FwdItem it(a, idx);
-        if (it.all_hi > it.all_lo) {
+        FwdItem following = it;
+        auto look_ahead = [&]() {                      // before the last wait of an item: its loads take a microsecond
+          idx = sched_next<false>(sched, n, a.status);
+          if (idx >= 0) following = FwdItem(a, idx);
+        };
+        if (it.all_hi <= it.all_lo) {
+          look_ahead();
+        } else {
           ok = mbar_wait(q_full, nq & 1, a.status);
           ++nq;
           // S of block j: its stage is nk % kK
@@ -208,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
               if (ok) keys_done(j + 1);
             }
             const int sv = nv % F::kV;
+            if (ok && !more) look_ahead();
             if (ok) ok = mbar_wait(&v_full[sv], (nv / F::kV) & 1, a.status);
             for (int i = 0; i < 2 && ok; ++i) {
               if (it.has(i, j)) {
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           }
           for (int i = 0; i < 2; ++i) no[i] += it.hi[i] > it.lo[i];
         }
-        if (ok) idx = sched_next<false>(sched, n, a.status);
+        it = following;
       }
       umma_commit(drain);                              // nothing of this CTA is in flight when tensor memory is given back
       mbar_wait(drain, 0, a.status);
@@ -243,13 +251,22 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int nb = 0, items = 0;
     bool ok = true, s_ready = false;
+    struct Mine {                                      // this group's tile
+      int h, q0, lo, hi, row, st, most;
+      SB_DEVICE Mine(const Args& a, int idx, int w) {
+        const FwdItem it(a, idx);
+        q0 = w ? it.q0[1] : it.q0[0];
+        lo = w ? it.lo[1] : it.lo[0];
+        hi = w ? it.hi[1] : it.hi[0];
+        h = w ? it.h[1] : it.h[0];
+        row = q0 + threadIdx.x % 128;
+        st = row < a.T ? a.start[row] : row + 1;
+        most = q0 < a.T ? a.start[min(q0 + 127, a.T - 1)] : 0;             // the tile's latest start
+      }
+    };
+    Mine now(a, blockIdx.x, w);
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-      const FwdItem it(a, idx);
-      const int q0 = w ? it.q0[1] : it.q0[0], lo = w ? it.lo[1] : it.lo[0], hi = w ? it.hi[1] : it.hi[0];
-      const int h = w ? it.h[1] : it.h[0];
-      const int row = q0 + (warp % 4) * 32 + lane;
-      const int st = row < a.T ? a.start[row] : row + 1;
-      const int most = q0 < a.T ? a.start[min(q0 + 127, a.T - 1)] : 0;     // the tile's latest start
+      const int h = now.h, q0 = now.q0, lo = now.lo, hi = now.hi, row = now.row, st = now.st, most = now.most;
       float m = -INFINITY, l = 0.f;
       for (int j = lo; j < hi; ++j, ++nb) {
         if (!warp_wait(&s_full[w], nb & 1, a.status, s_ready)) {
@@ -338,6 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
         l += l2[0].x + l2[0].y;
       }
       if (!ok) break;
+      idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
+      if (idx >= 0) now = Mine(a, idx, w);
       const bool covered = row < a.T && st <= row;
       float lse2 = -INFINITY;
       bool bad = false;
@@ -387,7 +406,6 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
         slow_o<D, T>(a, __shfl_sync(0xffffffffu, row, who), h, __shfl_sync(0xffffffffu, st, who),
                      __shfl_sync(0xffffffffu, lse2, who));
       }
-      idx = sched_next(sched, n, a.status);
     }
   }
   tc_fence_before();
