@@ -6,14 +6,16 @@
 // order in which they get there.
 //
 // In both, the other side comes in blocks of 64 and the two groups of softmax warps take them in turn: S and dP of block n
-// are in buffer n & 1 (64 columns each), P and dS go over them as 16-bit operands.  While a group works on block n, the
-// products of block n + 1 fill the other buffer.
+// are in buffer n & 1 (64 columns each).  P and dS have columns of their own where there are enough, so that S and dP of
+// block n + 2 are computed while the group is still at block n; in the dK / dV pass of heads of 128 they lie over S and dP,
+// and a group waits for the products of its block before and of its next one.
 #include "attention_packed.cuh"
 
 namespace sb {
 namespace pa {
 
 constexpr int kSub = 64 * 128;     // bytes of 64 rows of 64 16-bit columns
+constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe
 
 // -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
 // a row of a head.
@@ -48,6 +50,8 @@ template <int D>
 struct Dkv {
   static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
   static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock + 512;      // Q, dO, -lse and -delta of 64 queries
+  static constexpr bool kOver = D == 128;                                          // P, dS over S, dP
+  static constexpr int kP = kOver ? 0 : 384, kPStep = kOver ? 128 : 64, kDs = kOver ? 64 : 32, kAhead = kOver ? 1 : 2;
   static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
 };
 
@@ -81,8 +85,9 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
   uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
   uint64_t *kv_full = bar, *kv_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
   uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
-  const Sched sched{answer, p_full + 2, p_full + 4};
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_full + 6);
+  uint64_t *s_empty = p_full + 2, *p_free = s_empty + 2;
+  const Sched sched{answer, p_free + 2, p_free + 4};
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_free + 6);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -99,6 +104,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_free[i], 1);
       mbar_init(&sched.full[i], 1);
       mbar_init(&sched.empty[i], kReaders);
     }
@@ -176,6 +183,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       auto scores = [&](int g) -> bool {               // S^T and dP^T of block g to its buffer
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
+        if (!F::kOver && g >= 2 && !mbar_wait(&s_empty[g & 1], ((g >> 1) - 1) & 1, a.status)) return false;
         tc_fence_after();
         const uint64_t q = din + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
         const uint32_t ts = tbase + (g & 1) * 128;
@@ -195,31 +203,41 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       if (elect_one()) {
       int g = 0, nkv = 0;
       bool ok = true;
+      DkvItem it(a, blockIdx.x);
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-        const DkvItem it(a, idx);
-        if (it.subs > 0) {
+        DkvItem following = it;
+        auto look_ahead = [&]() {                      // before the last wait of an item: its loads take a microsecond
+          idx = sched_next<false>(sched, n, a.status);
+          if (idx >= 0) following = DkvItem(a, idx);
+        };
+        if (it.subs == 0) {
+          look_ahead();
+        } else {
           ok = mbar_wait(kv_full, nkv & 1, a.status);
-          if (ok) ok = scores(g);
+          for (int s = 0; s < min(F::kAhead, it.subs) && ok; ++s) ok = scores(g + s);
           for (int s = 0; s < it.subs && ok; ++s, ++g) {
-            if (s + 1 < it.subs) ok = scores(g + 1);
-            if (ok && s == max(0, it.subs - 2)) umma_commit(kv_empty);                    // the last scores were issued
+            if (s + F::kAhead < it.subs) ok = scores(g + F::kAhead);
+            if (ok && s == max(0, it.subs - 1 - F::kAhead)) umma_commit(kv_empty);        // the last scores were issued
+            if (ok && s + 1 == it.subs) look_ahead();
             if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
             if (ok && s == 0 && nkv > 0) ok = mbar_wait(acc_free, (nkv - 1) & 1, a.status);
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
             const uint64_t q = din_mn + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
-            const uint32_t ts = tbase + (g & 1) * 128;
+            const uint32_t tp = tbase + F::kP + (g & 1) * F::kPStep;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdV, ts + kk * 8, o + kk * (2048 >> 4), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdV, tp + kk * 8, o + kk * (2048 >> 4), idG, s > 0 || kk > 0);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdK, ts + 64 + kk * 8, q + kk * (2048 >> 4), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tdK, tp + F::kDs + kk * 8, q + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
+            if (!F::kOver) umma_commit(&p_free[g & 1]);
           }
           if (ok) umma_commit(acc_full);
           ++nkv;
         }
-        if (ok) idx = sched_next<false>(sched, n, a.status);
+        it = following;
       }
       umma_commit(drain);
       mbar_wait(drain, 0, a.status);
@@ -230,12 +248,12 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     regs_up<kSoftRegs>();
     const int w = warp / 4;                            // this group's buffer; at the end, 0 stores dV and 1 dK
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t ts = tbase + w * 128 + lane_off;
+    const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * F::kPStep + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, nkv = 0;
-    bool ok = true;
+    bool ok = true, in_ready = false, s_ready = false;
+    DkvItem it(a, blockIdx.x);
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-      const DkvItem it(a, idx);
       const int row = it.k0 + (warp % 4) * 32 + lane;
       const int end = row < a.T ? a.stop[row] : row;
       const int least = a.stop[it.k0];                 // the tile's earliest end
@@ -243,21 +261,26 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         if ((g & 1) != w) continue;
         const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * 64;
         // -lse and -delta came with Q and dO; S cannot be there before them
-        if (!__all_sync(0xffffffffu, mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status) &&
-                                         mbar_wait(&s_full[w], (g >> 1) & 1, a.status))) {
+        if (!warp_wait(&in_full[st], (g / F::kStages) & 1, a.status, in_ready) ||
+            !warp_wait(&s_full[w], (g >> 1) & 1, a.status, s_ready)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const bool p_ready = !F::kOver && g >= 2 && mbar_test(&p_free[w], ((g >> 1) - 1) & 1);
         const float4* nl4 = reinterpret_cast<const float4*>(sR + st * 128);
         const bool masked = q0 < it.k0 + 127 || q0 + 64 > least;
-        const int from = row - q0, to_c = end - q0;    // visible: from <= column < to_c
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t vs[32], vd[32];
           tmem_ld_32x32b_x32(ts + c, vs);
           tmem_ld_32x32b_x32(ts + 64 + c, vd);
           tmem_wait_ld();
+          if (!F::kOver && c == 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[w]);
+          }
           uint32_t pp[16], pd[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
@@ -269,27 +292,32 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
             e[1] = add2(make_float2(__uint_as_float(vd[k + 2]), __uint_as_float(vd[k + 3])), make_float2(nd.z, nd.w));
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              z[u].x = ex2(z[u].x);
-              z[u].y = ex2(z[u].y);
+              z[u] = (k / 2 + u) % 8 < kOnFma ? ex2_fma(z[u]) : make_float2(ex2(z[u].x), ex2(z[u].y));
               e[u] = mul2(e[u], z[u]);
-            }
-            if (masked) {
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int col = c + k + 2 * u;
-                if (col < from || col >= to_c) z[u].x = e[u].x = 0.f;
-                if (col + 1 < from || col + 1 >= to_c) z[u].y = e[u].y = 0.f;
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
               pp[k / 2 + u] = Half<T>::pack(z[u].x, z[u].y);
               pd[k / 2 + u] = Half<T>::pack(e[u].x, e[u].y);
             }
           }
-          tmem_st_32x32b_x16(ts + c / 2, pp);
-          tmem_st_32x32b_x16(ts + 64 + c / 2, pd);
+          if (masked) {                                // two packed values at a time
+            const uint32_t bits = seen(row - q0 - c, end - 1 - q0 - c);
+            if (!__all_sync(0xffffffffu, bits == 0xffffffffu))
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const uint32_t keep = (bits >> (2 * k) & 1 ? 0xffffu : 0u) | (bits >> (2 * k + 1) & 1 ? 0xffff0000u : 0u);
+                pp[k] &= keep;
+                pd[k] &= keep;
+              }
+          }
+          if (!F::kOver && c == 0 && g >= 2) {         // the products of this group's block before have read P and dS
+            if (!warp_wait(&p_free[w], ((g >> 1) - 1) & 1, a.status, p_ready)) ok = false;
+            tc_fence_after();
+          }
+          tmem_st_32x32b_x16(tp + c / 2, pp);
+          tmem_st_32x32b_x16(tp + F::kDs + c / 2, pd);
         }
+        if (!ok) break;
+        in_ready = mbar_test(&in_full[(g + 2) % F::kStages], ((g + 2) / F::kStages) & 1);
+        s_ready = mbar_test(&s_full[w], ((g >> 1) + 1) & 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -298,13 +326,16 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       if (!ok) break;
       const bool covered = row < a.T && end > row;
       const bool dk = w == 1;
-      const long col = static_cast<long>(a.Hq + (dk ? 0 : a.Hkv) + it.kvh) * D;
+      const DkvItem at = it;
+      idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
+      if (idx >= 0) it = DkvItem(a, idx);
+      const long col = static_cast<long>(a.Hq + (dk ? 0 : a.Hkv) + at.kvh) * D;
       T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + col;
       float* partial = nullptr;
       if (a.split > 1)
-        partial = a.partial + ((static_cast<long>(it.part) * a.Hkv + it.kvh) * a.T + row) * (2 * D) + (dk ? 0 : D);
+        partial = a.partial + ((static_cast<long>(at.part) * a.Hkv + at.kvh) * a.T + row) * (2 * D) + (dk ? 0 : D);
       bool bad = false;
-      if (it.subs > 0) {
+      if (at.subs > 0) {
         if (!__all_sync(0xffffffffu, mbar_wait(acc_full, nkv & 1, a.status))) {
           ok = false;
           break;
@@ -346,15 +377,14 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         }
         bad = covered && chk != 0.f;
       }
-      if (row < a.T && !covered && a.fill && it.part == 0)
+      if (row < a.T && !covered && a.fill && at.part == 0)
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
       for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
         const int who = __ffs(some) - 1, r = __shfl_sync(0xffffffffu, row, who);
-        slow_dkv<D, T>(a, r, it.kvh, it.first_h, it.first_h + it.heads, __shfl_sync(0xffffffffu, end, who), dk,
+        slow_dkv<D, T>(a, r, at.kvh, at.first_h, at.first_h + at.heads, __shfl_sync(0xffffffffu, end, who), dk,
                        partial == nullptr ? nullptr : partial + static_cast<long>(r - row) * (2 * D));
       }
-      idx = sched_next(sched, n, a.status);
     }
   }
   tc_fence_before();
@@ -388,6 +418,7 @@ template <int D>
 struct Dq {
   static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
   static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock;             // K, V of 64 keys
+  static constexpr int kP = 256 + D, kAhead = 2;                                   // dS, 32 columns a buffer
   static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
 };
 
@@ -419,8 +450,9 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
   uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
   uint64_t *q_full = bar, *q_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
   uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
-  const Sched sched{answer, p_full + 2, p_full + 4};
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_full + 6);
+  uint64_t *s_empty = p_full + 2, *p_free = s_empty + 2;
+  const Sched sched{answer, p_free + 2, p_free + 4};
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(p_free + 6);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -437,6 +469,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_free[i], 1);
       mbar_init(&sched.full[i], 1);
       mbar_init(&sched.empty[i], kReaders);
     }
@@ -511,6 +545,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       auto scores = [&](int g) -> bool {
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
+        if (g >= 2 && !mbar_wait(&s_empty[g & 1], ((g >> 1) - 1) & 1, a.status)) return false;
         tc_fence_after();
         const uint64_t k = din + st * (F::kStage >> 4), v = k + (F::kBlock >> 4);
         const uint32_t ts = tbase + (g & 1) * 128;
@@ -530,30 +565,39 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       if (elect_one()) {
       int g = 0, nq = 0;
       bool ok = true;
+      DqItem it(a, blockIdx.x);
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-        const DqItem it(a, idx);
+        DqItem following = it;
         const int subs = it.hi - it.lo;
-        if (subs > 0) {
+        auto look_ahead = [&]() {                      // before the last wait of an item: its loads take a microsecond
+          idx = sched_next<false>(sched, n, a.status);
+          if (idx >= 0) following = DqItem(a, idx);
+        };
+        if (subs == 0) {
+          look_ahead();
+        } else {
           ok = mbar_wait(q_full, nq & 1, a.status);
-          if (ok) ok = scores(g);
+          for (int s = 0; s < min(F::kAhead, subs) && ok; ++s) ok = scores(g + s);
           for (int s = 0; s < subs && ok; ++s, ++g) {
-            if (s + 1 < subs) ok = scores(g + 1);
-            if (ok && s == max(0, subs - 2)) umma_commit(q_empty);             // the last scores were issued
+            if (s + F::kAhead < subs) ok = scores(g + F::kAhead);
+            if (ok && s == max(0, subs - 1 - F::kAhead)) umma_commit(q_empty);  // the last scores were issued
+            if (ok && s + 1 == subs) look_ahead();
             if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
             if (ok && s == 0 && nq > 0) ok = mbar_wait(acc_free, (nq - 1) & 1, a.status);
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
             const uint64_t k = din_mn + st * (F::kStage >> 4);
-            const uint32_t ts = tbase + (g & 1) * 128;
+            const uint32_t tp = tbase + F::kP + (g & 1) * 32;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdQ, ts + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdQ, tp + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
+            umma_commit(&p_free[g & 1]);
           }
           if (ok) umma_commit(acc_full);
           ++nq;
         }
-        if (ok) idx = sched_next<false>(sched, n, a.status);
+        it = following;
       }
       umma_commit(drain);
       mbar_wait(drain, 0, a.status);
@@ -564,12 +608,12 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
     regs_up<kSoftRegs>();
     const int w = warp / 4;                            // this group's buffer; at the end, its half of the columns
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t ts = tbase + w * 128 + lane_off;
+    const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * 32 + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, nq = 0;
-    bool ok = true;
+    bool ok = true, s_ready = false;
+    DqItem it(a, blockIdx.x);
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
-      const DqItem it(a, idx);
       const int row = it.q0 + (warp % 4) * 32 + lane;
       const int st = row < a.T ? a.start[row] : row + 1;
       const int most = a.start[min(it.q0 + 127, a.T - 1)];
@@ -577,34 +621,47 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       const float2 nl = make_float2(rb[0], rb[0]), nd = make_float2(rb[64], rb[64]);
       for (int j = it.lo; j < it.hi; ++j, ++g) {
         if ((g & 1) != w) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (g >> 1) & 1, a.status))) {
+        if (!warp_wait(&s_full[w], (g >> 1) & 1, a.status, s_ready)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const bool p_ready = g >= 2 && mbar_test(&p_free[w], ((g >> 1) - 1) & 1);
         const bool masked = j * 64 < most || j * 64 + 63 > it.q0;
-        const int from = st - j * 64, to_c = row - j * 64;
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t vs[32], vd[32], pd[16];
           tmem_ld_32x32b_x32(ts + c, vs);
           tmem_ld_32x32b_x32(ts + 64 + c, vd);
           tmem_wait_ld();
+          if (c == 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[w]);
+          }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 z = fma2(make_float2(__uint_as_float(vs[k]), __uint_as_float(vs[k + 1])), sc2, nl);
             float2 e = add2(make_float2(__uint_as_float(vd[k]), __uint_as_float(vd[k + 1])), nd);
-            z.x = ex2(z.x);
-            z.y = ex2(z.y);
+            z = k / 2 % 8 < kOnFma ? ex2_fma(z) : make_float2(ex2(z.x), ex2(z.y));
             e = mul2(e, z);
-            if (masked) {
-              if (c + k < from || c + k > to_c) e.x = 0.f;
-              if (c + k + 1 < from || c + k + 1 > to_c) e.y = 0.f;
-            }
             pd[k / 2] = Half<T>::pack(e.x, e.y);
           }
-          tmem_st_32x32b_x16(ts + c / 2, pd);
+          if (masked) {
+            const uint32_t bits = seen(st - j * 64 - c, row - j * 64 - c);
+            if (!__all_sync(0xffffffffu, bits == 0xffffffffu))
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                pd[k] &= (bits >> (2 * k) & 1 ? 0xffffu : 0u) | (bits >> (2 * k + 1) & 1 ? 0xffff0000u : 0u);
+          }
+          if (c == 0 && g >= 2) {                      // the product of this group's block before has read dS
+            if (!warp_wait(&p_free[w], ((g >> 1) - 1) & 1, a.status, p_ready)) ok = false;
+            tc_fence_after();
+          }
+          tmem_st_32x32b_x16(tp + c / 2, pd);
         }
+        if (!ok) break;
+        s_ready = mbar_test(&s_full[w], ((g >> 1) + 1) & 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -612,9 +669,12 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       }
       if (!ok) break;
       const bool covered = row < a.T && st <= row;
-      T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(it.h) * D;
+      const DqItem at = it;
+      idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
+      if (idx >= 0) it = DqItem(a, idx);
+      T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(at.h) * D;
       bool bad = false;
-      if (it.hi > it.lo) {
+      if (at.hi > at.lo) {
         if (!__all_sync(0xffffffffu, mbar_wait(acc_full, nq & 1, a.status))) {
           ok = false;
           break;
@@ -652,10 +712,9 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
         for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + w * (D / 2) + c) = make_uint4(0, 0, 0, 0);
       for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
         const int who = __ffs(some) - 1;
-        slow_dq<D, T>(a, __shfl_sync(0xffffffffu, row, who), it.h, __shfl_sync(0xffffffffu, st, who), w * (D / 2),
+        slow_dq<D, T>(a, __shfl_sync(0xffffffffu, row, who), at.h, __shfl_sync(0xffffffffu, st, who), w * (D / 2),
                       (w + 1) * (D / 2));
       }
-      idx = sched_next(sched, n, a.status);
     }
   }
   tc_fence_before();
