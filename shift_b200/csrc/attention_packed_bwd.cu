@@ -5,16 +5,16 @@
 // queries (S = Q K^T, dP = dO V^T, dQ += dS K).  Seven products instead of five; one pass would add dQ across CTAs in the
 // order in which they get there.
 //
-// In both, the other side comes in blocks of 64 and the two groups of softmax warps take them in turn: S and dP of block n
-// are in buffer n & 1 (64 columns each).  P and dS have columns of their own where there are enough, so that S and dP of
-// block n + 2 are computed while the group is still at block n; in the dK / dV pass of heads of 128 they lie over S and dP,
-// and a group waits for the products of its block before and of its next one.
+// The other side comes in blocks of 128, of which each group of softmax warps has 64 columns; S and dP have columns of their
+// own in tensor memory and P and dS have too, so that S and dP of the next block are computed while the groups are still at
+// this one.  (Products of 64 columns cost as much as ones of 128: blocks of 64 that the groups took in turn made the dK / dV
+// pass of heads of 64 1.4 times as slow.)  The dK / dV pass of heads of 128 has no columns left for that: its blocks are of
+// 64, the groups take them in turn, and P and dS lie over S and dP.
 #include "attention_packed.cuh"
 
 namespace sb {
 namespace pa {
 
-constexpr int kSub = 64 * 128;     // bytes of 64 rows of 64 16-bit columns
 constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe
 
 // -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
@@ -48,16 +48,20 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args 
 // ============================ dK, dV ============================
 template <int D>
 struct Dkv {
-  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
-  static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock + 512;      // Q, dO, -lse and -delta of 64 queries
-  static constexpr bool kOver = D == 128;                                          // P, dS over S, dP
-  static constexpr int kP = kOver ? 0 : 384, kPStep = kOver ? 128 : 64, kDs = kOver ? 64 : 32, kAhead = kOver ? 1 : 2;
+  static constexpr bool kWide = D == 64;
+  static constexpr int kW = kWide ? 128 : 64;                                      // queries of a block
+  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kNext = kW * 128, kBlock = kHalves * kNext;
+  static constexpr int kStages = 4, kStage = 2 * kBlock + kW * 8;                  // Q, dO, -lse and -delta of the queries
+  // columns: S, dP (wide: one buffer of 2 x 128, else two of 2 x 64) | dV | dK | P, dS (else over S, dP)
+  static constexpr int kDp = kW, kP = kWide ? 384 : 0, kDs = 64;
   static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
+  static SB_DEVICE int buffer(int g) { return kWide ? 0 : g & 1; }
+  static SB_DEVICE int phase(int g) { return (kWide ? g : g >> 1) & 1; }
 };
 
 struct DkvItem {
-  int kvh, part, k0, first_h, heads, blocks, subs;      // `blocks` of 64 queries a head
-  SB_DEVICE DkvItem(const Args& a, int idx) {
+  int kvh, part, k0, first_h, heads, blocks, subs;      // `blocks` of w queries a head
+  SB_DEVICE DkvItem(const Args& a, int idx, int w) {
     const int per = a.Hkv * a.split, r = idx % per;
     kvh = r / a.split;
     part = r % a.split;
@@ -65,14 +69,14 @@ struct DkvItem {
     first_h = kvh * a.group + part * heads;
     k0 = a.order[idx / per] * 128;
     const int end = a.stop[min(k0 + 127, a.T - 1)];
-    blocks = k0 < a.ends[1] && k0 + 128 > a.ends[0] ? (end - k0 + 63) / 64 : 0;
+    blocks = k0 < a.ends[1] && k0 + 128 > a.ends[0] ? (end - k0 + w - 1) / w : 0;
     subs = blocks * heads;
   }
 };
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUtensorMap tm64,
+dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUtensorMap tmw,
            const __grid_constant__ CUtensorMap tmo, const __grid_constant__ Args a) {
   using F = Dkv<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -80,8 +84,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
   uint8_t* sK = smem_raw + (((raw + 1023) & ~1023u) - raw);
   uint8_t* sV = sK + F::kTile;
   uint8_t* sQ = sV + F::kTile;                                  // [stages][Q | dO]
-  float* sR = reinterpret_cast<float*>(sQ + F::kStages * 2 * F::kBlock);          // [stages][2][64]
-  uint4* answer = reinterpret_cast<uint4*>(sR + F::kStages * 128);
+  float* sR = reinterpret_cast<float*>(sQ + F::kStages * 2 * F::kBlock);          // [stages][blocks of 64][2][64]
+  uint4* answer = reinterpret_cast<uint4*>(sR + F::kStages * 2 * F::kW);
   uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
   uint64_t *kv_full = bar, *kv_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
   uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
@@ -103,8 +107,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], F::kWide ? 8 : 4);
+      mbar_init(&s_empty[i], 8);
       mbar_init(&p_free[i], 1);
       mbar_init(&sched.full[i], 1);
       mbar_init(&sched.empty[i], kReaders);
@@ -129,7 +133,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         if (lane == 0) ok = sched_request(sched, n, a.status);
         ok = __all_sync(0xffffffffu, ok);
-        const DkvItem it(a, idx);
+        const DkvItem it(a, idx, F::kW);
         if (ok && it.subs > 0) {
           if (lane == 0) {
             ok = mbar_wait(kv_empty, (nkv & 1) ^ 1, a.status);
@@ -144,8 +148,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
           ++nkv;
           ok = __all_sync(0xffffffffu, ok);
           for (int s = 0; s < it.subs && ok; ++s, ++g) {
-            const int st = g % F::kStages, h = it.first_h + s / it.blocks, row = it.k0 + s % it.blocks * 64;
-            const bool clear = row < first || min(row + 64, a.T) > last;
+            const int st = g % F::kStages, h = it.first_h + s / it.blocks, row = it.k0 + s % it.blocks * F::kW;
+            const bool clear = row < first || min(row + F::kW, a.T) > last;
             uint8_t* in = sQ + st * 2 * F::kBlock;
             if (lane == 0) {
               ok = mbar_wait(&in_empty[st], ((g / F::kStages) & 1) ^ 1, a.status);
@@ -153,10 +157,10 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
                 uint64_t* to = clear ? land : &in_full[st];
                 mbar_arrive_expect_tx(to, F::kStage);
                 for (int c = 0; c < F::kHalves; ++c) {
-                  tma_load_2d(in + c * kSub, &tm64, to, h * D + c * 64, row);
-                  tma_load_2d(in + F::kBlock + c * kSub, &tmo, to, h * D + c * 64, row);
+                  tma_load_2d(in + c * F::kNext, &tmw, to, h * D + c * 64, row);
+                  tma_load_2d(in + F::kBlock + c * F::kNext, &tmo, to, h * D + c * 64, row);
                 }
-                bulk_load(sR + st * 128, row_block(a, h, row), 512, to);
+                bulk_load(sR + st * 2 * F::kW, row_block(a, h, row), F::kW * 8, to);
               }
             }
             ok = __all_sync(0xffffffffu, ok);
@@ -164,8 +168,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
               ok = __all_sync(0xffffffffu, mbar_wait(land, nl & 1, a.status));
               ++nl;
               if (ok) {
-                clear_rows(in, 64, F::kHalves, kSub, row, first, last);
-                clear_rows(in + F::kBlock, 64, F::kHalves, kSub, row, first, last);
+                clear_rows(in, F::kW, F::kHalves, F::kNext, row, first, last);
+                clear_rows(in + F::kBlock, F::kW, F::kHalves, F::kNext, row, first, last);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&in_full[st]);
@@ -176,63 +180,63 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         if (ok) idx = sched_next(sched, n, a.status);
       }
     } else if (warp == kIssuer) {
-      constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
+      constexpr uint32_t idS = idesc<T>(128, F::kW, 0), idG = idesc<T>(128, D, 1);
       // all of shared memory lies below 256 KB: adding to a descriptor's address field (16-byte units) never carries out
       const uint64_t dk = kdesc(smem_u32(sK)), dv = kdesc(smem_u32(sV)), din = kdesc(smem_u32(sQ));
-      const uint64_t din_mn = mndesc(smem_u32(sQ), kSub);
+      const uint64_t din_mn = mndesc(smem_u32(sQ), F::kNext);
       auto scores = [&](int g) -> bool {               // S^T and dP^T of block g to its buffer
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
-        if (!F::kOver && g >= 2 && !mbar_wait(&s_empty[g & 1], ((g >> 1) - 1) & 1, a.status)) return false;
+        if (F::kWide && g >= 1 && !mbar_wait(&s_empty[0], (g - 1) & 1, a.status)) return false;
         tc_fence_after();
         const uint64_t q = din + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
-        const uint32_t ts = tbase + (g & 1) * 128;
+        const uint32_t ts = tbase + F::buffer(g) * 128;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * F::kNext + (kk & 3) * 32) >> 4;
           umma_f16(ts, dk + off, q + sub, idS, kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
-          umma_f16(ts + 64, dv + off, o + sub, idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * F::kNext + (kk & 3) * 32) >> 4;
+          umma_f16(ts + F::kDp, dv + off, o + sub, idS, kk > 0);
         }
-        umma_commit(&s_full[g & 1]);
+        umma_commit(&s_full[F::buffer(g)]);
         return true;
       };
       if (elect_one()) {
       int g = 0, nkv = 0;
       bool ok = true;
-      DkvItem it(a, blockIdx.x);
+      DkvItem it(a, blockIdx.x, F::kW);
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         DkvItem following = it;
         auto look_ahead = [&]() {                      // before the last wait of an item: its loads take a microsecond
           idx = sched_next<false>(sched, n, a.status);
-          if (idx >= 0) following = DkvItem(a, idx);
+          if (idx >= 0) following = DkvItem(a, idx, F::kW);
         };
         if (it.subs == 0) {
           look_ahead();
         } else {
           ok = mbar_wait(kv_full, nkv & 1, a.status);
-          for (int s = 0; s < min(F::kAhead, it.subs) && ok; ++s) ok = scores(g + s);
+          if (ok) ok = scores(g);
           for (int s = 0; s < it.subs && ok; ++s, ++g) {
-            if (s + F::kAhead < it.subs) ok = scores(g + F::kAhead);
-            if (ok && s == max(0, it.subs - 1 - F::kAhead)) umma_commit(kv_empty);        // the last scores were issued
+            if (s + 1 < it.subs) ok = scores(g + 1);
+            if (ok && s == max(0, it.subs - 2)) umma_commit(kv_empty);                    // the last scores were issued
             if (ok && s + 1 == it.subs) look_ahead();
-            if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
+            if (ok) ok = mbar_wait(&p_full[F::buffer(g)], F::phase(g), a.status);
             if (ok && s == 0 && nkv > 0) ok = mbar_wait(acc_free, (nkv - 1) & 1, a.status);
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
             const uint64_t q = din_mn + st * (2 * F::kBlock >> 4), o = q + (F::kBlock >> 4);
-            const uint32_t tp = tbase + F::kP + (g & 1) * F::kPStep;
+            const uint32_t tp = tbase + F::kP + F::buffer(g) * 128;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdV, tp + kk * 8, o + kk * (2048 >> 4), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < F::kW / 16; ++kk) umma_f16_ts(tdV, tp + kk * 8, o + kk * (2048 >> 4), idG, s > 0 || kk > 0);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
+            for (int kk = 0; kk < F::kW / 16; ++kk)
               umma_f16_ts(tdK, tp + F::kDs + kk * 8, q + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
-            if (!F::kOver) umma_commit(&p_free[g & 1]);
+            if (F::kWide) umma_commit(p_free);
           }
           if (ok) umma_commit(acc_full);
           ++nkv;
@@ -246,40 +250,42 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     }
   } else {
     regs_up<kSoftRegs>();
-    const int w = warp / 4;                            // this group's buffer; at the end, 0 stores dV and 1 dK
+    const int w = warp / 4;                            // this group's half of the columns or its buffer; 0 stores dV, 1 dK
+    const int b = F::buffer(w);
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * F::kPStep + lane_off;
+    const uint32_t ts = tbase + w * (F::kWide ? 64 : 128) + lane_off;
+    const uint32_t tp = tbase + F::kP + w * (F::kWide ? 32 : 128) + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, nkv = 0;
     bool ok = true, in_ready = false, s_ready = false;
-    DkvItem it(a, blockIdx.x);
+    DkvItem it(a, blockIdx.x, F::kW);
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int row = it.k0 + (warp % 4) * 32 + lane;
       const int end = row < a.T ? a.stop[row] : row;
       const int least = a.stop[it.k0];                 // the tile's earliest end
       for (int s = 0; s < it.subs; ++s, ++g) {
-        if ((g & 1) != w) continue;
-        const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * 64;
+        if (!F::kWide && (g & 1) != w) continue;
+        const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * F::kW + (F::kWide ? w * 64 : 0);
         // -lse and -delta came with Q and dO; S cannot be there before them
         if (!warp_wait(&in_full[st], (g / F::kStages) & 1, a.status, in_ready) ||
-            !warp_wait(&s_full[w], (g >> 1) & 1, a.status, s_ready)) {
+            !warp_wait(&s_full[b], F::phase(g), a.status, s_ready)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const bool p_ready = !F::kOver && g >= 2 && mbar_test(&p_free[w], ((g >> 1) - 1) & 1);
-        const float4* nl4 = reinterpret_cast<const float4*>(sR + st * 128);
+        const bool p_ready = F::kWide && g >= 1 && mbar_test(p_free, (g - 1) & 1);
+        const float4* nl4 = reinterpret_cast<const float4*>(sR + st * 2 * F::kW + (F::kWide ? w * 128 : 0));
         const bool masked = q0 < it.k0 + 127 || q0 + 64 > least;
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t vs[32], vd[32];
           tmem_ld_32x32b_x32(ts + c, vs);
-          tmem_ld_32x32b_x32(ts + 64 + c, vd);
+          tmem_ld_32x32b_x32(ts + F::kDp + c, vd);
           tmem_wait_ld();
-          if (!F::kOver && c == 32) {
+          if (F::kWide && c == 32) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[w]);
+            if (lane == 0) mbar_arrive(s_empty);
           }
           uint32_t pp[16], pd[16];
 #pragma unroll
@@ -308,27 +314,28 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
                 pd[k] &= keep;
               }
           }
-          if (!F::kOver && c == 0 && g >= 2) {         // the products of this group's block before have read P and dS
-            if (!warp_wait(&p_free[w], ((g >> 1) - 1) & 1, a.status, p_ready)) ok = false;
+          if (F::kWide && c == 0 && g >= 1) {          // the products of the block before have read P and dS
+            if (!warp_wait(p_free, (g - 1) & 1, a.status, p_ready)) ok = false;
             tc_fence_after();
           }
           tmem_st_32x32b_x16(tp + c / 2, pp);
           tmem_st_32x32b_x16(tp + F::kDs + c / 2, pd);
         }
         if (!ok) break;
-        in_ready = mbar_test(&in_full[(g + 2) % F::kStages], ((g + 2) / F::kStages) & 1);
-        s_ready = mbar_test(&s_full[w], ((g >> 1) + 1) & 1);
+        const int next = g + (F::kWide ? 1 : 2);       // this group's; what came before it on these barriers is over
+        in_ready = mbar_test(&in_full[next % F::kStages], (next / F::kStages) & 1);
+        s_ready = mbar_test(&s_full[b], F::phase(next));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[w]);
+        if (lane == 0) mbar_arrive(&p_full[b]);
       }
       if (!ok) break;
       const bool covered = row < a.T && end > row;
       const bool dk = w == 1;
       const DkvItem at = it;
       idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
-      if (idx >= 0) it = DkvItem(a, idx);
+      if (idx >= 0) it = DkvItem(a, idx, F::kW);
       const long col = static_cast<long>(a.Hq + (dk ? 0 : a.Hkv) + at.kvh) * D;
       T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + col;
       float* partial = nullptr;
@@ -416,30 +423,29 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 // ============================ dQ ============================
 template <int D>
 struct Dq {
-  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk, kBlock = kHalves * kSub;
-  static constexpr int kStages = D == 64 ? 6 : 4, kStage = 2 * kBlock;             // K, V of 64 keys
-  static constexpr int kP = 256 + D, kAhead = 2;                                   // dS, 32 columns a buffer
+  static constexpr int kHalves = D / 64, kTile = kHalves * kChunk;
+  static constexpr int kStages = D == 64 ? 4 : 2, kStage = 2 * kTile;              // K, V of 128 keys
+  static constexpr int kP = 256 + D;                                               // S | dP | dQ | dS
   static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
 };
 
 struct DqItem {
-  int h, kvh, q0, lo, hi;                              // blocks of 64 keys
+  int h, kvh, q0, lo, hi;                              // blocks of 128 keys
   SB_DEVICE DqItem(const Args& a, int idx) {
     h = idx % a.Hq;
     kvh = h / a.group;
     q0 = a.order[idx / a.Hq] * 128;
     lo = hi = 0;
     if (q0 < a.ends[1] && q0 + 128 > a.ends[0]) {
-      lo = a.start[q0] / 64;
-      hi = min(q0 / 64 + 2, (a.T + 63) / 64);
+      lo = a.start[q0] / 128;
+      hi = q0 / 128 + 1;
     }
   }
 };
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUtensorMap tm64,
-          const __grid_constant__ CUtensorMap tmo, const __grid_constant__ Args a) {
+dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tmo, const __grid_constant__ Args a) {
   using F = Dq<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -468,8 +474,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&s_empty[i], 8);
       mbar_init(&p_free[i], 1);
       mbar_init(&sched.full[i], 1);
       mbar_init(&sched.empty[i], kReaders);
@@ -501,7 +507,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
             if (ok) {
               mbar_arrive_expect_tx(q_full, 2 * F::kTile);
               for (int c = 0; c < F::kHalves; ++c) {
-                tma_load_2d(sQ + c * kChunk, &tm128, q_full, it.h * D + c * 64, it.q0);
+                tma_load_2d(sQ + c * kChunk, &tm, q_full, it.h * D + c * 64, it.q0);
                 tma_load_2d(sO + c * kChunk, &tmo, q_full, it.h * D + c * 64, it.q0);
               }
             }
@@ -509,8 +515,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
           ++nq;
           ok = __all_sync(0xffffffffu, ok);
           for (int j = it.lo; j < it.hi && ok; ++j, ++g) {
-            const int st = g % F::kStages, row = j * 64;
-            const bool clear = row < first || min(row + 64, a.T) > last;
+            const int st = g % F::kStages, row = j * 128;
+            const bool clear = row < first || min(row + 128, a.T) > last;
             uint8_t* in = sK + st * F::kStage;
             if (lane == 0) {
               ok = mbar_wait(&in_empty[st], ((g / F::kStages) & 1) ^ 1, a.status);
@@ -518,8 +524,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
                 uint64_t* to = clear ? land : &in_full[st];
                 mbar_arrive_expect_tx(to, F::kStage);
                 for (int c = 0; c < F::kHalves; ++c) {
-                  tma_load_2d(in + c * kSub, &tm64, to, (a.Hq + it.kvh) * D + c * 64, row);
-                  tma_load_2d(in + F::kBlock + c * kSub, &tm64, to, (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
+                  tma_load_2d(in + c * kChunk, &tm, to, (a.Hq + it.kvh) * D + c * 64, row);
+                  tma_load_2d(in + F::kTile + c * kChunk, &tm, to, (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
                 }
               }
             }
@@ -528,7 +534,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
               ok = __all_sync(0xffffffffu, mbar_wait(land, nl & 1, a.status));
               ++nl;
               if (ok) {
-                clear_rows(in, 64, F::kHalves, kSub, row, first, last);
+                clear_rows(in, 128, F::kHalves, kChunk, row, first, last);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&in_full[st]);
@@ -539,27 +545,26 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
         if (ok) idx = sched_next(sched, n, a.status);
       }
     } else if (warp == kIssuer) {
-      constexpr uint32_t idS = idesc<T>(128, 64, 0), idG = idesc<T>(128, D, 1);
+      constexpr uint32_t idS = idesc<T>(128, 128, 0), idG = idesc<T>(128, D, 1);
       const uint64_t dq = kdesc(smem_u32(sQ)), dob = kdesc(smem_u32(sO)), din = kdesc(smem_u32(sK));
-      const uint64_t din_mn = mndesc(smem_u32(sK), kSub);
+      const uint64_t din_mn = mndesc(smem_u32(sK), kChunk);
       auto scores = [&](int g) -> bool {
         const int st = g % F::kStages;
         if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
-        if (g >= 2 && !mbar_wait(&s_empty[g & 1], ((g >> 1) - 1) & 1, a.status)) return false;
+        if (g >= 1 && !mbar_wait(s_empty, (g - 1) & 1, a.status)) return false;
         tc_fence_after();
-        const uint64_t k = din + st * (F::kStage >> 4), v = k + (F::kBlock >> 4);
-        const uint32_t ts = tbase + (g & 1) * 128;
+        const uint64_t k = din + st * (F::kStage >> 4), v = k + (F::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
-          umma_f16(ts, dq + off, k + sub, idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+          umma_f16(tbase, dq + off, k + sub, idS, kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kSub + (kk & 3) * 32) >> 4;
-          umma_f16(ts + 64, dob + off, v + sub, idS, kk > 0);
+          const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+          umma_f16(tbase + 128, dob + off, v + sub, idS, kk > 0);
         }
-        umma_commit(&s_full[g & 1]);
+        umma_commit(s_full);
         return true;
       };
       if (elect_one()) {
@@ -577,22 +582,21 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
           look_ahead();
         } else {
           ok = mbar_wait(q_full, nq & 1, a.status);
-          for (int s = 0; s < min(F::kAhead, subs) && ok; ++s) ok = scores(g + s);
+          if (ok) ok = scores(g);
           for (int s = 0; s < subs && ok; ++s, ++g) {
-            if (s + F::kAhead < subs) ok = scores(g + F::kAhead);
-            if (ok && s == max(0, subs - 1 - F::kAhead)) umma_commit(q_empty);  // the last scores were issued
+            if (s + 1 < subs) ok = scores(g + 1);
+            if (ok && s == max(0, subs - 2)) umma_commit(q_empty);              // the last scores were issued
             if (ok && s + 1 == subs) look_ahead();
-            if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.status);
+            if (ok) ok = mbar_wait(p_full, g & 1, a.status);
             if (ok && s == 0 && nq > 0) ok = mbar_wait(acc_free, (nq - 1) & 1, a.status);
             if (!ok) break;
             tc_fence_after();
             const int st = g % F::kStages;
             const uint64_t k = din_mn + st * (F::kStage >> 4);
-            const uint32_t tp = tbase + F::kP + (g & 1) * 32;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tdQ, tp + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
+            for (int kk = 0; kk < 8; ++kk) umma_f16_ts(tdQ, tbase + F::kP + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
             umma_commit(&in_empty[st]);
-            umma_commit(&p_free[g & 1]);
+            umma_commit(p_free);
           }
           if (ok) umma_commit(acc_full);
           ++nq;
@@ -606,9 +610,9 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
     }
   } else {
     regs_up<kSoftRegs>();
-    const int w = warp / 4;                            // this group's buffer; at the end, its half of the columns
+    const int w = warp / 4;                            // this group's half of the columns, also of dQ
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t ts = tbase + w * 128 + lane_off, tp = tbase + F::kP + w * 32 + lane_off;
+    const uint32_t ts = tbase + w * 64 + lane_off, tp = tbase + F::kP + w * 32 + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, nq = 0;
     bool ok = true, s_ready = false;
@@ -620,24 +624,24 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
       const float* rb = row_block(a, it.h, row);       // there are rows up to a multiple of 128
       const float2 nl = make_float2(rb[0], rb[0]), nd = make_float2(rb[64], rb[64]);
       for (int j = it.lo; j < it.hi; ++j, ++g) {
-        if ((g & 1) != w) continue;
-        if (!warp_wait(&s_full[w], (g >> 1) & 1, a.status, s_ready)) {
+        if (!warp_wait(s_full, g & 1, a.status, s_ready)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const bool p_ready = g >= 2 && mbar_test(&p_free[w], ((g >> 1) - 1) & 1);
-        const bool masked = j * 64 < most || j * 64 + 63 > it.q0;
+        const bool p_ready = g >= 1 && mbar_test(p_free, (g - 1) & 1);
+        const int k0 = j * 128 + w * 64;
+        const bool masked = k0 < most || k0 + 63 > it.q0;
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t vs[32], vd[32], pd[16];
           tmem_ld_32x32b_x32(ts + c, vs);
-          tmem_ld_32x32b_x32(ts + 64 + c, vd);
+          tmem_ld_32x32b_x32(ts + 128 + c, vd);
           tmem_wait_ld();
           if (c == 32) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[w]);
+            if (lane == 0) mbar_arrive(s_empty);
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
@@ -648,24 +652,24 @@ dq_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CUt
             pd[k / 2] = Half<T>::pack(e.x, e.y);
           }
           if (masked) {
-            const uint32_t bits = seen(st - j * 64 - c, row - j * 64 - c);
+            const uint32_t bits = seen(st - k0 - c, row - k0 - c);
             if (!__all_sync(0xffffffffu, bits == 0xffffffffu))
 #pragma unroll
               for (int k = 0; k < 16; ++k)
                 pd[k] &= (bits >> (2 * k) & 1 ? 0xffffu : 0u) | (bits >> (2 * k + 1) & 1 ? 0xffff0000u : 0u);
           }
-          if (c == 0 && g >= 2) {                      // the product of this group's block before has read dS
-            if (!warp_wait(&p_free[w], ((g >> 1) - 1) & 1, a.status, p_ready)) ok = false;
+          if (c == 0 && g >= 1) {                      // the product of the block before has read dS
+            if (!warp_wait(p_free, (g - 1) & 1, a.status, p_ready)) ok = false;
             tc_fence_after();
           }
           tmem_st_32x32b_x16(tp + c / 2, pd);
         }
         if (!ok) break;
-        s_ready = mbar_test(&s_full[w], ((g >> 1) + 1) & 1);
+        s_ready = mbar_test(s_full, (g + 1) & 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[w]);
+        if (lane == 0) mbar_arrive(p_full);
       }
       if (!ok) break;
       const bool covered = row < a.T && st <= row;
@@ -732,13 +736,14 @@ static void launch(const CUtensorMap& tm128, const CUtensorMap& tm64, const CUte
   cudaFuncSetAttribute(dkv_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dkv<D>::kSmem);
   cudaFuncSetAttribute(dq_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dq<D>::kSmem);
   a.order = k_order;
-  dkv_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hkv * a.split), kThreads, Dkv<D>::kSmem, stream>>>(tm128, tm64, do64, a);
+  dkv_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hkv * a.split), kThreads, Dkv<D>::kSmem, stream>>>(
+      tm128, Dkv<D>::kWide ? tm128 : tm64, Dkv<D>::kWide ? do128 : do64, a);
   if (a.split > 1) {
     const long n = static_cast<long>(a.Hkv) * a.T * (2 * D / 8);
     join_kernel<D, T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(a);
   }
   a.order = q_order;
-  dq_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hq), kThreads, Dq<D>::kSmem, stream>>>(tm128, tm64, do128, a);
+  dq_kernel<D, T><<<static_cast<unsigned>(a.tiles * a.Hq), kThreads, Dq<D>::kSmem, stream>>>(tm128, do128, a);
 }
 
 void launch_bwd(int D, bool half, const CUtensorMap& tm128, const CUtensorMap& tm64, const CUtensorMap& do128,
