@@ -276,17 +276,20 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         const bool p_ready = F::kWide && g >= 1 && mbar_test(p_free, (g - 1) & 1);
         const float4* nl4 = reinterpret_cast<const float4*>(sR + st * 2 * F::kW + (F::kWide ? w * 128 : 0));
         const bool masked = q0 < it.k0 + 127 || q0 + 64 > least;
+        uint32_t ws[64], wd[64];
+        tmem_ld_32x32b_x32(ts, ws);
+        tmem_ld_32x32b_x32(ts + F::kDp, wd);
+        tmem_ld_32x32b_x32(ts + 32, ws + 32);
+        tmem_ld_32x32b_x32(ts + F::kDp + 32, wd + 32);
+        tmem_wait_ld();
+        if (F::kWide) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_empty);
+        }
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
-          uint32_t vs[32], vd[32];
-          tmem_ld_32x32b_x32(ts + c, vs);
-          tmem_ld_32x32b_x32(ts + F::kDp + c, vd);
-          tmem_wait_ld();
-          if (F::kWide && c == 32) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty);
-          }
+          const uint32_t *vs = ws + c, *vd = wd + c;
           uint32_t pp[16], pd[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
@@ -632,17 +635,19 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
         const bool p_ready = g >= 1 && mbar_test(p_free, (g - 1) & 1);
         const int k0 = j * 128 + w * 64;
         const bool masked = k0 < most || k0 + 63 > it.q0;
+        uint32_t ws[64], wd[64];
+        tmem_ld_32x32b_x32(ts, ws);
+        tmem_ld_32x32b_x32(ts + 128, wd);
+        tmem_ld_32x32b_x32(ts + 32, ws + 32);
+        tmem_ld_32x32b_x32(ts + 128 + 32, wd + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty);
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
-          uint32_t vs[32], vd[32], pd[16];
-          tmem_ld_32x32b_x32(ts + c, vs);
-          tmem_ld_32x32b_x32(ts + 128 + c, vd);
-          tmem_wait_ld();
-          if (c == 32) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty);
-          }
+          const uint32_t *vs = ws + c, *vd = wd + c;
+          uint32_t pd[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 z = fma2(make_float2(__uint_as_float(vs[k]), __uint_as_float(vs[k + 1])), sc2, nl);
