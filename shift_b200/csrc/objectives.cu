@@ -29,46 +29,77 @@ SB_DEVICE float ex2(float x) {
 // exp(z - m); m is finite.  The difference is rounded before it is scaled, so the error goes with |z - m|, not with |z|.
 SB_DEVICE float exp_diff(float z, float m) { return ex2((z - m) * kLog2e); }
 
+SB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+SB_DEVICE float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+// the same of two values, two operations an instruction; `minus`: -m twice
+SB_DEVICE float2 exp_diff2(float2 z, float2 minus) {
+  z = mul2(add2(z, minus), make_float2(kLog2e, kLog2e));
+  return make_float2(ex2(z.x), ex2(z.y));
+}
+
+// A 16-byte vector as pairs of fp32 values, back, and its largest value (NaN apart; 16-bit values two at a time).
 template <typename T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
-  static SB_DEVICE void unpack(const uint4& u, float* f) { bf16x8_to_float(reinterpret_cast<const bf16x8&>(u), f); }
-  static SB_DEVICE uint4 pack(const float* f) {
-    bf16x8 v = float_to_bf16x8(f);
-    return reinterpret_cast<uint4&>(v);
+  static SB_DEVICE void unpack(const uint4& u, float2* f) {
+    f[0] = unpack_bf16x2(u.x);
+    f[1] = unpack_bf16x2(u.y);
+    f[2] = unpack_bf16x2(u.z);
+    f[3] = unpack_bf16x2(u.w);
+  }
+  static SB_DEVICE uint4 pack(const float2* f) {
+    return make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                      pack_bf16x2(f[3].x, f[3].y));
+  }
+  static SB_DEVICE float top(const uint4& u, const float2*) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(m.x, m.y);
   }
 };
 template <>
 struct Elem<__half> {
-  static SB_DEVICE void unpack(const uint4& u, float* f) {
+  static SB_DEVICE void unpack(const uint4& u, float2* f) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = __half22float2(h[i]);
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
-    }
+    for (int i = 0; i < 4; ++i) f[i] = __half22float2(h[i]);
   }
-  static SB_DEVICE uint4 pack(const float* f) {
+  static SB_DEVICE uint4 pack(const float2* f) {
     uint4 u;
     __half2* h = reinterpret_cast<__half2*>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[i].x, f[i].y);
     return u;
+  }
+  static SB_DEVICE float top(const uint4& u, const float2*) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(m.x, m.y);
   }
 };
 template <>
 struct Elem<float> {
-  static SB_DEVICE void unpack(const uint4& u, float* f) {
-    f[0] = __uint_as_float(u.x);
-    f[1] = __uint_as_float(u.y);
-    f[2] = __uint_as_float(u.z);
-    f[3] = __uint_as_float(u.w);
+  static SB_DEVICE void unpack(const uint4& u, float2* f) {
+    f[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static SB_DEVICE uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static SB_DEVICE uint4 pack(const float2* f) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
   }
+  static SB_DEVICE float top(const uint4&, const float2* f) { return fmaxf(fmaxf(f[0].x, f[0].y), fmaxf(f[1].x, f[1].y)); }
 };
 
 // The part of a row that one CTA of a cluster has: whole 16-byte vectors [v0, v1) of the row's aligned middle; rank 0 also
@@ -98,26 +129,32 @@ struct Slice {
 // Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.
 struct Run {
   float m = -INFINITY, s = 0.f;
-  template <int N>
-  SB_DEVICE void add(const float* z) {
-    float b = z[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) b = fmaxf(b, z[i]);
+  SB_DEVICE void rise(float b) {
     if (b > m) {
       s *= m == -INFINITY ? 0.f : exp_diff(m, b);
       m = b;
     }
-    // NaN has no place in a maximum, so a row of NaN and -inf alone gets there with m = -inf
-    const float at = m == -INFINITY ? 0.f : m;
-    if (m == INFINITY) {                           // the sum counts the infinite ones, so that its logarithm adds nothing
+  }
+  // One vector, or one value.  NaN has no place in a maximum, so a row of NaN and -inf alone gets here with m = -inf;
+  // among infinite values the sum counts those, so that its logarithm adds nothing.
+  template <int N>
+  SB_DEVICE void add(const float2* z, float top) {
+    rise(top);
+    if (m == INFINITY) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += z[i] == INFINITY ? 1.f : exp_diff(z[i], at);
+      for (int i = 0; i < N; ++i)
+        s += (z[i].x == INFINITY ? 1.f : exp_diff(z[i].x, m)) + (z[i].y == INFINITY ? 1.f : exp_diff(z[i].y, m));
       return;
     }
-    float part[2] = {0.f, 0.f};
+    const float at = m == -INFINITY ? 0.f : -m;
+    float2 part = exp_diff2(z[0], make_float2(at, at));
 #pragma unroll
-    for (int i = 0; i < N; ++i) part[i & 1] += exp_diff(z[i], at);
-    s += part[0] + part[1];
+    for (int i = 1; i < N; ++i) part = add2(part, exp_diff2(z[i], make_float2(at, at)));
+    s += part.x + part.y;
+  }
+  SB_DEVICE void add(float z) {
+    rise(z);
+    s += z == INFINITY ? 1.f : exp_diff(z, m == -INFINITY ? 0.f : m);
   }
   static SB_DEVICE float share(float m, float s, float top) {
     return m == top ? 1.f : m == -INFINITY ? (s == s ? 0.f : 1.f) : exp_diff(m, top);
@@ -160,39 +197,71 @@ SB_DEVICE Run join_all(Run r, int ranks) {
   return row;
 }
 
-// d (onehot - softmax) over the slice.  `get` yields a vector's values, p(z) the softmax.
-template <typename T, typename Get, typename P>
-SB_DEVICE void write_grad(const Slice<T>& s, int label, float d, const Get& get, const P& p) {
-  constexpr int E = Slice<T>::E;
-  int owner = -1;                                  // the slice's vector that holds the label
-  if (label >= s.head && label < s.V - s.tail) owner = (label - s.head) / E;
-  if (d == 0.f) {                                  // rows without a label, or clipped: no value of theirs is looked at
-    for (int v = s.v0 + threadIdx.x; v < s.v1; v += kThreads) *s.vec(v) = make_uint4(0, 0, 0, 0);
-    const int e = s.edge();
-    if (e >= 0) s.row[e] = from_float<T>(0.f);
-    return;
-  }
-#pragma unroll 4
-  for (int v = s.v0 + threadIdx.x; v < s.v1; v += kThreads) {
-    float z[E];
-    Elem<T>::unpack(get(v), z);
+// d (onehot - softmax) of one vector; `p` of two values is their softmax
+template <typename T, typename P>
+SB_DEVICE uint4 grad_of(const uint4& u, int v, int owner, int at, float d, const P& p) {
+  constexpr int N = Slice<T>::E / 2;
+  float2 z[N];
+  Elem<T>::unpack(u, z);
 #pragma unroll
-    for (int i = 0; i < E; ++i) z[i] = -d * p(z[i]);
-    if (v == owner) {
-      const int at = (label - s.head) % E;
+  for (int i = 0; i < N; ++i) z[i] = mul2(p(z[i]), make_float2(-d, -d));
+  if (v == owner) {
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (i == at) z[i] += d;
+    for (int i = 0; i < N; ++i) {
+      if (2 * i == at) z[i].x += d;
+      if (2 * i + 1 == at) z[i].y += d;
     }
-    *s.vec(v) = Elem<T>::pack(z);
   }
+  return Elem<T>::pack(z);
+}
+// the slice's vector that holds the label, or -1
+template <typename T>
+SB_DEVICE int label_vec(const Slice<T>& s, int label) {
+  return label >= s.head && label < s.V - s.tail ? (label - s.head) / Slice<T>::E : -1;
+}
+template <typename T, typename P>
+SB_DEVICE void write_edge(const Slice<T>& s, int label, float d, const P& p) {
   const int e = s.edge();
-  if (e >= 0) s.row[e] = from_float<T>((e == label ? d : 0.f) - d * p(to_float(s.row[e])));
+  if (e >= 0) s.row[e] = from_float<T>((e == label ? d : 0.f) - d * p(make_float2(to_float(s.row[e]), 0.f)).x);
+}
+// rows without a label, or clipped: no value of theirs is looked at
+template <typename T>
+SB_DEVICE void write_zeros(const Slice<T>& s) {
+  for (int v = s.v0 + threadIdx.x; v < s.v1; v += kThreads) *s.vec(v) = make_uint4(0, 0, 0, 0);
+  const int e = s.edge();
+  if (e >= 0) s.row[e] = from_float<T>(0.f);
+}
+template <typename T, typename P>
+SB_DEVICE void write_grad(const Slice<T>& s, int label, float d, const P& p) {
+  const int owner = label_vec(s, label), at = owner < 0 ? 0 : (label - s.head) % Slice<T>::E;
+  constexpr int U = 4;                             // vectors in flight
+  for (int v = s.v0 + threadIdx.x; v < s.v1; v += U * kThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < s.v1) u[k] = *s.vec(v + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < s.v1) *s.vec(v + k * kThreads) = grad_of<T>(u[k], v + k * kThreads, owner, at, d, p);
+  }
+  write_edge(s, label, d, p);
 }
 
-template <typename T, typename Keep>
-SB_DEVICE Run read_row(const Slice<T>& s, const Keep& keep) {
-  constexpr int E = Slice<T>::E, U = 4;            // vectors in flight
+template <typename T>
+SB_DEVICE void add_vec(Run& r, const uint4& u) {
+  constexpr int N = Slice<T>::E / 2;
+  float2 z[N];
+  Elem<T>::unpack(u, z);
+  r.add<N>(z, Elem<T>::top(u, z));
+}
+template <typename T>
+SB_DEVICE void add_edge(Run& r, const Slice<T>& s) {
+  const int e = s.edge();
+  if (e >= 0) r.add(to_float(s.row[e]));
+}
+template <typename T>
+SB_DEVICE Run read_row(const Slice<T>& s) {
+  constexpr int U = 4;
   Run r;
   for (int v = s.v0 + threadIdx.x; v < s.v1; v += U * kThreads) {
     uint4 u[U];
@@ -201,18 +270,9 @@ SB_DEVICE Run read_row(const Slice<T>& s, const Keep& keep) {
       if (v + k * kThreads < s.v1) u[k] = *s.vec(v + k * kThreads);
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (v + k * kThreads < s.v1) {
-        float z[E];
-        keep(v + k * kThreads, u[k]);
-        Elem<T>::unpack(u[k], z);
-        r.add<E>(z);
-      }
+      if (v + k * kThreads < s.v1) add_vec<T>(r, u[k]);
   }
-  const int e = s.edge();
-  if (e >= 0) {
-    const float z = to_float(s.row[e]);
-    r.add<1>(&z);
-  }
+  add_edge(r, s);
   return r;
 }
 
@@ -221,13 +281,15 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) logp_kernel(const Args a) {
   const long r = blockIdx.x / a.ranks;
   const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
-  const Run run = join_all(read_row(s, [](int, const uint4&) {}), a.ranks);
+  const Run run = join_all(read_row(s), a.ranks);
   if (threadIdx.x == 0 && s.edges) {
     const int label = a.labels[r];
     const bool live = label >= 0 && label < a.V;
     const double l = log(static_cast<double>(run.s));
+    const double logp = live ? static_cast<double>(to_float(s.row[label])) - static_cast<double>(run.m) - l : 0.0;
     a.lse[r] = static_cast<float>(static_cast<double>(run.m) + l);
-    a.logp[r] = live ? static_cast<float>(static_cast<double>(to_float(s.row[label])) - static_cast<double>(run.m) - l) : 0.f;
+    if (a.logp64 != nullptr) a.logp64[r] = logp;
+    else a.logp[r] = static_cast<float>(logp);
   }
 }
 
@@ -239,21 +301,61 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Args a) {
   const int label = a.labels[r];
   const float d = label >= 0 && label < a.V ? a.dlogp[r] : 0.f;
   const float lse = a.lse[r];
-  write_grad(s, label, d, [&](int v) { return *s.vec(v); }, [&](float z) { return exp_diff(z, lse); });
+  if (d == 0.f) write_zeros(s);
+  else write_grad(s, label, d, [&](float2 z) { return exp_diff2(z, make_float2(-lse, -lse)); });
+}
+
+SB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+SB_DEVICE void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
 }
 
 // Loss, log-probability and gradient of every row in one pass: the row's slice waits in shared memory (KEEP) for its sum.
+// It comes and goes by bulk copies in kParts parts, so that all of it is in flight at once and three CTAs an SM keep the
+// memory busy while one of them computes (with loads and stores of the threads, 16 KB in flight a CTA: 494 us for 16384 x
+// 32768 bf16).
+constexpr int kParts = 4;
+
 template <typename T, bool KEEP>
 __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
   extern __shared__ uint4 held[];
+  __shared__ uint64_t bar[kParts];
+  __shared__ float s_d;
   const long r = blockIdx.x / a.ranks;
   const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
+  const int n = s.v1 - s.v0;
+  auto part = [&](int c) { return s.v0 + static_cast<int>(static_cast<long>(n) * c / kParts); };
+  if (KEEP && threadIdx.x == 0) {
+    for (int c = 0; c < kParts; ++c) mbar_init(&bar[c], 1);
+    fence_barrier_init();
+    for (int c = 0; c < kParts; ++c) {
+      const uint32_t bytes = static_cast<uint32_t>(part(c + 1) - part(c)) * 16;
+      mbar_arrive_expect_tx(&bar[c], bytes);
+      if (bytes > 0) bulk_load(held + (part(c) - s.v0), s.vec(part(c)), bytes, &bar[c]);
+    }
+  }
   const int label = a.labels[r];
   const bool live = label >= 0 && label < a.V;
-  __shared__ float s_d;
   float zl = 0.f;
-  if (threadIdx.x == 0 && live) zl = to_float(s.row[label]);          // before it is written over (by any CTA of the row)
-  const Run run = join_all(read_row(s, [&](int v, const uint4& u) { if (KEEP) held[v - s.v0] = u; }), a.ranks);
+  if (threadIdx.x == 0 && live) zl = to_float(s.row[label]);      // before it is written over (by any CTA of the row)
+  Run run;
+  if (KEEP) {
+    __syncthreads();                               // the barriers are there
+    for (int c = 0; c < kParts; ++c) {
+      mbar_wait(&bar[c], 0, a.status);
+      for (int v = part(c) + threadIdx.x; v < part(c + 1); v += kThreads) add_vec<T>(run, held[v - s.v0]);
+    }
+    add_edge(run, s);
+  } else {
+    run = read_row(s);
+  }
+  run = join_all(run, a.ranks);
   if (threadIdx.x == 0) {
     double loss = 0, logp = 0, d = 0;
     if (live) {
@@ -279,15 +381,36 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
     }
   }
   __syncthreads();
-  const float inv = 1.f / run.s, m = run.m;
-  write_grad(s, label, s_d, [&](int v) { return KEEP ? held[v - s.v0] : *s.vec(v); },
-             [&](float z) { return exp_diff(z, m) * inv; });
+  const float d = s_d, inv = 1.f / run.s, m = run.m;
+  if (d == 0.f) {
+    write_zeros(s);
+    return;
+  }
+  auto p = [&](float2 z) { return mul2(exp_diff2(z, make_float2(-m, -m)), make_float2(inv, inv)); };
+  if (!KEEP) {
+    write_grad(s, label, d, p);
+    return;
+  }
+  const int owner = label_vec(s, label), at = owner < 0 ? 0 : (label - s.head) % Slice<T>::E;
+  for (int c = 0; c < kParts; ++c) {
+    for (int v = part(c) + threadIdx.x; v < part(c + 1); v += kThreads)
+      held[v - s.v0] = grad_of<T>(held[v - s.v0], v, owner, at, d, p);
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (threadIdx.x == 0 && part(c + 1) > part(c))
+      bulk_store(s.vec(part(c)), held + (part(c) - s.v0), static_cast<uint32_t>(part(c + 1) - part(c)) * 16);
+  }
+  write_edge(s, label, d, p);
+  if (threadIdx.x == 0) {                          // shared memory stays until it was read
+    bulk_commit_group();
+    bulk_wait_group_read<0>();
+  }
 }
 
 // Pairs of sequences (2 p chosen, 2 p + 1 rejected): one CTA a pair sums logp - ref over each sequence's labelled rows,
 // and writes the loss, the margin and every row's dL/dlogp.  Rows of no pair get 0.
 __global__ void __launch_bounds__(kThreads)
-pair_kernel(const float* __restrict__ logp, const float* __restrict__ ref, const int* __restrict__ labels, int V,
+pair_kernel(const double* __restrict__ logp, const float* __restrict__ ref, const int* __restrict__ labels, int V,
             const int* __restrict__ offs, int T, float beta, float scale, float* __restrict__ loss,
             float* __restrict__ margin, float* __restrict__ dlogp) {
   __shared__ int bound[3];
@@ -304,7 +427,7 @@ pair_kernel(const float* __restrict__ logp, const float* __restrict__ ref, const
   for (int k = 0; k < 2; ++k) {
     double sum = 0;
     for (int r = bound[k] + threadIdx.x; r < bound[k + 1]; r += kThreads)
-      if (labels[r] >= 0 && labels[r] < V) sum += static_cast<double>(logp[r]) - static_cast<double>(ref[r]);
+      if (labels[r] >= 0 && labels[r] < V) sum += logp[r] - static_cast<double>(ref[r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (threadIdx.x % 32 == 0) part[warp] = sum;
@@ -363,7 +486,7 @@ cudaError_t run(Kernel k, Type type, const Args& a, cudaStream_t stream) {
          : type == kF16 ? run_typed<__half>(k, a, stream) : run_typed<float>(k, a, stream);
 }
 
-cudaError_t run_pairs(int pairs, const float* logp, const float* ref, const int* labels, int V, const int* offs, int T,
+cudaError_t run_pairs(int pairs, const double* logp, const float* ref, const int* labels, int V, const int* offs, int T,
                       float beta, float scale, float* loss, float* margin, float* dlogp, cudaStream_t stream) {
   pair_kernel<<<pairs, kThreads, 0, stream>>>(logp, ref, labels, V, offs, T, beta, scale, loss, margin, dlogp);
   return cudaGetLastError();

@@ -26,15 +26,17 @@ struct Args {
   long rows;
   int V, ranks;
   float* logp;
+  double* logp64;         // instead of logp, unrounded, for sums of many
   float* lse;             // written by the forward pass, read by the backward pass
   const float* dlogp;
   Terms t;
+  int* status;
 };
 
 enum Kernel { kLogp, kGrad, kPolicy };
 enum Type { kBf16, kF16, kF32 };
 cudaError_t run(Kernel k, Type type, const Args& a, cudaStream_t stream);
-cudaError_t run_pairs(int pairs, const float* logp, const float* ref, const int* labels, int V, const int* offs, int T,
+cudaError_t run_pairs(int pairs, const double* logp, const float* ref, const int* labels, int V, const int* offs, int T,
                       float beta, float scale, float* loss, float* margin, float* dlogp, cudaStream_t stream);
 
 }  // namespace obj

@@ -79,7 +79,7 @@ void logp_bwd(at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ls
 
 std::vector<at::Tensor> policy(at::Tensor& logits, const at::Tensor& labels, const at::Tensor& old, const at::Tensor& adv,
                                const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& weight, double low,
-                               double high, double kl, double scale) {
+                               double high, double kl, double scale, const at::Tensor& status) {
   const char* who = "policy_loss_fwd_bwd";
   Args a = base_args(logits, labels, who);
   a.t.old = row_floats(old, logits, who, "old_logp");
@@ -90,6 +90,7 @@ std::vector<at::Tensor> policy(at::Tensor& logits, const at::Tensor& labels, con
   a.t.high = high;
   a.t.kl = kl;
   a.t.scale = scale;
+  a.status = status.data_ptr<int>();
   const at::cuda::CUDAGuard guard(logits.device());
   auto loss = at::empty({a.rows}, logits.options().dtype(at::kFloat)), logp = at::empty_like(loss);
   if (a.rows == 0) return {loss, logp};
@@ -111,15 +112,16 @@ std::vector<at::Tensor> preference(at::Tensor& logits, const at::Tensor& labels,
   TORCH_CHECK(a.rows < (1L << 31), who, ": too many rows");
   const at::cuda::CUDAGuard guard(logits.device());
   const int64_t pairs = offs.numel() / 2;
-  auto rows = at::empty({3, a.rows}, logits.options().dtype(at::kFloat));
+  auto rows = at::empty({2, a.rows}, logits.options().dtype(at::kFloat));
+  auto logp = at::empty({a.rows}, logits.options().dtype(at::kDouble));
   auto loss = at::empty({pairs}, rows.options()), margin = at::empty_like(loss);
-  a.logp = rows.data_ptr<float>();
-  a.lse = a.logp + a.rows;
+  a.logp64 = logp.data_ptr<double>();
+  a.lse = rows.data_ptr<float>();
   float* dlogp = a.lse + a.rows;
   a.dlogp = dlogp;
   a.ranks = pick_ranks(a, size_of(logits), false);
   if (a.rows > 0) go(kLogp, a, logits);
-  C10_CUDA_CHECK(run_pairs(static_cast<int>(pairs), a.logp, rp, a.labels, a.V, offs.data_ptr<int>(), static_cast<int>(a.rows),
+  C10_CUDA_CHECK(run_pairs(static_cast<int>(pairs), a.logp64, rp, a.labels, a.V, offs.data_ptr<int>(), static_cast<int>(a.rows),
                            static_cast<float>(beta), static_cast<float>(scale), loss.data_ptr<float>(),
                            margin.data_ptr<float>(), dlogp, at::cuda::getCurrentCUDAStream()));
   if (a.rows > 0) go(kGrad, a, logits);

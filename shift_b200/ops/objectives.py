@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from . import reference as ref
-from ._ext import ext
+from ._ext import ext, status_word
 
 
 def _check(logits, labels, who, **rows):
@@ -73,7 +73,7 @@ def policy_loss_fwd_bwd(logits: torch.Tensor, labels: torch.Tensor, old_logp: to
         raise ValueError(f"{who}: a KL term needs ref_logp")
     if logits.is_cuda:
         return tuple(ext().policy_loss(logits, labels, old_logp, adv, ref_logp, weight, clip_low, clip_high, kl_coef,
-                                       scale))
+                                       scale, status_word(logits.device)))
     lse = torch.logsumexp(logits.double(), 1)
     logp = ref.label_logp(logits, labels, lse)
     loss, d = ref.policy_terms(logp, old_logp, adv, ref_logp, clip_low, clip_high, kl_coef)
