@@ -156,44 +156,42 @@ struct Run {
     rise(z);
     s += z == INFINITY ? 1.f : exp_diff(z, m == -INFINITY ? 0.f : m);
   }
-  static SB_DEVICE float share(float m, float s, float top) {
-    return m == top ? 1.f : m == -INFINITY ? (s == s ? 0.f : 1.f) : exp_diff(m, top);
-  }
-  SB_DEVICE void join(float m2, float s2) {
-    const float top = fmaxf(m, m2);
-    s = s * share(m, s, top) + s2 * share(m2, s2, top);
-    m = top;
-  }
+  // the sum over another maximum, at least this one
+  SB_DEVICE float over(float top) const { return m == top ? s : m == -INFINITY ? (s == s ? 0.f : s) : s * exp_diff(m, top); }
 };
 
 // All threads' runs joined over the CTA and the cluster, in an order that does not change; every thread gets the result.
+// The maximum first, so that every sum is scaled once (an exponential of the hardware's is 5e-8 too small on average, which
+// a tree of joins would add up).
 SB_DEVICE Run join_all(Run r, int ranks) {
-  __shared__ float2 warps[kThreads / 32];
+  __shared__ float tops[kThreads / 32], sums[kThreads / 32];
   __shared__ float2 mine;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r.join(__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o));
-  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = make_float2(r.m, r.s);
-  __syncthreads();
+  const int warp = threadIdx.x / 32;
   Run all;
-  all.m = warps[0].x;
-  all.s = warps[0].y;
+  all.m = warp_max(r.m);
+  if (threadIdx.x % 32 == 0) tops[warp] = all.m;
+  __syncthreads();
 #pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) all.join(warps[w].x, warps[w].y);
+  for (int w = 0; w < kThreads / 32; ++w) all.m = fmaxf(all.m, tops[w]);
+  const float s = warp_sum(r.over(all.m));
+  if (threadIdx.x % 32 == 0) sums[warp] = s;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) all.s += sums[w];
   if (ranks == 1) return all;
   if (threadIdx.x == 0) mine = make_float2(all.m, all.s);
   cg::cluster_group cl = cg::this_cluster();
   cl.sync();
   Run row;
+  for (int k = 0; k < ranks; ++k) row.m = fmaxf(row.m, cl.map_shared_rank(&mine, k)->x);
   for (int k = 0; k < ranks; ++k) {
     const float2 p = *cl.map_shared_rank(&mine, k);
-    if (k == 0) {
-      row.m = p.x;
-      row.s = p.y;
-    } else {
-      row.join(p.x, p.y);
-    }
+    Run one;
+    one.m = p.x;
+    one.s = p.y;
+    row.s += one.over(row.m);
   }
-  cl.sync();                                       // nobody leaves, or writes `mine` again, while it is read
+  cl.sync();                                       // nobody leaves while it is read
   return row;
 }
 
