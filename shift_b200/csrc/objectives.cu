@@ -316,9 +316,9 @@ SB_DEVICE void bulk_store(void* dst, const void* src, uint32_t bytes) {
 
 // Loss, log-probability and gradient of every row in one pass: the row's slice waits in shared memory (KEEP) for its sum.
 // It comes and goes by bulk copies in kParts parts, so that all of it is in flight at once and three CTAs an SM keep the
-// memory busy while one of them computes (with loads and stores of the threads, 16 KB in flight a CTA: 494 us for 16384 x
-// 32768 bf16).
-constexpr int kParts = 4;
+// memory busy while one of them computes.  16384 x 32768 bf16: with loads and stores of the threads 494 us (16 KB in flight
+// a CTA), in 8 / 4 / 2 / 1 parts 452 / 412 / 392 / 401 us; CTAs that go on to their next rows 468 us.
+constexpr int kParts = 2;
 
 template <typename T, bool KEEP>
 __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
@@ -340,14 +340,22 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
   }
   const int label = a.labels[r];
   const bool live = label >= 0 && label < a.V;
-  float zl = 0.f;
-  if (threadIdx.x == 0 && live) zl = to_float(s.row[label]);      // before it is written over (by any CTA of the row)
+  double zl = 0, old = 0, adv = 0, ref = 0, weight = 1;
+  const bool kl = a.t.ref != nullptr && a.t.kl != 0.0;
+  if (threadIdx.x == 0 && live) {                  // early; the label's logit before any CTA of the row writes over it
+    zl = to_float(s.row[label]);
+    old = a.t.old[r];
+    adv = a.t.adv[r];
+    if (kl) ref = a.t.ref[r];
+    if (a.t.weight != nullptr) weight = a.t.weight[r];
+  }
   Run run;
   if (KEEP) {
     __syncthreads();                               // the barriers are there
     for (int c = 0; c < kParts; ++c) {
       mbar_wait(&bar[c], 0, a.status);
-      for (int v = part(c) + threadIdx.x; v < part(c + 1); v += kThreads) add_vec<T>(run, held[v - s.v0]);
+      const int end = part(c + 1);
+      for (int v = part(c) + threadIdx.x; v < end; v += kThreads) add_vec<T>(run, held[v - s.v0]);
     }
     add_edge(run, s);
   } else {
@@ -357,20 +365,19 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
   if (threadIdx.x == 0) {
     double loss = 0, logp = 0, d = 0;
     if (live) {
-      logp = static_cast<double>(zl) - static_cast<double>(run.m) - log(static_cast<double>(run.s));
-      const double ratio = exp(logp - static_cast<double>(a.t.old[r])), adv = a.t.adv[r];
-      const double clipped = fmin(fmax(ratio, 1.0 - a.t.low), 1.0 + a.t.high);
+      logp = zl - static_cast<double>(run.m) - log(static_cast<double>(run.s));
+      const double ratio = exp(logp - old), clipped = fmin(fmax(ratio, 1.0 - a.t.low), 1.0 + a.t.high);
       const double gain = adv == 0.0 ? 0.0 : ratio * adv, cut = clipped * adv;
       const bool open = gain <= cut;
       loss = -(open ? gain : cut);
       d = open ? -gain : 0.0;
       if (gain != gain) loss = d = gain;
-      if (a.t.ref != nullptr && a.t.kl != 0.0) {
-        const double gap = static_cast<double>(a.t.ref[r]) - logp, e = expm1(gap);
+      if (kl) {
+        const double gap = ref - logp, e = expm1(gap);
         loss += a.t.kl * (e - gap);
         d -= a.t.kl * e;
       }
-      d *= a.t.weight != nullptr ? a.t.scale * a.t.weight[r] : a.t.scale;
+      d *= a.t.scale * weight;
     }
     s_d = static_cast<float>(d);
     if (s.edges) {
@@ -391,7 +398,8 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
   }
   const int owner = label_vec(s, label), at = owner < 0 ? 0 : (label - s.head) % Slice<T>::E;
   for (int c = 0; c < kParts; ++c) {
-    for (int v = part(c) + threadIdx.x; v < part(c + 1); v += kThreads)
+    const int end = part(c + 1);
+    for (int v = part(c) + threadIdx.x; v < end; v += kThreads)
       held[v - s.v0] = grad_of<T>(held[v - s.v0], v, owner, at, d, p);
     fence_proxy_async_smem();
     __syncthreads();
