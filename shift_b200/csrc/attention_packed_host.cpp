@@ -60,28 +60,26 @@ static void check_rows(const at::Tensor& t, const at::Tensor& qkv, int64_t rows,
               "bytes apart");
 }
 
-static void check_ints(const at::Tensor& t, const at::Tensor& qkv, int64_t n, const char* who) {
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n && t.device() == qkv.device(), who,
-              ": the plan of another buffer (ops.packed.sequences of ", qkv.size(0), " rows beside qkv)");
-}
+struct Plan {                        // of packed.cu's sequences()
+  const int *start, *stop, *ends, *q_order, *q2_order, *k_order;
+};
 
-static Args base_args(const at::Tensor& qkv, const at::Tensor& start, const at::Tensor& ends,
-                      const std::vector<at::Tensor>& orders, int64_t Hq, int64_t Hkv, int64_t D, double scale,
-                      const at::Tensor& status, const char* who) {
+static Args base_args(const at::Tensor& qkv, const at::Tensor& plan, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                      double scale, const at::Tensor& status, const char* who, Plan& pl) {
   TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 || qkv.scalar_type() == at::kHalf, who, ": bf16 or fp16, got ",
               qkv.scalar_type());
   TORCH_CHECK(D == 64 || D == 128, who, ": heads of 64 or 128 columns, got ", D);
   TORCH_CHECK(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq <= (1 << 20), who, ": ", Hq, " query heads for ", Hkv,
               " key heads");
   TORCH_CHECK(std::isfinite(scale) && scale > 0, who, ": scale ", scale, ", a number above 0 is expected");
-  const int64_t T = start.numel(), nt = (T + 127) / 128;
+  const int64_t nt = (T + 127) / 128, nt2 = (T + 255) / 256;
   check_rows(qkv, qkv, T, (Hq + 2 * Hkv) * D, who, "qkv");
-  check_ints(start, qkv, T, who);
-  check_ints(ends, qkv, 2, who);
-  TORCH_CHECK(orders.size() == 3, who, ": the plan of a buffer on the CPU");
-  check_ints(orders[0], qkv, nt, who);
-  check_ints(orders[1], qkv, (T + 255) / 256, who);
-  check_ints(orders[2], qkv, nt, who);
+  TORCH_CHECK(plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.numel() == 3 * T + 2 + 2 * nt + nt2 &&
+                  plan.device() == qkv.device(),
+              who, ": the plan of another buffer, or on another device (ops.packed.sequences of ", T, " rows beside qkv)");
+  const int* p = plan.data_ptr<int>();
+  const int* o = p + 3 * T + 2;
+  pl = Plan{p, p + 2 * T, p + 3 * T, o, o + nt, o + nt + nt2};
   TORCH_CHECK(nt * Hq < (1L << 31), who, ": too many rows and heads");
   Args a{};
   a.T = static_cast<int>(T);
@@ -90,8 +88,9 @@ static Args base_args(const at::Tensor& qkv, const at::Tensor& start, const at::
   a.group = static_cast<int>(Hq / Hkv);
   a.split = 1;
   a.tiles = static_cast<int>(nt);
-  a.start = start.data_ptr<int>();
-  a.ends = ends.data_ptr<int>();
+  a.start = pl.start;
+  a.stop = pl.stop;
+  a.ends = pl.ends;
   a.scale = static_cast<float>(scale);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.qkv = qkv.data_ptr();
@@ -100,11 +99,11 @@ static Args base_args(const at::Tensor& qkv, const at::Tensor& start, const at::
   return a;
 }
 
-std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& start, const at::Tensor& ends,
-                            const std::vector<at::Tensor>& orders, int64_t Hq, int64_t Hkv, int64_t D, double scale,
-                            const c10::optional<at::Tensor>& out, const at::Tensor& status) {
+std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& plan, int64_t rows, int64_t Hq, int64_t Hkv,
+                            int64_t D, double scale, const c10::optional<at::Tensor>& out, const at::Tensor& status) {
   const char* who = "attention_fwd";
-  Args a = base_args(qkv, start, ends, orders, Hq, Hkv, D, scale, status, who);
+  Plan pl;
+  Args a = base_args(qkv, plan, rows, Hq, Hkv, D, scale, status, who, pl);
   const at::cuda::CUDAGuard guard(qkv.device());
   auto o = out.has_value() ? *out : at::empty({a.T, Hq * D}, qkv.options());
   if (out.has_value()) check_rows(o, qkv, a.T, Hq * D, who, "out");
@@ -117,7 +116,7 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& start, cons
   // Two heads of one key head share every key block and have the same causal cost; without such pairs two consecutive
   // tiles of a head do.
   a.pair_heads = a.group % 2 == 0;
-  a.order = orders[a.pair_heads ? 0 : 1].data_ptr<int>();
+  a.order = a.pair_heads ? pl.q_order : pl.q2_order;
   const unsigned items = static_cast<unsigned>(a.pair_heads ? a.tiles * (Hq / 2) : (a.T + 255) / 256 * Hq);
   const CUtensorMap tm = tile_map(qkv, 128);
   const bool half = qkv.scalar_type() == at::kHalf;
@@ -127,12 +126,11 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& start, cons
 }
 
 at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse, const at::Tensor& dout,
-               const at::Tensor& start, const at::Tensor& stop, const at::Tensor& ends,
-               const std::vector<at::Tensor>& orders, int64_t Hq, int64_t Hkv, int64_t D, double scale,
+               const at::Tensor& plan, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, double scale,
                const c10::optional<at::Tensor>& out, const at::Tensor& status) {
   const char* who = "attention_bwd";
-  Args a = base_args(qkv, start, ends, orders, Hq, Hkv, D, scale, status, who);
-  check_ints(stop, qkv, a.T, who);
+  Plan pl;
+  Args a = base_args(qkv, plan, rows, Hq, Hkv, D, scale, status, who, pl);
   check_rows(o, qkv, a.T, Hq * D, who, "o");
   check_rows(dout, qkv, a.T, Hq * D, who, "do");
   TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.device() == qkv.device() && lse.dim() == 2 &&
@@ -143,7 +141,6 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
   if (out.has_value()) check_rows(dqkv, qkv, a.T, (Hq + 2 * Hkv) * D, who, "out");
   if (a.T == 0) return dqkv;
   a.fill = out.has_value() ? 0 : 1;
-  a.stop = stop.data_ptr<int>();
   a.o = o.data_ptr();
   a.o_ld = row_stride(o);
   a.lse = lse.data_ptr<float>();
@@ -151,7 +148,7 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
   a.do_ld = row_stride(dout);
   a.dqkv = dqkv.data_ptr();
   a.dqkv_ld = row_stride(dqkv);
-  auto rows = at::empty({Hq * a.tiles * 256}, lse.options());
+  auto row_values = at::empty({Hq * a.tiles * 256}, lse.options());
   // A key tile meets every later query of its sequence in every head of its group: with few tiles the group's heads are
   // dealt out over several CTAs, whose fp32 sums are added up in order afterwards.
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
@@ -162,7 +159,7 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
     a.partial = partial.data_ptr<float>();
   }
   launch_bwd(static_cast<int>(D), qkv.scalar_type() == at::kHalf, tile_map(qkv, 128), tile_map(qkv, 64), tile_map(dout, 128),
-             tile_map(dout, 64), a, orders[0].data_ptr<int>(), orders[2].data_ptr<int>(), rows.data_ptr<float>(),
+             tile_map(dout, 64), a, pl.q_order, pl.k_order, row_values.data_ptr<float>(),
              at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return dqkv;

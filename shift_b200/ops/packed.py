@@ -36,32 +36,41 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 class Sequences(NamedTuple):
-    """Of every row: the first row of its sequence, its place in it, and the row behind its end.  A row that no sequence
-    covers has ``start`` row + 1, ``pos`` -1 and ``stop`` row.  ``ends``: the first covered row and the one behind the
-    last; ``orders``: orders in which the attention kernels take their tiles (none on the CPU)."""
+    """What the offsets say of every row of a buffer, in one int32 tensor: ``start``, the first row of its sequence, ``pos``,
+    its place in it, and ``stop``, the row behind its end.  A row that no sequence covers has ``start`` row + 1, ``pos`` -1
+    and ``stop`` row.  ``ends``: the first covered row and the one behind the last.  (On the GPU orders follow in which the
+    attention kernels take their tiles.)"""
     offs: torch.Tensor
-    start: torch.Tensor
-    pos: torch.Tensor
-    stop: torch.Tensor
-    ends: torch.Tensor
-    orders: tuple
+    plan: torch.Tensor
+    rows: int
 
     @property
-    def rows(self) -> int:
-        return self.start.shape[0]
+    def start(self) -> torch.Tensor:
+        return self.plan[:self.rows]
+
+    @property
+    def pos(self) -> torch.Tensor:
+        return self.plan[self.rows:2 * self.rows]
+
+    @property
+    def stop(self) -> torch.Tensor:
+        return self.plan[2 * self.rows:3 * self.rows]
+
+    @property
+    def ends(self) -> torch.Tensor:
+        return self.plan[3 * self.rows:3 * self.rows + 2]
 
 
 def sequences(offs: torch.Tensor, rows: int) -> Sequences:
     """The plan of a buffer of ``rows`` rows.  It reads ``offs`` on the device, now: it can be captured into a graph, and
     is made again for other offsets."""
+    if offs.is_cuda:
+        return Sequences(offs, ext().packed_sequences(offs, rows), rows)
     if offs.dtype != torch.int32 or offs.dim() != 1 or offs.numel() < 2 or not offs.is_contiguous():
         raise ValueError(f"sequences: offs are int32 [sequences + 1], contiguous, got {tuple(offs.shape)} of {offs.dtype}")
-    if not 0 <= rows <= 1 << 30:
-        raise ValueError(f"sequences: 0 to 2^30 rows, got {rows}")
-    if offs.is_cuda:
-        start, pos, stop, ends, *orders = ext().packed_sequences(offs, rows)
-        return Sequences(offs, start, pos, stop, ends, tuple(orders))
-    return Sequences(offs, *ref.packed_rows(offs, rows), ())
+    if not 0 <= rows <= 1 << 29:
+        raise ValueError(f"sequences: 0 to 2^29 rows, got {rows}")
+    return Sequences(offs, torch.cat(ref.packed_rows(offs, rows)), rows)
 
 
 # ----------------------------------------------------------------------------- rotary positions
@@ -175,8 +184,7 @@ def attention_fwd(qkv: torch.Tensor, seqs: Sequences, Hq: int, Hkv: int, D: int,
     if out is not None and (tuple(out.shape) != (seqs.rows, Hq * D) or out.dtype != qkv.dtype or out.device != qkv.device):
         raise ValueError(f"attention_fwd: out [{seqs.rows}, {Hq * D}] of {qkv.dtype} beside qkv")
     if qkv.is_cuda:
-        return tuple(ext().packed_attn_fwd(qkv, seqs.start, seqs.ends, list(seqs.orders), Hq, Hkv, D, scale, out,
-                                           status_word(qkv.device)))
+        return tuple(ext().packed_attn_fwd(qkv, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out, status_word(qkv.device)))
     o, lse = ref.packed_attention(qkv, ref.segments(seqs.offs, seqs.rows), Hq, Hkv, D, scale)
     if out is not None:
         live = seqs.pos >= 0
@@ -197,8 +205,8 @@ def attention_bwd(qkv: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: tor
     if out is not None and (out.shape != qkv.shape or out.dtype != qkv.dtype or out.device != qkv.device):
         raise ValueError(f"attention_bwd: out {tuple(qkv.shape)} of {qkv.dtype} beside qkv")
     if qkv.is_cuda:
-        return ext().packed_attn_bwd(qkv, o, lse, do, seqs.start, seqs.stop, seqs.ends, list(seqs.orders), Hq, Hkv, D,
-                                     scale, out, status_word(qkv.device))
+        return ext().packed_attn_bwd(qkv, o, lse, do, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out,
+                                     status_word(qkv.device))
     segs = ref.segments(seqs.offs, seqs.rows)
     (g,) = ref.grad_of(lambda x: ref.packed_attention(x, segs, Hq, Hkv, D, scale)[0], [qkv], do.float())
     if out is not None:

@@ -23,6 +23,12 @@ def _randn(*shape, seed=0, dtype=torch.bfloat16, std=1.0):
     return (torch.randn(*shape, generator=g) * std).to(dtype).to(DEV)
 
 
+def _orders(seqs):
+    """The plan's tile orders: of 128 queries, of 256 queries, of 128 keys."""
+    n, n2 = -(-seqs.rows // 128), -(-seqs.rows // 256)
+    return seqs.plan[3 * seqs.rows + 2:].split([n, n2, n])
+
+
 # ----------------------------------------------------------------------------- the plan
 @pytest.mark.parametrize("offs,rows", [
     ([0, 1], 1), ([0, 0], 0), ([0, 300], 300), ([3, 3, 3, 200, 255, 256, 257, 600], 700), ([0, 5, 2, 9], 9),
@@ -33,7 +39,7 @@ def test_sequences(offs, rows):
     want = packed.sequences(torch.tensor(offs, dtype=torch.int32), rows)
     for name in ("start", "pos", "stop", "ends"):
         assert torch.equal(getattr(got, name).cpu(), getattr(want, name)), name
-    for order, tile in zip(got.orders, (128, 256, 128)):
+    for order, tile in zip(_orders(got), (128, 256, 128)):
         assert sorted(order.tolist()) == list(range(-(-rows // tile)))
 
 
@@ -41,8 +47,8 @@ def test_orders_put_the_costliest_tiles_first():
     offs, rows = [0, 100, 2100, 2400, 6000], 6100
     got = _seqs(offs, rows)
     start, stop = got.start.tolist(), got.stop.tolist()
-    fwd = [(min(128 * t + 128, rows) + 127) // 128 - start[128 * t] // 128 for t in got.orders[0].tolist()]
-    bwd = [(stop[min(128 * t + 128, rows) - 1] - 128 * t + 127) // 128 for t in got.orders[2].tolist()]
+    fwd = [(min(128 * t + 128, rows) + 127) // 128 - start[128 * t] // 128 for t in _orders(got)[0].tolist()]
+    bwd = [(stop[min(128 * t + 128, rows) - 1] - 128 * t + 127) // 128 for t in _orders(got)[2].tolist()]
     assert fwd == sorted(fwd, reverse=True) and bwd == sorted(bwd, reverse=True)
 
 
