@@ -81,6 +81,8 @@ std::vector<at::Tensor> policy(at::Tensor& logits, const at::Tensor& labels, con
                                const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& weight, double low,
                                double high, double kl, double scale, const at::Tensor& status) {
   const char* who = "policy_loss_fwd_bwd";
+  TORCH_CHECK(low >= 0 && high >= 0, who, ": clipped to 1 - ", low, ", 1 + ", high);
+  TORCH_CHECK(kl == 0 || ref.has_value(), who, ": a KL term needs ref_logp");
   Args a = base_args(logits, labels, who);
   a.t.old = row_floats(old, logits, who, "old_logp");
   a.t.adv = row_floats(adv, logits, who, "adv");

@@ -15,26 +15,25 @@
 namespace sb {
 namespace packed {
 
-constexpr int kRows = 256;     // rows (and threads) of a CTA of the plan kernel
+constexpr int kRows = 256;     // rows (and threads) of a CTA of the plan's first kernel
 constexpr int kBins = 4096;    // costs of the tile orders; larger ones share the last bin
 
 // start, pos, stop of every row.  A row's sequence begins at the last offset at or before it and ends at the first one
 // behind it, so the offsets that fall into a CTA's 256 rows are marked in a bit set and the nearest ones outside are kept
 // beside it: no search per row.  Every CTA walks all offsets (a prefix maximum, 256 at a time).
-__global__ void __launch_bounds__(kRows)
-rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start, int* __restrict__ pos,
-            int* __restrict__ stop, int* __restrict__ ends) {
-  __shared__ unsigned mark[kRows / 32];
-  __shared__ int part[kRows / 32], s_before, s_after;
-  const int r0 = blockIdx.x * kRows, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (threadIdx.x < kRows / 32) mark[threadIdx.x] = 0;
+template <int ROWS>
+SB_DEVICE void find_rows(const int* __restrict__ offs, int n, int T, int* start, int* pos, int* stop, int* ends) {
+  __shared__ unsigned mark[ROWS / 32];
+  __shared__ int part[ROWS / 32], s_before, s_after;
+  const int r0 = blockIdx.x * ROWS, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x < ROWS / 32) mark[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     s_before = -1;
     s_after = INT_MAX;
   }
   int carry = 0;                 // the largest offset so far, at least 0
   __syncthreads();
-  for (int base = 0; base < n; base += kRows) {
+  for (int base = 0; base < n; base += ROWS) {
     const int i = base + threadIdx.x;
     int b = i < n ? min(offs[i], T) : 0;
 #pragma unroll
@@ -45,7 +44,7 @@ rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start,
     if (lane == 31) part[warp] = b;
     __syncthreads();
     int top = carry;
-    for (int w = 0; w < kRows / 32; ++w) {
+    for (int w = 0; w < ROWS / 32; ++w) {
       if (w < warp) b = max(b, part[w]);
       top = max(top, part[w]);
     }
@@ -53,7 +52,7 @@ rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start,
     carry = top;
     if (i < n) {
       if (b < r0) atomicMax(&s_before, b);
-      else if (b < r0 + kRows) atomicOr(&mark[(b - r0) / 32], 1u << ((b - r0) % 32));
+      else if (b < r0 + ROWS) atomicOr(&mark[(b - r0) / 32], 1u << ((b - r0) % 32));
       else atomicMin(&s_after, b);
       if (blockIdx.x == 0 && i == 0) ends[0] = b;
     }
@@ -69,7 +68,7 @@ rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start,
   if (m != 0) first = r0 + w * 32 + 31 - __clz(m);
   m = lane == 31 ? 0 : mark[warp] & (0xffffffffu << (lane + 1));
   w = warp;
-  while (m == 0 && w < kRows / 32 - 1) m = mark[++w];
+  while (m == 0 && w < ROWS / 32 - 1) m = mark[++w];
   if (m != 0) behind = r0 + w * 32 + __ffs(m) - 1;
   const bool covered = first >= 0 && behind != INT_MAX;
   start[r] = covered ? first : r + 1;
@@ -78,18 +77,15 @@ rows_kernel(const int* __restrict__ offs, int n, int T, int* __restrict__ start,
 }
 
 // Orders of the attention kernels' tiles, the costliest first: a counting sort by the number of 128-row blocks that a
-// tile meets.  Block 0: tiles of 128 queries; 1: of 256 queries; 2: of 128 keys.  The order decides when a tile runs,
-// nothing else.
-__global__ void __launch_bounds__(1024)
-order_kernel(const int* __restrict__ start, const int* __restrict__ stop, int T, int* __restrict__ fwd,
-             int* __restrict__ fwd2, int* __restrict__ bwd) {
-  __shared__ int bins[kBins];
-  const int rows = blockIdx.x == 1 ? 256 : 128;
+// tile meets.  0: tiles of 128 queries; 1: of 256 queries; 2: of 128 keys.  The order decides when a tile runs, nothing
+// else.  By 1024 threads.
+SB_DEVICE void find_order(int which, const int* start, const int* stop, int T, int* out) {
+  __shared__ __align__(16) int bins[kBins];
+  const int rows = which == 1 ? 256 : 128;
   const int nt = (T + rows - 1) / rows;
-  int* out = blockIdx.x == 0 ? fwd : blockIdx.x == 1 ? fwd2 : bwd;
   auto cost = [&](int t) {
     const int lo = t * rows, hi = min(lo + rows, T);
-    const int blocks = blockIdx.x == 2 ? (stop[hi - 1] - lo + 127) / 128 : (hi + 127) / 128 - start[lo] / 128;
+    const int blocks = which == 2 ? (stop[hi - 1] - lo + 127) / 128 : (hi + 127) / 128 - start[lo] / 128;
     return kBins - 1 - max(0, min(blocks, kBins - 1));
   };
   for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
@@ -116,6 +112,25 @@ order_kernel(const int* __restrict__ start, const int* __restrict__ stop, int T,
   for (int t = threadIdx.x; t < nt; t += 1024) out[atomicAdd(&bins[cost(t)], 1)] = t;
 }
 
+__global__ void __launch_bounds__(kRows)
+rows_kernel(const int* __restrict__ offs, int n, int T, int* start, int* pos, int* stop, int* ends) {
+  find_rows<kRows>(offs, n, T, start, pos, stop, ends);
+}
+__global__ void __launch_bounds__(1024)
+order_kernel(const int* start, const int* stop, int T, int* fwd, int* fwd2, int* bwd) {
+  find_order(blockIdx.x, start, stop, T, blockIdx.x == 0 ? fwd : blockIdx.x == 1 ? fwd2 : bwd);
+}
+// both for a buffer of at most 1024 rows (one launch: 4 us less of 20 for a short batch)
+__global__ void __launch_bounds__(1024)
+small_kernel(const int* __restrict__ offs, int n, int T, int* start, int* pos, int* stop, int* ends, int* fwd, int* fwd2,
+             int* bwd) {
+  find_rows<1024>(offs, n, T, start, pos, stop, ends);
+  for (int which = 0; which < 3; ++which) {
+    __syncthreads();
+    find_order(which, start, stop, T, which == 0 ? fwd : which == 1 ? fwd2 : bwd);
+  }
+}
+
 // The plan: start, pos, stop of every row | first covered row, row behind the last one | tile orders (of 128 queries, 256
 // queries, 128 keys).
 at::Tensor sequences(const at::Tensor& offs, int64_t rows) {
@@ -129,14 +144,18 @@ at::Tensor sequences(const at::Tensor& offs, int64_t rows) {
   auto stream = at::cuda::getCurrentCUDAStream();
   const int T = static_cast<int>(rows);
   int* p = plan.data_ptr<int>();
-  rows_kernel<<<std::max(1, (T + kRows - 1) / kRows), kRows, 0, stream>>>(
-      offs.data_ptr<int>(), static_cast<int>(offs.numel()), T, p, p + T, p + 2L * T, p + 3L * T);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (T > 0) {
-    int* o = p + 3L * T + 2;
-    order_kernel<<<3, 1024, 0, stream>>>(p, p + 2L * T, T, o, o + nt, o + nt + nt2);
+  const int n = static_cast<int>(offs.numel());
+  int* o = p + 3L * T + 2;
+  if (T <= 1024) {
+    small_kernel<<<1, 1024, 0, stream>>>(offs.data_ptr<int>(), n, T, p, p + T, p + 2L * T, p + 3L * T, o, o + nt,
+                                         o + nt + nt2);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
+    return plan;
   }
+  rows_kernel<<<(T + kRows - 1) / kRows, kRows, 0, stream>>>(offs.data_ptr<int>(), n, T, p, p + T, p + 2L * T, p + 3L * T);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  order_kernel<<<3, 1024, 0, stream>>>(p, p + 2L * T, T, o, o + nt, o + nt + nt2);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
   return plan;
 }
 

@@ -26,6 +26,7 @@ from . import reference as ref
 from ._ext import ext, status_word
 
 
+# The CUDA entry points check their arguments themselves (csrc/objectives_host.cpp); this is for CPU tensors.
 def _check(logits, labels, who, **rows):
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"{who}: logits [rows, vocabulary] in bf16, fp16 or fp32, got {tuple(logits.shape)} of "
@@ -40,19 +41,19 @@ def _check(logits, labels, who, **rows):
 
 def token_logp_fwd(logits: torch.Tensor, labels: torch.Tensor):
     """(logp [T], lse [T]), fp32: the label's log-probability (0 without one) and every row's log-sum-exp."""
-    _check(logits, labels, "token_logp_fwd")
     if logits.is_cuda:
         return tuple(ext().token_logp_fwd(logits, labels))
+    _check(logits, labels, "token_logp_fwd")
     lse = torch.logsumexp(logits.double(), 1)
     return ref.label_logp(logits, labels, lse).float(), lse.float()
 
 
 def token_logp_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor) -> torch.Tensor:
     """Overwrites the logits of ``token_logp_fwd`` by dlogp (onehot - softmax), and returns them."""
-    _check(logits, labels, "token_logp_bwd", lse=lse, dlogp=dlogp)
     if logits.is_cuda:
         ext().token_logp_bwd(logits, labels, lse, dlogp)
         return logits
+    _check(logits, labels, "token_logp_bwd", lse=lse, dlogp=dlogp)
     return ref.label_logp_grad_(logits, labels, lse, dlogp)
 
 
@@ -65,15 +66,15 @@ def policy_loss_fwd_bwd(logits: torch.Tensor, labels: torch.Tensor, old_logp: to
 
     The logits are overwritten by scale * weight * dloss/dlogits (``weight`` [T], default 1).  Where the clip binds, the
     first term has no gradient; on its border it still has.  A row of zero advantage has none, whatever its ratio."""
+    if logits.is_cuda:
+        return tuple(ext().policy_loss(logits, labels, old_logp, adv, ref_logp, weight, clip_low, clip_high, kl_coef,
+                                       scale, status_word(logits.device)))
     who = "policy_loss_fwd_bwd"
     _check(logits, labels, who, old_logp=old_logp, adv=adv, ref_logp=ref_logp, weight=weight)
     if not (0 <= clip_low and 0 <= clip_high):
         raise ValueError(f"{who}: clipped to 1 - {clip_low}, 1 + {clip_high}")
     if kl_coef != 0 and ref_logp is None:
         raise ValueError(f"{who}: a KL term needs ref_logp")
-    if logits.is_cuda:
-        return tuple(ext().policy_loss(logits, labels, old_logp, adv, ref_logp, weight, clip_low, clip_high, kl_coef,
-                                       scale, status_word(logits.device)))
     lse = torch.logsumexp(logits.double(), 1)
     logp = ref.label_logp(logits, labels, lse)
     loss, d = ref.policy_terms(logp, old_logp, adv, ref_logp, clip_low, clip_high, kl_coef)
@@ -91,13 +92,13 @@ def preference_loss_fwd_bwd(logits: torch.Tensor, labels: torch.Tensor, ref_logp
     margin = beta (sum over the chosen of (logp - ref_logp) - the same over the rejected), over labelled rows;
     loss = -log sigmoid(margin).  ``offs``: int32 [2 P + 1] on the device, as for ``ops.packed.sequences``.  The logits are
     overwritten by scale * dloss/dlogits (zeros in rows of no pair)."""
+    if logits.is_cuda:
+        return tuple(ext().preference_loss(logits, labels, ref_logp, offs, beta, scale))
     who = "preference_loss_fwd_bwd"
     _check(logits, labels, who, ref_logp=ref_logp)
     if (offs.dtype != torch.int32 or offs.dim() != 1 or offs.numel() < 3 or offs.numel() % 2 == 0
             or offs.device != logits.device):
         raise ValueError(f"{who}: offs are int32 [2 pairs + 1] beside the logits")
-    if logits.is_cuda:
-        return tuple(ext().preference_loss(logits, labels, ref_logp, offs, beta, scale))
     lse = torch.logsumexp(logits.double(), 1)
     gap = torch.where(ref.has_label(labels, logits.shape[1]), ref.label_logp(logits, labels, lse) - ref_logp.double(),
                       torch.zeros_like(lse))

@@ -162,6 +162,7 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, plan: Rotary, heads: int, inverse
 
 
 # ----------------------------------------------------------------------------- attention
+# The CUDA entry points check their arguments themselves (csrc/attention_packed_host.cpp); this is for CPU tensors.
 def _check(x, width, seqs, Hq, Hkv, D, who, what="qkv"):
     if Hq < 1 or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{who}: {Hq} query heads for {Hkv} key heads")
@@ -180,11 +181,11 @@ def attention_fwd(qkv: torch.Tensor, seqs: Sequences, Hq: int, Hkv: int, D: int,
     covers get zeros (with ``out``: are left as they were) and an lse of minus infinity; what they hold is not looked
     at.  A row's result hangs on the rows it sees and on no other, also where others are not finite (such rows are
     computed one by one, slowly)."""
+    if qkv.is_cuda:
+        return tuple(ext().packed_attn_fwd(qkv, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out, status_word(qkv.device)))
     _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, "attention_fwd")
     if out is not None and (tuple(out.shape) != (seqs.rows, Hq * D) or out.dtype != qkv.dtype or out.device != qkv.device):
         raise ValueError(f"attention_fwd: out [{seqs.rows}, {Hq * D}] of {qkv.dtype} beside qkv")
-    if qkv.is_cuda:
-        return tuple(ext().packed_attn_fwd(qkv, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out, status_word(qkv.device)))
     o, lse = ref.packed_attention(qkv, ref.segments(seqs.offs, seqs.rows), Hq, Hkv, D, scale)
     if out is not None:
         live = seqs.pos >= 0
@@ -199,14 +200,14 @@ def attention_bwd(qkv: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: tor
 
     Deterministic: no sum's order hangs on timing.  Rows that no sequence covers get zeros (with ``out``: are left as
     they were)."""
+    if qkv.is_cuda:
+        return ext().packed_attn_bwd(qkv, o, lse, do, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out,
+                                     status_word(qkv.device))
     _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, "attention_bwd")
     _check(o, Hq * D, seqs, Hq, Hkv, D, "attention_bwd", "o")
     _check(do, Hq * D, seqs, Hq, Hkv, D, "attention_bwd", "do")
     if out is not None and (out.shape != qkv.shape or out.dtype != qkv.dtype or out.device != qkv.device):
         raise ValueError(f"attention_bwd: out {tuple(qkv.shape)} of {qkv.dtype} beside qkv")
-    if qkv.is_cuda:
-        return ext().packed_attn_bwd(qkv, o, lse, do, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out,
-                                     status_word(qkv.device))
     segs = ref.segments(seqs.offs, seqs.rows)
     (g,) = ref.grad_of(lambda x: ref.packed_attention(x, segs, Hq, Hkv, D, scale)[0], [qkv], do.float())
     if out is not None:
