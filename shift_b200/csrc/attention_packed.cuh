@@ -86,12 +86,13 @@ SB_DEVICE float max3(float a, float b, float c) {
 }
 
 // 2^x of two values on the FMA and integer pipes, for x <= 126: x = j + r with j the nearest whole number (left in the low
-// bits of x + 1.5 * 2^23) and r in [-1/2, 1/2]; 2^r by a polynomial of degree 4 fitted to the relative error over that
-// interval (least squares, reweighted; at most 2.7e-6), j added to the exponent.  Values below -126 count as -126.
-__device__ constexpr float kEx2[5] = {0.99999928f, 0.69312179f, 0.24024744f, 0.055917863f, 0.0095701013f};
+// bits of x + 1.5 * 2^23) and r in [-1/2, 1/2]; 2^r by a polynomial of degree 4 that is 1 at 0, fitted to the relative error
+// over that interval (least squares, reweighted; at most 2.9e-6), j added to the exponent.  At -127 and below, masked -inf
+// among it, that leaves exactly 0: a masked probability must not carry another row's value, however large that is.
+__device__ constexpr float kEx2[5] = {1.f, 0.693124175f, 0.240240991f, 0.0559064262f, 0.00958285294f};
 SB_DEVICE float2 ex2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
   const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
   const float2 j = add2(t, make_float2(-12582912.f, -12582912.f));
   const float2 r = fma2(j, make_float2(-1.f, -1.f), x);

@@ -141,15 +141,18 @@ class Engine:
     # ------------------------------------------------------------------ compute
     def forward_backward(self, batches: list, B: int, S: int):
         """batches: list of (tokens [B,S], labels [B,S]) device tensors for a
-        single-stage model.  Returns the device scalar sum of token losses
-        (already scaled into the mean by ``loss_scale``)."""
+        single-stage model, each followed, where it wants them, by a dict of
+        further arguments of ``QwenMoE.forward`` (``seqs``: the rows hold
+        packed sequences; ``objective``: another loss, which scales its own
+        gradient).  Returns the device scalar sum of token losses (already
+        scaled into the mean by ``loss_scale``)."""
         n_tok = B * S * len(batches)
         self.store.zero_grad()
         total = None
         self.model._accumulate = False
         hook = self.model.layer_done_hook
-        for mb, (tok, lab) in enumerate(batches):
-            _, loss = self.model.forward(tok, None, lab, B, S, loss_scale=1.0 / n_tok)
+        for mb, (tok, lab, *more) in enumerate(batches):
+            _, loss = self.model.forward(tok, None, lab, B, S, loss_scale=1.0 / n_tok, **(more[0] if more else {}))
             # bucket-completion hooks fire only while the last microbatch's
             # backward writes the final gradients
             self.model.layer_done_hook = hook if mb == len(batches) - 1 else None

@@ -15,6 +15,11 @@ needs; backward writes weight gradients straight into the flat gradient
 buffer (``FlatParams.grad``) and reports per-layer completion so that the
 cross-replica reduction of a bucket can start as soon as its layers are done.
 
+Sequences of different lengths may lie one after the other in a batch's rows (``ops.packed.Sequences``): attention then
+stays inside each of them, positions restart, and rows of none take no part but in the router's load.  Heads may be rotated
+in part, interleaved or with frequencies scaled for longer contexts.  Another objective than cross entropy
+(``ops.objectives``) takes the logits in its place.
+
 Layout of the fused weights:
 * ``attn.qkv``  [(Hq + 2 Hkv) * D, H]   rows q | k | v
 * ``mlp.w1``    [E_local, 2F, H]        rows in blocks of 16 gate / 16 up
@@ -30,6 +35,7 @@ import torch
 
 from ..ops import functional as Fn
 from ..ops import gemm as G
+from ..ops import packed
 from ..ops import reference as ref
 from ..parallel.flat import FlatParams, ParamSpec
 
@@ -51,6 +57,9 @@ class MoEConfig:
     aux_coef: float = 1.0e-3
     init_std: float = 0.02
     max_seq: int = 4096
+    rope_dim: int | None = None                              # rotated columns of a head; all by default
+    rope_layout: str = "half"                                # or "interleaved"
+    rope_scaling: packed.RotaryScaling | None = None
 
     @classmethod
     def bench(cls) -> "MoEConfig":
@@ -62,6 +71,9 @@ class MoEConfig:
         """2 layers, hidden 256, 4 heads, 8 experts top-2, FFN 256, vocab 1024."""
         return cls(vocab=1024, hidden=256, layers=2, heads=4, kv_heads=4, head_dim=64, experts=8, top_k=2,
                    expert_ffn=256, max_seq=512)
+
+    def plain_rope(self) -> bool:
+        return self.rope_dim in (None, self.head_dim) and self.rope_layout == "half" and self.rope_scaling is None
 
     def param_count(self) -> int:
         H, F, E = self.hidden, self.expert_ffn, self.experts
@@ -136,6 +148,7 @@ class QwenMoE:
         self.e_hi = cfg.experts if self.part.expert_hi < 0 else self.part.expert_hi
         dev = store.device
         self.cos, self.sin = ref.rope_tables(cfg.max_seq, cfg.head_dim, cfg.rope_theta, dev)
+        self.rotary = packed.Rotary(cfg.head_dim, cfg.rope_theta, cfg.rope_dim, cfg.rope_layout, cfg.rope_scaling, dev)
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
         self.dt = store.compute_dtype
         self._saved: list = []
@@ -154,13 +167,25 @@ class QwenMoE:
 
     # ------------------------------------------------------------------ forward
     def forward(self, tokens: torch.Tensor | None, hidden: torch.Tensor | None, labels: torch.Tensor | None,
-                B: int, S: int, loss_scale: float = 1.0):
+                B: int, S: int, loss_scale: float = 1.0, seqs: packed.Sequences | None = None, objective=None):
         """Run this stage.  Returns (hidden_out, loss_sum) where hidden_out is
         the residual stream (h, delta) pair flattened as one tensor for the
-        next stage, and loss_sum a device scalar on the last stage."""
+        next stage, and loss_sum a device scalar on the last stage.
+
+        ``seqs``: the B * S rows hold these sequences instead of B of length S
+        (every stage is given them).  ``objective``: called as
+        ``objective(logits, labels)`` on the last stage in place of cross
+        entropy; it overwrites the logits by their gradient and returns losses
+        to be summed (``ops.objectives``; the rows of one rank only, so not
+        with tensor parallelism)."""
         cfg, st = self.cfg, self.store
         T = B * S
-        saved = {"B": B, "S": S, "layers": [], "loss_scale": loss_scale}
+        if seqs is not None and seqs.rows != T:
+            raise ValueError(f"forward: sequences of a buffer of {seqs.rows} rows, the batch has {T}")
+        if objective is not None and self.tp is not None:
+            raise ValueError("forward: an objective of its own sees whole sequences, which tensor parallelism splits")
+        saved = {"B": B, "S": S, "layers": [], "loss_scale": loss_scale, "seqs": seqs,
+                 "pos": self._positions(T, S, seqs, st.device)}
         if self.part.has_embed:
             tok = tokens.reshape(-1).to(torch.int32)
             if self.tp is not None:
@@ -174,9 +199,9 @@ class QwenMoE:
         pend = None      # (peer-written partial of delta, the layer whose flag covers it)
         for i in self.layers:
             if fused:
-                resid, delta, pend, ctx = self._layer_fwd_peer(i, resid, delta, pend, B, S)
+                resid, delta, pend, ctx = self._layer_fwd_peer(i, resid, delta, pend, B, S, seqs, saved["pos"])
             else:
-                resid, delta, ctx = self._layer_fwd(i, resid, delta, B, S)
+                resid, delta, ctx = self._layer_fwd(i, resid, delta, B, S, seqs, saved["pos"])
             saved["layers"].append(ctx)
         if pend is not None and not self.part.has_head:
             self.tp.wait("rMoe", pend[1])          # the next stage needs delta in one tensor
@@ -193,7 +218,10 @@ class QwenMoE:
             lab = labels.reshape(-1).to(torch.int32)
             if self.tp is not None:
                 lab = self.tp.local_rows(lab).contiguous()
-            per_tok = Fn.xent_fwd_bwd(logits, lab, loss_scale)   # logits now hold dlogits
+            if objective is None:
+                per_tok = Fn.xent_fwd_bwd(logits, lab, loss_scale)   # logits now hold dlogits
+            else:
+                per_tok = objective(logits, lab)
             loss_sum = per_tok.sum()
             saved.update(final_h=h, final_rstd=rstd, final_y=y, dlogits=logits)
             out = None
@@ -202,23 +230,47 @@ class QwenMoE:
         self._saved.append(saved)
         return out, loss_sum
 
+    # ------------------------------------------------------------------ attention of equal or packed sequences
+    def _positions(self, T, S, seqs, device):
+        """Rows' positions, or None where ``rope_`` and its tables express them."""
+        if seqs is not None:
+            return seqs.pos
+        return None if self.cfg.plain_rope() else torch.arange(T, dtype=torch.int32, device=device).remainder_(S)
+
+    def _rotate(self, qkv, S, pos, inverse=False):
+        heads = self.hq + self.hkv
+        if pos is None:
+            Fn.rope_(qkv, self.cos, self.sin, S, heads, self.cfg.head_dim, inverse=inverse)
+        else:
+            packed.rotary(qkv, pos, self.rotary, heads, inverse=inverse)
+
+    def _attend(self, qkv, B, S, seqs):
+        if seqs is None:
+            return Fn.attention_fwd(qkv, B, S, self.hq, self.hkv, self.cfg.head_dim, self.scale)
+        return packed.attention_fwd(qkv, seqs, self.hq, self.hkv, self.cfg.head_dim, self.scale)
+
+    def _attend_bwd(self, c, d_o, B, S, seqs):
+        heads = (self.hq, self.hkv, self.cfg.head_dim, self.scale)
+        if seqs is None:
+            return Fn.attention_bwd(c["qkv"], c["o"], c["lse"], d_o, B, S, *heads)
+        return packed.attention_bwd(c["qkv"], c["o"], c["lse"], d_o, seqs, *heads)
+
     def _ag(self, x):
         return self.tp.all_gather(x) if self.tp is not None else x
 
     def _rs(self, x):
         return self.tp.reduce_scatter(x) if self.tp is not None else x
 
-    def _layer_fwd(self, i, resid, delta, B, S):
+    def _layer_fwd(self, i, resid, delta, B, S, seqs=None, pos=None):
         """resid / delta / outputs are this rank's token rows (all rows without TP)."""
         cfg, st = self.cfg, self.store
         p = f"layers.{i}."
-        Hq, Hkv, D = self.hq, self.hkv, cfg.head_dim
         T = B * S
         a_loc, rstd1, h = Fn.rmsnorm_fwd(resid, st.w(p + "ln1.weight"), cfg.eps, delta)
         a_in = self._ag(a_loc)                                  # [T, H]
         qkv = G.linear_fwd(a_in, st.w(p + "attn.qkv"))          # column parallel: local heads
-        Fn.rope_(qkv, self.cos, self.sin, S, Hq + Hkv, D)
-        o, lse = Fn.attention_fwd(qkv, B, S, Hq, Hkv, D, self.scale)
+        self._rotate(qkv, S, pos)
+        o, lse = self._attend(qkv, B, S, seqs)
         attn_out = self._rs(G.linear_fwd(o, st.w(p + "attn.o")))  # row parallel partial -> token rows
         m_loc, rstd2, h2 = Fn.rmsnorm_fwd(h, st.w(p + "ln2.weight"), cfg.eps, attn_out)
         m_in = self._ag(m_loc)
@@ -231,13 +283,12 @@ class QwenMoE:
     def _fused_tp(self) -> bool:
         return self.tp is not None and getattr(self.tp, "fused", False)
 
-    def _layer_fwd_peer(self, i, resid, delta, pend, B, S):
+    def _layer_fwd_peer(self, i, resid, delta, pend, B, S, seqs=None, pos=None):
         """One layer with the TP exchanges inside our kernels (see
         parallel.tp.TPPeer).  resid/delta/outputs are this rank's token rows;
         ``pend`` is (peer partial of delta, layer of its flag) or None."""
         cfg, st, tp = self.cfg, self.store, self.tp
         p = f"layers.{i}."
-        Hq, Hkv, D = self.hq, self.hkv, cfg.head_dim
         T = B * S
         own = tp.own()
         plo, phi = tp.peer_range()
@@ -250,8 +301,8 @@ class QwenMoE:
         # column-parallel QKV: own rows first, the peer's after its flag
         qkv = G.linear_fwd(gA, st.w(p + "attn.qkv"), xchg=tp.xchg(wait=("gA", i)),
                            tp=(plo, phi, tp.rot_own_first(), 0, 0, 0))
-        Fn.rope_(qkv, self.cos, self.sin, S, Hq + Hkv, D)
-        o, lse = Fn.attention_fwd(qkv, B, S, Hq, Hkv, D, self.scale)
+        self._rotate(qkv, S, pos)
+        o, lse = self._attend(qkv, B, S, seqs)
         # row-parallel output projection: the peer's rows go straight to it
         attn_own = torch.empty(T // 2, cfg.hidden, dtype=o.dtype, device=o.device)
         G.linear_fwd(o, st.w(p + "attn.o"), out=attn_own,
@@ -267,14 +318,13 @@ class QwenMoE:
         ctx = dict(h=h, rstd1=rstd1, a_in=gA, qkv=qkv, o=o, lse=lse, h2=h2, rstd2=rstd2, m_in=gM, **mctx)
         return h2, moe_own, (tp.buf("rMoe", i), i), ctx
 
-    def _layer_bwd_peer(self, i, c, B, S, accumulate):
+    def _layer_bwd_peer(self, i, c, B, S, accumulate, seqs=None, pos=None):
         """Backward of _layer_fwd_peer.  The gradient w.r.t. the layer output
         is already in gather buffer gD of layer i (own rows written by our
         producer, the peer's by the peer).  Returns dh (own rows), written
         into gD of layer i-1 (both ranks) when that layer is in this stage."""
         cfg, st, tp = self.cfg, self.store, self.tp
         p = f"layers.{i}."
-        Hq, Hkv, D = self.hq, self.hkv, cfg.head_dim
         T = B * S
         own = tp.own()
         plo, phi = tp.peer_range()
@@ -292,8 +342,8 @@ class QwenMoE:
                                    xchg=tp.xchg(wait=("gH", i)), tp=(plo, phi, 0, 0, 0, 0)))
         d_o = G.linear_dgrad(gH, st.w(p + "attn.o"), xchg=tp.xchg(wait=("gH", i)),
                              tp=(plo, phi, tp.rot_own_first(), 0, 0, 0))
-        dqkv = Fn.attention_bwd(c["qkv"], c["o"], c["lse"], d_o, B, S, Hq, Hkv, D, self.scale)
-        Fn.rope_(dqkv, self.cos, self.sin, S, Hq + Hkv, D, inverse=True)
+        dqkv = self._attend_bwd(c, d_o, B, S, seqs)
+        self._rotate(dqkv, S, pos, inverse=True)
         self._wg(functools.partial(G.linear_wgrad, dqkv, c["a_in"], st.g(p + "attn.qkv"), accumulate))
         da_own = torch.empty(T // 2, cfg.hidden, dtype=dqkv.dtype, device=dqkv.device)
         G.linear_dgrad(dqkv, st.w(p + "attn.qkv"), out=da_own,
@@ -365,9 +415,11 @@ class QwenMoE:
         for idx_l in reversed(range(len(saved["layers"]))):
             i = self.part.layer_lo + idx_l
             if self._fused_tp():
-                dres = self._layer_bwd_peer(i, saved["layers"][idx_l], B, S, accumulate)
+                dres = self._layer_bwd_peer(i, saved["layers"][idx_l], B, S, accumulate, saved["seqs"],
+                                            saved["pos"])
             else:
-                dres = self._layer_bwd(i, saved["layers"][idx_l], dres, B, S, accumulate)
+                dres = self._layer_bwd(i, saved["layers"][idx_l], dres, B, S, accumulate, saved["seqs"],
+                                            saved["pos"])
             self._hook(i)
         if self.part.has_embed:
             tok = saved["tokens"]
@@ -413,11 +465,10 @@ class QwenMoE:
         for fn in q:
             fn()
 
-    def _layer_bwd(self, i, c, dout, B, S, accumulate):
+    def _layer_bwd(self, i, c, dout, B, S, accumulate, seqs=None, pos=None):
         """dout: gradient w.r.t. the layer output h_out = h2 + moe_out."""
         cfg, st = self.cfg, self.store
         p = f"layers.{i}."
-        Hq, Hkv, D = self.hq, self.hkv, cfg.head_dim
         T = B * S
         # ---- MoE (the gradient of a reduce-scatter is an all-gather and vice versa) ----
         dm_in = self._rs(self._moe_bwd(p, c, self._ag(dout), T, accumulate))
@@ -427,8 +478,8 @@ class QwenMoE:
         dattn = self._ag(dh2)
         self._wg(functools.partial(G.linear_wgrad, dattn, c["o"], st.g(p + "attn.o"), accumulate))
         d_o = G.linear_dgrad(dattn, st.w(p + "attn.o"))
-        dqkv = Fn.attention_bwd(c["qkv"], c["o"], c["lse"], d_o, B, S, Hq, Hkv, D, self.scale)
-        Fn.rope_(dqkv, self.cos, self.sin, S, Hq + Hkv, D, inverse=True)
+        dqkv = self._attend_bwd(c, d_o, B, S, seqs)
+        self._rotate(dqkv, S, pos, inverse=True)
         self._wg(functools.partial(G.linear_wgrad, dqkv, c["a_in"], st.g(p + "attn.qkv"), accumulate))
         da = self._rs(G.linear_dgrad(dqkv, st.w(p + "attn.qkv")))
         dh = Fn.rmsnorm_bwd(da, c["h"], c["rstd1"], st.w(p + "ln1.weight"), cfg.eps, st.g(p + "ln1.weight"), dh2,

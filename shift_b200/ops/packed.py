@@ -104,6 +104,8 @@ class Rotary:
             raise ValueError(f"Rotary: layout {layout!r}, expected 'half' or 'interleaved'")
         if not (math.isfinite(theta) and theta > 0):
             raise ValueError(f"Rotary: theta {theta}")
+        if scaling is not None and not isinstance(scaling, RotaryScaling):
+            scaling = RotaryScaling(*scaling)              # as a configuration file gives it
         self.head_dim, self.rot_dim, self.layout, self.theta, self.scaling = head_dim, rot, layout, theta, scaling
         freq, self.magnitude = self._frequencies()
         self.freq = torch.tensor(freq, dtype=torch.float64)
@@ -209,6 +211,8 @@ def attention_bwd(qkv: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: tor
     if out is not None and (out.shape != qkv.shape or out.dtype != qkv.dtype or out.device != qkv.device):
         raise ValueError(f"attention_bwd: out {tuple(qkv.shape)} of {qkv.dtype} beside qkv")
     segs = ref.segments(seqs.offs, seqs.rows)
+    if all(lo == hi for lo, hi in segs):
+        return torch.zeros_like(qkv) if out is None else out
     (g,) = ref.grad_of(lambda x: ref.packed_attention(x, segs, Hq, Hkv, D, scale)[0], [qkv], do.float())
     if out is not None:
         live = seqs.pos >= 0

@@ -203,6 +203,24 @@ def test_sequences_do_not_hear_each_other(D):
         assert torch.isnan(got[0][120:250]).any(1).all()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_masked_values_count_as_nothing_however_large(D):
+    """Other sequences' finite values of 3e38, in shared tiles, leave results as they are to the bit."""
+    offs, rows = [0, 100, 250, 390, 600], 600
+    for heads in ((4, 2), (3, 3)):
+        qkv, do, seqs, heads = _case(offs, rows, *heads, D=D)
+        kv = (heads[0] + heads[1]) * D
+        qkv[100:250] = 0
+        do[100:250] = 0
+        want = _step(qkv, do, seqs, heads)
+        qkv[100:250, kv:], do[100:250, ::3] = 3e38, 3e38
+        got = _step(qkv, do, seqs, heads)
+        check_status()
+        for rows_ in (slice(0, 100), slice(250, 600)):
+            assert torch.equal(got[0][rows_], want[0][rows_]) and torch.equal(got[1][:, rows_], want[1][:, rows_])
+            assert torch.equal(got[2][rows_], want[2][rows_])
+
+
 def test_attention_leaves_rows_of_no_sequence_in_a_given_out():
     offs, rows = [10, 140, 300], 400
     qkv, do, seqs, heads = _case(offs, rows)
