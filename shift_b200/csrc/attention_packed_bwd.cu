@@ -7,9 +7,13 @@
 //
 // The other side comes in blocks of 128, of which each group of softmax warps has 64 columns; S and dP have columns of their
 // own in tensor memory and P and dS have too, so that S and dP of the next block are computed while the groups are still at
-// this one.  (Products of 64 columns cost as much as ones of 128: blocks of 64 that the groups took in turn made the dK / dV
-// pass of heads of 64 1.4 times as slow.)  The dK / dV pass of heads of 128 has no columns left for that: its blocks are of
-// 64, the groups take them in turn, and P and dS lie over S and dP.
+// this one (blocks of 64 that the groups took in turn: 412 us where this takes 335, 8 x 2048 rows, 16 / 4 heads of 64).  The
+// dK / dV pass of heads of 128 has no columns left for that: its blocks are of 64, the groups take them in turn, and P and dS
+// lie over S and dP.
+//
+// At those sizes (heads of 64) the products take 1024 of the 2290 clocks that a 128 x 128 block of the dK / dV pass takes,
+// and 768 of 2180 of the dQ pass; the rest is the chain scores - exponentials - operands of one block.  Four groups of warps
+// instead of two, with 32 columns a thread, take as long.
 #include "attention_packed.cuh"
 
 namespace sb {
@@ -427,9 +431,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 template <int D>
 struct Dq {
   static constexpr int kHalves = D / 64, kTile = kHalves * kChunk;
-  static constexpr int kStages = D == 64 ? 4 : 2, kStage = 2 * kTile;              // K, V of 128 keys
+  // tiles of 128 keys: V is done with after the scores, K after dQ
+  static constexpr int kK = D == 64 ? 4 : 3, kV = D == 64 ? 4 : 2;
   static constexpr int kP = 256 + D;                                               // S | dP | dQ | dS
-  static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + 512;
+  static constexpr int kSmem = 1024 + (2 + kK + kV) * kTile + 512;
 };
 
 struct DqItem {
@@ -454,12 +459,13 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sQ = smem_raw + (((raw + 1023) & ~1023u) - raw);
   uint8_t* sO = sQ + F::kTile;
-  uint8_t* sK = sO + F::kTile;                                  // [stages][K | V]
-  uint4* answer = reinterpret_cast<uint4*>(sK + F::kStages * F::kStage);
+  uint8_t* sK = sO + F::kTile;
+  uint8_t* sV = sK + F::kK * F::kTile;
+  uint4* answer = reinterpret_cast<uint4*>(sV + F::kV * F::kTile);
   uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
   uint64_t *q_full = bar, *q_empty = bar + 1, *land = bar + 2, *acc_full = bar + 3, *acc_free = bar + 4, *drain = bar + 5;
-  uint64_t *in_full = bar + 6, *in_empty = in_full + F::kStages, *s_full = in_empty + F::kStages, *p_full = s_full + 2;
-  uint64_t *s_empty = p_full + 2, *p_free = s_empty + 2;
+  uint64_t *k_full = bar + 6, *k_empty = k_full + F::kK, *v_full = k_empty + F::kK, *v_empty = v_full + F::kV;
+  uint64_t *s_full = v_empty + F::kV, *p_full = s_full + 2, *s_empty = p_full + 2, *p_free = s_empty + 2;
   const Sched sched{answer, p_free + 2, p_free + 4};
   uint32_t* tslot = reinterpret_cast<uint32_t*>(p_free + 6);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -471,9 +477,13 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 8);
     mbar_init(drain, 1);
-    for (int i = 0; i < F::kStages; ++i) {
-      mbar_init(&in_full[i], 1);
-      mbar_init(&in_empty[i], 1);
+    for (int i = 0; i < F::kK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < F::kV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -518,18 +528,22 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
           ++nq;
           ok = __all_sync(0xffffffffu, ok);
           for (int j = it.lo; j < it.hi && ok; ++j, ++g) {
-            const int st = g % F::kStages, row = j * 128;
+            const int sk = g % F::kK, sv = g % F::kV, row = j * 128;
             const bool clear = row < first || min(row + 128, a.T) > last;
-            uint8_t* in = sK + st * F::kStage;
+            uint8_t* in = sK + sk * F::kTile;
             if (lane == 0) {
-              ok = mbar_wait(&in_empty[st], ((g / F::kStages) & 1) ^ 1, a.status);
+              ok = mbar_wait(&k_empty[sk], ((g / F::kK) & 1) ^ 1, a.status);
               if (ok) {
-                uint64_t* to = clear ? land : &in_full[st];
-                mbar_arrive_expect_tx(to, F::kStage);
-                for (int c = 0; c < F::kHalves; ++c) {
+                uint64_t* to = clear ? land : &k_full[sk];
+                mbar_arrive_expect_tx(to, F::kTile);
+                for (int c = 0; c < F::kHalves; ++c)
                   tma_load_2d(in + c * kChunk, &tm, to, (a.Hq + it.kvh) * D + c * 64, row);
-                  tma_load_2d(in + F::kTile + c * kChunk, &tm, to, (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
-                }
+                ok = mbar_wait(&v_empty[sv], ((g / F::kV) & 1) ^ 1, a.status);
+              }
+              if (ok) {
+                mbar_arrive_expect_tx(&v_full[sv], F::kTile);
+                for (int c = 0; c < F::kHalves; ++c)
+                  tma_load_2d(sV + sv * F::kTile + c * kChunk, &tm, &v_full[sv], (a.Hq + a.Hkv + it.kvh) * D + c * 64, row);
               }
             }
             ok = __all_sync(0xffffffffu, ok);
@@ -540,7 +554,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
                 clear_rows(in, 128, F::kHalves, kChunk, row, first, last);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&in_full[st]);
+                if (lane == 0) mbar_arrive(&k_full[sk]);
               }
             }
           }
@@ -549,14 +563,15 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 128, 0), idG = idesc<T>(128, D, 1);
-      const uint64_t dq = kdesc(smem_u32(sQ)), dob = kdesc(smem_u32(sO)), din = kdesc(smem_u32(sK));
-      const uint64_t din_mn = mndesc(smem_u32(sK), kChunk);
+      const uint64_t dq = kdesc(smem_u32(sQ)), dob = kdesc(smem_u32(sO)), dk = kdesc(smem_u32(sK)), dv = kdesc(smem_u32(sV));
+      const uint64_t dk_mn = mndesc(smem_u32(sK), kChunk);
       auto scores = [&](int g) -> bool {
-        const int st = g % F::kStages;
-        if (!mbar_wait(&in_full[st], (g / F::kStages) & 1, a.status)) return false;
+        const int sk = g % F::kK, sv = g % F::kV;
+        if (!mbar_wait(&k_full[sk], (g / F::kK) & 1, a.status)) return false;
+        if (!mbar_wait(&v_full[sv], (g / F::kV) & 1, a.status)) return false;
         if (g >= 1 && !mbar_wait(s_empty, (g - 1) & 1, a.status)) return false;
         tc_fence_after();
-        const uint64_t k = din + st * (F::kStage >> 4), v = k + (F::kTile >> 4);
+        const uint64_t k = dk + sk * (F::kTile >> 4), v = dv + sv * (F::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4, sub = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
@@ -568,6 +583,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
           umma_f16(tbase + 128, dob + off, v + sub, idS, kk > 0);
         }
         umma_commit(s_full);
+        umma_commit(&v_empty[sv]);
         return true;
       };
       if (elect_one()) {
@@ -594,11 +610,11 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
             if (ok && s == 0 && nq > 0) ok = mbar_wait(acc_free, (nq - 1) & 1, a.status);
             if (!ok) break;
             tc_fence_after();
-            const int st = g % F::kStages;
-            const uint64_t k = din_mn + st * (F::kStage >> 4);
+            const int sk = g % F::kK;
+            const uint64_t k = dk_mn + sk * (F::kTile >> 4);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) umma_f16_ts(tdQ, tbase + F::kP + kk * 8, k + kk * (2048 >> 4), idG, s > 0 || kk > 0);
-            umma_commit(&in_empty[st]);
+            umma_commit(&k_empty[sk]);
             umma_commit(p_free);
           }
           if (ok) umma_commit(acc_full);

@@ -1,6 +1,6 @@
 """Kernel micro-benchmarks at the shapes of the 0.494B MoE training step.
 
-    python -m shift_b200.ops.microbench [--ops gemm,attn,mem,fused,fp8] [--iters N]
+    python -m shift_b200.ops.microbench [--ops gemm,attn,mem,fused,fp8,packed] [--iters N]
 
 Each case is timed with CUDA events on the launching stream after warm-up,
 with a synchronize on both sides; inputs of the timed cases are larger than
@@ -333,6 +333,45 @@ def run_fp8(iters, T=16384, H=1024):
     return rows
 
 
+def run_packed(iters, T=16384):
+    """Packed-sequence operators: attention against the bf16 rate (visible pairs only), the rest against the copy
+    bandwidth."""
+    from . import objectives, packed
+    from ._ext import check_status
+    pk = peaks()
+    rows = []
+    for name, length, hq, hkv, d in (("equal", 2048, 16, 4, 64), ("short", 700, 16, 4, 64), ("equal", 2048, 16, 4, 128),
+                                     ("one", T, 32, 8, 128)):
+        ends = list(range(0, T, length)) + [T]
+        seqs = packed.sequences(torch.tensor(ends, dtype=torch.int32, device="cuda"), T)
+        qkv, do, args = bf(T, (hq + 2 * hkv) * d), bf(T, hq * d), (hq, hkv, d, d ** -0.5)
+        o, lse = packed.attention_fwd(qkv, seqs, *args)
+        pairs = sum((b - a) * (b - a + 1) // 2 for a, b in zip(ends, ends[1:])) * hq * d
+        for kind, fn, flops in (("fwd", lambda: packed.attention_fwd(qkv, seqs, *args), 4 * pairs),
+                                ("bwd", lambda: packed.attention_bwd(qkv, o, lse, do, seqs, *args), 10 * pairs)):
+            t = timeit(fn, iters)
+            rows.append({"case": f"packed.attention_{kind} {name} {len(ends) - 1}x{length} {hq}/{hkv}x{d}", "ms": round(t, 4),
+                         "tflops": round(flops / t / 1e9, 1), "frac_of_peak": round(flops / t / 1e9 / pk["bf16_tflops"], 3)})
+
+    def mem(name, fn, nbytes):
+        t = timeit(fn, iters)
+        rows.append({"case": name, "ms": round(t, 4), "gbs": round(nbytes / t / 1e6, 1),
+                     "frac_of_peak": round(nbytes / t / 1e6 / pk["hbm_gbs"], 3)})
+
+    plan, pos, x = packed.Rotary(64, 1.0e6), torch.arange(T, dtype=torch.int32, device="cuda"), bf(T, 24 * 64)
+    mem(f"packed.rotary {T}x20x64 in place", lambda: packed.rotary(x, pos, plan, 20), T * 20 * 64 * 4)
+    V = 32768
+    z, labels = bf(T, V), torch.randint(0, V, (T,), dtype=torch.int32, device="cuda")
+    old, adv = torch.full((T,), -10.0, device="cuda"), torch.randn(T, device="cuda")
+    offs = torch.arange(0, T + 1, T // 32, dtype=torch.int32, device="cuda")
+    mem(f"objectives.token_logp_fwd {T}x{V}", lambda: objectives.token_logp_fwd(z, labels), T * V * 2)
+    mem(f"objectives.policy_loss {T}x{V}", lambda: objectives.policy_loss_fwd_bwd(z, labels, old, adv), T * V * 4)
+    mem(f"objectives.preference_loss {T}x{V}", lambda: objectives.preference_loss_fwd_bwd(z, labels, old, offs), T * V * 6)
+    torch.cuda.synchronize()
+    check_status()
+    return rows
+
+
 def main():
     p = argparse.ArgumentParser()
     p.add_argument("--ops", default="gemm,attn,mem")
@@ -355,6 +394,8 @@ def main():
         out["fused"] = run_fused(args.iters)
     if "fp8" in ops:
         out["fp8"] = run_fp8(args.iters)
+    if "packed" in ops:
+        out["packed"] = run_packed(args.iters)
     for k, v in out.items():
         if isinstance(v, list):
             for r in v:
