@@ -257,7 +257,20 @@ SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // -lse, -d
   return a.rows + (static_cast<long>(h) * (a.tiles * 2) + q / 64) * 128 + q % 64;
 }
 
-// One row of dQ, columns [c0, c1).
+// What dS is multiplied by before it is rounded to T, as a power of two's exponent: fp16 would lose the small gradients of a
+// long row (do of 1e-4 over 1000 keys: dS near 1e-6, where its steps are 6e-8) and overflow with large ones.  do times it
+// has its largest value in [1, 2).  Nothing for bf16, which has fp32's range.
+template <typename T>
+SB_DEVICE int ds_shift(const Args& a);
+template <>
+SB_DEVICE int ds_shift<__nv_bfloat16>(const Args&) { return 0; }
+template <>
+SB_DEVICE int ds_shift<__half>(const Args& a) {
+  const int e = *a.largest >> 23;                      // 0: no gradient, 255: an infinite one
+  return e == 0 || e == 255 ? 0 : max(-100, min(100, 127 - e));
+}
+
+// Columns [c0, c1) of one row of dQ.
 template <int D, typename T>
 __device__ __noinline__ void slow_dq(const Args& a, int row, int h, int st, int c0, int c1) {
   constexpr int N = D / 32;

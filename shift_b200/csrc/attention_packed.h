@@ -28,6 +28,7 @@ struct Args {
   void* dqkv;
   long dqkv_ld;
   float* partial;             // split > 1: fp32 [split][Hkv][T][2 D]
+  int* largest;               // backward, fp16: bits of the largest |do|, else null
   int fill;                   // rows that no sequence covers get zeros
   int* status;
 };

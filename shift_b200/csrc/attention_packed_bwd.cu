@@ -29,20 +29,33 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args 
   const long i = static_cast<long>(blockIdx.x) * (256 / L) + threadIdx.x / L;
   const int sub = threadIdx.x % L, h = static_cast<int>(i % a.Hq);
   const long row = i / a.Hq;
-  if (row >= static_cast<long>(a.tiles) * 128) return;         // whole groups of L lanes; a warp's last group shuffles alone
+  const bool there = row < static_cast<long>(a.tiles) * 128;   // the same in all L lanes of a group
   const unsigned lanes = (L == 8 ? 0xffu : 0xffffu) << (threadIdx.x % 32 / L * L);
-  float s = 0.f, nl = 0.f;
-  if (row < a.T && a.start[row] <= row) {
+  float s = 0.f, nl = 0.f, top = 0.f;
+  if (there && row < a.T && a.start[row] <= row) {
     const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D + sub * 8);
     const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D + sub * 8);
     const T *x = reinterpret_cast<const T*>(&u), *y = reinterpret_cast<const T*>(&g);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += to_float(x[k]) * to_float(y[k]);
+    for (int k = 0; k < 8; ++k) {
+      s += to_float(x[k]) * to_float(y[k]);
+      top = fmaxf(top, fabsf(to_float(y[k])));
+    }
     nl = -a.lse[static_cast<long>(h) * a.T + row] * kLog2e;
   }
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(lanes, s, o);
-  if (sub == 0) {
+  if (a.largest != nullptr) {                        // one atomic a CTA; a maximum does not hang on their order
+    __shared__ float tops[8];
+    top = warp_max(top);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) top = fmaxf(top, tops[w]);
+      atomicMax(a.largest, __float_as_int(top));
+    }
+  }
+  if (there && sub == 0) {
     float* p = out + (static_cast<long>(h) * (a.tiles * 2) + row / 64) * 128 + row % 64;
     p[0] = nl;
     p[64] = -s;
@@ -260,6 +273,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     const uint32_t ts = tbase + w * (F::kWide ? 64 : 128) + lane_off;
     const uint32_t tp = tbase + F::kP + w * (F::kWide ? 32 : 128) + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    const int shift = ds_shift<T>(a);
+    const float2 up = make_float2(ldexpf(1.f, shift), ldexpf(1.f, shift));
     int g = 0, nkv = 0;
     bool ok = true, in_ready = false, s_ready = false;
     DkvItem it(a, blockIdx.x, F::kW);
@@ -308,6 +323,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
               z[u] = (k / 2 + u) % 8 < kOnFma ? ex2_fma(z[u]) : make_float2(ex2(z[u].x), ex2(z[u].y));
               e[u] = mul2(e[u], z[u]);
               pp[k / 2 + u] = Half<T>::pack(z[u].x, z[u].y);
+              if constexpr (Half<T>::kFormat == 0) e[u] = mul2(e[u], up);
               pd[k / 2 + u] = Half<T>::pack(e[u].x, e[u].y);
             }
           }
@@ -356,7 +372,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         }
         ++nkv;
         tc_fence_after();
-        const float f = dk ? a.scale : 1.f;
+        const float f = dk ? ldexpf(a.scale, -shift) : 1.f;
         float chk = 0.f;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -633,6 +649,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tbase + w * 64 + lane_off, tp = tbase + F::kP + w * 32 + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    const int shift = ds_shift<T>(a);                  // of dS: in its exponential's argument
+    const float out_scale = ldexpf(a.scale, -shift);
     int g = 0, nq = 0;
     bool ok = true, s_ready = false;
     DqItem it(a, blockIdx.x);
@@ -641,7 +659,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       const int st = row < a.T ? a.start[row] : row + 1;
       const int most = a.start[min(it.q0 + 127, a.T - 1)];
       const float* rb = row_block(a, it.h, row);       // there are rows up to a multiple of 128
-      const float2 nl = make_float2(rb[0], rb[0]), nd = make_float2(rb[64], rb[64]);
+      const float2 nl = make_float2(rb[0] + shift, rb[0] + shift), nd = make_float2(rb[64], rb[64]);
       for (int j = it.lo; j < it.hi; ++j, ++g) {
         if (!warp_wait(s_full, g & 1, a.status, s_ready)) {
           ok = false;
@@ -723,7 +741,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
             uint32_t y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float y0 = __uint_as_float(o[k + 2 * e]) * a.scale, y1 = __uint_as_float(o[k + 2 * e + 1]) * a.scale;
+              const float y0 = __uint_as_float(o[k + 2 * e]) * out_scale, y1 = __uint_as_float(o[k + 2 * e + 1]) * out_scale;
               chk = fmaf(y0, 0.f, fmaf(y1, 0.f, chk));
               y[e] = Half<T>::pack(y0, y1);
             }

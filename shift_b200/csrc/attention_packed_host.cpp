@@ -6,6 +6,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "apart.h"
 #include "attention_packed.h"
 
 namespace sb {
@@ -106,7 +107,10 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& plan, int64
   Args a = base_args(qkv, plan, rows, Hq, Hkv, D, scale, status, who, pl);
   const at::cuda::CUDAGuard guard(qkv.device());
   auto o = out.has_value() ? *out : at::empty({a.T, Hq * D}, qkv.options());
-  if (out.has_value()) check_rows(o, qkv, a.T, Hq * D, who, "out");
+  if (out.has_value()) {
+    check_rows(o, qkv, a.T, Hq * D, who, "out");
+    TORCH_CHECK(!share_memory(o, qkv), who, ": out overlaps qkv");
+  }
   auto lse = at::empty({Hq, a.T}, qkv.options().dtype(at::kFloat));
   if (a.T == 0) return {o, lse};
   a.fill = out.has_value() ? 0 : 1;
@@ -138,7 +142,11 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
               who, ": lse [", Hq, ", ", a.T, "] fp32, contiguous, beside qkv");
   const at::cuda::CUDAGuard guard(qkv.device());
   auto dqkv = out.has_value() ? *out : at::empty({a.T, (Hq + 2 * Hkv) * D}, qkv.options());
-  if (out.has_value()) check_rows(dqkv, qkv, a.T, (Hq + 2 * Hkv) * D, who, "out");
+  if (out.has_value()) {
+    check_rows(dqkv, qkv, a.T, (Hq + 2 * Hkv) * D, who, "out");
+    TORCH_CHECK(!share_memory(dqkv, qkv) && !share_memory(dqkv, o) && !share_memory(dqkv, dout), who,
+                ": out overlaps qkv, o or do");
+  }
   if (a.T == 0) return dqkv;
   a.fill = out.has_value() ? 0 : 1;
   a.o = o.data_ptr();
@@ -149,6 +157,11 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
   a.dqkv = dqkv.data_ptr();
   a.dqkv_ld = row_stride(dqkv);
   auto row_values = at::empty({Hq * a.tiles * 256}, lse.options());
+  at::Tensor largest;
+  if (qkv.scalar_type() == at::kHalf) {              // fp16 holds dS over some 2^30: it is scaled by the largest |do|
+    largest = at::zeros({1}, lse.options().dtype(at::kInt));
+    a.largest = largest.data_ptr<int>();
+  }
   // A key tile meets every later query of its sequence in every head of its group: with few tiles the group's heads are
   // dealt out over several CTAs, whose fp32 sums are added up in order afterwards.
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

@@ -9,6 +9,7 @@
 
 #include <limits>
 
+#include "apart.h"
 #include "common.cuh"
 #include "lowp.cuh"
 
@@ -296,14 +297,7 @@ void rotary(const at::Tensor& x, at::Tensor& out, const at::Tensor& pos, const a
     TORCH_CHECK((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
                 "rotary: rows of stride 1 inside that do not overlap");
   const bool same = x.data_ptr() == out.data_ptr() && (x.size(0) <= 1 || x.stride(0) == out.stride(0));
-  if (!same && x.numel() > 0) {
-    auto range = [](const at::Tensor& t) {
-      const char* p = static_cast<const char*>(t.data_ptr());
-      return std::make_pair(p, p + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size());
-    };
-    const auto a = range(x), b = range(out);
-    TORCH_CHECK(a.second <= b.first || b.second <= a.first, "rotary: out overlaps x and is not x itself");
-  }
+  TORCH_CHECK(same || !share_memory(x, out), "rotary: out overlaps x and is not x itself");
   if (x.size(0) == 0 || heads == 0) return;
   const at::cuda::CUDAGuard guard(x.device());
   RotaryArgs a{x.data_ptr(), out.data_ptr(), pos.data_ptr<int>(),

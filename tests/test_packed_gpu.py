@@ -265,3 +265,19 @@ def test_attention_of_large_scores(dtype):
     want = orc.attention(qkv, offs, Hq, Hkv, D, D ** -0.5)
     orc.close(o, want["o"], want["o_tol"], "o")
     orc.close(lse, want["lse"], 1e-5 * (1 + want["lse"].abs()), "lse")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** 9])
+def test_fp16_gradients_of_any_size(size, D):
+    """dS of a long row is near 2^-20 of do's size, below what fp16 holds well, or above what it holds at all."""
+    rows, heads = 1500, (2, 1, D, D ** -0.5)
+    qkv, do = _randn(rows, 4 * D, seed=11, dtype=torch.float16), _randn(rows, 2 * D, seed=12, dtype=torch.float16) * size
+    got = _step(qkv, do, _seqs([0, rows], rows), heads)[2].double()
+    check_status()
+    want = orc.attention(qkv, [0, rows], *heads, do)["dqkv"]
+    for cols in (slice(0, 2 * D), slice(2 * D, 3 * D), slice(3 * D, None)):
+        w = want[:, cols]
+        # roundings of P, dS and the result, 2^-11 each of a value of random sign, and the result's own smallest step
+        bound = 3 * 2.0 ** -11 * w.norm() + 2.0 ** -25 * w.numel() ** 0.5
+        assert (got[:, cols] - w).norm() <= bound

@@ -64,6 +64,8 @@ def test_refusals():
         lambda: packed.attention_bwd(qkv, o, lse, o[:, :64], seqs, 2, 1, 64, 1.0),
         lambda: packed.attention_bwd(qkv, o, lse, o.half(), seqs, 2, 1, 64, 1.0),
         lambda: packed.attention_bwd(qkv, o, lse, o, seqs, 2, 1, 64, 1.0, out=o),
+        lambda: packed.attention_bwd(qkv, o, lse, o, seqs, 2, 1, 64, 1.0, out=qkv),
+        lambda: packed.attention_fwd(qkv, seqs, 2, 1, 64, 1.0, out=qkv[:, 64:192]),
         lambda: ob.token_logp_fwd(z.double(), labels),
         lambda: ob.token_logp_fwd(z, labels.long()),
         lambda: ob.token_logp_fwd(z, labels[:5]),
@@ -84,6 +86,22 @@ def test_refusals():
             pytest.fail(f"case {k} was not refused")
     torch.cuda.synchronize()
     check_status()
+
+
+def test_columns_of_one_buffer_side_by_side():
+    """Views of a buffer's rows that lie next to each other are not refused as overlapping."""
+    seqs = packed.sequences(_offs(0, 40, 90), 90)
+    wide = _randn(90, 256 + 128 + 256)
+    qkv, o, g = wide[:, :256], wide[:, 256:384], wide[:, 384:]
+    do = _randn(90, 128, seed=1)
+    want, lse = packed.attention_fwd(qkv.contiguous(), seqs, 2, 1, 64, 0.125)
+    packed.attention_fwd(qkv, seqs, 2, 1, 64, 0.125, out=o)
+    packed.attention_bwd(qkv, o, lse, do, seqs, 2, 1, 64, 0.125, out=g)
+    assert torch.equal(o, want)
+    assert torch.equal(g, packed.attention_bwd(qkv.contiguous(), want, lse, do, seqs, 2, 1, 64, 0.125))
+    plan = packed.Rotary(64)
+    packed.rotary(qkv, seqs.pos, plan, 3, out=g)
+    assert torch.equal(g[:, :192], packed.rotary(qkv.clone(), seqs.pos, plan, 3)[:, :192])
 
 
 # ----------------------------------------------------------------------------- streams and graphs
