@@ -9,9 +9,9 @@ from shift_b200.ops import objectives as ob
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-# A term of a row's sum is an exponential (2^-22), and every time its running maximum rises or two runs are joined (once a
-# thread, 5 times over the lanes, once over the warps and once over the cluster) it is scaled by another one: 9 x 2^-22,
-# and a few fp32 roundings of 2^-24 with them, less than 2^-18.5 of the sum, so of lse and logp in absolute terms.
+# A term of a row's sum is an exponential (2^-22, and the rounding of its argument), scaled by another one each time its
+# thread's running maximum rises and once when the threads' sums are joined: at most ten of them with fp32 roundings of 2^-24
+# between, less than 2^-18.5 of the sum, so of lse and logp in absolute terms.
 SUM = 2.0 ** -18.5
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
 SIZES = [(1, 1), (3, 7), (5, 64), (2, 1021), (17, 4096), (1, 32768), (200, 2056), (3, 100003), (2, 262144), (149, 9)]
