@@ -232,9 +232,9 @@ SB_DEVICE float dot(const float* a, const float* b) {
   return warp_sum(s);
 }
 
-// One row of O by a whole warp, from what the row sees alone.
+// Columns [c0, c1) of one row of O by a whole warp, from what the row sees alone.
 template <int D, typename T>
-__device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float lse2) {
+__device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float lse2, int c0, int c1) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x % 32;
   const T* x = static_cast<const T*>(a.qkv);
@@ -248,9 +248,10 @@ __device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] += p * v[i];
   }
-  T* out = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D + lane * N;
+  T* out = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D;
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = from_float<T>(acc[i]);
+  for (int i = 0; i < N; ++i)
+    if (lane * N + i >= c0 && lane * N + i < c1) out[lane * N + i] = from_float<T>(acc[i]);
 }
 
 SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // -lse, -delta of query q (64 apart)

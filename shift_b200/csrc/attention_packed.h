@@ -10,6 +10,7 @@ namespace pa {
 struct Args {
   int T, Hq, Hkv, group;
   int pair_heads;             // forward: an item is two heads over 128 queries (they share keys); else 256 queries of a head
+  int split_keys;             // forward: an item is one tile of a head, its key blocks dealt out to the two groups
   int split;                  // dK / dV: CTAs that share a key tile's query heads
   int tiles;
   const int* start;

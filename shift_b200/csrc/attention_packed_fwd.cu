@@ -10,25 +10,32 @@ namespace pa {
 //   softmax  a thread's whole row of S to registers, running maximum and sum, P back to tensor memory
 // Heads of 64: S, P and O of both tiles have columns of their own (2 x (128 + 64 + 64)), so the next S is computed while a
 // group is still at its exponentials.  Heads of 128: P lies over S (2 x (128 + 128)).
-template <int D>
+//
+// SPLIT: with few tiles (launch rule in attention_packed_host.cpp) the two tiles are one: group w has every second key block
+// of it, from the w-th, and the two partial results are joined at the end, half of the columns a group.  An item then takes
+// half of its blocks' time, which is what counts when every SM has one or two.
+template <int D, bool SPLIT>
 struct Fwd {
   static constexpr int kHalves = D / 64, kTile = kHalves * kChunk;
   static constexpr int kK = D == 64 ? 4 : 3, kV = D == 64 ? 4 : 2;     // stages
   static constexpr bool kOver = D == 128;                              // P over S
-  static constexpr int kSmem = 1024 + 2 * kTile + (kK + kV) * kTile + 512;
+  static constexpr int kQ = SPLIT ? 1 : 2;                             // tiles of Q
+  static constexpr int kSmem = 1024 + (kQ + kK + kV) * kTile + 512 + (SPLIT ? 2 * 2 * 128 * 8 : 0);
   static constexpr int kP = kOver ? 0 : 256, kPStep = kOver ? 128 : 64, kO = kOver ? 256 : 384;
 };
 
+template <bool SPLIT>
 struct FwdItem {
   int h[2], q0[2], lo[2], hi[2], all_lo, all_hi, kvh;
   SB_DEVICE FwdItem(const Args& a, int idx) {
-    const int per = a.pair_heads ? a.Hq / 2 : a.Hq;
+    const bool pair = !SPLIT && a.pair_heads;
+    const int per = pair ? a.Hq / 2 : a.Hq;
     const int t = a.order[idx / per], r = idx % per;
     const int first = a.ends[0], last = a.ends[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      h[i] = a.pair_heads ? 2 * r + i : r;
-      q0[i] = a.pair_heads ? t * 128 : t * 256 + i * 128;
+      h[i] = pair ? 2 * r + i : r;
+      q0[i] = SPLIT || pair ? t * 128 : t * 256 + i * 128;
       lo[i] = hi[i] = 0;
       if (q0[i] < a.T && q0[i] < last && q0[i] + 128 > first) {
         lo[i] = a.start[q0[i]] / 128;
@@ -40,26 +47,32 @@ struct FwdItem {
     all_hi = max(hi[0], hi[1]);
     kvh = h[0] / a.group;
   }
-  SB_DEVICE bool has(int i, int j) const { return j >= lo[i] && j < hi[i]; }
+  SB_DEVICE bool has(int i, int j) const { return j >= lo[i] && j < hi[i] && (!SPLIT || ((j - lo[i]) & 1) == i); }
+  SB_DEVICE bool first(int i, int j) const { return j == lo[i] + (SPLIT ? i : 0); }
+  SB_DEVICE bool last(int i, int j) const { return j + (SPLIT ? 2 : 1) >= hi[i]; }
+  SB_DEVICE bool any(int i) const { return hi[i] > lo[i] + (SPLIT ? i : 0); }
 };
 
 constexpr int kOnFma = 3;      // of 8 exponentials, those computed on the FMA pipe
 
-template <int D, typename T>
+template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Args a) {
-  using F = Fwd<D>;
+  using F = Fwd<D, SPLIT>;
+  using FwdItem = FwdItem<SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sQ = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  uint8_t* sK = sQ + 2 * F::kTile;
+  uint8_t* sK = sQ + F::kQ * F::kTile;
   uint8_t* sV = sK + F::kK * F::kTile;
-  uint4* answer = reinterpret_cast<uint4*>(sV + F::kV * F::kTile);
+  float2* s_ml = reinterpret_cast<float2*>(sV + F::kV * F::kTile);           // SPLIT: [item parity][group][row] (m, l)
+  uint4* answer = reinterpret_cast<uint4*>(s_ml + (SPLIT ? 2 * 2 * 128 : 0));
   uint64_t* bar = reinterpret_cast<uint64_t*>(answer + 2);
   uint64_t *q_full = bar, *q_empty = bar + 1, *land = bar + 2, *k_full = bar + 3, *k_empty = k_full + F::kK;
   uint64_t *v_full = k_empty + F::kK, *v_empty = v_full + F::kV, *s_full = v_empty + F::kV, *s_empty = s_full + 2;
   uint64_t *p_full = s_empty + 2, *o_full = p_full + 2, *o_free = o_full + 2, *drain = o_free + 2;
   const Sched sched{answer, drain + 1, drain + 3};
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 5);
+  uint64_t* ml_full = drain + 5;                       // SPLIT: a group's maxima and sums
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 7);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -80,7 +93,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       mbar_init(&s_empty[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
-      mbar_init(&o_free[i], 4);
+      mbar_init(&o_free[i], SPLIT ? 8 : 4);
+      mbar_init(&ml_full[i], 4);
       mbar_init(&sched.full[i], 1);
       mbar_init(&sched.empty[i], kReaders);
     }
@@ -110,8 +124,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           if (lane == 0) {
             ok = mbar_wait(q_empty, (nq & 1) ^ 1, a.status);
             if (ok) {
-              mbar_arrive_expect_tx(q_full, 2 * F::kTile);
-              for (int i = 0; i < 2; ++i)
+              mbar_arrive_expect_tx(q_full, F::kQ * F::kTile);
+              for (int i = 0; i < F::kQ; ++i)
                 for (int c = 0; c < F::kHalves; ++c)
                   tma_load_2d(sQ + i * F::kTile + c * kChunk, &tm, q_full, it.h[i] * D + c * 64, it.q0[i]);
             }
@@ -156,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       // all of shared memory lies below 256 KB: adding to a descriptor's address field (16-byte units) never carries out
       const uint64_t dq = kdesc(smem_u32(sQ)), dk = kdesc(smem_u32(sK)), dv = mndesc(smem_u32(sV), kChunk);
       auto issue_s = [&](int i, int sk) {              // S_i of the key block in stage sk
-        const uint64_t q = dq + i * (F::kTile >> 4), k = dk + sk * (F::kTile >> 4);
+        const uint64_t q = dq + (SPLIT ? 0 : i) * (F::kTile >> 4), k = dk + sk * (F::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
@@ -202,38 +216,43 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
             if (j == it.all_hi - 1) umma_commit(q_empty);
           };
           int np[2] = {nb[0], nb[1]};                  // blocks whose P was used
-          if (ok) ok = keys();
-          for (int i = 0; i < 2 && ok; ++i)
-            if (it.has(i, it.all_lo)) ok = scores(it.all_lo, i);
-          if (ok) keys_done(it.all_lo);
+          // scores are issued one block ahead, SPLIT two (one for each group)
+          constexpr int kAhead = SPLIT ? 2 : 1;
+          for (int j = it.all_lo; j < min(it.all_lo + kAhead, it.all_hi) && ok; ++j) {
+            ok = keys();
+            for (int i = 0; i < 2 && ok; ++i)
+              if (it.has(i, j)) ok = scores(j, i);
+            if (ok) keys_done(j);
+          }
           for (int j = it.all_lo; j < it.all_hi && ok; ++j) {
-            const bool more = j + 1 < it.all_hi;
+            const int next = j + kAhead;
+            const bool more = next < it.all_hi;
             if (more) ok = keys();
             if (!F::kOver && more) {
               for (int i = 0; i < 2 && ok; ++i)
-                if (it.has(i, j + 1)) ok = scores(j + 1, i);
-              if (ok) keys_done(j + 1);
+                if (it.has(i, next)) ok = scores(next, i);
+              if (ok) keys_done(next);
             }
             const int sv = nv % F::kV;
-            if (ok && !more) look_ahead();
+            if (ok && j + 1 == it.all_hi) look_ahead();
             if (ok) ok = mbar_wait(&v_full[sv], (nv / F::kV) & 1, a.status);
             for (int i = 0; i < 2 && ok; ++i) {
               if (it.has(i, j)) {
                 ok = mbar_wait(&p_full[i], np[i] & 1, a.status);
                 ++np[i];
-                if (ok && j == it.lo[i] && no[i] > 0) ok = mbar_wait(&o_free[i], (no[i] - 1) & 1, a.status);
+                if (ok && it.first(i, j) && no[i] > 0) ok = mbar_wait(&o_free[i], (no[i] - 1) & 1, a.status);
                 if (!ok) break;
                 tc_fence_after();
-                issue_o(i, sv, j == it.lo[i], j == it.hi[i] - 1);
+                issue_o(i, sv, it.first(i, j), it.last(i, j));
               }
-              if (F::kOver && more && it.has(i, j + 1)) ok = scores(j + 1, i);
+              if (F::kOver && more && it.has(i, next)) ok = scores(next, i);
             }
             if (!ok) break;
             umma_commit(&v_empty[sv]);
             ++nv;
-            if (F::kOver && more) keys_done(j + 1);
+            if (F::kOver && more) keys_done(next);
           }
-          for (int i = 0; i < 2; ++i) no[i] += it.hi[i] > it.lo[i];
+          for (int i = 0; i < 2; ++i) no[i] += it.any(i);
         }
         it = following;
       }
@@ -250,13 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     const uint32_t to = tbase + F::kO + w * D + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
     int nb = 0, items = 0;
+    int live = 0, other_nb = 0, other_items = 0;       // SPLIT: items with blocks; the other group's blocks and items
     bool ok = true, s_ready = false;
-    struct Mine {                                      // this group's tile
+    constexpr int kStep = SPLIT ? 2 : 1;
+    struct Mine {                                      // this group's tile: blocks lo, lo + kStep ... below hi
       int h, q0, lo, hi, row, st, most;
       SB_DEVICE Mine(const Args& a, int idx, int w) {
         const FwdItem it(a, idx);
         q0 = w ? it.q0[1] : it.q0[0];
-        lo = w ? it.lo[1] : it.lo[0];
+        lo = w ? it.lo[1] + (SPLIT ? 1 : 0) : it.lo[0];
         hi = w ? it.hi[1] : it.hi[0];
         h = w ? it.h[1] : it.h[0];
         row = q0 + threadIdx.x % 128;
@@ -268,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int h = now.h, q0 = now.q0, lo = now.lo, hi = now.hi, row = now.row, st = now.st, most = now.most;
       float m = -INFINITY, l = 0.f;
-      for (int j = lo; j < hi; ++j, ++nb) {
+      for (int j = lo; j < hi; j += kStep, ++nb) {
         if (!warp_wait(&s_full[w], nb & 1, a.status, s_ready)) {
           ok = false;
           break;
@@ -346,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           }
           tmem_st_32x32b_x16(tp + c / 2, pk);
         }
-        s_ready = j + 1 < hi && mbar_test(&s_full[w], (nb + 1) & 1);
+        s_ready = j + kStep < hi && mbar_test(&s_full[w], (nb + 1) & 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -360,26 +381,68 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       const bool covered = row < a.T && st <= row;
       float lse2 = -INFINITY;
       bool bad = false;
+      constexpr int kCols = SPLIT ? D / 2 : D;         // columns of O that this group stores, from c0
+      const int c0 = SPLIT ? w * kCols : 0;
       T* orow = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D;
-      if (hi > lo) {
-        if (!warp_wait(&o_full[w], (F::kOver ? items : nb - 1) & 1, a.status)) {
-          ok = false;
-          break;
+      const bool mine = hi > lo, theirs = SPLIT && hi > lo + (w ? -1 : 1);         // who has blocks
+      if (mine || theirs) {
+        float f = 1.f, g = 0.f, top = m;               // factors of this group's O and of the other's
+        if (SPLIT) {
+          s_ml[(live & 1) * 256 + w * 128 + threadIdx.x % 128] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ml_full[w]);
+          // what the other group waited for before it came here tells which phase its O's barrier is in
+          if (!warp_wait(&ml_full[w ^ 1], live & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          const float2 other = s_ml[(live & 1) * 256 + (w ^ 1) * 128 + threadIdx.x % 128];
+          ++live;
+          top = fmaxf(m, other.x);
+          f = m == -INFINITY ? 0.f : ex2(m - top);
+          g = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+          l = l * f + other.y * g;
+          if (theirs) {
+            other_nb += (hi - (w ? lo - 1 : lo + 1) + 1) / 2;
+            if (!warp_wait(&o_full[w ^ 1], (F::kOver ? other_items : other_nb - 1) & 1, a.status)) {
+              ok = false;
+              break;
+            }
+            ++other_items;
+          }
         }
-        ++items;
+        if (mine) {
+          if (!warp_wait(&o_full[w], (F::kOver ? items : nb - 1) & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          ++items;
+        }
         tc_fence_after();
         const float inv = 1.f / l;
         float chk = 0.f;
-        lse2 = m + log2f(l);
+        lse2 = top + log2f(l);
+        const uint32_t from = tbase + F::kO + lane_off + c0;
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < kCols; c += 32) {
           uint32_t o[32];
-          tmem_ld_32x32b_x32(to + c, o);
-          tmem_wait_ld();
-          if (c + 32 == D) {
+          if (SPLIT) {
+            uint32_t p[32];
+            if (mine) tmem_ld_32x32b_x32(from + w * D + c, o);
+            if (theirs) tmem_ld_32x32b_x32(from + (w ^ 1) * D + c, p);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k)               // O without a block is not there, not even as zeros
+              o[k] = __float_as_uint((mine ? __uint_as_float(o[k]) * f : 0.f) + (theirs ? __uint_as_float(p[k]) * g : 0.f));
+          } else {
+            tmem_ld_32x32b_x32(from + w * D + c, o);
+            tmem_wait_ld();
+          }
+          if (c + 32 == kCols) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[w]);
+            if (lane == 0 && mine) mbar_arrive(&o_free[w]);
+            if (lane == 0 && theirs) mbar_arrive(&o_free[w ^ 1]);
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
@@ -390,21 +453,21 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
               chk = fmaf(y0, 0.f, fmaf(y1, 0.f, chk));
               y[e] = Half<T>::pack(y0, y1);
             }
-            if (covered) *reinterpret_cast<uint4*>(orow + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
+            if (covered) *reinterpret_cast<uint4*>(orow + c0 + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
           }
         }
         bad = covered && chk != 0.f && fabsf(lse2) < INFINITY;
       }
       if (row < a.T) {
-        a.lse[static_cast<long>(h) * a.T + row] = covered ? lse2 * kLn2 : -INFINITY;
+        if (!SPLIT || w == 0) a.lse[static_cast<long>(h) * a.T + row] = covered ? lse2 * kLn2 : -INFINITY;
         if (!covered && a.fill)
 #pragma unroll
-          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < kCols; c += 8) *reinterpret_cast<uint4*>(orow + c0 + c) = make_uint4(0, 0, 0, 0);
       }
       for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
         const int who = __ffs(some) - 1;
         slow_o<D, T>(a, __shfl_sync(0xffffffffu, row, who), h, __shfl_sync(0xffffffffu, st, who),
-                     __shfl_sync(0xffffffffu, lse2, who));
+                     __shfl_sync(0xffffffffu, lse2, who), c0, c0 + kCols);
       }
     }
   }
@@ -414,15 +477,21 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
   if (warp == kIssuer) tmem_dealloc(tbase, 512);
 }
 
-template <int D, typename T>
+template <int D, typename T, bool SPLIT>
 static void launch(const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
-  cudaFuncSetAttribute(fwd_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fwd<D>::kSmem);
-  fwd_kernel<D, T><<<items, kThreads, Fwd<D>::kSmem, stream>>>(tm, a);
+  using F = Fwd<D, SPLIT>;
+  cudaFuncSetAttribute(fwd_kernel<D, T, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  fwd_kernel<D, T, SPLIT><<<items, kThreads, F::kSmem, stream>>>(tm, a);
+}
+
+template <typename T>
+static void launch_typed(int D, const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
+  if (D == 64) a.split_keys ? launch<64, T, true>(tm, a, items, stream) : launch<64, T, false>(tm, a, items, stream);
+  else a.split_keys ? launch<128, T, true>(tm, a, items, stream) : launch<128, T, false>(tm, a, items, stream);
 }
 
 void launch_fwd(int D, bool half, const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
-  if (D == 64) half ? launch<64, __half>(tm, a, items, stream) : launch<64, __nv_bfloat16>(tm, a, items, stream);
-  else half ? launch<128, __half>(tm, a, items, stream) : launch<128, __nv_bfloat16>(tm, a, items, stream);
+  half ? launch_typed<__half>(D, tm, a, items, stream) : launch_typed<__nv_bfloat16>(D, tm, a, items, stream);
 }
 
 }  // namespace pa

@@ -120,8 +120,12 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& plan, int64
   // Two heads of one key head share every key block and have the same causal cost; without such pairs two consecutive
   // tiles of a head do.
   a.pair_heads = a.group % 2 == 0;
-  a.order = a.pair_heads ? pl.q_order : pl.q2_order;
-  const unsigned items = static_cast<unsigned>(a.pair_heads ? a.tiles * (Hq / 2) : (a.T + 255) / 256 * Hq);
+  // With at most two tiles an SM an item is one tile, whose key blocks the two groups share.
+  a.split_keys = a.tiles * Hq <= 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  a.order = a.split_keys || a.pair_heads ? pl.q_order : pl.q2_order;
+  const unsigned items = static_cast<unsigned>(a.split_keys     ? a.tiles * Hq
+                                               : a.pair_heads ? a.tiles * (Hq / 2)
+                                                              : (a.T + 255) / 256 * Hq);
   const CUtensorMap tm = tile_map(qkv, 128);
   const bool half = qkv.scalar_type() == at::kHalf;
   launch_fwd(static_cast<int>(D), half, tm, a, items, at::cuda::getCurrentCUDAStream());
