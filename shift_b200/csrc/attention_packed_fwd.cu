@@ -11,7 +11,7 @@ namespace pa {
 // Heads of 64: S, P and O of both tiles have columns of their own (2 x (128 + 64 + 64)), so the next S is computed while a
 // group is still at its exponentials.  Heads of 128: P lies over S (2 x (128 + 128)).
 //
-// SPLIT: with few tiles (launch rule in attention_packed_host.cpp) the two tiles are one: group w has every second key block
+// SPLIT: with few tiles of heads of 64 (the rule stands in attention_packed_host.cpp) the two tiles are one: group w has every second key block
 // of it, from the w-th, and the two partial results are joined at the end, half of the columns a group.  An item then takes
 // half of its blocks' time, which is what counts when every SM has one or two.
 template <int D, bool SPLIT>
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
   uint64_t* ml_full = drain + 5;                       // SPLIT: a group's maxima and sums
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 7);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const FwdItem first_item(a, blockIdx.x);             // its dependent loads run under the set-up
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -116,10 +117,11 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       int nk = 0, nv = 0, nq = 0, nl = 0;
       bool ok = true;
       if (lane == 0) tma_prefetch_desc(&tm);
+      FwdItem it = first_item;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         if (lane == 0) ok = sched_request(sched, n, a.status);
         ok = __all_sync(0xffffffffu, ok);
-        const FwdItem it(a, idx);
+        if (n > 0) it = FwdItem(a, idx);
         if (ok && it.all_hi > it.all_lo) {
           if (lane == 0) {
             ok = mbar_wait(q_empty, (nq & 1) ^ 1, a.status);
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       if (elect_one()) {
       int nk = 0, nv = 0, nq = 0, nb[2] = {0, 0}, no[2] = {0, 0};   // blocks and items of each tile so far
       bool ok = true;
-      FwdItem it(a, blockIdx.x);
+      FwdItem it = first_item;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         FwdItem following = it;
         auto look_ahead = [&]() {                      // before the last wait of an item: its loads take a microsecond
@@ -274,8 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     constexpr int kStep = SPLIT ? 2 : 1;
     struct Mine {                                      // this group's tile: blocks lo, lo + kStep ... below hi
       int h, q0, lo, hi, row, st, most;
-      SB_DEVICE Mine(const Args& a, int idx, int w) {
-        const FwdItem it(a, idx);
+      SB_DEVICE Mine(const Args& a, const FwdItem& it, int w) {
         q0 = w ? it.q0[1] : it.q0[0];
         lo = w ? it.lo[1] + (SPLIT ? 1 : 0) : it.lo[0];
         hi = w ? it.hi[1] : it.hi[0];
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
         most = q0 < a.T ? a.start[min(q0 + 127, a.T - 1)] : 0;             // the tile's latest start
       }
     };
-    Mine now(a, blockIdx.x, w);
+    Mine now(a, first_item, w);
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int h = now.h, q0 = now.q0, lo = now.lo, hi = now.hi, row = now.row, st = now.st, most = now.most;
       float m = -INFINITY, l = 0.f;
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       }
       if (!ok) break;
       idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
-      if (idx >= 0) now = Mine(a, idx, w);
+      if (idx >= 0) now = Mine(a, FwdItem(a, idx), w);
       const bool covered = row < a.T && st <= row;
       float lse2 = -INFINITY;
       bool bad = false;
@@ -487,7 +488,7 @@ static void launch(const CUtensorMap& tm, const Args& a, unsigned items, cudaStr
 template <typename T>
 static void launch_typed(int D, const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {
   if (D == 64) a.split_keys ? launch<64, T, true>(tm, a, items, stream) : launch<64, T, false>(tm, a, items, stream);
-  else a.split_keys ? launch<128, T, true>(tm, a, items, stream) : launch<128, T, false>(tm, a, items, stream);
+  else launch<128, T, false>(tm, a, items, stream);
 }
 
 void launch_fwd(int D, bool half, const CUtensorMap& tm, const Args& a, unsigned items, cudaStream_t stream) {

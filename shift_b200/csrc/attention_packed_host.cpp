@@ -120,8 +120,10 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& plan, int64
   // Two heads of one key head share every key block and have the same causal cost; without such pairs two consecutive
   // tiles of a head do.
   a.pair_heads = a.group % 2 == 0;
-  // With at most two tiles an SM an item is one tile, whose key blocks the two groups share.
-  a.split_keys = a.tiles * Hq <= 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // With at most two tiles an SM an item is one tile, whose key blocks the two groups share (one sequence, 16 / 4 heads of
+  // 64: 512 rows 16.4 -> 14.3 us, 1024 22.5 -> 18.4, 2048 36.9 -> 34.8).  Not for heads of 128, where a block is then loaded
+  // for one tile in as long as it takes for two, and shared memory has no stages left to hide it (2048 rows 41 -> 57 us).
+  a.split_keys = D == 64 && a.tiles * Hq <= 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.order = a.split_keys || a.pair_heads ? pl.q_order : pl.q2_order;
   const unsigned items = static_cast<unsigned>(a.split_keys     ? a.tiles * Hq
                                                : a.pair_heads ? a.tiles * (Hq / 2)

@@ -77,18 +77,19 @@ SB_DEVICE void find_rows(const int* __restrict__ offs, int n, int T, int* start,
   stop[r] = covered ? behind : r;
 }
 
+// How many blocks of 128 rows a tile meets.  which: 0 tiles of 128 queries, 1 of 256 queries, 2 of 128 keys.
+SB_DEVICE int tile_cost(int which, const int* start, const int* stop, int T, int t) {
+  const int rows = which == 1 ? 256 : 128, lo = t * rows, hi = min(lo + rows, T);
+  return which == 2 ? (stop[hi - 1] - lo + 127) / 128 : (hi + 127) / 128 - start[lo] / 128;
+}
+
 // Orders of the attention kernels' tiles, the costliest first: a counting sort by the number of 128-row blocks that a
-// tile meets.  0: tiles of 128 queries; 1: of 256 queries; 2: of 128 keys.  The order decides when a tile runs, nothing
-// else.  By 1024 threads.
+// tile meets.  The order decides when a tile runs, nothing else.  By 1024 threads.
 SB_DEVICE void find_order(int which, const int* start, const int* stop, int T, int* out) {
   __shared__ __align__(16) int bins[kBins];
   const int rows = which == 1 ? 256 : 128;
   const int nt = (T + rows - 1) / rows;
-  auto cost = [&](int t) {
-    const int lo = t * rows, hi = min(lo + rows, T);
-    const int blocks = which == 2 ? (stop[hi - 1] - lo + 127) / 128 : (hi + 127) / 128 - start[lo] / 128;
-    return kBins - 1 - max(0, min(blocks, kBins - 1));
-  };
+  auto cost = [&](int t) { return kBins - 1 - max(0, min(tile_cost(which, start, stop, T, t), kBins - 1)); };
   for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
   __syncthreads();
   for (int t = threadIdx.x; t < nt; t += 1024) atomicAdd(&bins[cost(t)], 1);
@@ -126,10 +127,18 @@ __global__ void __launch_bounds__(1024)
 small_kernel(const int* __restrict__ offs, int n, int T, int* start, int* pos, int* stop, int* ends, int* fwd, int* fwd2,
              int* bwd) {
   find_rows<1024>(offs, n, T, start, pos, stop, ends);
-  for (int which = 0; which < 3; ++which) {
-    __syncthreads();
-    find_order(which, start, stop, T, which == 0 ? fwd : which == 1 ? fwd2 : bwd);
+  __syncthreads();
+  // at most eight tiles: one warp an order, a lane a tile, whose place is the number of costlier ones (or alike and before)
+  const int which = threadIdx.x / 32, t = threadIdx.x % 32;
+  if (which >= 3) return;
+  const int rows = which == 1 ? 256 : 128, nt = (T + rows - 1) / rows;
+  const int mine = t < nt ? tile_cost(which, start, stop, T, t) : -1;
+  int place = 0;
+  for (int k = 0; k < nt; ++k) {
+    const int other = __shfl_sync(0xffffffffu, mine, k);
+    place += other > mine || (other == mine && k < t);
   }
+  if (t < nt) (which == 0 ? fwd : which == 1 ? fwd2 : bwd)[place] = t;
 }
 
 // The plan: start, pos, stop of every row | first covered row, row behind the last one | tile orders (of 128 queries, 256
