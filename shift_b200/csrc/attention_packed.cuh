@@ -85,14 +85,19 @@ SB_DEVICE float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two values on the FMA and integer pipes, for x <= 126: x = j + r with j the nearest whole number (left in the low
+// 2^x of two values on the FMA and integer pipes, for x <= 127: x = j + r with j the nearest whole number (left in the low
 // bits of x + 1.5 * 2^23) and r in [-1/2, 1/2]; 2^r by a polynomial of degree 4 that is 1 at 0, fitted to the relative error
-// over that interval (least squares, reweighted; at most 2.9e-6), j added to the exponent.  At -127 and below, masked -inf
-// among it, that leaves exactly 0: a masked probability must not carry another row's value, however large that is.
+// over that interval (least squares, reweighted; at most 2.9e-6), times 2^j.  At -127 and below, masked -inf among
+// it, 2^j is exactly 0: a masked probability must not carry another row's value, however large that is.  NaN stays NaN.
 __device__ constexpr float kEx2[5] = {1.f, 0.693124175f, 0.240240991f, 0.0559064262f, 0.00958285294f};
+SB_DEVICE float max_nan(float a, float b) {            // NaN where one of them is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 SB_DEVICE float2 ex2_fma(float2 x) {
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
   const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
   const float2 j = add2(t, make_float2(-12582912.f, -12582912.f));
   const float2 r = fma2(j, make_float2(-1.f, -1.f), x);
@@ -100,8 +105,8 @@ SB_DEVICE float2 ex2_fma(float2 x) {
   p = fma2(p, r, make_float2(kEx2[2], kEx2[2]));
   p = fma2(p, r, make_float2(kEx2[1], kEx2[1]));
   p = fma2(p, r, make_float2(kEx2[0], kEx2[0]));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                             __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 
 // Whether a barrier's phase is over; asked early, since the answer takes a hundred clocks.
@@ -232,7 +237,36 @@ SB_DEVICE float dot(const float* a, const float* b) {
   return warp_sum(s);
 }
 
-// Columns [c0, c1) of one row of O by a whole warp, from what the row sees alone.
+// Whether rows [lo, st) and [end, hi) of an operand, which a result's masked zeros met, have something there that zero times
+// it is NaN, in a column that is not NaN by the result's own rows (`own`: a bit for each of this lane's columns).  Where they
+// have not, what is not finite in the result is its own, and a step that has gone wrong as a whole takes no longer for it.
+template <int D, typename T>
+SB_DEVICE bool touched(const T* p, long ld, int lo, int st, int end, int hi, uint32_t own) {
+  constexpr int N = D / 32;
+  constexpr int kMost = 1024;                          // rows: with more of them it is the result that is computed
+  const bool open = (~own & ((1u << N) - 1)) != 0;
+  if (!__any_sync(0xffffffffu, open)) return false;
+  const int before = max(st - lo, 0), n = before + max(hi - end, 0);
+  if (n > kMost) return true;
+  uint32_t bad = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    float f[N];
+    load_part<D>(p + static_cast<long>(i < before ? lo + i : end + i - before) * ld, f);
+#pragma unroll
+    for (int k = 0; k < N; ++k) bad |= fabsf(f[k]) < INFINITY ? 0u : 1u << k;
+  }
+  return __any_sync(0xffffffffu, (bad & ~own) != 0);
+}
+template <int N>
+SB_DEVICE uint32_t nan_columns(const float* f) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) bits |= f[k] != f[k] ? 1u << k : 0u;
+  return bits;
+}
+
+// Columns [c0, c1) of one row of O by a whole warp, from what the row sees alone, if others have got into it.
 template <int D, typename T>
 __device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float lse2, int c0, int c1) {
   constexpr int N = D / 32;
@@ -240,6 +274,9 @@ __device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float
   const T* x = static_cast<const T*>(a.qkv);
   const long kc = static_cast<long>(a.Hq + h / a.group) * D, vc = kc + static_cast<long>(a.Hkv) * D;
   float q[N], k[N], v[N], acc[N] = {};
+  load_part<D>(x + row * a.ld + vc, v);
+  const int q0 = row / 128 * 128;
+  if (!touched<D>(x + vc, a.ld, a.start[q0] / 128 * 128, st, row + 1, min(q0 + 128, a.T), nan_columns<N>(v))) return;
   load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
   for (int j = st; j <= row; ++j) {
     load_part<D>(x + j * a.ld + kc, k);
@@ -282,6 +319,9 @@ __device__ __noinline__ void slow_dq(const Args& a, int row, int h, int st, int 
   load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
   load_part<D>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D, g);
   const float* rb = row_block(a, h, row);
+  const int q0 = row / 128 * 128;
+  const uint32_t own = rb[0] != rb[0] || rb[64] != rb[64] ? ~0u : 0u;
+  if (!touched<D>(x + kc, a.ld, a.start[q0] / 128 * 128, st, row + 1, min(q0 + 128, a.T), own)) return;
   for (int j = st; j <= row; ++j) {
     load_part<D>(x + j * a.ld + kc, k);
     load_part<D>(x + j * a.ld + vc, v);
@@ -303,6 +343,19 @@ __device__ __noinline__ void slow_dkv(const Args& a, int row, int kvh, int h0, i
   const T* x = static_cast<const T*>(a.qkv);
   const long kc = static_cast<long>(a.Hq + kvh) * D, vc = kc + static_cast<long>(a.Hkv) * D;
   float q[N], g[N], k[N], v[N], acc[N] = {};
+  const int k0 = row / 128 * 128, hi = min(k0 + (a.stop[min(k0 + 127, a.T - 1)] - k0 + 127) / 128 * 128, a.T);
+  uint32_t own = 0;
+  for (int h = h0; h < h1; ++h) {
+    const float* rb = row_block(a, h, row);
+    load_part<D>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D, g);
+    own |= rb[0] != rb[0] || (want_k && rb[64] != rb[64]) ? ~0u : want_k ? 0u : nan_columns<N>(g);
+  }
+  bool others = false;
+  for (int h = h0; h < h1 && !others; ++h) {
+    const T* p = want_k ? x : static_cast<const T*>(a.dout);
+    others = touched<D>(p + static_cast<long>(h) * D, want_k ? a.ld : a.do_ld, k0, row, end, hi, own);
+  }
+  if (!others) return;
   load_part<D>(x + row * a.ld + kc, k);
   load_part<D>(x + row * a.ld + vc, v);
   for (int h = h0; h < h1; ++h)

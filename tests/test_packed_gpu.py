@@ -281,3 +281,42 @@ def test_fp16_gradients_of_any_size(size, D):
         # roundings of P, dS and the result, 2^-11 each of a value of random sign, and the result's own smallest step
         bound = 3 * 2.0 ** -11 * w.norm() + 2.0 ** -25 * w.numel() ** 0.5
         assert (got[:, cols] - w).norm() <= bound
+
+
+def test_a_step_of_nan_takes_no_longer():
+    """Where everything is NaN, nothing is computed again row by row (that would take some hundred times as long)."""
+    rows, heads = 8192, (4, 2, 64, 0.125)
+    qkv, do, seqs = _randn(rows, 8 * 64, seed=1), _randn(rows, 4 * 64, seed=2), _seqs([0, rows], rows)
+    bad = torch.full_like(qkv, math.nan)
+    times = []
+    for x, g in ((qkv, do), (bad, do), (qkv, torch.full_like(do, math.nan))):
+        _step(x, g, seqs, heads)
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        got = _step(x, g, seqs, heads)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    check_status()
+    assert torch.isnan(got[2][:, :6 * 64]).all() and max(times[1:]) < 20 * times[0], times
+
+
+@pytest.mark.parametrize("where", [0, 1, 5, 14, 63, 130, 255])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_score_of_nan_stays(where, D):
+    """One key that is NaN makes every later row of its sequence NaN, statistics and gradients among it, and no earlier one.
+    Its value is finite, so that it is the score that has to tell."""
+    rows, first, heads = 256, 3, (2, 1, D, D ** -0.5)
+    qkv, do = _randn(rows, 4 * D, seed=where + 1), _randn(rows, 2 * D, seed=where + 2)
+    seqs = _seqs([first, rows], rows)
+    at = max(where, first)
+    qkv[at, 2 * D + 1] = math.nan
+    o, lse, d = _step(qkv, do, seqs, heads)
+    check_status()
+    late = torch.arange(rows, device=DEV) >= at
+    inside = torch.arange(rows, device=DEV) >= first
+    assert torch.isnan(o[late]).all() and torch.isfinite(o[~late]).all()
+    assert torch.isnan(lse[:, late]).all() and torch.isfinite(lse[:, inside & ~late]).all()
+    assert torch.isnan(d[late, :2 * D]).all() and torch.isfinite(d[~late, :2 * D]).all()
+    # every key of the sequence is met by its last row, which is NaN
+    assert torch.isnan(d[inside, 2 * D:]).all() and torch.isfinite(d[~inside]).all()
