@@ -7,7 +7,7 @@
 //
 // The other side comes in blocks of 128, of which each group of softmax warps has 64 columns; S and dP have columns of their
 // own in tensor memory and P and dS have too, so that S and dP of the next block are computed while the groups are still at
-// this one (blocks of 64 that the groups took in turn: 412 us where this takes 335, 8 x 2048 rows, 16 / 4 heads of 64).  The
+// this one (blocks of 64 that the groups took in turn: 412 us where this took 335, 8 x 2048 rows, 16 / 4 heads of 64).  The
 // dK / dV pass of heads of 128 has no columns left for that: its blocks are of 64, the groups take them in turn, and P and dS
 // lie over S and dP.
 //
@@ -19,7 +19,7 @@
 namespace sb {
 namespace pa {
 
-constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe
+constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe (of 64, 8 x 2048: 342 us, 1: 345)
 
 // -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
 // a row of a head.

@@ -11,9 +11,9 @@ namespace pa {
 // Heads of 64: S, P and O of both tiles have columns of their own (2 x (128 + 64 + 64)), so the next S is computed while a
 // group is still at its exponentials.  Heads of 128: P lies over S (2 x (128 + 128)).
 //
-// SPLIT: with few tiles of heads of 64 (the rule stands in attention_packed_host.cpp) the two tiles are one: group w has every second key block
-// of it, from the w-th, and the two partial results are joined at the end, half of the columns a group.  An item then takes
-// half of its blocks' time, which is what counts when every SM has one or two.
+// SPLIT: with few tiles of heads of 64 (the rule stands in attention_packed_host.cpp) the two tiles are one: group w has every
+// second key block of it, from the w-th, and the two partial results are joined at the end, half of the columns a group.  An
+// item then takes half of its blocks' time, which is what counts when every SM has one or two.
 template <int D, bool SPLIT>
 struct Fwd {
   static constexpr int kHalves = D / 64, kTile = kHalves * kChunk;
@@ -53,7 +53,10 @@ struct FwdItem {
   SB_DEVICE bool any(int i) const { return hi[i] > lo[i] + (SPLIT ? i : 0); }
 };
 
-constexpr int kOnFma = 3;      // of 8 exponentials, those computed on the FMA pipe
+// Of 8 exponentials, those computed on the FMA pipe.  3 and 2: heads of 64, 8 x 2048 rows, 16 / 4 heads 123 and 122 us, 8 / 8
+// heads 80 and 86; heads of 128, 16 / 4 heads 144 and 142, one sequence of 16384, 32 / 8 heads 1676 and 1645.
+template <int D>
+constexpr int kOnFma = D == 64 ? 3 : 2;
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Args a) {
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           for (int k = 0; k < 16; ++k)
             z[k] = fma2(make_float2(__uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1])), sc2, nm2);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) z[k] = k % 8 < kOnFma ? ex2_fma(z[k]) : make_float2(ex2(z[k].x), ex2(z[k].y));
+          for (int k = 0; k < 16; ++k) z[k] = k % 8 < kOnFma<D> ? ex2_fma(z[k]) : make_float2(ex2(z[k].x), ex2(z[k].y));
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             l2[k & 3] = add2(l2[k & 3], z[k]);

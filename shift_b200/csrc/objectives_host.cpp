@@ -47,7 +47,8 @@ static float* row_floats(const at::Tensor& t, const at::Tensor& logits, const ch
 }
 
 // CTAs a row: enough that a slice can be held (where `hold`), and more while the grid would leave SMs idle and a slice
-// keeps at least 8 KB (below that the cluster's two barriers cost more than the shorter slice saves).
+// keeps at least 8 KB.  (token_logp_fwd, one row: 100003 of bf16 20.5 us by one CTA, 10.4 by eight; 8192 of fp32 8.2 us by one,
+// two or four CTAs, 9.3 by eight, of slices of 4 KB.)
 static int pick_ranks(const Args& a, int64_t bytes, bool hold) {
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, row = bytes * a.V;
   int c = 1;

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(1024)
 order_kernel(const int* start, const int* stop, int T, int* fwd, int* fwd2, int* bwd) {
   find_order(blockIdx.x, start, stop, T, blockIdx.x == 0 ? fwd : blockIdx.x == 1 ? fwd2 : bwd);
 }
-// both for a buffer of at most 1024 rows (one launch: 4 us less of 20 for a short batch)
+// both for a buffer of at most 1024 rows: one launch of 4.0 us instead of two of 5.1 together (200 rows), and 3 us less of host
 __global__ void __launch_bounds__(1024)
 small_kernel(const int* __restrict__ offs, int n, int T, int* start, int* pos, int* stop, int* ends, int* fwd, int* fwd2,
              int* bwd) {
@@ -274,7 +274,7 @@ static void rotary_launch(RotaryArgs a, bool inter, bool copy, cudaStream_t stre
 }
 
 // Elements per access: the most, up to 16 bytes, that divide every column that a chunk begins at, the row strides and the
-// bases.  (16384 rows of 24 heads of 64, bf16: 16-byte accesses 17 us, 2-byte ones 70 us.)
+// bases.  (16384 rows of 24 heads of 64, bf16: 16-byte accesses 25 us, 2-byte ones 33 us.)
 template <typename T>
 static void rotary_typed(const RotaryArgs& a, bool inter, bool copy, cudaStream_t stream) {
   const uint64_t all = static_cast<uint64_t>(a.dim) | static_cast<uint64_t>(inter ? a.rot : a.rot / 2) |
