@@ -19,7 +19,7 @@
 namespace sb {
 namespace pa {
 
-constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe (of 64, 8 x 2048: 342 us, 1: 345)
+constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe (of 64, 8 x 2048: 343 us, 1: 345)
 
 // -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
 // a row of a head.

@@ -53,10 +53,9 @@ struct FwdItem {
   SB_DEVICE bool any(int i) const { return hi[i] > lo[i] + (SPLIT ? i : 0); }
 };
 
-// Of 8 exponentials, those computed on the FMA pipe.  3 and 2: heads of 64, 8 x 2048 rows, 16 / 4 heads 123 and 122 us, 8 / 8
-// heads 80 and 86; heads of 128, 16 / 4 heads 144 and 142, one sequence of 16384, 32 / 8 heads 1676 and 1645.
-template <int D>
-constexpr int kOnFma = D == 64 ? 3 : 2;
+// Of 8 exponentials, those computed on the FMA pipe.  3 and 2, 16 / 4 heads: 8 x 2048 rows, heads of 64 122 and 122 us, of 128
+// 144 and 141; 24 x 700, of 64 79 and 77.
+constexpr int kOnFma = 2;
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Args a) {
@@ -363,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
           for (int k = 0; k < 16; ++k)
             z[k] = fma2(make_float2(__uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1])), sc2, nm2);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) z[k] = k % 8 < kOnFma<D> ? ex2_fma(z[k]) : make_float2(ex2(z[k].x), ex2(z[k].y));
+          for (int k = 0; k < 16; ++k) z[k] = k % 8 < kOnFma ? ex2_fma(z[k]) : make_float2(ex2(z[k].x), ex2(z[k].y));
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             l2[k & 3] = add2(l2[k & 3], z[k]);
