@@ -15,8 +15,9 @@
 //
 // What others hold.  Products run over whole blocks, so a masked value is a product with zero, which is zero unless the
 // other factor is infinite or NaN.  Rows that no sequence covers are cleared in shared memory after they were loaded.  Rows
-// of other sequences (or later ones of the same) that are not finite would leave NaN in a result: such results are
-// recognised when they are stored and computed again row by row from what they see.
+// of other sequences (or later ones of the same) that are not finite would leave NaN in a result: results
+// that are not finite are recognised when they are stored and, where such a row met them, computed again row by row from
+// what they see.
 //
 // Every wait is bounded; on expiry the kernel records a status code and winds down.
 #pragma once

@@ -294,6 +294,7 @@ void rotary(const at::Tensor& x, at::Tensor& out, const at::Tensor& pos, const a
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && out.dim() == 2, "rotary: matrices [rows, columns] on the device");
   TORCH_CHECK(x.device() == out.device() && x.device() == pos.device() && x.device() == turns.device(),
               "rotary: x, out, positions and the plan on one device");
+  TORCH_CHECK(x.size(0) <= (1 << 29), "rotary: at most 2^29 rows, got ", x.size(0));
   TORCH_CHECK(x.scalar_type() == out.scalar_type(), "rotary: out is ", out.scalar_type(), ", x ", x.scalar_type());
   TORCH_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.numel() == x.size(0) && pos.is_contiguous(),
               "rotary: positions are int32, one for each of the ", x.size(0), " rows, contiguous");

@@ -120,12 +120,12 @@ class Rotary:
         if not (math.isfinite(s.factor) and s.factor > 0):
             raise ValueError(f"Rotary: scaled by {s.factor}")
         if s.kind == "linear":
-            return [f / s.factor for f in plain], s.magnitude or 1.0
+            return [f / s.factor for f in plain], 1.0 if s.magnitude is None else s.magnitude
         if s.kind == "base":
             if rot < 4:
                 raise ValueError("Rotary: a scaled base needs two pairs or more")
             theta *= s.factor ** (rot / (rot - 2))
-            return [theta ** (-2.0 * i / rot) for i in range(rot // 2)], s.magnitude or 1.0
+            return [theta ** (-2.0 * i / rot) for i in range(rot // 2)], 1.0 if s.magnitude is None else s.magnitude
         if s.kind != "ramp":
             raise ValueError(f"Rotary: scaling {s.kind!r}, expected 'linear', 'base' or 'ramp'")
         if s.original < 1 or not s.fast > s.slow > 0 or theta <= 1:
@@ -182,7 +182,7 @@ def attention_fwd(qkv: torch.Tensor, seqs: Sequences, Hq: int, Hkv: int, D: int,
     multiple of 16 bytes apart.  ``lse`` is the natural logarithm of the sum of exp(scale q k).  Rows that no sequence
     covers get zeros (with ``out``: are left as they were) and an lse of minus infinity; what they hold is not looked
     at.  A row's result hangs on the rows it sees and on no other, also where others are not finite (such rows are
-    computed one by one, slowly)."""
+    computed one by one, slowly).  A score of NaN or plus infinity makes its row NaN, on the GPU its lse too."""
     if qkv.is_cuda:
         return tuple(ext().packed_attn_fwd(qkv, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out, status_word(qkv.device)))
     _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, "attention_fwd")

@@ -233,3 +233,14 @@ def test_model_takes_an_objective():
     assert math.isclose(loss * 12, math.log(2.0), rel_tol=1e-5) and torch.isfinite(grad).all() and grad.any()
     with pytest.raises(ValueError, match="16 rows"):
         eng.forward_backward([(tok, lab, {"seqs": _seqs([0, 16], 16)})], 1, 12)
+
+
+@pytest.mark.parametrize("kind", ["linear", "base", "ramp"])
+@pytest.mark.parametrize("magnitude", [0.0, 1.0, 2.5])
+def test_a_given_magnitude_is_taken(kind, magnitude):
+    scaling = packed.RotaryScaling(kind, 8.0, 4096, magnitude=magnitude)
+    plan = packed.Rotary(64, 1.0e4, scaling=scaling, device="cpu")
+    assert plan.magnitude == magnitude
+    x = torch.randn(3, 64)
+    turned = packed.rotary(x.clone(), torch.tensor([0, 1, 5], dtype=torch.int32), plan, 1)
+    assert torch.allclose(turned.norm(dim=1), magnitude * x.norm(dim=1), atol=1e-5)

@@ -320,3 +320,33 @@ def test_a_score_of_nan_stays(where, D):
     assert torch.isnan(d[late, :2 * D]).all() and torch.isfinite(d[~late, :2 * D]).all()
     # every key of the sequence is met by its last row, which is NaN
     assert torch.isnan(d[inside, 2 * D:]).all() and torch.isfinite(d[~inside]).all()
+
+
+@pytest.mark.parametrize("rows,Hq,Hkv", [(300, 2, 1), (5000, 8, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinite_scores(D, rows, Hq, Hkv):
+    at, seqs, heads = 137, _seqs([0, rows], rows), (Hq, Hkv, D, D ** -0.5)
+    late = torch.arange(rows, device=DEV) >= at
+    x, do = _randn(rows, (Hq + 2 * Hkv) * D, seed=8), _randn(rows, Hq * D, seed=9)
+    x[:, :(Hq + Hkv) * D:D] = x[:, :(Hq + Hkv) * D:D].abs() + 1                  # the first column of every head
+    # one row of one head whose scores are all minus infinity: 0 / 0, and an empty sum's logarithm
+    y = x.clone()
+    y[at, 0] = -math.inf
+    o, lse, d = _step(y, do, seqs, heads)
+    check_status()
+    assert torch.isnan(o[at, :D]).all() and torch.isfinite(o[~(torch.arange(rows, device=DEV) == at)]).all()
+    assert torch.isfinite(o[at, D:]).all() and lse[0, at] == -math.inf and (~torch.isfinite(lse)).sum() == 1
+    assert torch.isnan(d[:at + 1, Hq * D:Hq * D + D]).all() and torch.isfinite(d[at + 1:]).all()
+    # a key whose score is minus infinity counts for nothing
+    y = x.clone()
+    y[at, Hq * D] = -math.inf
+    o, lse, d = _step(y, do, seqs, heads)
+    check_status()
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all() and torch.isfinite(d[:, Hq * D:]).all()
+    # a score of plus infinity makes its row NaN
+    y[at, Hq * D] = math.inf
+    o, lse, d = _step(y, do, seqs, heads)
+    check_status()
+    group = Hq // Hkv * D
+    assert torch.isnan(o[late, :group]).all() and torch.isfinite(o[~late]).all() and torch.isfinite(o[:, group:]).all()
+    assert not torch.isfinite(lse[:Hq // Hkv, late]).any() and torch.isfinite(lse[:, ~late]).all()
