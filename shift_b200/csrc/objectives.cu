@@ -469,7 +469,8 @@ static cudaError_t launch(F* kernel, const Args& a, size_t smem, cudaStream_t st
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (smem > 48 * 1024) {
+  // Without opting in a kernel has 48 KB, its static shared memory (some 100 bytes: barriers, sums) among it.
+  if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMost);
     if (e != cudaSuccess) return e;
   }
