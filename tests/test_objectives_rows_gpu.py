@@ -1,5 +1,5 @@
 """Losses of label log-probabilities on the GPU: vocabularies whose slice fills shared memory to the limit without opt-in, each
-as the first call of a process."""
+as the first call of a process; rows behind 2^31 elements."""
 import os
 import subprocess
 import sys
@@ -46,3 +46,40 @@ def test_policy_loss_as_the_first_call(dtype, vocab):
     env = {**os.environ, "PYTHONPATH": os.pathsep.join([here, os.path.dirname(here)])}
     got = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert got.returncode == 0, got.stderr[-2000:]
+
+
+def test_gradients_of_rows_behind_two_to_the_31():
+    """What is written there, not only what is read: the last rows of 2.2e9 logits, and a row on each side of 2^31 elements."""
+    rows, vocab = 17000, 131072
+    at = torch.tensor([0, (1 << 31) // vocab - 1, (1 << 31) // vocab, rows - 2, rows - 1], device=DEV)
+    g = torch.Generator().manual_seed(6)
+    some = torch.randn(len(at), vocab, generator=g).to(torch.bfloat16).to(DEV)
+    labels = torch.full((rows,), -1, dtype=torch.int32, device=DEV)
+    labels[at] = torch.tensor([5, 9, 131071, 0, 77], dtype=torch.int32, device=DEV)
+    z = torch.ones(rows, vocab, dtype=torch.bfloat16, device=DEV)
+    d = torch.zeros(rows, device=DEV)
+    d[at] = torch.tensor([1.5, -2.0, 0.5, 3.0, -1.0], device=DEV)
+    want_logp, *_ = orc.label_logp(some, labels[at])
+
+    def compare(got, d_at, slack):
+        want = orc.logits_grad(some, labels[at], d_at)
+        tol = (torch.finfo(torch.bfloat16).eps / 2 + slack) * want.abs() + orc.tiny(torch.bfloat16) + orc.tiny(torch.float32)
+        tol.scatter_add_(1, labels[at].long()[:, None], slack * d_at.double().abs()[:, None])
+        orc.close(got[at], want, tol, "dlogits")
+        assert int(torch.count_nonzero(got.view(torch.int16).view(rows, -1).any(1))) == len(at)      # the others are zeros
+
+    z[at] = some
+    logp, lse = ob.token_logp_fwd(z, labels)
+    orc.close(logp[at], want_logp, SUM + 2.0 ** -23 * want_logp.abs(), "logp")
+    ob.token_logp_bwd(z, labels, lse, d)
+    compare(z, d[at], 2 * SUM)
+    z.fill_(1)
+    z[at] = some
+    old = torch.zeros(rows, device=DEV)
+    old[at] = (want_logp + 0.1).float()
+    adv = torch.zeros(rows, device=DEV)
+    adv[at] = d[at]
+    _, logp = ob.policy_loss_fwd_bwd(z, labels, old, adv, clip_low=10.0, clip_high=1e9)
+    orc.close(logp[at], want_logp, SUM + 2.0 ** -23 * want_logp.abs(), "logp")
+    compare(z, -torch.exp(want_logp - old[at].double()) * d[at].double(), 4 * SUM)
+    check_status()
