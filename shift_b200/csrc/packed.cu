@@ -209,6 +209,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   T* yr = static_cast<T*>(a.out) + row * a.os + static_cast<long>(h0) * a.dim;
   if (c >= a.live) {                                       // columns behind the rotated ones
     const int at = a.rot + (c - a.live) * V;
+    if (at + V > a.dim) {                                  // the last column of an odd head, whose pairs still go by two
+      for (int h = 0; h < nh; ++h)
+        for (int k = at; k < a.dim; ++k) yr[h * a.dim + k] = xr[h * a.dim + k];
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < kHeads; ++h)
       if (h < nh) *reinterpret_cast<VT*>(yr + h * a.dim + at) = *reinterpret_cast<const VT*>(xr + h * a.dim + at);
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 template <typename T, int V, int ALIGN = V * static_cast<int>(sizeof(T))>
 static void rotary_launch(RotaryArgs a, bool inter, bool copy, cudaStream_t stream) {
   a.live = (inter ? a.rot : a.rot / 2) / V;
-  a.chunks = a.live + (copy ? (a.dim - a.rot) / V : 0);
+  a.chunks = a.live + (copy ? (a.dim - a.rot + V - 1) / V : 0);
   // a row of threads has a row's chunks, so that no index is divided
   const int bx = std::min(a.chunks, 256), by = 256 / bx;
   const dim3 block(bx, by), grid((a.T + by - 1) / by, (a.heads + kHeads - 1) / kHeads, (a.chunks + bx - 1) / bx);
