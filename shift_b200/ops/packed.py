@@ -131,8 +131,10 @@ class Rotary:
         if s.original < 1 or not s.fast > s.slow > 0 or theta <= 1:
             raise ValueError(f"Rotary: a ramp needs the original context, fast > slow > 0 and theta > 1, got {s}, {theta}")
         place = [rot * math.log(s.original / (2 * math.pi * t)) / (2 * math.log(theta)) for t in (s.fast, s.slow)]
-        low, high = max(math.floor(place[0]), 0), min(math.ceil(place[1]), rot // 2 - 1)
-        ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rot // 2)]
+        # The ramp's end may lie behind the last pair, which then keeps a part of its speed; it is held to the columns, the
+        # guard that scaled models are trained with.
+        low, high = max(math.floor(place[0]), 0), min(math.ceil(place[1]), rot - 1)
+        ramp = [1.0 if i >= place[1] else min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rot // 2)]
         size = 0.1 * math.log(s.factor) + 1.0 if s.magnitude is None else s.magnitude
         return [f * (1 - r) + f / s.factor * r for f, r in zip(plain, ramp)], size
 
