@@ -80,7 +80,7 @@ class RotaryScaling(NamedTuple):
     ``"linear"``: all divided by factor.  ``"base"``: theta becomes theta * factor^(rot / (rot - 2)), so that the
     slowest pair is stretched by factor and the fastest stays.  ``"ramp"``: pairs that turn more than ``fast`` times
     within ``original`` positions stay, those that turn less than ``slow`` times are divided by factor, a ramp over the
-    pairs between; rotated values are multiplied by ``magnitude`` (``None``: 0.1 ln(factor) + 1)."""
+    pairs between; rotated values are multiplied by ``magnitude`` (``None``: 0.1 ln(factor) + 1, at least 1)."""
     kind: str
     factor: float
     original: int = 0
@@ -135,7 +135,7 @@ class Rotary:
         # guard that scaled models are trained with.
         low, high = max(math.floor(place[0]), 0), min(math.ceil(place[1]), rot - 1)
         ramp = [1.0 if i >= place[1] else min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rot // 2)]
-        size = 0.1 * math.log(s.factor) + 1.0 if s.magnitude is None else s.magnitude
+        size = 0.1 * math.log(max(s.factor, 1.0)) + 1.0 if s.magnitude is None else s.magnitude
         return [f * (1 - r) + f / s.factor * r for f, r in zip(plain, ramp)], size
 
 

@@ -44,3 +44,9 @@ def test_ramp_of_the_published_rule(theta, rot, original, factor):
     want = plain / factor * (1 - keep) + plain * keep
     plan = packed.Rotary(rot, theta, scaling=packed.RotaryScaling("ramp", factor, original), device="cpu")
     assert torch.allclose(plan.freq, want, rtol=1e-12)
+
+
+@pytest.mark.parametrize("factor,magnitude", [(0.25, 1.0), (1.0, 1.0), (1e-8, 1.0), (8.0, 0.1 * math.log(8) + 1)])
+def test_contexts_no_longer_than_the_original_keep_their_magnitude(factor, magnitude):
+    plan = packed.Rotary(64, 1.0e4, scaling=packed.RotaryScaling("ramp", factor, 4096), device="cpu")
+    assert plan.magnitude == magnitude
