@@ -183,6 +183,13 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------------------------------------ one pass, own
+def _slowest(case):
+    """How often a pair turns within the original context that is slowed all the way: once, or as often as the last pair does,
+    at which a case's ramp ends at the latest."""
+    last = case["original"] / (2 * math.pi) * case["theta"] ** (2.0 / case["rot"] - 1.0) * (1 + 1e-9)
+    return last if 1.0 < last < 32.0 else 1.0
+
+
 def _run_own(s):
     case, op = s["case"], s["op"]
     if op in ("logp", "policy", "preference"):
@@ -204,7 +211,7 @@ def _run_own(s):
     if op == "rotary":
         if "plan" not in s:
             scaling = None if case["scaling"] == "none" else packed.RotaryScaling(case["scaling"], case["factor"],
-                                                                                  case["original"])
+                                                                                  case["original"], slow=_slowest(case))
             s["plan"] = packed.Rotary(case["dim"], case["theta"], rot_dim=case["rot"], layout=case["layout"],
                                       scaling=scaling, device=s["x"].device)
         return packed.rotary(s["x"], s["pos"], s["plan"], case["heads"], inverse=case["inverse"], out=s["out"])
