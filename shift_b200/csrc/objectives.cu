@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
     if (live) {
       logp = zl - static_cast<double>(run.m) - log(static_cast<double>(run.s));
       const double ratio = exp(logp - old), clipped = fmin(fmax(ratio, 1.0 - a.t.low), 1.0 + a.t.high);
-      const double gain = adv == 0.0 ? 0.0 : ratio * adv, cut = clipped * adv;
+      const double gain = adv == 0.0 && ratio == ratio ? 0.0 : ratio * adv, cut = clipped * adv;
       const bool open = gain <= cut;
       loss = -(open ? gain : cut);
       d = open ? -gain : 0.0;

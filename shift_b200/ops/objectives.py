@@ -65,7 +65,8 @@ def policy_loss_fwd_bwd(logits: torch.Tensor, labels: torch.Tensor, old_logp: to
     loss = -min(r adv, clip(r, 1 - clip_low, 1 + clip_high) adv) + kl_coef (exp(g) - g - 1),  g = ref_logp - logp
 
     The logits are overwritten by scale * weight * dloss/dlogits (``weight`` [T], default 1).  Where the clip binds, the
-    first term has no gradient; on its border it still has.  A row of zero advantage has none, whatever its ratio."""
+    first term has no gradient; on its border it still has.  A row of zero advantage has none, however
+    large its ratio; a ratio of NaN makes loss and gradient NaN with any advantage."""
     if logits.is_cuda:
         return tuple(ext().policy_loss(logits, labels, old_logp, adv, ref_logp, weight, clip_low, clip_high, kl_coef,
                                        scale, status_word(logits.device)))

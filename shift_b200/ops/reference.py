@@ -251,7 +251,7 @@ def policy_terms(logp, old_logp, adv, ref_logp, low: float, high: float, kl: flo
     """Loss and its derivative at logp (64 bits) of the clipped policy loss with a KL term."""
     adv = adv.double()
     ratio = torch.exp(logp - old_logp.double())
-    gain = torch.where(adv == 0, torch.zeros_like(adv), ratio * adv)
+    gain = torch.where((adv == 0) & ~ratio.isnan(), torch.zeros_like(adv), ratio * adv)
     cut = ratio.clamp(1 - low, 1 + high) * adv
     loss = -torch.minimum(gain, cut)
     d = torch.where(gain <= cut, -gain, torch.where(gain.isnan(), gain, torch.zeros_like(gain)))
