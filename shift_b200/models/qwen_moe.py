@@ -16,9 +16,9 @@ buffer (``FlatParams.grad``) and reports per-layer completion so that the
 cross-replica reduction of a bucket can start as soon as its layers are done.
 
 Sequences of different lengths may lie one after the other in a batch's rows (``ops.packed.Sequences``): attention then
-stays inside each of them, positions restart, and rows of none take no part but in the router's load.  Heads may be rotated
-in part, interleaved or with frequencies scaled for longer contexts.  Another objective than cross entropy
-(``ops.objectives``) takes the logits in its place.
+stays inside each of them, positions restart, and rows of none have no label and take no part but in the router's load.
+Heads may be rotated in part, interleaved or with frequencies scaled for longer contexts.  Another objective than cross
+entropy (``ops.objectives``) takes the logits in its place.
 
 Layout of the fused weights:
 * ``attn.qkv``  [(Hq + 2 Hkv) * D, H]   rows q | k | v
@@ -216,6 +216,8 @@ class QwenMoE:
                 y, rstd, h = Fn.rmsnorm_fwd(resid, st.w("norm.weight"), cfg.eps, delta)
             logits = G.linear_fwd(y, st.w("lm_head.weight"))
             lab = labels.reshape(-1).to(torch.int32)
+            if seqs is not None:
+                lab = torch.where(seqs.pos >= 0, lab, -100)          # rows of no sequence have no label
             if self.tp is not None:
                 lab = self.tp.local_rows(lab).contiguous()
             if objective is None:
