@@ -91,6 +91,7 @@ void bind_adamw_many(pybind11::module& m);        // adamw_many.cu
 void bind_packed(pybind11::module& m);            // packed.cu
 void bind_packed_attention(pybind11::module& m);  // attention_packed_host.cpp
 void bind_objectives(pybind11::module& m);        // objectives_host.cpp
+void bind_status(pybind11::module& m);            // status_host.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "shift_b200 sm_100a kernels";
@@ -134,6 +135,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_packed(m);
   bind_packed_attention(m);
   bind_objectives(m);
+  bind_status(m);
   m.def("fp8_quantize", &sb::fp8::quantize, "block quantiser to 8-bit floating point");
   m.def("fp8_matmul", &sb::fp8::matmul, "product of 8-bit matrices with block scales (dense / grouped)");
   m.def("attn_fwd", &sb::fa::fwd, "tcgen05 causal flash attention forward");

@@ -59,8 +59,11 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
-        t = torch.zeros(16, dtype=torch.int32, device=device)
-        _status[idx] = t
+        make = ext().fresh_words
+        with _lock:
+            t = _status.get(idx)
+            if t is None:
+                t = _status[idx] = make(idx, 16)
     return t
 
 
