@@ -103,6 +103,8 @@ class EagerBlock(nn.Module):
 class EagerMoE(nn.Module):
     def __init__(self, cfg: MoEConfig, seed: int = 0):
         super().__init__()
+        if not cfg.plain_rope():
+            raise ValueError("EagerMoE: rotary positions of whole heads in halves, unscaled; this configuration has others")
         self.cfg = cfg
         H = cfg.hidden
         self.embed = nn.Embedding(cfg.vocab, H)

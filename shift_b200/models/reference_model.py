@@ -7,6 +7,7 @@ import math
 
 import torch
 
+from ..ops import packed
 from ..ops import reference as ref
 from .qwen_moe import MoEConfig
 
@@ -16,7 +17,17 @@ def reference_loss(cfg: MoEConfig, params: dict, tokens: torch.Tensor, labels: t
     """Mean token loss (+ auxiliary router loss) for fp32 leaf tensors ``params``."""
     H, D, Hq, Hkv = cfg.hidden, cfg.head_dim, cfg.heads, cfg.kv_heads
     T = B * S
-    cos, sin = ref.rope_tables(cfg.max_seq, D, cfg.rope_theta)
+    if cfg.plain_rope():
+        cos, sin = ref.rope_tables(cfg.max_seq, D, cfg.rope_theta)
+    else:
+        plan = packed.Rotary(D, cfg.rope_theta, cfg.rope_dim, cfg.rope_layout, cfg.rope_scaling, device="cpu")
+        pos = torch.arange(T, dtype=torch.int32) % S
+
+    def rope(t):
+        if cfg.plain_rope():
+            return ref.rope(t, cos, sin, S)
+        return ref.rotary(t, pos, plan.freq, plan.rot_dim, plan.layout, plan.magnitude, inverse=False)
+
     scale = 1.0 / math.sqrt(D)
     x = params["embed.weight"][tokens.reshape(-1).long()]
     aux_total = 0.0
@@ -24,8 +35,8 @@ def reference_loss(cfg: MoEConfig, params: dict, tokens: torch.Tensor, labels: t
         p = f"layers.{i}."
         a = ref.rmsnorm(x, params[p + "ln1.weight"], cfg.eps)
         qkv = a @ params[p + "attn.qkv"].t()
-        q = ref.rope(qkv[:, : Hq * D].reshape(T, Hq, D), cos, sin, S)
-        k = ref.rope(qkv[:, Hq * D:(Hq + Hkv) * D].reshape(T, Hkv, D), cos, sin, S)
+        q = rope(qkv[:, : Hq * D].reshape(T, Hq, D))
+        k = rope(qkv[:, Hq * D:(Hq + Hkv) * D].reshape(T, Hkv, D))
         v = qkv[:, (Hq + Hkv) * D:].reshape(T, Hkv, D)
         o = ref.attention(q, k, v, B, S, scale).reshape(T, Hq * D)
         x = x + o @ params[p + "attn.o"].t()
