@@ -139,6 +139,28 @@ class Rotary:
         return [f * (1 - r) + f / s.factor * r for f, r in zip(plain, ramp)], size
 
 
+def _share_memory(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two matrices (inner stride 1, rows that do not overlap) share a byte, as csrc/apart.h says it."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    (a, a_end, a_row, a_step), (b, b_end, b_row, b_step) = (
+        (t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * step + t.shape[1]) * t.element_size(),
+         t.shape[1] * t.element_size(), step * t.element_size())
+        for t in (x, y) for step in [t.stride(0) if t.shape[0] > 1 else t.shape[1]])
+    if a_end <= b or b_end <= a:
+        return False
+    if a_step != b_step:
+        return True
+    shift = (b - a) % a_step                               # columns of one buffer, side by side?
+    return not (shift >= a_row and shift + b_row <= a_step)
+
+
+def _check_apart(out, who, **others):
+    for name, t in others.items():
+        if _share_memory(out, t):
+            raise ValueError(f"{who}: out overlaps {name}")
+
+
 def rotary(x: torch.Tensor, pos: torch.Tensor, plan: Rotary, heads: int, inverse: bool = False,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotates the first ``heads`` heads of every row of x [T, >= heads * head_dim] (bf16, fp16 or fp32, any row stride)
@@ -159,6 +181,12 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, plan: Rotary, heads: int, inverse
         raise ValueError(f"rotary: bf16, fp16 or fp32, x and out alike, got {x.dtype} and {out.dtype}")
     if pos.dtype != torch.int32 or tuple(pos.shape) != (x.shape[0],):
         raise ValueError(f"rotary: positions are int32, one for each of the {x.shape[0]} rows")
+    for t in (x, out):
+        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError("rotary: rows of stride 1 inside that do not overlap")
+    same = x.data_ptr() == out.data_ptr() and (x.shape[0] <= 1 or x.stride(0) == out.stride(0))
+    if not same:
+        _check_apart(out, "rotary", x=x)
     y = ref.rotary(x[:, :n].reshape(-1, heads, plan.head_dim), pos, plan.freq, plan.rot_dim, plan.layout, plan.magnitude,
                    inverse)
     out[:, :n] = y.reshape(-1, n)
@@ -167,13 +195,21 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, plan: Rotary, heads: int, inverse
 
 # ----------------------------------------------------------------------------- attention
 # The CUDA entry points check their arguments themselves (csrc/attention_packed_host.cpp); this is for CPU tensors.
-def _check(x, width, seqs, Hq, Hkv, D, who, what="qkv"):
+def _check(x, width, seqs, Hq, Hkv, D, scale, who):
     if Hq < 1 or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{who}: {Hq} query heads for {Hkv} key heads")
     if D not in (64, 128):
         raise ValueError(f"{who}: heads of 64 or 128 columns, got {D}")
-    if x.dim() != 2 or tuple(x.shape) != (seqs.rows, width):
-        raise ValueError(f"{who}: {what} [{seqs.rows}, {width}], got {tuple(x.shape)}")
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"{who}: scale {scale}, a number above 0 is expected")
+    if x.dtype not in _FLOATS:
+        raise ValueError(f"{who}: bf16, fp16 or fp32, got {x.dtype}")
+    _check_rows(x, x, seqs.rows, width, who, "qkv")
+
+
+def _check_rows(t, qkv, rows, cols, who, what):
+    if t.dim() != 2 or tuple(t.shape) != (rows, cols) or t.dtype != qkv.dtype or t.device != qkv.device:
+        raise ValueError(f"{who}: {what} [{rows}, {cols}] of {qkv.dtype} beside qkv, got {tuple(t.shape)} of {t.dtype}")
 
 
 def attention_fwd(qkv: torch.Tensor, seqs: Sequences, Hq: int, Hkv: int, D: int, scale: float,
@@ -187,9 +223,10 @@ def attention_fwd(qkv: torch.Tensor, seqs: Sequences, Hq: int, Hkv: int, D: int,
     computed one by one, slowly).  A score of NaN or plus infinity makes its row NaN, on the GPU its lse too."""
     if qkv.is_cuda:
         return tuple(ext().packed_attn_fwd(qkv, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out, status_word(qkv.device)))
-    _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, "attention_fwd")
-    if out is not None and (tuple(out.shape) != (seqs.rows, Hq * D) or out.dtype != qkv.dtype or out.device != qkv.device):
-        raise ValueError(f"attention_fwd: out [{seqs.rows}, {Hq * D}] of {qkv.dtype} beside qkv")
+    _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, scale, "attention_fwd")
+    if out is not None:
+        _check_rows(out, qkv, seqs.rows, Hq * D, "attention_fwd", "out")
+        _check_apart(out, "attention_fwd", qkv=qkv)
     o, lse = ref.packed_attention(qkv, ref.segments(seqs.offs, seqs.rows), Hq, Hkv, D, scale)
     if out is not None:
         live = seqs.pos >= 0
@@ -207,11 +244,15 @@ def attention_bwd(qkv: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: tor
     if qkv.is_cuda:
         return ext().packed_attn_bwd(qkv, o, lse, do, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out,
                                      status_word(qkv.device))
-    _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, "attention_bwd")
-    _check(o, Hq * D, seqs, Hq, Hkv, D, "attention_bwd", "o")
-    _check(do, Hq * D, seqs, Hq, Hkv, D, "attention_bwd", "do")
-    if out is not None and (out.shape != qkv.shape or out.dtype != qkv.dtype or out.device != qkv.device):
-        raise ValueError(f"attention_bwd: out {tuple(qkv.shape)} of {qkv.dtype} beside qkv")
+    who = "attention_bwd"
+    _check(qkv, (Hq + 2 * Hkv) * D, seqs, Hq, Hkv, D, scale, who)
+    _check_rows(o, qkv, seqs.rows, Hq * D, who, "o")
+    _check_rows(do, qkv, seqs.rows, Hq * D, who, "do")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, seqs.rows) or lse.device != qkv.device:
+        raise ValueError(f"{who}: lse [{Hq}, {seqs.rows}] fp32 beside qkv, got {tuple(lse.shape)} of {lse.dtype}")
+    if out is not None:
+        _check_rows(out, qkv, seqs.rows, qkv.shape[1], who, "out")
+        _check_apart(out, who, qkv=qkv, o=o, do=do)
     segs = ref.segments(seqs.offs, seqs.rows)
     if all(lo == hi for lo, hi in segs):
         return torch.zeros_like(qkv) if out is None else out
