@@ -297,16 +297,23 @@ SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // -lse, -d
 }
 
 // What dS is multiplied by before it is rounded to T, as a power of two's exponent: fp16 would lose the small gradients of a
-// long row (do of 1e-4 over 1000 keys: dS near 1e-6, where its steps are 6e-8) and overflow with large ones.  do times it
-// has its largest value in [1, 2).  Nothing for bf16, which has fp32's range.
-template <typename T>
-SB_DEVICE int ds_shift(const Args& a);
-template <>
-SB_DEVICE int ds_shift<__nv_bfloat16>(const Args&) { return 0; }
-template <>
-SB_DEVICE int ds_shift<__half>(const Args& a) {
-  const int e = *a.largest >> 23;                      // 0: no gradient, 255: an infinite one
+// long row (do of 1e-4 over 1000 keys: dS near 1e-6, where its steps are 6e-8) and overflow with large ones.  The largest |do|
+// times it lies in [1, 2): of the query's own row and head for dQ, and for dK and dV of the rows that see the key, from it to
+// its sequence's end, in the heads of its group.  So what scales a row's sums hangs on what is in them and on nothing else.
+// Nothing for bf16, which has fp32's range.
+SB_DEVICE int shift_for(float top) {
+  const int e = __float_as_int(top) >> 23;             // 0: no gradient, 255: an infinite one
   return e == 0 || e == 255 ? 0 : max(-100, min(100, 127 - e));
+}
+template <typename T>
+SB_DEVICE int query_shift(const Args& a, int h, int row) {
+  if constexpr (Half<T>::kFormat == 0) return shift_for(a.tops[static_cast<long>(h) * (a.tiles * 128) + row]);
+  return 0;
+}
+template <typename T>
+SB_DEVICE int key_shift(const Args& a, int kvh, int row) {
+  if constexpr (Half<T>::kFormat == 0) return a.shifts[static_cast<long>(kvh) * (a.tiles * 128) + row];
+  return 0;
 }
 
 // Columns [c0, c1) of one row of dQ.

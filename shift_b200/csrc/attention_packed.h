@@ -29,7 +29,8 @@ struct Args {
   void* dqkv;
   long dqkv_ld;
   float* partial;             // split > 1: fp32 [split][Hkv][T][2 D]
-  int* largest;               // backward, fp16: bits of the largest |do|, else null
+  float* tops;                // backward, fp16: [Hq][tiles * 128] the largest |do| of a row of a head, else null
+  int* shifts;                // and [Hkv][tiles * 128] what dS of a key is scaled by
   int fill;                   // rows that no sequence covers get zeros
   int* status;
 };

@@ -45,21 +45,49 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args 
   }
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(lanes, s, o);
-  if (a.largest != nullptr) {                        // one atomic a CTA; a maximum does not hang on their order
-    __shared__ float tops[8];
-    top = warp_max(top);
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 8; ++w) top = fmaxf(top, tops[w]);
-      atomicMax(a.largest, __float_as_int(top));
-    }
+  if (a.tops != nullptr) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
+    if (there && sub == 0) a.tops[static_cast<long>(h) * (a.tiles * 128) + row] = top;
   }
   if (there && sub == 0) {
     float* p = out + (static_cast<long>(h) * (a.tiles * 2) + row / 64) * 128 + row % 64;
     p[0] = nl;
     p[64] = -s;
   }
+}
+
+// fp16: every key's shift, from the largest |do| of the rows that see it.  A CTA has 1024 rows of a key head: maxima from a row to
+// its sequence's end within a warp, then over the warps behind it, then over what the sequence has behind the CTA's rows, which
+// it reads itself (for one sequence of n rows that is n^2 / 2048 values in all, beside n^2 / 2 products).
+__global__ void __launch_bounds__(1024) shift_kernel(const __grid_constant__ Args a) {
+  __shared__ float first[32], behind[32];
+  const long pad = static_cast<long>(a.tiles) * 128;
+  const float* tops = a.tops + static_cast<long>(blockIdx.y) * a.group * pad;
+  const int c0 = blockIdx.x * 1024, row = c0 + threadIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto top_of = [&](int r) {
+    float m = 0.f;
+    for (int h = 0; h < a.group; ++h) m = fmaxf(m, tops[h * pad + r]);
+    return m;
+  };
+  const int stop = row < a.T ? a.stop[row] : row;      // of a row of no sequence: the row itself
+  float m = row < a.T ? top_of(row) : 0.f;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float other = __shfl_down_sync(0xffffffffu, m, o);
+    if (lane + o < 32 && row + o < stop) m = fmaxf(m, other);
+  }
+  if (lane == 0) first[warp] = m;
+  const int c1 = min(c0 + 1024, a.T), end = a.stop[c1 - 1];
+  float far = 0.f;
+  for (int r = c1 + threadIdx.x; r < end; r += 1024) far = fmaxf(far, top_of(r));
+  far = warp_max(far);
+  if (lane == 0) behind[warp] = far;
+  __syncthreads();
+  for (int w = warp + 1; w < 32 && c0 + w * 32 < stop; ++w) m = fmaxf(m, first[w]);
+  if (stop > c1)
+    for (int w = 0; w < 32; ++w) m = fmaxf(m, behind[w]);
+  if (row < pad) a.shifts[blockIdx.y * pad + row] = shift_for(m);
 }
 
 // ============================ dK, dV ============================
@@ -273,8 +301,6 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     const uint32_t ts = tbase + w * (F::kWide ? 64 : 128) + lane_off;
     const uint32_t tp = tbase + F::kP + w * (F::kWide ? 32 : 128) + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-    const int shift = ds_shift<T>(a);
-    const float2 up = make_float2(ldexpf(1.f, shift), ldexpf(1.f, shift));
     int g = 0, nkv = 0;
     bool ok = true, in_ready = false, s_ready = false;
     DkvItem it(a, blockIdx.x, F::kW);
@@ -282,6 +308,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       const int row = it.k0 + (warp % 4) * 32 + lane;
       const int end = row < a.T ? a.stop[row] : row;
       const int least = a.stop[it.k0];                 // the tile's earliest end
+      const int shift = key_shift<T>(a, it.kvh, row);
+      const float2 up = make_float2(ldexpf(1.f, shift), ldexpf(1.f, shift));
       for (int s = 0; s < it.subs; ++s, ++g) {
         if (!F::kWide && (g & 1) != w) continue;
         const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * F::kW + (F::kWide ? w * 64 : 0);
@@ -649,8 +677,6 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tbase + w * 64 + lane_off, tp = tbase + F::kP + w * 32 + lane_off;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-    const int shift = ds_shift<T>(a);                  // of dS: in its exponential's argument
-    const float out_scale = ldexpf(a.scale, -shift);
     int g = 0, nq = 0;
     bool ok = true, s_ready = false;
     DqItem it(a, blockIdx.x);
@@ -659,6 +685,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       const int st = row < a.T ? a.start[row] : row + 1;
       const int most = a.start[min(it.q0 + 127, a.T - 1)];
       const float* rb = row_block(a, it.h, row);       // there are rows up to a multiple of 128
+      const int shift = query_shift<T>(a, it.h, row);  // of dS: in its exponential's argument
+      const float out_scale = ldexpf(a.scale, -shift);
       const float2 nl = make_float2(rb[0] + shift, rb[0] + shift), nd = make_float2(rb[64], rb[64]);
       for (int j = it.lo; j < it.hi; ++j, ++g) {
         if (!warp_wait(s_full, g & 1, a.status, s_ready)) {
@@ -772,6 +800,8 @@ static void launch(const CUtensorMap& tm128, const CUtensorMap& tm64, const CUte
   const long work = static_cast<long>(a.tiles) * 128 * a.Hq;
   rows_kernel<D, T><<<static_cast<unsigned>((work + 256 / (D / 8) - 1) / (256 / (D / 8))), 256, 0, stream>>>(a, rows);
   a.rows = rows;
+  if (a.tops != nullptr)
+    shift_kernel<<<dim3((a.tiles * 128 + 1023) / 1024, a.Hkv), 1024, 0, stream>>>(a);
   cudaFuncSetAttribute(dkv_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dkv<D>::kSmem);
   cudaFuncSetAttribute(dq_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dq<D>::kSmem);
   a.order = k_order;

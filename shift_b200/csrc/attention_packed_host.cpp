@@ -163,10 +163,12 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
   a.dqkv = dqkv.data_ptr();
   a.dqkv_ld = row_stride(dqkv);
   auto row_values = at::empty({Hq * a.tiles * 256}, lse.options());
-  at::Tensor largest;
-  if (qkv.scalar_type() == at::kHalf) {              // fp16 holds dS over some 2^30: it is scaled by the largest |do|
-    largest = at::zeros({1}, lse.options().dtype(at::kInt));
-    a.largest = largest.data_ptr<int>();
+  at::Tensor scales;
+  if (qkv.scalar_type() == at::kHalf) {              // fp16 holds dS over some 2^30: rows and keys scale it by powers of two
+    TORCH_CHECK(Hkv <= 65535, who, ": at most 65535 key heads in fp16, got ", Hkv);
+    scales = at::empty({(Hq + Hkv) * a.tiles * 128}, lse.options());
+    a.tops = scales.data_ptr<float>();
+    a.shifts = reinterpret_cast<int*>(a.tops + Hq * a.tiles * 128);
   }
   // A key tile meets every later query of its sequence in every head of its group: with few tiles the group's heads are
   // dealt out over several CTAs, whose fp32 sums are added up in order afterwards.
