@@ -292,7 +292,12 @@ __device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float
     if (lane * N + i >= c0 && lane * N + i < c1) out[lane * N + i] = from_float<T>(acc[i]);
 }
 
-SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // -lse, -delta of query q (64 apart)
+// P of the backward pass is normalised, so over 16384 keys a usual one is where fp16's numbers lose bits and below 3e-8 it would
+// be 0.  It is at most 1 and fp16 goes to 2^16: the row values that it is computed from hold 15 more, and dV is scaled back.
+template <typename T>
+__device__ constexpr int kUpP = Half<T>::kFormat == 0 ? 15 : 0;
+
+SB_DEVICE const float* row_block(const Args& a, int h, int q) {      // kUpP - lse, -delta of query q (64 apart)
   return a.rows + (static_cast<long>(h) * (a.tiles * 2) + q / 64) * 128 + q % 64;
 }
 
@@ -333,7 +338,7 @@ __device__ __noinline__ void slow_dq(const Args& a, int row, int h, int st, int 
   for (int j = st; j <= row; ++j) {
     load_part<D>(x + j * a.ld + kc, k);
     load_part<D>(x + j * a.ld + vc, v);
-    const float ds = ex2(dot<N>(q, k) * a.scale_log2 + rb[0]) * (dot<N>(g, v) + rb[64]);
+    const float ds = ex2(dot<N>(q, k) * a.scale_log2 + (rb[0] - kUpP<T>)) * (dot<N>(g, v) + rb[64]);
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] += ds * k[i];
   }
@@ -371,7 +376,7 @@ __device__ __noinline__ void slow_dkv(const Args& a, int row, int kvh, int h0, i
       load_part<D>(x + j * a.ld + static_cast<long>(h) * D, q);
       load_part<D>(static_cast<const T*>(a.dout) + j * a.do_ld + static_cast<long>(h) * D, g);
       const float* rb = row_block(a, h, j);
-      const float p = ex2(dot<N>(q, k) * a.scale_log2 + rb[0]);
+      const float p = ex2(dot<N>(q, k) * a.scale_log2 + (rb[0] - kUpP<T>));
       const float ds = p * (dot<N>(g, v) + rb[64]);
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] += want_k ? ds * q[i] : p * g[i];

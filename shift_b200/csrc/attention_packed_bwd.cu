@@ -21,8 +21,8 @@ namespace pa {
 
 constexpr int kOnFma = 2;          // of 8 exponentials, those computed on the FMA pipe (of 64, 8 x 2048: 343 us, 1: 345)
 
-// -lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes have
-// a row of a head.
+// kUpP - lse log2(e) and -delta of every query, [Hq][2 tiles][2][64]; zeros for rows of no sequence.  Eight or sixteen lanes
+// have a row of a head.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args a, float* __restrict__ out) {
   constexpr int L = D / 8;
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args 
       s += to_float(x[k]) * to_float(y[k]);
       top = fmaxf(top, fabsf(to_float(y[k])));
     }
-    nl = -a.lse[static_cast<long>(h) * a.T + row] * kLog2e;
+    nl = fmaf(-a.lse[static_cast<long>(h) * a.T + row], kLog2e, static_cast<float>(kUpP<T>));
   }
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(lanes, s, o);
@@ -57,9 +57,9 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args 
   }
 }
 
-// fp16: every key's shift, from the largest |do| of the rows that see it.  A CTA has 1024 rows of a key head: maxima from a row to
-// its sequence's end within a warp, then over the warps behind it, then over what the sequence has behind the CTA's rows, which
-// it reads itself (for one sequence of n rows that is n^2 / 2048 values in all, beside n^2 / 2 products).
+// fp16: every key's shift, from the largest |do| of the rows that see it.  A CTA has 1024 rows of a key head: maxima from a row
+// to its sequence's end within a warp, then over the warps behind it, then over what the sequence has behind the CTA's rows,
+// which it reads itself (for one sequence of n rows that is n^2 / 2048 values in all, beside n^2 / 2 products).
 __global__ void __launch_bounds__(1024) shift_kernel(const __grid_constant__ Args a) {
   __shared__ float first[32], behind[32];
   const long pad = static_cast<long>(a.tiles) * 128;
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(1024) shift_kernel(const __grid_constant__ Arg
   if (lane == 0) first[warp] = m;
   const int c1 = min(c0 + 1024, a.T), end = a.stop[c1 - 1];
   float far = 0.f;
+#pragma unroll 4
   for (int r = c1 + threadIdx.x; r < end; r += 1024) far = fmaxf(far, top_of(r));
   far = warp_max(far);
   if (lane == 0) behind[warp] = far;
@@ -309,7 +310,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       const int end = row < a.T ? a.stop[row] : row;
       const int least = a.stop[it.k0];                 // the tile's earliest end
       const int shift = key_shift<T>(a, it.kvh, row);
-      const float2 up = make_float2(ldexpf(1.f, shift), ldexpf(1.f, shift));
+      const float2 up = make_float2(ldexpf(1.f, shift - kUpP<T>), ldexpf(1.f, shift - kUpP<T>));
       for (int s = 0; s < it.subs; ++s, ++g) {
         if (!F::kWide && (g & 1) != w) continue;
         const int st = g % F::kStages, q0 = it.k0 + s % it.blocks * F::kW + (F::kWide ? w * 64 : 0);
@@ -400,7 +401,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
         }
         ++nkv;
         tc_fence_after();
-        const float f = dk ? ldexpf(a.scale, -shift) : 1.f;
+        const float f = dk ? ldexpf(a.scale, -shift) : ldexpf(1.f, -kUpP<T>);
         float chk = 0.f;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -687,7 +688,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       const float* rb = row_block(a, it.h, row);       // there are rows up to a multiple of 128
       const int shift = query_shift<T>(a, it.h, row);  // of dS: in its exponential's argument
       const float out_scale = ldexpf(a.scale, -shift);
-      const float2 nl = make_float2(rb[0] + shift, rb[0] + shift), nd = make_float2(rb[64], rb[64]);
+      const float2 nl = make_float2(rb[0] + (shift - kUpP<T>), rb[0] + (shift - kUpP<T>)), nd = make_float2(rb[64], rb[64]);
       for (int j = it.lo; j < it.hi; ++j, ++g) {
         if (!warp_wait(s_full, g & 1, a.status, s_ready)) {
           ok = false;

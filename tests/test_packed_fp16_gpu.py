@@ -1,4 +1,4 @@
-"""fp16 gradients of packed attention: what scales them for one row is not seen by others."""
+"""fp16 gradients of packed attention: what scales them for one row is not seen by others, and probabilities of long rows count."""
 import math
 
 import pytest
@@ -85,3 +85,15 @@ def test_an_infinite_gradient_elsewhere(D):
             w = exact["dqkv"][rows_, cols]
             assert (got[rows_, cols].double() - w).norm() <= 3 * 2.0 ** -11 * w.norm() + 2.0 ** -25 * w.numel() ** 0.5
     assert not torch.isfinite(got[350, :D]).any() and not torch.isfinite(got[300:351, 4 * D:5 * D]).any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_probabilities_below_what_fp16_holds(D):
+    """70000 keys of equal scores: a probability is 1.4e-5, in fp16 a number of eight bits.  dV is their sum over the last rows'
+    do alone, so nothing averages the error out; each is rounded to 11 bits, and so is the result."""
+    rows, heads = 70001, (1, 1, D, 1.0)
+    qkv, do = torch.zeros(rows, 3 * D, dtype=torch.float16, device=DEV), torch.zeros(rows, D, dtype=torch.float16, device=DEV)
+    do[-1] = _randn(D, seed=10) * 64 + 256
+    got = _step(qkv, do, [0, rows], heads)[:, 2 * D:].double()
+    want = do[-1].double() / rows
+    assert ((got - want).abs() <= 2.0 ** -11 * 2.02 * want.abs() + 2.0 ** -20 * want.abs() + orc.tiny(torch.float16)).all()
