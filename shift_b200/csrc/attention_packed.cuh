@@ -15,9 +15,9 @@
 //
 // What others hold.  Products run over whole blocks, so a masked value is a product with zero, which is zero unless the
 // other factor is infinite or NaN.  Rows that no sequence covers are cleared in shared memory after they were loaded.  Rows
-// of other sequences (or later ones of the same) that are not finite would leave NaN in a result: results
-// that are not finite are recognised when they are stored and, where such a row met them, computed again row by row from
-// what they see.
+// of other sequences (or later ones of the same) that are not finite would leave NaN in a result: results that are not finite
+// are recognised when they are stored and, where such a row met them, computed again row by row from what they see.  That may
+// take long, so it comes after a CTA's last item, when no wait of its pipeline hangs on it.
 //
 // Every wait is bounded; on expiry the kernel records a status code and winds down.
 #pragma once
@@ -225,17 +225,78 @@ SB_DEVICE void clear_rows(uint8_t* tile, int n, int chunks, int next, int row0, 
         *reinterpret_cast<uint4*>(tile + c * next + r * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
 }
 
+// ---------------------------------------------------------------------------
+// Results that are computed again.  A warp keeps those that it found in a list through global memory, a slot for each of its
+// items; when the CTA has no item left its eight softmax warps share all of them, row by row.
+// ---------------------------------------------------------------------------
+struct Later {
+  int2* slots;                // [items][8]: a bit for each row (lane), the slot before or -1
+  int last;
+  SB_DEVICE void add(unsigned bits, int item) {        // by a whole warp
+    if (bits == 0) return;
+    const int slot = item * 8 + static_cast<int>(threadIdx.x) / 32;
+    if (threadIdx.x % 32 == 0) slots[slot] = make_int2(static_cast<int>(bits), last);
+    last = slot;
+  }
+  // `again(item, warp that found it, row's lane)`; `heads`: shared memory of 8 ints
+  template <typename F>
+  SB_DEVICE void run(int* heads, const F& again) const {
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0) heads[warp] = last;
+    __syncwarp();
+    asm volatile("bar.sync 1, 256;" ::: "memory");     // the softmax warps alone
+    int n = 0;
+    for (int w = 0; w < 8; ++w)
+      for (int slot = heads[w]; slot >= 0;) {
+        const int2 s = slots[slot];
+        for (unsigned bits = static_cast<unsigned>(s.x); bits != 0; bits &= bits - 1)
+          if (n++ % 8 == warp) again(slot / 8, w, __ffs(bits) - 1);
+        slot = s.y;
+      }
+  }
+};
+
+// A warp has four rows of an operand at a time, eight lanes a row: this lane's D / 8 columns, from `first_column`.
+template <int D>
+SB_DEVICE int first_column() { return static_cast<int>(threadIdx.x) % 8 * (D / 8); }
+SB_DEVICE int quarter() { return static_cast<int>(threadIdx.x) % 32 / 8; }
 template <int D, typename T>
-SB_DEVICE void load_part(const T* p, float* f) {       // this lane's D / 32 columns
+SB_DEVICE void load_part(const T* p, float* f) {
+  const uint4* v = reinterpret_cast<const uint4*>(p + first_column<D>());
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) f[i] = to_float(p[(threadIdx.x % 32) * (D / 32) + i]);
+  for (int i = 0; i < D / 64; ++i) {
+    const uint4 u = v[i];
+    const T* x = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[i * 8 + k] = to_float(x[k]);
+  }
 }
 template <int N>
-SB_DEVICE float dot(const float* a, const float* b) {
+SB_DEVICE float dot(const float* a, const float* b) {   // over a row's eight lanes
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) s += a[i] * b[i];
-  return warp_sum(s);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+// the four quarters' sums joined, to columns [c0, c1) of 16-bit rows
+template <int D, typename T>
+SB_DEVICE void store_part(T* out, float* acc, float scale, int c0, int c1) {
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);
+    acc[i] *= scale;
+  }
+  const int c = first_column<D>();
+  if (quarter() != 0 || out == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < D / 8; i += 8)
+    if (c + i >= c0 && c + i < c1)
+      *reinterpret_cast<uint4*>(out + c + i) =
+          make_uint4(Half<T>::pack(acc[i], acc[i + 1]), Half<T>::pack(acc[i + 2], acc[i + 3]),
+                     Half<T>::pack(acc[i + 4], acc[i + 5]), Half<T>::pack(acc[i + 6], acc[i + 7]));
 }
 
 // Whether rows [lo, st) and [end, hi) of an operand, which a result's masked zeros met, have something there that zero times
@@ -243,7 +304,7 @@ SB_DEVICE float dot(const float* a, const float* b) {
 // have not, what is not finite in the result is its own, and a step that has gone wrong as a whole takes no longer for it.
 template <int D, typename T>
 SB_DEVICE bool touched(const T* p, long ld, int lo, int st, int end, int hi, uint32_t own) {
-  constexpr int N = D / 32;
+  constexpr int N = D / 8;
   constexpr int kMost = 1024;                          // rows: with more of them it is the result that is computed
   const bool open = (~own & ((1u << N) - 1)) != 0;
   if (!__any_sync(0xffffffffu, open)) return false;
@@ -251,7 +312,7 @@ SB_DEVICE bool touched(const T* p, long ld, int lo, int st, int end, int hi, uin
   if (n > kMost) return true;
   uint32_t bad = 0;
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = quarter(); i < n; i += 4) {
     float f[N];
     load_part<D>(p + static_cast<long>(i < before ? lo + i : end + i - before) * ld, f);
 #pragma unroll
@@ -269,27 +330,27 @@ SB_DEVICE uint32_t nan_columns(const float* f) {
 
 // Columns [c0, c1) of one row of O by a whole warp, from what the row sees alone, if others have got into it.
 template <int D, typename T>
-__device__ __noinline__ void slow_o(const Args& a, int row, int h, int st, float lse2, int c0, int c1) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x % 32;
+__device__ __noinline__ void slow_o(const Args& a, int row, int h, int c0, int c1) {
+  constexpr int N = D / 8;
   const T* x = static_cast<const T*>(a.qkv);
   const long kc = static_cast<long>(a.Hq + h / a.group) * D, vc = kc + static_cast<long>(a.Hkv) * D;
   float q[N], k[N], v[N], acc[N] = {};
   load_part<D>(x + row * a.ld + vc, v);
-  const int q0 = row / 128 * 128;
+  const int q0 = row / 128 * 128, st = a.start[row];
   if (!touched<D>(x + vc, a.ld, a.start[q0] / 128 * 128, st, row + 1, min(q0 + 128, a.T), nan_columns<N>(v))) return;
+  const float lse2 = a.lse[static_cast<long>(h) * a.T + row] * kLog2e;
   load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
-  for (int j = st; j <= row; ++j) {
+#pragma unroll 2
+  for (int j0 = st; j0 <= row; j0 += 4) {              // the same number of times in every lane
+    const int j = min(j0 + quarter(), row);
     load_part<D>(x + j * a.ld + kc, k);
     load_part<D>(x + j * a.ld + vc, v);
     const float p = ex2(dot<N>(q, k) * a.scale_log2 - lse2);
+    if (j0 + quarter() <= row)
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += p * v[i];
+      for (int i = 0; i < N; ++i) acc[i] += p * v[i];
   }
-  T* out = static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane * N + i >= c0 && lane * N + i < c1) out[lane * N + i] = from_float<T>(acc[i]);
+  store_part<D>(static_cast<T*>(a.o) + row * a.o_ld + static_cast<long>(h) * D, acc, 1.f, c0, c1);
 }
 
 // P of the backward pass is normalised, so over 16384 keys a usual one is where fp16's numbers lose bits and below 3e-8 it would
@@ -323,71 +384,72 @@ SB_DEVICE int key_shift(const Args& a, int kvh, int row) {
 
 // Columns [c0, c1) of one row of dQ.
 template <int D, typename T>
-__device__ __noinline__ void slow_dq(const Args& a, int row, int h, int st, int c0, int c1) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x % 32;
+__device__ __noinline__ void slow_dq(const Args& a, int row, int h, int c0, int c1) {
+  constexpr int N = D / 8;
   const T* x = static_cast<const T*>(a.qkv);
   const long kc = static_cast<long>(a.Hq + h / a.group) * D, vc = kc + static_cast<long>(a.Hkv) * D;
   float q[N], g[N], k[N], v[N], acc[N] = {};
+  const float* rb = row_block(a, h, row);
+  const float nl = rb[0] - kUpP<T>, nd = rb[64];
+  const int q0 = row / 128 * 128, st = a.start[row];
+  const uint32_t own = nl != nl || nd != nd ? ~0u : 0u;
+  if (!touched<D>(x + kc, a.ld, a.start[q0] / 128 * 128, st, row + 1, min(q0 + 128, a.T), own)) return;
   load_part<D>(x + row * a.ld + static_cast<long>(h) * D, q);
   load_part<D>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D, g);
-  const float* rb = row_block(a, h, row);
-  const int q0 = row / 128 * 128;
-  const uint32_t own = rb[0] != rb[0] || rb[64] != rb[64] ? ~0u : 0u;
-  if (!touched<D>(x + kc, a.ld, a.start[q0] / 128 * 128, st, row + 1, min(q0 + 128, a.T), own)) return;
-  for (int j = st; j <= row; ++j) {
+#pragma unroll 2
+  for (int j0 = st; j0 <= row; j0 += 4) {
+    const int j = min(j0 + quarter(), row);
     load_part<D>(x + j * a.ld + kc, k);
     load_part<D>(x + j * a.ld + vc, v);
-    const float ds = ex2(dot<N>(q, k) * a.scale_log2 + (rb[0] - kUpP<T>)) * (dot<N>(g, v) + rb[64]);
+    const float p = ex2(dot<N>(q, k) * a.scale_log2 + nl), ds = p * (dot<N>(g, v) + nd);
+    if (j0 + quarter() <= row)
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += ds * k[i];
+      for (int i = 0; i < N; ++i) acc[i] += ds * k[i];
   }
-  T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(h) * D;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane * N + i >= c0 && lane * N + i < c1) out[lane * N + i] = from_float<T>(acc[i] * a.scale);
+  store_part<D>(static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(h) * D, acc, a.scale, c0, c1);
 }
 
 // One row of dK (want_k) or dV of key head kvh, over query heads [h0, h1), to 16 bits or, where a split's sum follows, fp32.
 template <int D, typename T>
-__device__ __noinline__ void slow_dkv(const Args& a, int row, int kvh, int h0, int h1, int end, bool want_k, float* partial) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x % 32;
+__device__ __noinline__ void slow_dkv(const Args& a, int row, int kvh, int h0, int h1, bool want_k, float* partial) {
+  constexpr int N = D / 8;
   const T* x = static_cast<const T*>(a.qkv);
+  const T* dout = static_cast<const T*>(a.dout);
   const long kc = static_cast<long>(a.Hq + kvh) * D, vc = kc + static_cast<long>(a.Hkv) * D;
   float q[N], g[N], k[N], v[N], acc[N] = {};
   const int k0 = row / 128 * 128, hi = min(k0 + (a.stop[min(k0 + 127, a.T - 1)] - k0 + 127) / 128 * 128, a.T);
+  const int end = a.stop[row];
   uint32_t own = 0;
   for (int h = h0; h < h1; ++h) {
     const float* rb = row_block(a, h, row);
-    load_part<D>(static_cast<const T*>(a.dout) + row * a.do_ld + static_cast<long>(h) * D, g);
+    load_part<D>(dout + row * a.do_ld + static_cast<long>(h) * D, g);
     own |= rb[0] != rb[0] || (want_k && rb[64] != rb[64]) ? ~0u : want_k ? 0u : nan_columns<N>(g);
   }
   bool others = false;
-  for (int h = h0; h < h1 && !others; ++h) {
-    const T* p = want_k ? x : static_cast<const T*>(a.dout);
-    others = touched<D>(p + static_cast<long>(h) * D, want_k ? a.ld : a.do_ld, k0, row, end, hi, own);
-  }
+  for (int h = h0; h < h1 && !others; ++h)
+    others = touched<D>((want_k ? x : dout) + static_cast<long>(h) * D, want_k ? a.ld : a.do_ld, k0, row, end, hi, own);
   if (!others) return;
   load_part<D>(x + row * a.ld + kc, k);
   load_part<D>(x + row * a.ld + vc, v);
   for (int h = h0; h < h1; ++h)
-    for (int j = row; j < end; ++j) {
+#pragma unroll 2
+    for (int j0 = row; j0 < end; j0 += 4) {
+      const int j = min(j0 + quarter(), end - 1);
       load_part<D>(x + j * a.ld + static_cast<long>(h) * D, q);
-      load_part<D>(static_cast<const T*>(a.dout) + j * a.do_ld + static_cast<long>(h) * D, g);
+      load_part<D>(dout + j * a.do_ld + static_cast<long>(h) * D, g);
       const float* rb = row_block(a, h, j);
       const float p = ex2(dot<N>(q, k) * a.scale_log2 + (rb[0] - kUpP<T>));
       const float ds = p * (dot<N>(g, v) + rb[64]);
+      if (j0 + quarter() < end)
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += want_k ? ds * q[i] : p * g[i];
+        for (int i = 0; i < N; ++i) acc[i] += want_k ? ds * q[i] : p * g[i];
     }
   T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + (want_k ? kc : vc);
+  store_part<D>(partial != nullptr ? static_cast<T*>(nullptr) : out, acc, want_k ? a.scale : 1.f, 0, D);
+  if (partial != nullptr && quarter() == 0)
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = want_k ? acc[i] * a.scale : acc[i];
-    if (partial != nullptr) partial[lane * N + i] = y;
-    else out[lane * N + i] = from_float<T>(y);
-  }
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(partial + first_column<D>() + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
 }
 
 }  // namespace pa

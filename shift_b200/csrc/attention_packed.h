@@ -31,6 +31,7 @@ struct Args {
   float* partial;             // split > 1: fp32 [split][Hkv][T][2 D]
   float* tops;                // backward, fp16: [Hq][tiles * 128] the largest |do| of a row of a head, else null
   int* shifts;                // and [Hkv][tiles * 128] what dS of a key is scaled by
+  int2* later;                // [items][8 warps]: results to be computed again
   int fill;                   // rows that no sequence covers get zeros
   int* status;
 };

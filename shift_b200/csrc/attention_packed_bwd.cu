@@ -138,6 +138,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
   uint64_t *s_empty = p_full + 2, *p_free = s_empty + 2;
   const Sched sched{answer, p_free + 2, p_free + 4};
   uint32_t* tslot = reinterpret_cast<uint32_t*>(p_free + 6);
+  int* lists = reinterpret_cast<int*>(tslot + 1);      // [8]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -305,6 +306,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     int g = 0, nkv = 0;
     bool ok = true, in_ready = false, s_ready = false;
     DkvItem it(a, blockIdx.x, F::kW);
+    Later later{a.later, -1};
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int row = it.k0 + (warp % 4) * 32 + lane;
       const int end = row < a.T ? a.stop[row] : row;
@@ -386,6 +388,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       const bool covered = row < a.T && end > row;
       const bool dk = w == 1;
       const DkvItem at = it;
+      const int item = idx;
       idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
       if (idx >= 0) it = DkvItem(a, idx, F::kW);
       const long col = static_cast<long>(a.Hq + (dk ? 0 : a.Hkv) + at.kvh) * D;
@@ -439,12 +442,17 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
       if (row < a.T && !covered && a.fill && at.part == 0)
 #pragma unroll
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
-      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
-        const int who = __ffs(some) - 1, r = __shfl_sync(0xffffffffu, row, who);
-        slow_dkv<D, T>(a, r, at.kvh, at.first_h, at.first_h + at.heads, __shfl_sync(0xffffffffu, end, who), dk,
-                       partial == nullptr ? nullptr : partial + static_cast<long>(r - row) * (2 * D));
-      }
+      later.add(__ballot_sync(0xffffffffu, bad), item);
     }
+    later.run(lists, [&](int item, int finder, int who) {
+      const DkvItem at(a, item, F::kW);
+      const int row = at.k0 + finder % 4 * 32 + who;
+      const bool dk = finder / 4 == 1;
+      float* partial = nullptr;
+      if (a.split > 1)
+        partial = a.partial + ((static_cast<long>(at.part) * a.Hkv + at.kvh) * a.T + row) * (2 * D) + (dk ? 0 : D);
+      slow_dkv<D, T>(a, row, at.kvh, at.first_h, at.first_h + at.heads, dk, partial);
+    });
   }
   tc_fence_before();
   __syncthreads();
@@ -513,6 +521,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
   uint64_t *s_full = v_empty + F::kV, *p_full = s_full + 2, *s_empty = p_full + 2, *p_free = s_empty + 2;
   const Sched sched{answer, p_free + 2, p_free + 4};
   uint32_t* tslot = reinterpret_cast<uint32_t*>(p_free + 6);
+  int* lists = reinterpret_cast<int*>(tslot + 1);      // [8]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -681,6 +690,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
     int g = 0, nq = 0;
     bool ok = true, s_ready = false;
     DqItem it(a, blockIdx.x);
+    Later later{a.later, -1};
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int row = it.q0 + (warp % 4) * 32 + lane;
       const int st = row < a.T ? a.start[row] : row + 1;
@@ -742,6 +752,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       if (!ok) break;
       const bool covered = row < a.T && st <= row;
       const DqItem at = it;
+      const int item = idx;
       idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
       if (idx >= 0) it = DqItem(a, idx);
       T* out = static_cast<T*>(a.dqkv) + row * a.dqkv_ld + static_cast<long>(at.h) * D;
@@ -782,12 +793,12 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
       if (row < a.T && !covered && a.fill)
 #pragma unroll
         for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(out + w * (D / 2) + c) = make_uint4(0, 0, 0, 0);
-      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
-        const int who = __ffs(some) - 1;
-        slow_dq<D, T>(a, __shfl_sync(0xffffffffu, row, who), at.h, __shfl_sync(0xffffffffu, st, who), w * (D / 2),
-                      (w + 1) * (D / 2));
-      }
+      later.add(__ballot_sync(0xffffffffu, bad), item);
     }
+    later.run(lists, [&](int item, int finder, int who) {
+      const DqItem at(a, item);
+      slow_dq<D, T>(a, at.q0 + finder % 4 * 32 + who, at.h, finder / 4 * (D / 2), (finder / 4 + 1) * (D / 2));
+    });
   }
   tc_fence_before();
   __syncthreads();

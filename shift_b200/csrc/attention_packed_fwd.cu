@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
   const Sched sched{answer, drain + 1, drain + 3};
   uint64_t* ml_full = drain + 5;                       // SPLIT: a group's maxima and sums
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 7);
+  int* lists = reinterpret_cast<int*>(tslot + 1);      // [8]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const FwdItem first_item(a, blockIdx.x);             // its dependent loads run under the set-up
 
@@ -289,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
       }
     };
     Mine now(a, first_item, w);
+    Later later{a.later, -1};
     for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
       const int h = now.h, q0 = now.q0, lo = now.lo, hi = now.hi, row = now.row, st = now.st, most = now.most;
       float m = -INFINITY, l = 0.f;
@@ -379,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
         l += l2[0].x + l2[0].y;
       }
       if (!ok) break;
+      const int item = idx;
       idx = sched_next(sched, n, a.status);            // its tile is looked up while the last products run
       if (idx >= 0) now = Mine(a, FwdItem(a, idx), w);
       const bool covered = row < a.T && st <= row;
@@ -467,12 +470,14 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
 #pragma unroll
           for (int c = 0; c < kCols; c += 8) *reinterpret_cast<uint4*>(orow + c0 + c) = make_uint4(0, 0, 0, 0);
       }
-      for (unsigned some = __ballot_sync(0xffffffffu, bad); some != 0; some &= some - 1) {
-        const int who = __ffs(some) - 1;
-        slow_o<D, T>(a, __shfl_sync(0xffffffffu, row, who), h, __shfl_sync(0xffffffffu, st, who),
-                     __shfl_sync(0xffffffffu, lse2, who), c0, c0 + kCols);
-      }
+      later.add(__ballot_sync(0xffffffffu, bad), item);
     }
+    later.run(lists, [&](int item, int finder, int who) {
+      const Mine m(a, FwdItem(a, item), finder / 4);
+      constexpr int kCols = SPLIT ? D / 2 : D;
+      const int c0 = SPLIT ? finder / 4 * kCols : 0;
+      slow_o<D, T>(a, m.q0 + finder % 4 * 32 + who, m.h, c0, c0 + kCols);
+    });
   }
   tc_fence_before();
   __syncthreads();

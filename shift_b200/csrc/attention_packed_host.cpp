@@ -1,6 +1,7 @@
 // Causal attention over packed sequences: arguments, workspaces and launches.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
@@ -81,7 +82,7 @@ static Args base_args(const at::Tensor& qkv, const at::Tensor& plan, int64_t T, 
   const int* p = plan.data_ptr<int>();
   const int* o = p + 3 * T + 2;
   pl = Plan{p, p + 2 * T, p + 3 * T, o, o + nt, o + nt + nt2};
-  TORCH_CHECK(nt * Hq < (1L << 31), who, ": too many rows and heads");
+  TORCH_CHECK(nt * Hq <= (1L << 28), who, ": too many rows and heads");
   Args a{};
   a.T = static_cast<int>(T);
   a.Hq = static_cast<int>(Hq);
@@ -128,6 +129,8 @@ std::vector<at::Tensor> fwd(const at::Tensor& qkv, const at::Tensor& plan, int64
   const unsigned items = static_cast<unsigned>(a.split_keys     ? a.tiles * Hq
                                                : a.pair_heads ? a.tiles * (Hq / 2)
                                                               : (a.T + 255) / 256 * Hq);
+  const auto later = c10::cuda::CUDACachingAllocator::get()->allocate(items * 8 * sizeof(int2));
+  a.later = static_cast<int2*>(later.get());
   const CUtensorMap tm = tile_map(qkv, 128);
   const bool half = qkv.scalar_type() == at::kHalf;
   launch_fwd(static_cast<int>(D), half, tm, a, items, at::cuda::getCurrentCUDAStream());
@@ -162,7 +165,8 @@ at::Tensor bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& lse
   a.do_ld = row_stride(dout);
   a.dqkv = dqkv.data_ptr();
   a.dqkv_ld = row_stride(dqkv);
-  auto row_values = at::empty({Hq * a.tiles * 256}, lse.options());
+  auto row_values = at::empty({Hq * a.tiles * (256 + 16)}, lse.options());     // behind them [tiles * Hq][8] pairs of ints
+  a.later = reinterpret_cast<int2*>(row_values.data_ptr<float>() + Hq * a.tiles * 256);
   at::Tensor scales;
   if (qkv.scalar_type() == at::kHalf) {              // fp16 holds dS over some 2^30: rows and keys scale it by powers of two
     TORCH_CHECK(Hkv <= 65535, who, ": at most 65535 key heads in fp16, got ", Hkv);
