@@ -128,6 +128,12 @@ SB_DEVICE bool warp_wait(uint64_t* bar, uint32_t phase, int* status, bool ready 
   return __all_sync(0xffffffffu, mbar_wait(bar, phase, status));
 }
 
+// Before a CTA ends: the last `n` copies to these barriers' stages have landed in its memory.  They have, unless a wait ran out,
+// and then they take no longer than this.
+SB_DEVICE void landed(uint64_t* full, int stages, int n) {
+  for (int i = max(0, n - stages); i < n; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, nullptr, 10000000ull);
+}
+
 // Bits [from, to] of a word, clipped to it: which of 32 columns are seen.
 SB_DEVICE uint32_t seen(int from, int to) {
   const uint32_t low = to >= 31 ? 0xffffffffu : to < 0 ? 0u : (2u << to) - 1u;

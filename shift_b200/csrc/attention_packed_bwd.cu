@@ -175,7 +175,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
     regs_down<kOtherRegs>();
     if (warp == kLoader) {
       const int first = a.ends[0], last = min(a.ends[1], a.T);
-      int g = 0, nkv = 0, nl = 0;
+      int g = 0, nkv = 0, nl = 0, asked = 0;
       bool ok = true;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         if (lane == 0) ok = sched_request(sched, n, a.status);
@@ -224,7 +224,13 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm128, const __grid_constant__ CU
             }
           }
         }
+        asked = n + 1;
         if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {
+        landed(kv_full, 1, nkv);
+        landed(in_full, F::kStages, g);
+        landed(sched.full, 2, asked);
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, F::kW, 0), idG = idesc<T>(128, D, 1);
@@ -562,7 +568,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
     regs_down<kOtherRegs>();
     if (warp == kLoader) {
       const int first = a.ends[0], last = min(a.ends[1], a.T);
-      int g = 0, nq = 0, nl = 0;
+      int g = 0, nq = 0, nl = 0, asked = 0;
       bool ok = true;
       for (int n = 0, idx = blockIdx.x; idx >= 0 && ok; ++n) {
         if (lane == 0) ok = sched_request(sched, n, a.status);
@@ -613,7 +619,14 @@ dq_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtens
             }
           }
         }
+        asked = n + 1;
         if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {
+        landed(q_full, 1, nq);
+        landed(k_full, F::kK, g);
+        landed(v_full, F::kV, g);
+        landed(sched.full, 2, asked);
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 128, 0), idG = idesc<T>(128, D, 1);

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
     regs_down<kOtherRegs>();
     if (warp == kLoader) {
       const int first = a.ends[0], last = min(a.ends[1], a.T);
-      int nk = 0, nv = 0, nq = 0, nl = 0;
+      int nk = 0, nv = 0, nq = 0, nl = 0, asked = 0;
       bool ok = true;
       if (lane == 0) tma_prefetch_desc(&tm);
       FwdItem it = first_item;
@@ -168,7 +168,14 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_kernel(const __grid_constant_
             }
           }
         }
+        asked = n + 1;
         if (ok) idx = sched_next(sched, n, a.status);
+      }
+      if (lane == 0) {
+        landed(q_full, 1, nq);
+        landed(k_full, F::kK, nk);
+        landed(v_full, F::kV, nv);
+        landed(sched.full, 2, asked);
       }
     } else if (warp == kIssuer) {
       constexpr uint32_t idS = idesc<T>(128, 128, 0), idO = idesc<T>(128, D, 1);

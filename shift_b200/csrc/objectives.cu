@@ -350,14 +350,17 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
     if (a.t.weight != nullptr) weight = a.t.weight[r];
   }
   Run run;
+  bool late = false;
   if (KEEP) {
     __syncthreads();                               // the barriers are there
     for (int c = 0; c < kParts; ++c) {
-      mbar_wait(&bar[c], 0, a.status);
+      late |= !mbar_wait(&bar[c], 0, a.status);
       const int end = part(c + 1);
       for (int v = part(c) + threadIdx.x; v < end; v += kThreads) add_vec<T>(run, held[v - s.v0]);
     }
     add_edge(run, s);
+    if (late)                                      // the status says so; what was on its way here lands before anything else
+      for (int c = 0; c < kParts; ++c) mbar_wait(&bar[c], 0, nullptr, 10000000ull);
   } else {
     run = read_row(s);
   }
