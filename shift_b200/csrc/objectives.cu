@@ -43,6 +43,13 @@ SB_DEVICE float2 mul2(float2 a, float2 b) {
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
+SB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
 // the same of two values, two operations an instruction; `minus`: -m twice
 SB_DEVICE float2 exp_diff2(float2 z, float2 minus) {
   z = mul2(add2(z, minus), make_float2(kLog2e, kLog2e));
@@ -285,7 +292,9 @@ __global__ void __launch_bounds__(kThreads) logp_kernel(const Args a) {
     const bool live = label >= 0 && label < a.V;
     const double l = log(static_cast<double>(run.s));
     const double logp = live ? static_cast<double>(to_float(s.row[label])) - static_cast<double>(run.m) - l : 0.0;
-    a.lse[r] = static_cast<float>(static_cast<double>(run.m) + l);
+    const double lse = static_cast<double>(run.m) + l, left = lse - static_cast<double>(static_cast<float>(lse));
+    a.lse[r] = static_cast<float>(lse);
+    if (a.lse_low != nullptr) a.lse_low[r] = left == left ? static_cast<float>(left) : 0.f;     // infinities have none
     if (a.logp64 != nullptr) a.logp64[r] = logp;
     else a.logp[r] = static_cast<float>(logp);
   }
@@ -299,8 +308,14 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Args a) {
   const int label = a.labels[r];
   const float d = label >= 0 && label < a.V ? a.dlogp[r] : 0.f;
   const float lse = a.lse[r];
+  // lse near 1000 has steps of 6e-5, which every softmax value would carry; what it left comes in with the scaling
+  const float low = a.lse_low != nullptr ? a.lse_low[r] * -kLog2e : 0.f;
   if (d == 0.f) write_zeros(s);
-  else write_grad(s, label, d, [&](float2 z) { return exp_diff2(z, make_float2(-lse, -lse)); });
+  else
+    write_grad(s, label, d, [&](float2 z) {
+      z = fma2(add2(z, make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e), make_float2(low, low));
+      return make_float2(ex2(z.x), ex2(z.y));
+    });
 }
 
 SB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

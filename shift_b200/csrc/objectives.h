@@ -28,6 +28,7 @@ struct Args {
   float* logp;
   double* logp64;         // instead of logp, unrounded, for sums of many
   float* lse;             // written by the forward pass, read by the backward pass
+  float* lse_low;         // and what its rounding left, where both belong to one call; may be null
   const float* dlogp;
   Terms t;
   int* status;

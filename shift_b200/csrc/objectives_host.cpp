@@ -115,12 +115,13 @@ std::vector<at::Tensor> preference(at::Tensor& logits, const at::Tensor& labels,
   TORCH_CHECK(a.rows < (1L << 31), who, ": too many rows");
   const at::cuda::CUDAGuard guard(logits.device());
   const int64_t pairs = offs.numel() / 2;
-  auto rows = at::empty({2, a.rows}, logits.options().dtype(at::kFloat));
+  auto rows = at::empty({3, a.rows}, logits.options().dtype(at::kFloat));
   auto logp = at::empty({a.rows}, logits.options().dtype(at::kDouble));
   auto loss = at::empty({pairs}, rows.options()), margin = at::empty_like(loss);
   a.logp64 = logp.data_ptr<double>();
   a.lse = rows.data_ptr<float>();
-  float* dlogp = a.lse + a.rows;
+  a.lse_low = a.lse + a.rows;
+  float* dlogp = a.lse_low + a.rows;
   a.dlogp = dlogp;
   a.ranks = pick_ranks(a, size_of(logits), false);
   if (a.rows > 0) go(kLogp, a, logits);

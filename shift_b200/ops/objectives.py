@@ -49,7 +49,8 @@ def token_logp_fwd(logits: torch.Tensor, labels: torch.Tensor):
 
 
 def token_logp_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor) -> torch.Tensor:
-    """Overwrites the logits of ``token_logp_fwd`` by dlogp (onehot - softmax), and returns them."""
+    """Overwrites the logits of ``token_logp_fwd`` by dlogp (onehot - softmax), and returns them.  ``lse`` is fp32: where
+    logits lie near 1000 it has steps of 6e-5, and half of one is in every softmax value."""
     if logits.is_cuda:
         ext().token_logp_bwd(logits, labels, lse, dlogp)
         return logits

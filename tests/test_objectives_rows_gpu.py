@@ -83,3 +83,27 @@ def test_gradients_of_rows_behind_two_to_the_31():
     orc.close(logp[at], want_logp, SUM + 2.0 ** -23 * want_logp.abs(), "logp")
     compare(z, -torch.exp(want_logp - old[at].double()) * d[at].double(), 4 * SUM)
     check_status()
+
+
+@pytest.mark.parametrize("shift", [0.0, 1000.0, -3000.0])
+def test_preference_gradients_far_from_zero(shift):
+    """fp32 logits that are all far from zero: a log-sum-exp near 1000 has steps of 6e-5, its softmax must not."""
+    rows, vocab = 40, 3001
+    g = torch.Generator().manual_seed(8)
+    z = (torch.randn(rows, vocab, generator=g) * 2 + shift).to(DEV)
+    labels = torch.randint(0, vocab, (rows,), generator=g, dtype=torch.int32).to(DEV)
+    logp, *_ = orc.label_logp(z, labels)
+    ref = (logp + torch.randn(rows, generator=g).to(DEV) * 0.1).float()
+    gap = logp - ref.double()
+    h = 0.01 * (gap[:25].sum() - gap[25:].sum())
+    d = torch.full((rows,), 0.01 * float(torch.sigmoid(-h)), dtype=torch.float64, device=DEV)
+    d[:25] *= -1
+    want = orc.logits_grad(z, labels, d)
+    offs = torch.tensor([0, 25, 40], dtype=torch.int32, device=DEV)
+    ob.preference_loss_fwd_bwd(z, labels, ref, offs, beta=0.01)
+    # d: the margin is off by 0.01 SUM a row, and so is its sigmoid at most; softmax: SUM for the sum, 2^-20 for the difference
+    # z - lse (up to some tens) and its exponential; at the label two parts cancel
+    slack = 0.01 * rows * SUM + SUM + 2.0 ** -20
+    tol = (slack + 2.0 ** -24) * want.abs() + orc.tiny(torch.float32)
+    tol.scatter_add_(1, labels.long()[:, None], slack * d.abs()[:, None])
+    orc.close(z, want, tol, "dlogits")
