@@ -5,9 +5,10 @@
 //
 // All of them move logits: a row has V values of 2 or 4 bytes and a few of its own.  Rows are cut over a cluster of 1, 2,
 // 4 or 8 CTAs (joined over distributed shared memory in rank order) where a slice would not stay in shared memory, or
-// where there are too few rows for the SMs.  Maxima and sums are fp32, one running pair a thread; what follows from a
-// row's sum (its logarithm, ratios, the clip's comparison) is computed once a row in 64 bits, because a ratio next to the
-// clip's border decides a whole row's gradient.
+// where there are too few rows for the SMs.  Maxima are fp32, one running pair of maximum and sum a thread; the sums are
+// joined in 64 bits, and so is computed what follows from a row's sum (its logarithm, ratios, the clip's comparison), because
+// a ratio next to the clip's border decides a whole row's gradient and a pair of sequences adds up hundreds of rows.  A row's
+// log-probability is off by 2e-8 (rms, 32768 logits; on average 1e-8).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -26,8 +27,10 @@ SB_DEVICE float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// exp(z - m); m is finite.  The difference is rounded before it is scaled, so the error goes with |z - m|, not with |z|.
-SB_DEVICE float exp_diff(float z, float m) { return ex2((z - m) * kLog2e); }
+// exp(z - m); m is finite.  The difference is rounded before it is scaled, so the error goes with |z - m|, not with |z|.  For
+// sums log2(e) has 48 bits: with 24 a value far below the maximum is too large, by 8e-8 at -6 and 1.9e-7 at -14.
+constexpr float kLog2eLow = 1.9259630e-8f;
+SB_DEVICE float exp_diff(float z, float m) { return ex2(__fmaf_rn(z - m, kLog2e, (z - m) * kLog2eLow)); }
 
 SB_DEVICE float2 add2(float2 a, float2 b) {
   float2 d;
@@ -51,6 +54,12 @@ SB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 // the same of two values, two operations an instruction; `minus`: -m twice
+SB_DEVICE float2 exp_sum2(float2 z, float2 minus) {
+  z = add2(z, minus);
+  z = fma2(z, make_float2(kLog2e, kLog2e), mul2(z, make_float2(kLog2eLow, kLog2eLow)));
+  return make_float2(ex2(z.x), ex2(z.y));
+}
+// for a gradient's value, which is rounded by itself
 SB_DEVICE float2 exp_diff2(float2 z, float2 minus) {
   z = mul2(add2(z, minus), make_float2(kLog2e, kLog2e));
   return make_float2(ex2(z.x), ex2(z.y));
@@ -133,20 +142,32 @@ struct Slice {
   }
 };
 
-// Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.
+// The hardware's exponential is too small on average: by 2.2e-8 over arguments in [-0.7, 0] and 5.1e-8 below (of 4 million each),
+// 3.6e-8 where arguments are spread evenly and count by their values; at 0 it is exact.  All sums of a row would share that, and
+// a pair of sequences adds up hundreds of rows, so sums put it back.
+constexpr float kTooSmall = 3.6e-8f;
+
+// Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.  The sum is s + low:
+// beside the term of a likely label, which is 1, a rounding of each of a thread's additions would be as large as the rest.
 struct Run {
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, s = 0.f, low = 0.f;
   SB_DEVICE void rise(float b) {
     if (b > m) {
-      s *= m == -INFINITY ? 0.f : exp_diff(m, b);
+      const float f = m == -INFINITY ? 0.f : exp_diff(m, b);
+      s = __fmaf_rn(s, f, __fmaf_rn(s, f * kTooSmall, low * f));     // rounded once, after it was put back
+      low = 0.f;
       m = b;
     }
   }
-  // One vector, or one value.  NaN has no place in a maximum, so a row of NaN and -inf alone gets here with m = -inf;
-  // among infinite values the sum counts those, so that its logarithm adds nothing.
+  SB_DEVICE void plus(float x) {                   // exactly: what t does not hold goes to `low`
+    const float t = s + x, y = t - s;
+    low += (s - (t - y)) + (x - y);
+    s = t;
+  }
+  // One vector of values that are at most m, or one value.  NaN has no place in a maximum, so a row of NaN and -inf alone gets
+  // here with m = -inf; among infinite values the sum counts those, so that its logarithm adds nothing.
   template <int N>
-  SB_DEVICE void add(const float2* z, float top) {
-    rise(top);
+  SB_DEVICE void add(const float2* z) {
     if (m == INFINITY) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -154,48 +175,67 @@ struct Run {
       return;
     }
     const float at = m == -INFINITY ? 0.f : -m;
-    float2 part = exp_diff2(z[0], make_float2(at, at));
+    float2 part = exp_sum2(z[0], make_float2(at, at));
 #pragma unroll
-    for (int i = 1; i < N; ++i) part = add2(part, exp_diff2(z[i], make_float2(at, at)));
-    s += part.x + part.y;
+    for (int i = 1; i < N; ++i) part = add2(part, exp_sum2(z[i], make_float2(at, at)));
+    plus(part.x + part.y);
   }
   SB_DEVICE void add(float z) {
     rise(z);
-    s += z == INFINITY ? 1.f : exp_diff(z, m == -INFINITY ? 0.f : m);
+    plus(z == INFINITY ? 1.f : exp_diff(z, m == -INFINITY ? 0.f : m));
   }
+  // in 64 bits; the largest term was exact
+  SB_DEVICE double sum() const {
+    const double t = static_cast<double>(s) + static_cast<double>(low);
+    return s > 1.f && m < INFINITY ? t + static_cast<double>(kTooSmall) * (t - 1.0) : t;
+  }
+};
+
+// The same of a whole row, or of a part of it, in 64 bits.
+struct RowRun {
+  float m = -INFINITY;
+  double s = 0.0;
   // the sum over another maximum, at least this one
-  SB_DEVICE float over(float top) const { return m == top ? s : m == -INFINITY ? (s == s ? 0.f : s) : s * exp_diff(m, top); }
+  SB_DEVICE double over(float top) const {
+    return m == top ? s : m == -INFINITY ? (s == s ? 0.0 : s) : s * (static_cast<double>(exp_diff(m, top)) * (1.0 + kTooSmall));
+  }
 };
 
 // All threads' runs joined over the CTA and the cluster, in an order that does not change; every thread gets the result.
-// The maximum first, so that every sum is scaled once (an exponential of the hardware's is 5e-8 too small on average, which
-// a tree of joins would add up).
-SB_DEVICE Run join_all(Run r, int ranks) {
-  __shared__ float tops[kThreads / 32], sums[kThreads / 32];
-  __shared__ float2 mine;
+// The maximum first, so that every sum is scaled once.
+SB_DEVICE RowRun join_all(Run r, int ranks) {
+  __shared__ float tops[kThreads / 32], mine_m;
+  __shared__ double sums[kThreads / 32], mine_s;
   const int warp = threadIdx.x / 32;
-  Run all;
+  RowRun all;
   all.m = warp_max(r.m);
   if (threadIdx.x % 32 == 0) tops[warp] = all.m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) all.m = fmaxf(all.m, tops[w]);
-  const float s = warp_sum(r.over(all.m));
+  RowRun own;
+  own.m = r.m;
+  own.s = r.sum();
+  double s = own.over(all.m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (threadIdx.x % 32 == 0) sums[warp] = s;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) all.s += sums[w];
   if (ranks == 1) return all;
-  if (threadIdx.x == 0) mine = make_float2(all.m, all.s);
+  if (threadIdx.x == 0) {
+    mine_m = all.m;
+    mine_s = all.s;
+  }
   cg::cluster_group cl = cg::this_cluster();
   cl.sync();
-  Run row;
-  for (int k = 0; k < ranks; ++k) row.m = fmaxf(row.m, cl.map_shared_rank(&mine, k)->x);
+  RowRun row;
+  for (int k = 0; k < ranks; ++k) row.m = fmaxf(row.m, *cl.map_shared_rank(&mine_m, k));
   for (int k = 0; k < ranks; ++k) {
-    const float2 p = *cl.map_shared_rank(&mine, k);
-    Run one;
-    one.m = p.x;
-    one.s = p.y;
+    RowRun one;
+    one.m = *cl.map_shared_rank(&mine_m, k);
+    one.s = *cl.map_shared_rank(&mine_s, k);
     row.s += one.over(row.m);
   }
   cl.sync();                                       // nobody leaves while it is read
@@ -253,30 +293,40 @@ SB_DEVICE void write_grad(const Slice<T>& s, int label, float d, const P& p) {
 }
 
 template <typename T>
-SB_DEVICE void add_vec(Run& r, const uint4& u) {
-  constexpr int N = Slice<T>::E / 2;
-  float2 z[N];
-  Elem<T>::unpack(u, z);
-  r.add<N>(z, Elem<T>::top(u, z));
-}
-template <typename T>
 SB_DEVICE void add_edge(Run& r, const Slice<T>& s) {
   const int e = s.edge();
   if (e >= 0) r.add(to_float(s.row[e]));
 }
+// This thread's vectors of [v0, v1), four at a time, whose maximum is taken first: it then rises a few times a row.
+template <typename T, typename L>
+SB_DEVICE void add_vectors(Run& r, int v0, int v1, const L& load) {
+  constexpr int U = 4, N = Slice<T>::E / 2;
+  for (int v = v0 + static_cast<int>(threadIdx.x); v < v1; v += U * kThreads) {
+    uint4 u[U];
+    float2 z[N];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < v1) u[k] = load(v + k * kThreads);
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < v1) {
+        Elem<T>::unpack(u[k], z);
+        top = fmaxf(top, Elem<T>::top(u[k], z));
+      }
+    r.rise(top);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < v1) {
+        Elem<T>::unpack(u[k], z);
+        r.add<N>(z);
+      }
+  }
+}
 template <typename T>
 SB_DEVICE Run read_row(const Slice<T>& s) {
-  constexpr int U = 4;
   Run r;
-  for (int v = s.v0 + threadIdx.x; v < s.v1; v += U * kThreads) {
-    uint4 u[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (v + k * kThreads < s.v1) u[k] = *s.vec(v + k * kThreads);
-#pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (v + k * kThreads < s.v1) add_vec<T>(r, u[k]);
-  }
+  add_vectors<T>(r, s.v0, s.v1, [&](int v) { return *s.vec(v); });
   add_edge(r, s);
   return r;
 }
@@ -286,11 +336,11 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) logp_kernel(const Args a) {
   const long r = blockIdx.x / a.ranks;
   const Slice<T> s(static_cast<T*>(a.logits) + r * a.stride, a.V, blockIdx.x % a.ranks, a.ranks);
-  const Run run = join_all(read_row(s), a.ranks);
+  const RowRun run = join_all(read_row(s), a.ranks);
   if (threadIdx.x == 0 && s.edges) {
     const int label = a.labels[r];
     const bool live = label >= 0 && label < a.V;
-    const double l = log(static_cast<double>(run.s));
+    const double l = log(run.s);
     const double logp = live ? static_cast<double>(to_float(s.row[label])) - static_cast<double>(run.m) - l : 0.0;
     const double lse = static_cast<double>(run.m) + l, left = lse - static_cast<double>(static_cast<float>(lse));
     a.lse[r] = static_cast<float>(lse);
@@ -364,26 +414,25 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
     if (kl) ref = a.t.ref[r];
     if (a.t.weight != nullptr) weight = a.t.weight[r];
   }
-  Run run;
+  Run mine;
   bool late = false;
   if (KEEP) {
     __syncthreads();                               // the barriers are there
     for (int c = 0; c < kParts; ++c) {
       late |= !mbar_wait(&bar[c], 0, a.status);
-      const int end = part(c + 1);
-      for (int v = part(c) + threadIdx.x; v < end; v += kThreads) add_vec<T>(run, held[v - s.v0]);
+      add_vectors<T>(mine, part(c), part(c + 1), [&](int v) { return held[v - s.v0]; });
     }
-    add_edge(run, s);
+    add_edge(mine, s);
     if (late)                                      // the status says so; what was on its way here lands before anything else
       for (int c = 0; c < kParts; ++c) mbar_wait(&bar[c], 0, nullptr, 10000000ull);
   } else {
-    run = read_row(s);
+    mine = read_row(s);
   }
-  run = join_all(run, a.ranks);
+  const RowRun run = join_all(mine, a.ranks);
   if (threadIdx.x == 0) {
     double loss = 0, logp = 0, d = 0;
     if (live) {
-      logp = zl - static_cast<double>(run.m) - log(static_cast<double>(run.s));
+      logp = zl - static_cast<double>(run.m) - log(run.s);
       const double ratio = exp(logp - old), clipped = fmin(fmax(ratio, 1.0 - a.t.low), 1.0 + a.t.high);
       const double gain = adv == 0.0 && ratio == ratio ? 0.0 : ratio * adv, cut = clipped * adv;
       const bool open = gain <= cut;
@@ -404,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(const Args a) {
     }
   }
   __syncthreads();
-  const float d = s_d, inv = 1.f / run.s, m = run.m;
+  const float d = s_d, inv = static_cast<float>(1.0 / run.s), m = run.m;
   if (d == 0.f) {
     write_zeros(s);
     return;
