@@ -240,7 +240,8 @@ def attention_bwd(qkv: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: tor
     """dqkv of ``attention_fwd``, from its results and do [T, Hq * D] (rows a multiple of 16 bytes apart).
 
     Deterministic: no sum's order hangs on timing.  Rows that no sequence covers get zeros (with ``out``: are left as
-    they were)."""
+    they were).  fp16 scales what it rounds by powers of two, each row by the gradients that are in its own sums; the
+    scaled values stay below fp16's largest where the magnitudes of a row of v add up to less than 16000."""
     if qkv.is_cuda:
         return ext().packed_attn_bwd(qkv, o, lse, do, seqs.plan, seqs.rows, Hq, Hkv, D, scale, out,
                                      status_word(qkv.device))

@@ -97,3 +97,23 @@ def test_probabilities_below_what_fp16_holds(D):
     got = _step(qkv, do, [0, rows], heads)[:, 2 * D:].double()
     want = do[-1].double() / rows
     assert ((got - want).abs() <= 2.0 ** -11 * 2.02 * want.abs() + 2.0 ** -20 * want.abs() + orc.tiny(torch.float16)).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0])
+def test_values_as_large_as_documented(size, D):
+    """Rows of v whose magnitudes add up to 15900 and a `do` that goes along with one half of them and against the other: the
+    largest dS that there can be, 2 * 15900 * |do|, scaled to 2 at most, is below 65504."""
+    rows, heads = 300, (2, 1, D, D ** -0.5)
+    g = torch.Generator().manual_seed(11)
+    way = torch.randint(0, 2, (D,), generator=g) * 2 - 1
+    side = torch.randint(0, 2, (rows, 1), generator=g) * 2 - 1
+    qkv = _randn(rows, 4 * D, seed=12, std=0.3)
+    qkv[:, 3 * D:] = (side * way * (15900 / D)).half()
+    do = (way.repeat(2) * 1.99 * size * torch.ones(rows, 1)).half().to(DEV)
+    got = _step(qkv, do, [0, rows], heads)
+    want = orc.attention(qkv, [0, rows], *heads, do)["dqkv"]
+    big = want.abs() > 6e4                                 # what fp16 does not hold as a result
+    for cols in _parts(heads):
+        w, off = want[:, cols], (got[:, cols].double() - want[:, cols])[~big[:, cols]]
+        assert torch.isfinite(off).all() and off.norm() <= 3 * 2.0 ** -11 * w.norm() + 2.0 ** -25 * w.numel() ** 0.5
