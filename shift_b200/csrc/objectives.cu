@@ -142,13 +142,14 @@ struct Slice {
   }
 };
 
-// The hardware's exponential is too small on average: by 2.2e-8 over arguments in [-0.7, 0] and 5.1e-8 below (of 4 million each),
-// 3.6e-8 where arguments are spread evenly and count by their values; at 0 it is exact.  All sums of a row would share that, and
-// a pair of sequences adds up hundreds of rows, so sums put it back.
+// The hardware's exponential is too small on average: by 2.2e-8 over arguments in [-0.7, 0] and 5.1e-8 below (of 4 million
+// each), 3.6e-8 where arguments are spread evenly and count by their values; at 0 it is exact.  All sums of a row would share
+// that, and a pair of sequences adds up hundreds of rows, so sums put it back.
 constexpr float kTooSmall = 3.6e-8f;
 
-// Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.  The sum is s + low:
-// beside the term of a likely label, which is 1, a rounding of each of a thread's additions would be as large as the rest.
+// Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.  The sum is
+// s + low: beside the term of a likely label, which is 1, the roundings of a thread's additions would be as large as the rest
+// (rows whose label has 20 more than the others: off by 1.2e-7 rms instead of 4.2e-8, where the kernel saves 2 %).
 struct Run {
   float m = -INFINITY, s = 0.f, low = 0.f;
   SB_DEVICE void rise(float b) {

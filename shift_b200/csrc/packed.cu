@@ -236,7 +236,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
                                                   static_cast<unsigned long long>(a.turns[p0 + j]));
     // half turns in [-1, 1): the 64-bit fraction keeps its leading bits however small the angle is
     const float turn = __ll2float_rn(frac) * 1.0842021724855044e-19f /* 2^-63 */;
-    if constexpr (sizeof(T) == 2) {     // within half a turn the hardware's are off by 2^-21, far below a 16-bit rounding
+    // Within half a turn the hardware's sines are off by 2^-21, so a rotated value by 2^-20 of its pair's size: far below a
+    // 16-bit rounding of values of that size, more than that of the few that come out near 0.
+    if constexpr (sizeof(T) == 2) {
       sn[j] = __sinf(turn * 3.14159265f);
       cs[j] = __cosf(turn * 3.14159265f);
     } else {

@@ -144,8 +144,10 @@ class Engine:
         single-stage model, each followed, where it wants them, by a dict of
         further arguments of ``QwenMoE.forward`` (``seqs``: the rows hold
         packed sequences; ``objective``: another loss, which scales its own
-        gradient).  Returns the device scalar sum of token losses (already
-        scaled into the mean by ``loss_scale``)."""
+        gradient).  Returns the device scalar sum of all losses over the
+        number of rows (B * S of every microbatch): for cross entropy the mean
+        whose gradient ``loss_scale`` makes; what an objective returned is
+        summed and divided alike, whatever its own scale and weights."""
         n_tok = B * S * len(batches)
         self.store.zero_grad()
         total = None
