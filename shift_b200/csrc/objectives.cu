@@ -8,7 +8,7 @@
 // where there are too few rows for the SMs.  Maxima are fp32, one running pair of maximum and sum a thread; the sums are
 // joined in 64 bits, and so is computed what follows from a row's sum (its logarithm, ratios, the clip's comparison), because
 // a ratio next to the clip's border decides a whole row's gradient and a pair of sequences adds up hundreds of rows.  A row's
-// log-probability is off by 2e-8 (rms, 32768 logits; on average 1e-8).
+// log-probability is off by 1e-8 (rms, 32768 logits of a model's spread; on average by less than 1e-9).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -142,10 +142,11 @@ struct Slice {
   }
 };
 
-// The hardware's exponential is too small on average: by 2.2e-8 over arguments in [-0.7, 0] and 5.1e-8 below (of 4 million
+// The hardware's exponential is too small on average: by 2.2e-8 over arguments in [-ln 2, 0] and 5.05e-8 below (of 4 million
 // each), 3.6e-8 where arguments are spread evenly and count by their values; at 0 it is exact.  All sums of a row would share
 // that, and a pair of sequences adds up hundreds of rows, so sums put it back.
 constexpr float kTooSmall = 3.6e-8f;
+SB_DEVICE float too_small(float x) { return x > -0.6931472f ? 2.2e-8f : 5.05e-8f; }
 
 // Running (maximum, sum of exp(z - maximum)); an empty one, or one of -inf alone, has maximum -inf and sum 0.  The sum is
 // s + low: beside the term of a likely label, which is 1, the roundings of a thread's additions would be as large as the rest
@@ -155,7 +156,7 @@ struct Run {
   SB_DEVICE void rise(float b) {
     if (b > m) {
       const float f = m == -INFINITY ? 0.f : exp_diff(m, b);
-      s = __fmaf_rn(s, f, __fmaf_rn(s, f * kTooSmall, low * f));     // rounded once, after it was put back
+      s = __fmaf_rn(s, f, __fmaf_rn(s, f * too_small(m - b), low * f));            // rounded once, after it was put back
       low = 0.f;
       m = b;
     }
@@ -198,7 +199,9 @@ struct RowRun {
   double s = 0.0;
   // the sum over another maximum, at least this one
   SB_DEVICE double over(float top) const {
-    return m == top ? s : m == -INFINITY ? (s == s ? 0.0 : s) : s * (static_cast<double>(exp_diff(m, top)) * (1.0 + kTooSmall));
+    if (m == top) return s;
+    if (m == -INFINITY) return s == s ? 0.0 : s;
+    return s * (static_cast<double>(exp_diff(m, top)) * (1.0 + too_small(m - top)));
   }
 };
 
