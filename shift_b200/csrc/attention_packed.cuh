@@ -13,6 +13,11 @@
 // row of 128), one warp that loads tiles by TMA, one that issues tcgen05.mma.  Scores live in tensor memory; the
 // probabilities go back there as 16-bit operands of the second product and never to shared memory.
 //
+// What is rounded to 16 bits: P and dS, since the tensor cores take them so (two operands for each, the value and what its
+// rounding left, would double the products that bound these kernels), o, from which delta is taken, and the results.  Scores,
+// statistics and sums are fp32; the sum behind lse takes P unrounded.  Outputs are 1.1 to 1.5 times as far from 64 bits as fp32
+// arithmetic that rounds its results alone.
+//
 // What others hold.  Products run over whole blocks, so a masked value is a product with zero, which is zero unless the
 // other factor is infinite or NaN.  Rows that no sequence covers are cleared in shared memory after they were loaded.  Rows
 // of other sequences (or later ones of the same) that are not finite would leave NaN in a result: results that are not finite
